@@ -222,6 +222,38 @@ int qraf_hip_paged_attention_noalloc_dev(const float* q, const void* k_cache, co
                                          int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                          int32_t page_size, float scale, int32_t max_ctx, float* out, void* stream);
 uint64_t qraf_hip_attention_noalloc_max_bytes(void);
+/* Attention of rows that share the first positions of their caches, those
+ * positions read once for all of them: the batch of qraf_hip_paged_attention_dev
+ * (its caches, page types, page table, out and scale), its rows in groups.
+ *   group_starts [n_groups + 1] group g is rows group_starts[g] ..
+ *            group_starts[g+1] - 1 (ascending; a group may be empty)
+ *   prefix_lens [n_groups] positions that the rows of the group share: at
+ *            position t < prefix_lens[g] every row of the group that attends
+ *            to t has the same K and V, so they are read through the page
+ *            table of the group's first row (which must map them all, up to
+ *            the longest ctx of the group), the others through each row's own
+ *   ctx_lens [n_rows] as there, and 0: the row's output is zero.  A row may
+ *            attend to less than the prefix.
+ * (All three on the device; entries are taken into 0 .. n_rows, 0 .. max_ctx.)
+ * Sequences with one system prompt are a group that shares the prompt.  The
+ * rows of one sequence in one step (drafted tokens, a prompt chunk) are a group
+ * whose prefix is its whole cache, each row with its own ctx.  prefix 0 is plain
+ * attention.  Rows outside every group are left as they were.
+ * n_rows 1..1024, n_groups 1..n_rows; head_dim 16, 32, 64 or 128, any page_size
+ * and any number of query heads per KV head.  The workspace (qraf_hip_group_attention_workspace_bytes, 16-byte
+ * aligned) needs no initialisation; calls that share one must not overlap.
+ * Results are within the attention tolerance of qraf_hip_paged_attention_dev's
+ * on the same rows, and the same from call to call.  An infinity or NaN in the
+ * K or V of a position reaches the rows that attend to it and no others.
+ * No counterpart in the reference, which runs one sequence at a time. */
+uint64_t qraf_hip_group_attention_workspace_bytes(int32_t n_rows, int32_t n_groups, int32_t n_heads,
+                                                  int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx);
+int qraf_hip_group_attention_dev(const float* q, const void* k_cache, const void* v_cache, uint32_t kv_dtype,
+                                 const int32_t* page_table, int32_t max_pages_per_seq, const int32_t* ctx_lens,
+                                 const int32_t* group_starts, const int32_t* prefix_lens, int32_t n_rows,
+                                 int32_t n_groups, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                 int32_t page_size, float scale, int32_t max_ctx, float* out, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
 /* RoPE angle table, RopeCache::init (ops.cpp:179-193) computed on the host
  * with the host libm: table[pos*head_dim + i] = cos(pos*f_i),
  * table[pos*head_dim + i + 1] = sin(pos*f_i), f_i = 1/powf(theta, i/head_dim)
@@ -423,6 +455,52 @@ typedef struct qraf_sampling_params {
 int qraf_hip_sample_dev(float* logits, int32_t rows, int32_t vocab, const qraf_sampling_params* params,
                         const uint32_t* recent, const int32_t* recent_count, int32_t recent_stride,
                         const float* uniforms, uint32_t* tokens, void* stream);
+
+/* The distribution that qraf_hip_sample_dev draws from, as probabilities:
+ * probs [rows][vocab] (may be logits itself) from logits [rows][vocab], for
+ * verification against a draft (below).  With 64-bit weights w_i = exp((l_i -
+ * max) / T): of the top_k largest logits (all when top_k <= 0 or >= vocab;
+ * equal logits in index order) the shortest prefix whose weight reaches top_p
+ * times theirs (all of them unless 0 < top_p < 1), w_i over their sum; 0 elsewhere.
+ * temperature <= 0: 1 at the first of the largest logits (Sampler::argmax,
+ * sampler.cpp:25-35).  repetition_penalty, recent, recent_count and
+ * recent_stride as for qraf_hip_sample_dev (the logits are penalised in place).
+ * A NaN counts as -inf; of infinite logits each has the same probability; a row
+ * without a logit above -inf is all zero.  The workspace
+ * (qraf_hip_sample_probs_workspace_bytes, 16-byte aligned) needs no
+ * initialisation; calls that share one must not overlap.  The same from call to
+ * call.  Sampler::sample (sampler.cpp:57-128) is the counterpart in the reference,
+ * which draws from these probabilities (rounded sums in fp32) and drops them. */
+uint64_t qraf_hip_sample_probs_workspace_bytes(int32_t rows, int32_t vocab);
+int qraf_hip_sample_probs_dev(float* logits, int32_t rows, int32_t vocab, const qraf_sampling_params* params,
+                              const uint32_t* recent, const int32_t* recent_count, int32_t recent_stride, float* probs,
+                              void* workspace, uint64_t workspace_bytes, void* stream);
+/* Verification of drafted tokens (speculative decoding), many sequences at
+ * once, on the device.  Sequence s has rows row_starts[s] .. row_starts[s+1]-1
+ * (row_starts [n_seqs + 1] ascending, on the device, entries taken into 0 ..
+ * n_rows): with k drafted tokens k + 1 rows, row j the target's distribution
+ * behind its first j drafts.
+ *   probs [n_rows][vocab] those distributions (qraf_hip_sample_probs_dev)
+ *   draft_probs [n_rows][vocab] the distribution each draft was drawn from, or
+ *            NULL: the drafts were not drawn (a prompt's own n-grams)
+ *   draft_tokens [n_rows] the draft behind row j (a sequence's last row: unused)
+ *   accept_uniforms [n_rows], pick_uniforms [n_seqs] draws from [0, 1)
+ * Draft x of row j is accepted while accept * q(x) < p(x), compared in 64 bits
+ * (q = 1 without draft_probs; a token outside the vocabulary never is).  The
+ * first rejected row's next token is drawn from max(p - q, 0) (without
+ * draft_probs: from p without x; where nothing is left, from p), the last row's
+ * from p: the lowest token whose running sum over the vocabulary in 64 bits
+ * passes pick times the whole.  So the emitted tokens are distributed as the
+ * target's own samples.
+ *   accepted [n_seqs] drafts accepted;  tokens [n_rows]: at row_starts[s] the
+ *   accepted drafts, then the next token, then 0xFFFFFFFF up to the last row.
+ * A sequence without rows has accepted 0.  Workspace as above
+ * (qraf_hip_verify_draft_workspace_bytes).  No counterpart in the reference. */
+uint64_t qraf_hip_verify_draft_workspace_bytes(int32_t n_seqs, int32_t vocab);
+int qraf_hip_verify_draft_dev(const float* probs, const float* draft_probs, const uint32_t* draft_tokens,
+                              const int32_t* row_starts, int32_t n_seqs, int32_t n_rows, int32_t vocab,
+                              const float* accept_uniforms, const float* pick_uniforms, int32_t* accepted,
+                              uint32_t* tokens, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* QRAF file -> HBM.  The file layout of include/qraf/format.h:26-132 is
  * checked as validate_header (src/qraf/header.cpp:8-45) and get_string

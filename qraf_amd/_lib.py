@@ -73,6 +73,9 @@ SIGNATURES = {
     "qraf_hip_paged_attention_noalloc_dev": (C.c_int, [vp, vp, vp, C.c_uint32, vp, C.c_int32, vp] + [C.c_int32] * 5 +
                                              [C.c_float, C.c_int32, vp, vp]),
     "qraf_hip_attention_noalloc_max_bytes": (C.c_uint64, []),
+    "qraf_hip_group_attention_workspace_bytes": (C.c_uint64, [C.c_int32] * 6),
+    "qraf_hip_group_attention_dev": (C.c_int, [vp, vp, vp, C.c_uint32, vp, C.c_int32, vp, vp, vp] + [C.c_int32] * 6 +
+                                     [C.c_float, C.c_int32, vp, vp, C.c_uint64, vp]),
     "qraf_hip_split_bf16_dev": (C.c_int, [vp, vp, vp, C.c_int32, C.c_int32, vp]),
     "qraf_hip_set_qgemm_tuning": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "qraf_hip_set_qgemm_schedule": (C.c_int, [C.c_int32, C.c_int32]),
@@ -123,6 +126,11 @@ class SamplingParams(C.Structure):
 SIGNATURES.update({
     "qraf_hip_sample_dev": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), vp, vp, C.c_int32, vp, vp,
                                       vp]),
+    "qraf_hip_sample_probs_workspace_bytes": (C.c_uint64, [C.c_int32] * 2),
+    "qraf_hip_sample_probs_dev": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), vp, vp, C.c_int32, vp,
+                                            vp, C.c_uint64, vp]),
+    "qraf_hip_verify_draft_workspace_bytes": (C.c_uint64, [C.c_int32] * 2),
+    "qraf_hip_verify_draft_dev": (C.c_int, [vp, vp, vp, vp] + [C.c_int32] * 3 + [vp, vp, vp, vp, vp, C.c_uint64, vp]),
     "qraf_engine_sample": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), u32p, i32p, C.c_int32, fp,
                                      u32p]),
     "qraf_engine_create": (C.c_int, [C.POINTER(ModelConfig), C.POINTER(EngineOptions), C.POINTER(vp)]),

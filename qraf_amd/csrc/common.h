@@ -170,6 +170,18 @@ size_t sample_sort_bytes(int rows, int V, const qraf_sampling_params& sp);
 int launch_sample(float* logits, int rows, int V, const qraf_sampling_params& sp, const uint32_t* recent,
                   const int32_t* counts, int stride, const float* uniforms, uint32_t* out, void* sort_ws,
                   size_t sort_bytes, hipStream_t s);
+// Sampler::apply_repetition_penalty of every row, in place
+int launch_penalty(float* logits, int rows, int V, float penalty, const uint32_t* recent, const int32_t* counts,
+                   int stride, hipStream_t s);
+// a Sampler's distribution as probabilities, and drafted tokens verified against such rows (speculate.hip)
+size_t sample_probs_workspace_bytes(int rows, int V);
+int launch_sample_probs(float* logits, int rows, int V, const qraf_sampling_params& sp, const uint32_t* recent,
+                        const int32_t* counts, int stride, float* probs, void* ws, size_t ws_bytes, hipStream_t s);
+size_t verify_draft_workspace_bytes(int n, int V);
+int launch_verify_draft(const float* probs, const float* draft_probs, const uint32_t* draft_tokens,
+                        const int32_t* row_starts, int n, int n_rows, int V, const float* accept_uniforms,
+                        const float* pick_uniforms, int32_t* accepted, uint32_t* tokens, void* ws, size_t ws_bytes,
+                        hipStream_t s);
 
 // x may be S slices of `slice` floats each (GEMM partials), summed in slice order
 int launch_split_bf16(const float* x, uint16_t* hi, uint16_t* lo, int M, int K, int op, float* xout, hipStream_t s,
@@ -206,6 +218,12 @@ int launch_attention(const float* q, const void* kc, const void* vc, uint32_t kv
                      int max_pages, const int32_t* ctx, int n, int H, int Hkv, int hd, int page_size, float scale,
                      int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st, uint16_t* out_hi = nullptr,
                      uint16_t* out_lo = nullptr);
+// rows of a group share the first positions of their caches (attention_group.hip)
+size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd, int max_ctx);
+int launch_group_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype,
+                           const int32_t* page_table, int max_pages, const int32_t* ctx, const int32_t* group_starts,
+                           const int32_t* prefix, int n, int groups, int H, int Hkv, int hd, int page_size, float scale,
+                           int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st);
 int launch_rope_append(const float* qkv, const float* bias, int n, int H, int Hkv, int hd, const int32_t* pos,
                        const float* rope, float* q_out, void* kc, void* vc, uint32_t kv_dtype,
                        const int32_t* page_table, int max_pages, int page_size, hipStream_t st, int S = 1,

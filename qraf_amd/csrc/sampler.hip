@@ -912,6 +912,22 @@ size_t sample_sort_bytes(int rows, int V, const qraf_sampling_params& sp) {
     return greedy || cutoff <= CAND_CAP ? 0 : (size_t)rows * V * 16;
 }
 
+// Sampler::apply_repetition_penalty of every row, in place (nothing without recent tokens)
+int launch_penalty(float* logits, int rows, int V, float penalty, const uint32_t* recent, const int32_t* counts,
+                   int stride, hipStream_t s) {
+    if (penalty == 1.0f) return QRAF_HIP_OK;  // sampler.cpp:39
+    QH_REQUIRE(!recent || (counts && stride > 0), QRAF_HIP_ERR_INVALID, "sample: recent tokens need counts");
+    if (!recent) return QRAF_HIP_OK;
+    if (stride <= PEN_LDS)
+        hipLaunchKernelGGL(penalty_rows_lds_kernel, dim3(rows), dim3(256), 0, s, logits, V, recent, counts, stride,
+                           penalty);
+    else
+        hipLaunchKernelGGL(penalty_rows_kernel, dim3((rows + 63) / 64), dim3(64), 0, s, logits, V, rows, recent,
+                           counts, stride, penalty);
+    QH_CHECK_HIP(hipGetLastError());
+    return QRAF_HIP_OK;
+}
+
 int launch_sample(float* logits, int rows, int V, const qraf_sampling_params& sp, const uint32_t* recent,
                   const int32_t* counts, int stride, const float* uniforms, uint32_t* out, void* sort_ws,
                   size_t sort_bytes, hipStream_t s) {
@@ -923,18 +939,7 @@ int launch_sample(float* logits, int rows, int V, const qraf_sampling_params& sp
                QRAF_HIP_ERR_INVALID, "sample: sort storage of %zu bytes, %zu needed", sort_bytes,
                sample_sort_bytes(rows, V, sp));
     (void)cutoff;
-    if (sp.repetition_penalty != 1.0f) {  // sampler.cpp:39
-        QH_REQUIRE(!recent || (counts && stride > 0), QRAF_HIP_ERR_INVALID, "sample: recent tokens need counts");
-        if (recent) {
-            if (stride <= PEN_LDS)
-                hipLaunchKernelGGL(penalty_rows_lds_kernel, dim3(rows), dim3(256), 0, s, logits, V, recent, counts,
-                                   stride, sp.repetition_penalty);
-            else
-                hipLaunchKernelGGL(penalty_rows_kernel, dim3((rows + 63) / 64), dim3(64), 0, s, logits, V, rows,
-                                   recent, counts, stride, sp.repetition_penalty);
-            QH_CHECK_HIP(hipGetLastError());
-        }
-    }
+    QH_TRY(launch_penalty(logits, rows, V, sp.repetition_penalty, recent, counts, stride, s));
     hipLaunchKernelGGL(sample_rows_kernel, dim3(rows), dim3(SNT), 0, s, logits, V, sp.temperature, cutoff, sp.top_p,
                        uniforms, out, (float*)sort_ws);
     QH_CHECK_HIP(hipGetLastError());
