@@ -3,6 +3,18 @@
 //
 // Row r of group g attends to positions t < ctx[r]; those below prefix[g] hold
 // the same K and V for every row of the group.  Pages as in attention.hip.
+//
+// The work of one KV head is a list of jobs: per group its query vectors (rows x
+// the G query heads of the KV head, "columns") in blocks of up to 128 over the
+// positions below the prefix that some row of the block attends to, and per row
+// its G columns over its own positions behind the prefix.  A job is cut into
+// tiles of 32 positions per wave, and the tiles of all jobs, in order, into
+// equal shares for the workgroups (group_tile_kernel), all from the
+// device-resident lengths: a long prefix of few columns spreads over the chip,
+// and ragged lengths balance.  A share that holds all there is of a column
+// writes the output; the others write (max, sum, unnormalised output) parts,
+// which group_merge_kernel joins in position order.  group_any_kernel takes the
+// shapes that the tiles do not.
 #include <math.h>
 
 #include <algorithm>
@@ -20,8 +32,13 @@ struct GroupArgs {
     const int32_t* starts;      // [groups + 1]
     const int32_t* prefix;      // [groups]
     float* out;                 // [n][H][HD]
+    float* part_o;              // [Hkv][slots][HD] unnormalised outputs of parts
+    float2* part_ml;            // [Hkv][slots] their maxima (in powers of two) and sums
+    int* plan;                  // for the merge: tiles, prefix jobs, {column, any of the prefix} of each row, tile prefix
     int n, groups, H, Hkv, G, page_size, max_pages, max_ctx;
     float scale;
+    int ps_log2, job_cap;       // page_size = 1 << ps_log2; prefix jobs at most
+    long long slots;            // part slots of a KV head
 };
 
 // entries of the device-resident layout, taken into their ranges
@@ -149,9 +166,820 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// The tiles: head_dim 64 or 128, pages of 16, 32, 64, ... positions, up to 128
+// query heads per KV head.
+//
+// One wave holds 32 columns and takes 32 positions at a time, on the 32x32x16
+// fp16 matrix products, transposed:
+//     S^T[position][column] = K q^T     A = K (lane: position, 8 dims), B = q
+//     O^T[dim][column]     += V^T p^T   A = V (lane: dim, 8 positions), B = p
+// In the result of the first, lane l holds 16 scores of column l % 32 (its other
+// 16 are in lane l ^ 32), so a softmax row's maximum, sum and rescaling factor
+// are one register a lane and one exchange between the halves; and with
+// position(A row) permuted as in key_of() those 16 are, 8 by 8, the B operand of
+// the second: nothing moves between lanes.  32 columns and not 16: half the
+// operand reads per product, and the reads are what bounds it.
+//
+// q, p and f32 K and V enter as fp16 hi + lo pairs (22 bits; q scaled per column,
+// f32 K per tile and V per wave by powers of two, p by 2^14, so that neither
+// half leaves fp16's range: what is smaller than 2^-39 of the largest may be lost),
+// fp16 K and V as they are, int8 widened; a product of two pairs is three
+// matrix products (lo x lo is below 2^-22).  int8 scales: K's on the scores, V's
+// on p.  Sums in fp32.
+//
+// K of the next tile is requested behind this tile's scores, V behind its
+// outputs, straight into registers (a wave shares no tile with others but through the
+// caches): two waves per SIMD cover each other's waits.
+// ---------------------------------------------------------------------------
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int GW = 8, GTH = 64 * GW;  // waves and threads of a workgroup
+constexpr int BLK = 128;              // columns of a block: 4 waves of 32
+constexpr float P_UNIT = 14.f;        // p is held times 2^14
+
+template <int CTRL>
+__device__ __forceinline__ int gdpp(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, true);
+}
+enum : int { GDPP_XOR1 = 0xB1, GDPP_XOR2 = 0x4E, GDPP_ROR4 = 0x124, GDPP_ROR8 = 0x128 };
+// op over all lanes / over lanes l and l ^ 32, in every lane
+template <typename T, typename F>
+__device__ __forceinline__ T over_halves(T x, F op) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return op(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
+}
+template <typename T, typename F>
+__device__ __forceinline__ T over_wave(T x, F op) {
+    auto in = [](T v) { return __builtin_bit_cast(int, v); };
+    auto back = [](int v) { return __builtin_bit_cast(T, v); };
+    x = op(x, back(gdpp<GDPP_XOR1>(in(x))));
+    x = op(x, back(gdpp<GDPP_XOR2>(in(x))));
+    x = op(x, back(gdpp<GDPP_ROR4>(in(x))));
+    x = op(x, back(gdpp<GDPP_ROR8>(in(x))));
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = op(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
+    return over_halves(x, op);
+}
+__device__ __forceinline__ float fmax2(float x, float y) { return fmaxf(x, y); }
+__device__ __forceinline__ int imax2(int x, int y) { return max(x, y); }
+__device__ __forceinline__ int imin2(int x, int y) { return min(x, y); }
+
+// the position, of a tile's 32, that row rho of the first product's A holds
+__device__ __forceinline__ int key_of(int rho) {
+    return 16 * ((rho >> 4) & 1) + 8 * ((rho >> 2) & 1) + 4 * ((rho >> 3) & 1) + (rho & 3);
+}
+// power of two that brings a largest magnitude into [2^14, 2^15), as its exponent
+__device__ __forceinline__ int unit_exp(float mx) {
+    if (!(mx > 0.f)) return 110;
+    int e;
+    frexpf(mx, &e);
+    return max(-110, min(15 - e, 110));
+}
+// two values as fp16 hi + lo
+__device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
+    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x - (float)hi[0], y - (float)hi[1]));
+}
+__device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        f16x2 h, l;
+        split2(x[i], x[i + 1], h, l);
+        hi[i] = h[0], hi[i + 1] = h[1];
+        lo[i] = l[0], lo[i + 1] = l[1];
+    }
+}
+// 4 int8 (one dword) -> 4 fp16, exactly: the biased byte q + 128 under the
+// exponent of 1024, less 1152
+__device__ __forceinline__ uint2 widen4(uint32_t w) {
+    const uint32_t u = w ^ 0x80808080u;
+    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const f16x2 x = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+    const f16x2 y = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+    return make_uint2(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y));
+}
+__device__ __forceinline__ f16x8 widen8(uint32_t w0, uint32_t w1) {
+    const uint2 x = widen4(w0), y = widen4(w1);
+    return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
+}
+
+// ---- the plan: jobs and tiles, from the device-resident lengths, by every workgroup
+struct GroupPlan {
+    int* pref;   // [jobs + 1] first tile of each job: prefix blocks, then a tail per row
+    int* jb;     // [groups + 1] first prefix job of each group
+    int* gs;     // [groups + 1] group starts
+    int np;      // prefix jobs
+};
+// the last entry of ascending v[0..n) at or below x (v[0] <= x)
+__device__ __forceinline__ int last_at(const int* v, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+// v[0..n) to its exclusive prefix sums, v[n] the sum; a barrier before and behind
+__device__ void prefix_sum(int* v, int n, int* s_wave) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (n + GTH - 1) / GTH, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    __syncthreads();
+    int sum = 0;
+    for (int i = i0; i < i1; i++) sum += v[i];
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(inc, o);
+        if (lane >= o) inc += x;
+    }
+    if (lane == 63) s_wave[wave] = inc;
+    __syncthreads();
+    int run = inc - sum, all = 0;
+#pragma unroll
+    for (int w = 0; w < GW; w++) {
+        const int x = s_wave[w];
+        run += w < wave ? x : 0;
+        all += x;
+    }
+    for (int i = i0; i < i1; i++) {
+        const int x = v[i];
+        v[i] = run;
+        run += x;
+    }
+    if (tid == 0) v[n] = all;
+    __syncthreads();
+}
+// waves of a job of `cols` columns side by side along them (the others along the positions)
+__device__ __forceinline__ int waves_over(int cols) { return cols > 64 ? 4 : cols > 32 ? 2 : 1; }
+__device__ __forceinline__ int tiles_of(int positions, int cols) {
+    const int step = 32 * (GW / waves_over(cols));
+    return (positions + step - 1) / step;
+}
+__device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return max(0, min(a.prefix[g], a.max_ctx)); }
+// a tail begins with the 16 positions that hold the prefix's end, one page's
+__device__ __forceinline__ int tail_base(int prefix) { return prefix & ~15; }
+
+__device__ void group_plan(const GroupArgs& a, GroupPlan& p, int* s_wave) {
+    const int tid = threadIdx.x;
+    for (int g = tid; g <= a.groups; g += GTH) p.gs[g] = group_start(a, g);
+    __syncthreads();
+    for (int g = tid; g < a.groups; g += GTH) p.jb[g] = (max(0, p.gs[g + 1] - p.gs[g]) * a.G + BLK - 1) / BLK;
+    prefix_sum(p.jb, a.groups, s_wave);
+    p.np = min(p.jb[a.groups], a.job_cap);
+    for (int j = tid; j < p.np + a.n; j += GTH) p.pref[j] = 0;
+    __syncthreads();
+    for (int r = tid; r < a.n; r += GTH) {
+        if (r < p.gs[0] || r >= p.gs[a.groups]) continue;
+        const int g = last_at(p.gs, a.groups, r), ctx = row_ctx(a, r), pre = prefix_len(a, g);
+        const int c0 = (r - p.gs[g]) * a.G, j0 = p.jb[g] + c0 / BLK, j1 = p.jb[g] + (c0 + a.G - 1) / BLK;
+        for (int j = j0; j <= j1 && j < p.np; j++) atomicMax(&p.pref[j], min(ctx, pre));
+        if (ctx > pre) p.pref[p.np + r] = tiles_of(ctx - tail_base(pre), a.G);
+    }
+    __syncthreads();
+    for (int j = tid; j < p.np; j += GTH) {
+        const int g = last_at(p.jb, a.groups, j);
+        p.pref[j] = tiles_of(p.pref[j], min(BLK, (p.gs[g + 1] - p.gs[g]) * a.G - BLK * (j - p.jb[g])));
+    }
+    prefix_sum(p.pref, p.np + a.n, s_wave);
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        const int jobs = p.np + a.n;
+        for (int j = tid; j <= jobs; j += GTH) a.plan[2 + 2 * a.n + j] = p.pref[j];
+        for (int r = tid; r < a.n; r += GTH) {
+            const bool in = r >= p.gs[0] && r < p.gs[a.groups];
+            const int g = in ? last_at(p.gs, a.groups, r) : 0;
+            a.plan[2 + 2 * r] = in ? p.jb[g] * BLK + (r - p.gs[g]) * a.G : -1;
+            a.plan[3 + 2 * r] = in && min(row_ctx(a, r), prefix_len(a, g)) > 0;
+        }
+        if (tid == 0) {
+            a.plan[0] = p.pref[jobs];
+            a.plan[1] = p.np;
+        }
+    }
+}
+
+// ---- a wave's K and V of one tile
+template <int HD, int KV>
+struct GroupTile;
+template <int HD>
+struct GroupTile<HD, (int)DT_F16> {
+    f16x8 k[HD / 16];
+    uint4 v[HD / 32][2];
+};
+template <int HD>
+struct GroupTile<HD, (int)DT_I8> {
+    uint4 k[HD / 32];
+    uint2 v[HD / 32][2];
+    float4 ks[4], vs[4];
+};
+template <int HD>
+struct GroupTile<HD, (int)DT_F32> {
+    typedef float vrow __attribute__((ext_vector_type(HD / 32)));
+    float4 k[HD / 8];
+    vrow v[16];
+};
+
+template <int HD, int KV>
+__global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
+    constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
+    constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
+    constexpr int OS = HD + 4;  // row stride of the waves' outputs
+    extern __shared__ __align__(16) float s_dyn[];
+    __shared__ float s_m[GW][32], s_l[GW][32];
+    __shared__ int s_wave[GW];
+    float* s_o = s_dyn;           // [GW][32][OS] the waves' outputs, behind a segment's tiles
+    uint4* s_q = (uint4*)s_dyn;   // [4][KS][2][64] q's operands lane by lane, during them
+    GroupPlan plan;
+    plan.pref = (int*)(s_dyn + GW * 32 * OS);
+    plan.jb = plan.pref + a.job_cap + a.n + 1;
+    plan.gs = plan.jb + a.groups + 1;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.y, w = blockIdx.x, G = a.G, psl = a.ps_log2, psm = (1 << psl) - 1;
+
+    group_plan(a, plan, s_wave);
+    const int jobs = plan.np + a.n, T = plan.pref[jobs], shares = min((int)gridDim.x, T);
+    if (w >= shares) return;
+    const int t0 = (int)(((long long)w * T) / shares), t1 = (int)(((long long)(w + 1) * T) / shares);
+
+    for (int j = __builtin_amdgcn_readfirstlane(last_at(plan.pref, jobs, t0)); j < jobs; j++) {
+        const int p0 = plan.pref[j], p1 = plan.pref[j + 1];
+        if (p0 >= t1) break;
+        if (p0 == p1) continue;
+        const int ja = max(t0, p0) - p0, jend = min(t1, p1) - p0;  // the segment: tiles [ja, jend) of the job
+        const bool whole = ja == 0 && jend == p1 - p0;
+
+        // ---- the job
+        const bool tail = j >= plan.np;
+        int g, colbase, cols, trow;
+        if (tail) {
+            trow = j - plan.np;
+            g = last_at(plan.gs, a.groups, trow);
+            colbase = trow * G;
+            cols = G;
+        } else {
+            g = last_at(plan.jb, a.groups, j);
+            const int b = j - plan.jb[g];
+            trow = plan.gs[g];
+            colbase = trow * G + BLK * b;
+            cols = min(BLK, (plan.gs[g + 1] - trow) * G - BLK * b);
+        }
+        const int pre = prefix_len(a, g), lo = tail ? pre : 0, base = tail ? tail_base(pre) : 0;
+        const int wq = waves_over(cols), wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
+        const int32_t* ptab = a.page_table + (size_t)trow * a.max_pages;
+
+        // ---- the lane's column (past the block's end: its last, not written)
+        const int ab = colbase + min(qt * 32 + col, cols - 1), r = ab / G;
+        const float* qrow = a.q + ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
+        const int ctx = row_ctx(a, r), lim = tail ? ctx : min(ctx, pre);
+        const int kend = __builtin_amdgcn_readfirstlane(over_wave(lim, imax2));  // behind the last that some column attends to
+        const int least = __builtin_amdgcn_readfirstlane(over_wave(lim, imin2));
+
+        float4 qraw[2 * KS];
+#pragma unroll
+        for (int kk = 0; kk < KS; kk++) {
+            const int d = I8 ? 32 * (kk >> 1) + 16 * half + 8 * (kk & 1) : 16 * kk + 8 * half;
+            qraw[2 * kk] = *(const float4*)(qrow + d);
+            qraw[2 * kk + 1] = *(const float4*)(qrow + d + 4);
+        }
+
+        // ---- loads of the tile at position t
+        GroupTile<HD, KV> tl;
+        int pg0 = 0, pg1 = 0;
+        auto ids = [&](int t) {
+            pg0 = __builtin_amdgcn_readfirstlane(ptab[min(t, kend - 1) >> psl]);
+            pg1 = __builtin_amdgcn_readfirstlane(ptab[min(t + 16, kend - 1) >> psl]);
+        };
+        const size_t blk = (size_t)a.page_size * (I8 ? HD + 4 : F16 ? 2 * HD : 4 * HD);  // bytes of a (page, KV head)
+        auto block = [&](const void* pool, int pg) { return (const char*)pool + ((size_t)pg * a.Hkv + kvh) * blk; };
+        auto load_k = [&](int t) {
+            const int pc = min(t + key_of(col), kend - 1);  // (past the end: the last position's, masked below)
+            const char* kp = pc >= t + 16 ? block(a.kc, pg1) : block(a.kc, pg0);
+            if constexpr (F16) {
+                const uint32_t o = (uint32_t)((pc & psm) * HD + 8 * half) * 2u;
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) tl.k[kk] = *(const f16x8*)(kp + (o + 32u * kk));
+            } else if constexpr (I8) {
+                const uint32_t o = (uint32_t)((pc & psm) * HD + 16 * half);
+#pragma unroll
+                for (int kk = 0; kk < KS / 2; kk++) tl.k[kk] = *(const uint4*)(kp + (o + 32u * kk));
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const char* sp = block(a.kc, b ? pg1 : pg0) + (size_t)a.page_size * HD + 4 * (((t + 16 * b) & psm) + 8 * half);
+                    tl.ks[2 * b] = *(const float4*)sp;
+                    tl.ks[2 * b + 1] = *(const float4*)(sp + 16);
+                }
+            } else {
+                const uint32_t o = (uint32_t)((pc & psm) * HD + 8 * half) * 4u;
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) {
+                    tl.k[2 * kk] = *(const float4*)(kp + (o + 64u * kk));
+                    tl.k[2 * kk + 1] = *(const float4*)(kp + (o + 64u * kk + 16u));
+                }
+            }
+        };
+        auto load_v = [&](int t) {
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const char* vp = block(a.vc, b ? pg1 : pg0);
+                const int off = ((t + 16 * b) & psm) + 8 * half;
+                if constexpr (F16) {
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+                        tl.v[d][b] = *(const uint4*)(vp + (uint32_t)((32 * d + col) * a.page_size + off) * 2u);
+                } else if constexpr (I8) {
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+                        tl.v[d][b] = *(const uint2*)(vp + (uint32_t)((32 * d + col) * a.page_size + off));
+                    const char* sp = vp + (size_t)a.page_size * HD + 4 * off;
+                    tl.vs[2 * b] = *(const float4*)sp;
+                    tl.vs[2 * b + 1] = *(const float4*)(sp + 16);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int pc = min(t + 16 * b + 8 * half + i, kend - 1);
+                        const char* xp = pc >= t + 16 ? block(a.vc, pg1) : block(a.vc, pg0);
+                        tl.v[8 * b + i] = *(const typename GroupTile<HD, (int)DT_F32>::vrow*)(
+                            xp + (uint32_t)((pc & psm) * HD + DT * col) * 4u);
+                    }
+                }
+            }
+        };
+
+        // f32 rows of 128 fill the registers: V is requested behind the scores, the next K behind the outputs
+        constexpr bool TURNS = F32 && HD == 128;
+        int i = ja, t = base + (i * wk + kw) * 32;  // the wave's tiles: every wk-th 32 positions
+        const int dt = 32 * wk;
+        bool more = i < jend && t < kend;
+        if (more) {
+            ids(t);
+            load_k(t);
+            if (!TURNS) load_v(t);
+        }
+
+        // ---- q as fp16 hi + lo, scaled per column (waves of the same columns write the same)
+        float qs;
+        uint4* qop = s_q + qt * KS * 128 + lane;
+        {
+            float mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * KS; k++)
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(qraw[k].x), fabsf(qraw[k].y)), fmaxf(fabsf(qraw[k].z), fabsf(qraw[k].w))));
+            mx = over_halves(mx, fmax2);
+            const int e = mx <= 3.0e38f ? unit_exp(mx) : 0;
+            const float sg = ldexpf(1.f, e);
+            if (kw == 0) {
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) {
+                    const float4 x = qraw[2 * kk], y = qraw[2 * kk + 1];
+                    const float v[8] = {x.x * sg, x.y * sg, x.z * sg, x.w * sg, y.x * sg, y.y * sg, y.z * sg, y.w * sg};
+                    f16x8 hi, lw;
+                    split8(v, hi, lw);
+                    qop[128 * kk] = __builtin_bit_cast(uint4, hi);
+                    qop[128 * kk + 64] = __builtin_bit_cast(uint4, lw);
+                }
+            }
+            qs = ldexpf(a.scale * 1.44269504088896340736f, -e);  // scores in powers of two
+        }
+        __syncthreads();
+
+        float m = -INFINITY, l = 0.f;  // running maximum; sum of the lane's own positions, times 2^14
+        int vexp = 110;                // V's unit: outputs are held times 2^vexp (f32, int8)
+        f32x16 o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) o[d][x] = 0.f;
+
+        while (more) {
+            // opaque to the compiler: else q's operands are read once, ahead of the loop, and spilled
+            int qat = qt * KS * 128 + lane;
+            asm volatile("" : "+v"(qat));
+            const uint4* qtile = s_q + qat;
+            const bool edge = t < lo || t + 32 > least;  // some column does not attend to all 32
+            // ---- scores
+            f32x16 s;
+#pragma unroll
+            for (int x = 0; x < 16; x++) s[x] = 0.f;
+            float fs = qs;
+            if constexpr (F32) {
+                float mx = 0.f;
+#pragma unroll
+                for (int k = 0; k < 2 * KS; k++)
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(tl.k[k].x), fabsf(tl.k[k].y)), fmaxf(fabsf(tl.k[k].z), fabsf(tl.k[k].w))));
+                mx = over_wave(mx, fmax2);
+                if (mx > 3.0e38f) {  // an infinity: the unit of the others
+                    mx = 0.f;
+                    for (int k = 0; k < 2 * KS; k++) {
+                        const float v[4] = {tl.k[k].x, tl.k[k].y, tl.k[k].z, tl.k[k].w};
+                        for (int c = 0; c < 4; c++) mx = fabsf(v[c]) <= 3.0e38f ? fmaxf(mx, fabsf(v[c])) : mx;
+                    }
+                    mx = over_wave(mx, fmax2);
+                }
+                const int e = unit_exp(mx);
+                const float sg = ldexpf(1.f, e);
+                fs = ldexpf(qs, -e);
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) {
+                    const float4 x = tl.k[2 * kk], y = tl.k[2 * kk + 1];
+                    const float v[8] = {x.x * sg, x.y * sg, x.z * sg, x.w * sg, y.x * sg, y.y * sg, y.z * sg, y.w * sg};
+                    f16x8 kh, kl;
+                    split8(v, kh, kl);
+                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[128 * kk]);
+                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[128 * kk + 64]);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh, s, 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) {
+                    f16x8 kf;
+                    if constexpr (I8) {
+                        const uint4 x = tl.k[kk >> 1];
+                        kf = (kk & 1) ? widen8(x.z, x.w) : widen8(x.x, x.y);
+                    } else {
+                        kf = tl.k[kk];
+                    }
+                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[128 * kk]);
+                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[128 * kk + 64]);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh, s, 0, 0, 0);
+                }
+            }
+            float vsc[16];
+            if constexpr (I8) {
+#pragma unroll
+                for (int x = 0; x < 16; x++) s[x] *= ((const float*)&tl.ks[x >> 2])[x & 3];
+#pragma unroll
+                for (int x = 0; x < 16; x++) vsc[x] = ((const float*)&tl.vs[x >> 2])[x & 3];
+            }
+            // the next tile's ids and K
+            const int tn = t + dt;
+            const bool go = i + 1 < jend && tn < kend;
+            if (TURNS) {
+                load_v(t);
+                if (go) ids(tn);
+            } else if (go) {
+                ids(tn);
+                load_k(tn);
+            }
+
+            // ---- softmax: register x is position t + 16 (x / 8) + 8 half + x % 8
+            float mt = -INFINITY;
+            if (edge) {
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const int pos = t + 16 * (x >> 3) + 8 * half + (x & 7);
+                    s[x] = pos >= lo && pos < lim ? s[x] * fs : -INFINITY;
+                    if constexpr (I8) vsc[x] = pos < kend ? vsc[x] : 0.f;
+                    mt = fmaxf(mt, s[x]);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    s[x] *= fs;
+                    mt = fmaxf(mt, s[x]);
+                }
+            }
+            mt = over_halves(mt, fmax2);
+            const float mn = fmaxf(m, mt);
+            if (__any(mn > m)) {
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) o[d][x] *= alpha;
+                m = mn;
+            }
+            const float sub = (mn == -INFINITY ? 0.f : mn) - P_UNIT;
+            float p[16];
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                p[x] = __builtin_amdgcn_exp2f(s[x] - sub);
+                l += p[x];
+            }
+            // V's unit, as small as the largest V so far needs
+            if constexpr (F32 || I8) {
+                float mx = 0.f;
+                if constexpr (I8) {
+#pragma unroll
+                    for (int x = 0; x < 16; x++) mx = fabsf(vsc[x]) <= 3.0e38f ? fmaxf(mx, fabsf(vsc[x])) : mx;
+                    mx = over_halves(mx, fmax2);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+#pragma unroll
+                        for (int c = 0; c < DT; c++) mx = fmaxf(mx, fabsf(tl.v[k][c]));
+                    mx = over_wave(mx, fmax2);
+                    if (mx > 3.0e38f) {
+                        mx = 0.f;
+                        for (int k = 0; k < 16; k++)
+                            for (int c = 0; c < DT; c++)
+                                mx = fabsf(tl.v[k][c]) <= 3.0e38f ? fmaxf(mx, fabsf(tl.v[k][c])) : mx;
+                        mx = over_wave(mx, fmax2);
+                    }
+                }
+                const int e = __builtin_amdgcn_readfirstlane(I8 ? unit_exp(mx) - 15 : unit_exp(mx));
+                if (e < vexp) {
+                    const float f = ldexpf(1.f, max(e - vexp, -126));
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int x = 0; x < 16; x++) o[d][x] *= f;
+                    vexp = e;
+                }
+                if constexpr (I8) {
+                    const float f = ldexpf(1.f, vexp);
+#pragma unroll
+                    for (int x = 0; x < 16; x++) p[x] = !edge || s[x] > -INFINITY ? p[x] * (vsc[x] * f) : 0.f;
+                }
+            }
+            f16x8 ph[2], pl[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float v[8] = {p[8 * b], p[8 * b + 1], p[8 * b + 2], p[8 * b + 3],
+                                    p[8 * b + 4], p[8 * b + 5], p[8 * b + 6], p[8 * b + 7]};
+                split8(v, ph[b], pl[b]);
+            }
+
+            // ---- outputs
+            if constexpr (!I8) {
+                if (edge) {
+                    // V past the end: zeros, whatever the page holds there (f32: the last position's)
+                    if constexpr (F16) {
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            const int valid = kend - (t + 16 * b + 8 * half);
+#pragma unroll
+                            for (int d = 0; d < DT; d++) {
+                                uint32_t* u = (uint32_t*)&tl.v[d][b];
+#pragma unroll
+                                for (int k = 0; k < 4; k++)
+                                    u[k] &= valid >= 2 * k + 2 ? 0xFFFFFFFFu : valid == 2 * k + 1 ? 0xFFFFu : 0u;
+                            }
+                        }
+                    }
+                    // An infinity or NaN in V times a weight of 0 is NaN, in columns that do not attend to it.
+                    // Tiles that hold one: NaN to the outputs of the columns that do (a product of indicators
+                    // counts them), then zeros in its place.
+                    auto value = [&](int d, int b, int k) {
+                        if constexpr (F32) return tl.v[8 * b + k][d];
+                        else return (float)__builtin_bit_cast(f16x8, tl.v[d][b])[k];
+                    };
+                    bool bad = false;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int k = 0; k < 16; k++) bad |= !(fabsf(value(d, k >> 3, k & 7)) <= 3.4e38f);
+                    if (__any(bad)) {
+                        f16x8 att[2];
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            const int pos = t + 16 * (x >> 3) + 8 * half + (x & 7);
+                            att[x >> 3][x & 7] = pos >= lo && pos < lim ? (_Float16)1.f : (_Float16)0.f;
+                        }
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            f32x16 c;
+#pragma unroll
+                            for (int x = 0; x < 16; x++) c[x] = 0.f;
+#pragma unroll
+                            for (int b = 0; b < 2; b++) {
+                                f16x8 f;
+#pragma unroll
+                                for (int k = 0; k < 8; k++)
+                                    f[k] = fabsf(value(d, b, k)) <= 3.4e38f ? (_Float16)0.f : (_Float16)1.f;
+                                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, att[b], c, 0, 0, 0);
+#pragma unroll
+                                for (int k = 0; k < 8; k++) {
+                                    if constexpr (F32) {
+                                        tl.v[8 * b + k][d] = f[k] > (_Float16)0.f ? 0.f : tl.v[8 * b + k][d];
+                                    } else {
+                                        uint32_t* u = (uint32_t*)&tl.v[d][b];
+                                        u[k >> 1] &= f[k] > (_Float16)0.f ? (k & 1 ? 0xFFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int x = 0; x < 16; x++) o[d][x] = c[x] > 0.f ? NAN : o[d][x];
+                        }
+                    }
+                }
+            }
+            const float vg = F32 ? ldexpf(1.f, vexp) : 1.f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    if constexpr (F32) {  // dims DT * row + d
+                        float x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) x[k] = tl.v[8 * b + k][d] * vg;
+                        f16x8 vh, vl;
+                        split8(x, vh, vl);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[b], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[b], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[b], o[d], 0, 0, 0);
+                    } else {  // dims 32 d + row
+                        f16x8 vf;
+                        if constexpr (I8) vf = widen8(tl.v[d][b].x, tl.v[d][b].y);
+                        else vf = __builtin_bit_cast(f16x8, tl.v[d][b]);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b], o[d], 0, 0, 0);
+                    }
+                }
+            if (go) {
+                if (TURNS) load_k(tn);
+                else load_v(tn);
+            }
+            more = go;
+            i++;
+            t = tn;
+        }
+
+        // ---- join the waves of a column
+        __syncthreads();  // q's operands lie where the outputs go
+        l = over_halves(l, [](float x, float y) { return x + y; });
+        if (half == 0) {
+            s_m[wave][col] = m;
+            s_l[wave][col] = l;
+        }
+        const float unit = F16 ? 1.f : ldexpf(1.f, -vexp);
+        {
+            float* row = s_o + (wave * 32 + col) * OS;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                if constexpr (F32) {  // register 4 b + c of tile d: dim DT * (8 b + 4 half + c) + d
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int d = 0; d < DT; d++) row[DT * (8 * b + 4 * half + c) + d] = o[d][4 * b + c] * unit;
+                } else {  // dim 32 d + 8 b + 4 half + c
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+                        *(float4*)(row + 32 * d + 8 * b + 4 * half) = float4{
+                            o[d][4 * b] * unit, o[d][4 * b + 1] * unit, o[d][4 * b + 2] * unit, o[d][4 * b + 3] * unit};
+                }
+            }
+        }
+        __syncthreads();
+        const size_t slot0 = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + colbase + (size_t)BLK * w;
+        for (int e = tid; e < cols * (HD / 4); e += GTH) {
+            const int c = e / (HD / 4), d = e % (HD / 4) * 4;
+            const int cq = c >> 5, ci = c & 31;
+            float M = -INFINITY;
+            for (int k = 0; k < wk; k++) M = fmaxf(M, s_m[cq + wq * k][ci]);
+            const float mu = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < wk; k++) {
+                const int v = cq + wq * k;
+                const float f = __builtin_amdgcn_exp2f(s_m[v][ci] - mu);
+                const float4 x = *(const float4*)(s_o + (v * 32 + ci) * OS + d);
+                L = __builtin_fmaf(s_l[v][ci], f, L);
+                if (f > 0.f || f != f) {
+                    O.x = __builtin_fmaf(x.x, f, O.x);
+                    O.y = __builtin_fmaf(x.y, f, O.y);
+                    O.z = __builtin_fmaf(x.z, f, O.z);
+                    O.w = __builtin_fmaf(x.w, f, O.w);
+                }
+            }
+            const int cab = colbase + c, cr = cab / G, hh = cab - cr * G;
+            const int cctx = row_ctx(a, cr);
+            const bool any_pre = min(cctx, pre) > 0, any_tail = cctx > pre;
+            if (whole && (tail ? !any_pre : any_pre && !any_tail)) {
+                *(float4*)(a.out + ((size_t)cr * a.H + kvh * G + hh) * HD + d) =
+                    make_float4(O.x / L, O.y / L, O.z / L, O.w / L);
+            } else if (tail || any_pre) {
+                *(float4*)(a.part_o + (slot0 + c) * HD + d) = O;
+                if (d == 0) a.part_ml[slot0 + c] = make_float2(M, L);
+            }
+        }
+        __syncthreads();  // s_o, s_m, s_l are written again
+    }
+}
+
+// The parts of a column, joined in order: one wave per (row, query head).  A row
+// whose one part was the output itself is left; one without any is zero.
+template <int HD>
+__global__ __launch_bounds__(64) void group_merge_kernel(GroupArgs a, int gx) {
+    constexpr int DPL = HD / 64;
+    const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / a.G, hh = h - kvh * a.G;
+    const int pos = a.plan[2 + 2 * r], any_pre = a.plan[3 + 2 * r];
+    if (pos < 0) return;  // outside every group
+    const int T = a.plan[0], np = a.plan[1], shares = min(gx, T);
+    const int* pref = a.plan + 2 + 2 * a.n;
+    // (first share, parts) of the prefix and of the tail: tile x lies in share ((x + 1) shares - 1) / T
+    int first[2] = {0, 0}, count[2] = {0, 0};
+    const int jobs[2] = {(pos + hh) / BLK, np + r};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        if (k == 0 && !any_pre) continue;
+        const long long x0 = pref[jobs[k]], x1 = pref[jobs[k] + 1];
+        if (x1 <= x0) continue;
+        first[k] = (int)(((x0 + 1) * shares - 1) / T);
+        count[k] = (int)((x1 * shares - 1) / T) - first[k] + 1;
+    }
+    const int all = count[0] + count[1];
+    float* out = a.out + ((size_t)r * a.H + h) * HD;
+    if (all == 0) {
+#pragma unroll
+        for (int k = 0; k < DPL; k++) out[lane + 64 * k] = 0.f;
+        return;
+    }
+    if (all == 1) return;
+    const size_t column = (size_t)kvh * a.slots + (size_t)r * a.G + hh;
+    auto slot = [&](int i) {
+        return i < count[0] ? column + (size_t)BLK * (first[0] + i)
+                            : column + (size_t)a.n * a.G + (size_t)BLK * (first[1] + i - count[0]);
+    };
+    float M = -INFINITY;
+    for (int i = lane; i < all; i += 64) M = fmaxf(M, a.part_ml[slot(i)].x);
+    M = over_wave(M, fmax2);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O[DPL];
+#pragma unroll
+    for (int k = 0; k < DPL; k++) O[k] = 0.f;
+    for (int i0 = 0; i0 < all; i0 += 64) {
+        float wgt = 0.f, lw = 0.f;
+        if (i0 + lane < all) {
+            const float2 ml = a.part_ml[slot(i0 + lane)];
+            wgt = __builtin_amdgcn_exp2f(ml.x - mu);
+            lw = ml.y * wgt;
+        }
+        L += over_wave(lw, [](float x, float y) { return x + y; });
+        const int n = min(64, all - i0);
+        for (int u0 = 0; u0 < n; u0 += 8) {  // 8 parts' loads in flight
+            float v[8][DPL];
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+#pragma unroll
+                for (int k = 0; k < DPL; k++) v[u][k] = a.part_o[slot(i0 + min(u0 + u, n - 1)) * HD + lane + 64 * k];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float f = __shfl(wgt, u0 + u);
+                if (u0 + u < n && (f > 0.f || f != f))
+#pragma unroll
+                    for (int k = 0; k < DPL; k++) O[k] = __builtin_fmaf(v[u][k], f, O[k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < DPL; k++) out[lane + 64 * k] = O[k] / L;
+}
+
+// workgroups per KV head: as many as are resident at once, one per CU, whose
+// registers its 8 waves fill
+static int group_grid(int Hkv) { return std::max(1, 256 / Hkv); }
+
+struct GroupSizes {
+    int job_cap;
+    long long slots;
+    size_t plan_bytes, ml_bytes, o_bytes;
+};
+static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
+    const int G = H / Hkv;
+    GroupSizes z;
+    z.job_cap = (int)((long long)n * G / BLK) + groups;
+    z.slots = 2ll * n * G + (long long)BLK * group_grid(Hkv);
+    z.plan_bytes = ((size_t)(2 + 2 * n + z.job_cap + n + 1) * 4 + 255) / 256 * 256;
+    z.ml_bytes = ((size_t)Hkv * z.slots * sizeof(float2) + 255) / 256 * 256;
+    z.o_bytes = (size_t)Hkv * z.slots * hd * 4;
+    return z;
+}
+static size_t group_lds(int hd, int n, int groups, int job_cap) {
+    return (size_t)GW * 32 * (hd + 4) * 4 + (size_t)(job_cap + n + 1 + 2 * (groups + 1)) * 4;
+}
+// shapes of the tiles (their LDS bounds what few very wide layouts would need)
+static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
+    const int G = H / Hkv;
+    return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 &&
+           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd).job_cap) + 3072 <= 160 * 1024;
+}
+
+int group_attention_init() {
+#define QH_GROUP_LDS(HDv, KVv)                                                         \
+    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv>,    \
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, 157 * 1024));
+    QH_GROUP_LDS(64, DT_F32) QH_GROUP_LDS(64, DT_F16) QH_GROUP_LDS(64, DT_I8)
+    QH_GROUP_LDS(128, DT_F32) QH_GROUP_LDS(128, DT_F16) QH_GROUP_LDS(128, DT_I8)
+#undef QH_GROUP_LDS
+    return QRAF_HIP_OK;
+}
+
+// (of any page size: one that the tiles do not take needs less)
 size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd, int max_ctx) {
-    (void)n, (void)groups, (void)H, (void)Hkv, (void)hd, (void)max_ctx;
-    return 16;
+    (void)max_ctx;
+    if (H % Hkv || !group_tiles(n, groups, H, Hkv, hd, 16)) return 16;
+    const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
+    return z.plan_bytes + z.ml_bytes + z.o_bytes;
 }
 
 int launch_group_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype,
@@ -173,8 +1001,46 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
     QH_REQUIRE(ws_bytes >= group_attention_workspace_bytes(n, groups, H, Hkv, hd, max_ctx), QRAF_HIP_ERR_INVALID,
                "group attention: workspace of %zu bytes, %zu needed", ws_bytes,
                group_attention_workspace_bytes(n, groups, H, Hkv, hd, max_ctx));
-    GroupArgs a{q, kc, vc, page_table, ctx, group_starts, prefix, out, n, groups, H, Hkv, H / Hkv, page_size, max_pages,
-                max_ctx, scale};
+    GroupArgs a{};
+    a.q = q;
+    a.kc = kc;
+    a.vc = vc;
+    a.page_table = page_table;
+    a.ctx = ctx;
+    a.starts = group_starts;
+    a.prefix = prefix;
+    a.out = out;
+    a.n = n;
+    a.groups = groups;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.G = H / Hkv;
+    a.page_size = page_size;
+    a.max_pages = max_pages;
+    a.max_ctx = max_ctx;
+    a.scale = scale;
+    if (group_tiles(n, groups, H, Hkv, hd, page_size)) {
+        const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
+        a.job_cap = z.job_cap;
+        a.slots = z.slots;
+        while ((1 << a.ps_log2) < page_size) a.ps_log2++;
+        a.plan = (int*)ws;
+        a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
+        a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
+        const int gx = group_grid(Hkv);
+        const size_t lds = group_lds(hd, n, groups, z.job_cap);
+#define QH_GROUP_TILE(HDv, KVv)   \
+    if (hd == HDv && kv_dtype == KVv) \
+        hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv>), dim3(gx, Hkv), dim3(GTH), lds, st, a);
+        QH_GROUP_TILE(64, DT_F32) QH_GROUP_TILE(64, DT_F16) QH_GROUP_TILE(64, DT_I8)
+        QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)
+#undef QH_GROUP_TILE
+        QH_CHECK_HIP(hipGetLastError());
+        if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, H), dim3(64), 0, st, a, gx);
+        else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, H), dim3(64), 0, st, a, gx);
+        QH_CHECK_HIP(hipGetLastError());
+        return QRAF_HIP_OK;
+    }
     const dim3 grid(n, H);
 #define QH_GROUP_ANY(HDv, KVv)                                                                     \
     if (hd == HDv && kv_dtype == KVv) {                                                            \

@@ -6,7 +6,11 @@ operands keep at least 21 bits, so they are off by at most
     d = scale * sum_d |q_d k_d| * (2^-20 + head_dim * 2^-24),
 which moves every probability by a factor within exp(+-2 d); and the weighted sum
 and its divisor are chains of at most ctx + 64 fp32 additions:
-    |got - want| <= (2 max_t d + (ctx + 64) * 2^-24) * sum_t p_t |v_t| + 1e-30.
+    |got - want| <= (2 max_t d + (ctx + 64) * 2^-24) * sum_t p_t |v_t| + ctx * 2^-37 * max_t |v_t| + 1e-30.
+The last but one: a weight enters its product as two fp16 values, times 2^14 (the largest weight is at most 1, and
+at least one is 1).  fp16 has steps of 2^-24 at its least, so a weight is off by up to 2^-38 however small it is;
+int8 pages multiply it by the position's V scale over a power of two that may be twice the largest scale, which
+makes that 2^-37 of the largest |v| for each of ctx positions.  (f32 V is held in steps of 2^-40 of the largest.)
 """
 import numpy as np
 import pytest
@@ -164,7 +168,7 @@ def expected(c, q, H):
             p = np.exp(s - s.max())
             p /= p.sum()
             out[r, h] = p @ v
-            tol[r, h] += (2 * d.max() + (n + 64) * 2.0 ** -24) * (p @ np.abs(v))
+            tol[r, h] += (2 * d.max() + (n + 64) * 2.0 ** -24) * (p @ np.abs(v)) + n * 2.0 ** -37 * np.abs(v).max()
     return out, tol
 
 
