@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -268,11 +269,21 @@ __device__ __forceinline__ f16x8 widen8(uint32_t w0, uint32_t w1) {
     return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
 }
 
+// A barrier for what lies in LDS: loads and stores to memory stay in flight
+// (__syncthreads waits for all of them, 3 to 6 us a segment here).
+__device__ __forceinline__ void lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // ---- the plan: jobs and tiles, from the device-resident lengths, by every workgroup
 struct GroupPlan {
     int* pref;   // [jobs + 1] first tile of each job: prefix blocks, then a tail per row
     int* jb;     // [groups + 1] first prefix job of each group
     int* gs;     // [groups + 1] group starts
+    int* pre;    // [groups] prefix lengths
+    int* ctx;    // [n] context lengths
     int np;      // prefix jobs
 };
 // the last entry of ascending v[0..n) at or below x (v[0] <= x)
@@ -285,11 +296,19 @@ __device__ __forceinline__ int last_at(const int* v, int n, int x) {
     }
     return lo;
 }
+// the same by a whole wave, n <= 4096: two reads instead of one per halving
+__device__ __forceinline__ int wave_last_at(const int* v, int n, int x) {
+    const int lane = threadIdx.x & 63, step = (n + 63) >> 6;
+    int i = lane * step;
+    const int b = (__popcll(__ballot(i < n && v[min(i, n - 1)] <= x)) - 1) * step;
+    i = b + lane;
+    return b + __popcll(__ballot(lane < step && i < n && v[min(i, n - 1)] <= x)) - 1;
+}
 // v[0..n) to its exclusive prefix sums, v[n] the sum; a barrier before and behind
 __device__ void prefix_sum(int* v, int n, int* s_wave) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (n + GTH - 1) / GTH, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    __syncthreads();
+    lds_sync();
     int sum = 0;
     for (int i = i0; i < i1; i++) sum += v[i];
     int inc = sum;
@@ -299,7 +318,7 @@ __device__ void prefix_sum(int* v, int n, int* s_wave) {
         if (lane >= o) inc += x;
     }
     if (lane == 63) s_wave[wave] = inc;
-    __syncthreads();
+    lds_sync();
     int run = inc - sum, all = 0;
 #pragma unroll
     for (int w = 0; w < GW; w++) {
@@ -313,7 +332,7 @@ __device__ void prefix_sum(int* v, int n, int* s_wave) {
         run += x;
     }
     if (tid == 0) v[n] = all;
-    __syncthreads();
+    lds_sync();
 }
 // waves of a job of `cols` columns side by side along them (the others along the positions)
 __device__ __forceinline__ int waves_over(int cols) { return cols > 64 ? 4 : cols > 32 ? 2 : 1; }
@@ -327,21 +346,26 @@ __device__ __forceinline__ int tail_base(int prefix) { return prefix & ~15; }
 
 __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int* s_wave) {
     const int tid = threadIdx.x;
-    for (int g = tid; g <= a.groups; g += GTH) p.gs[g] = group_start(a, g);
-    __syncthreads();
+    for (int i = tid; i < max(a.n, a.groups + 1); i += GTH) {  // (all requested at once)
+        const int c = row_ctx(a, min(i, a.n - 1)), s = group_start(a, min(i, a.groups)), e = prefix_len(a, min(i, a.groups - 1));
+        if (i < a.n) p.ctx[i] = c;
+        if (i <= a.groups) p.gs[i] = s;
+        if (i < a.groups) p.pre[i] = e;
+    }
+    lds_sync();
     for (int g = tid; g < a.groups; g += GTH) p.jb[g] = (max(0, p.gs[g + 1] - p.gs[g]) * a.G + BLK - 1) / BLK;
     prefix_sum(p.jb, a.groups, s_wave);
     p.np = min(p.jb[a.groups], a.job_cap);
     for (int j = tid; j < p.np + a.n; j += GTH) p.pref[j] = 0;
-    __syncthreads();
+    lds_sync();
     for (int r = tid; r < a.n; r += GTH) {
         if (r < p.gs[0] || r >= p.gs[a.groups]) continue;
-        const int g = last_at(p.gs, a.groups, r), ctx = row_ctx(a, r), pre = prefix_len(a, g);
+        const int g = last_at(p.gs, a.groups, r), ctx = p.ctx[r], pre = p.pre[g];
         const int c0 = (r - p.gs[g]) * a.G, j0 = p.jb[g] + c0 / BLK, j1 = p.jb[g] + (c0 + a.G - 1) / BLK;
         for (int j = j0; j <= j1 && j < p.np; j++) atomicMax(&p.pref[j], min(ctx, pre));
         if (ctx > pre) p.pref[p.np + r] = tiles_of(ctx - tail_base(pre), a.G);
     }
-    __syncthreads();
+    lds_sync();
     for (int j = tid; j < p.np; j += GTH) {
         const int g = last_at(p.jb, a.groups, j);
         p.pref[j] = tiles_of(p.pref[j], min(BLK, (p.gs[g + 1] - p.gs[g]) * a.G - BLK * (j - p.jb[g])));
@@ -354,7 +378,7 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int* s_wave) {
             const bool in = r >= p.gs[0] && r < p.gs[a.groups];
             const int g = in ? last_at(p.gs, a.groups, r) : 0;
             a.plan[2 + 2 * r] = in ? p.jb[g] * BLK + (r - p.gs[g]) * a.G : -1;
-            a.plan[3 + 2 * r] = in && min(row_ctx(a, r), prefix_len(a, g)) > 0;
+            a.plan[3 + 2 * r] = in && min(p.ctx[r], p.pre[g]) > 0;
         }
         if (tid == 0) {
             a.plan[0] = p.pref[jobs];
@@ -388,18 +412,31 @@ template <int HD, int KV>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
-    constexpr int OS = HD + 4;  // row stride of the waves' outputs
     extern __shared__ __align__(16) float s_dyn[];
-    __shared__ float s_m[GW][32], s_l[GW][32];
+    __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK];
+    __shared__ float* s_to[BLK];
     __shared__ int s_wave[GW];
-    float* s_o = s_dyn;           // [GW][32][OS] the waves' outputs, behind a segment's tiles
+    // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
+    // c ^ (column % 16), which spreads a wave's writes over the banks
+    float* s_o = s_dyn;
     uint4* s_q = (uint4*)s_dyn;   // [4][KS][2][64] q's operands lane by lane, during them
     GroupPlan plan;
-    plan.pref = (int*)(s_dyn + GW * 32 * OS);
+    plan.pref = (int*)(s_dyn + GW * 32 * HD);
     plan.jb = plan.pref + a.job_cap + a.n + 1;
     plan.gs = plan.jb + a.groups + 1;
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    plan.pre = plan.gs + a.groups + 1;
+    plan.ctx = plan.pre + a.groups;
+    // opaque to the compiler before each use of many (here and below): else addresses made of it are formed once,
+    // ahead of the loops, and spilled across them
+    int tid = threadIdx.x;
+    int lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto lanes_again = [&] {
+        asm volatile("" : "+v"(tid));
+        lane = tid & 63;
+        col = lane & 31;
+        half = lane >> 5;
+    };
     const int kvh = blockIdx.y, w = blockIdx.x, G = a.G, psl = a.ps_log2, psm = (1 << psl) - 1;
 
     group_plan(a, plan, s_wave);
@@ -407,10 +444,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     if (w >= shares) return;
     const int t0 = (int)(((long long)w * T) / shares), t1 = (int)(((long long)(w + 1) * T) / shares);
 
-    for (int j = __builtin_amdgcn_readfirstlane(last_at(plan.pref, jobs, t0)); j < jobs; j++) {
+    for (int j = wave_last_at(plan.pref, jobs, t0); j < jobs; j++) {
         const int p0 = plan.pref[j], p1 = plan.pref[j + 1];
         if (p0 >= t1) break;
         if (p0 == p1) continue;
+        lanes_again();
         const int ja = max(t0, p0) - p0, jend = min(t1, p1) - p0;  // the segment: tiles [ja, jend) of the job
         const bool whole = ja == 0 && jend == p1 - p0;
 
@@ -419,25 +457,28 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         int g, colbase, cols, trow;
         if (tail) {
             trow = j - plan.np;
-            g = last_at(plan.gs, a.groups, trow);
+            g = wave_last_at(plan.gs, a.groups, trow);
             colbase = trow * G;
             cols = G;
         } else {
-            g = last_at(plan.jb, a.groups, j);
+            g = wave_last_at(plan.jb, a.groups, j);
             const int b = j - plan.jb[g];
             trow = plan.gs[g];
             colbase = trow * G + BLK * b;
             cols = min(BLK, (plan.gs[g + 1] - trow) * G - BLK * b);
         }
-        const int pre = prefix_len(a, g), lo = tail ? pre : 0, base = tail ? tail_base(pre) : 0;
+        const int pre = plan.pre[g], lo = tail ? pre : 0, base = tail ? tail_base(pre) : 0;
         const int wq = waves_over(cols), wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
-        const int32_t* ptab = a.page_table + (size_t)trow * a.max_pages;
+        // the page table through scalar loads: an id does not wait for vector loads ahead of it
+        typedef const __attribute__((address_space(4))) int32_t ConstInt;
+        ConstInt* ptab = (ConstInt*)(uintptr_t)(a.page_table + (size_t)__builtin_amdgcn_readfirstlane(trow) * a.max_pages);
 
         // ---- the lane's column (past the block's end: its last, not written)
         const int ab = colbase + min(qt * 32 + col, cols - 1), r = ab / G;
         const float* qrow = a.q + ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
-        const int ctx = row_ctx(a, r), lim = tail ? ctx : min(ctx, pre);
-        const int kend = __builtin_amdgcn_readfirstlane(over_wave(lim, imax2));  // behind the last that some column attends to
+        const int ctx = plan.ctx[r], lim = tail ? ctx : min(ctx, pre);
+        // behind the last position that some of the wave's columns attends to
+        const int kend = __builtin_amdgcn_readfirstlane(over_wave(lim, imax2)), klast = max(kend - 1, 0);
         const int least = __builtin_amdgcn_readfirstlane(over_wave(lim, imin2));
 
         float4 qraw[2 * KS];
@@ -452,13 +493,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         GroupTile<HD, KV> tl;
         int pg0 = 0, pg1 = 0;
         auto ids = [&](int t) {
-            pg0 = __builtin_amdgcn_readfirstlane(ptab[min(t, kend - 1) >> psl]);
-            pg1 = __builtin_amdgcn_readfirstlane(ptab[min(t + 16, kend - 1) >> psl]);
+            pg0 = ptab[min(t, klast) >> psl];
+            pg1 = ptab[min(t + 16, klast) >> psl];
         };
         const size_t blk = (size_t)a.page_size * (I8 ? HD + 4 : F16 ? 2 * HD : 4 * HD);  // bytes of a (page, KV head)
         auto block = [&](const void* pool, int pg) { return (const char*)pool + ((size_t)pg * a.Hkv + kvh) * blk; };
         auto load_k = [&](int t) {
-            const int pc = min(t + key_of(col), kend - 1);  // (past the end: the last position's, masked below)
+            const int pc = min(t + key_of(col), klast);  // (past the end: the last position's, masked below)
             const char* kp = pc >= t + 16 ? block(a.kc, pg1) : block(a.kc, pg0);
             if constexpr (F16) {
                 const uint32_t o = (uint32_t)((pc & psm) * HD + 8 * half) * 2u;
@@ -502,7 +543,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int pc = min(t + 16 * b + 8 * half + i, kend - 1);
+                        const int pc = min(t + 16 * b + 8 * half + i, klast);
                         const char* xp = pc >= t + 16 ? block(a.vc, pg1) : block(a.vc, pg0);
                         tl.v[8 * b + i] = *(const typename GroupTile<HD, (int)DT_F32>::vrow*)(
                             xp + (uint32_t)((pc & psm) * HD + DT * col) * 4u);
@@ -513,14 +554,15 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 
         // f32 rows of 128 fill the registers: V is requested behind the scores, the next K behind the outputs
         constexpr bool TURNS = F32 && HD == 128;
-        int i = ja, t = base + (i * wk + kw) * 32;  // the wave's tiles: every wk-th 32 positions
+        int i = ja, t = __builtin_amdgcn_readfirstlane(base + (i * wk + kw) * 32);  // the wave's tiles: every wk-th 32 positions
         const int dt = 32 * wk;
         bool more = i < jend && t < kend;
-        if (more) {
-            ids(t);
-            load_k(t);
-            if (!TURNS) load_v(t);
-        }
+        // No load depends on a branch, here and below: where paths with more and with fewer loads behind one meet,
+        // a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
+        ids(more ? t : 0);
+        pg0 = more ? pg0 : 0;
+        pg1 = more ? pg1 : 0;
+        load_k(more ? t : 0);
 
         // ---- q as fp16 hi + lo, scaled per column (waves of the same columns write the same)
         float qs;
@@ -546,7 +588,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             }
             qs = ldexpf(a.scale * 1.44269504088896340736f, -e);  // scores in powers of two
         }
-        __syncthreads();
+        if (!TURNS) load_v(more ? t : 0);  // (behind q: their registers)
+        lds_sync();
 
         float m = -INFINITY, l = 0.f;  // running maximum; sum of the lane's own positions, times 2^14
         int vexp = 110;                // V's unit: outputs are held times 2^vexp (f32, int8)
@@ -557,10 +600,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             for (int x = 0; x < 16; x++) o[d][x] = 0.f;
 
         while (more) {
-            // opaque to the compiler: else q's operands are read once, ahead of the loop, and spilled
-            int qat = qt * KS * 128 + lane;
-            asm volatile("" : "+v"(qat));
-            const uint4* qtile = s_q + qat;
+            lanes_again();
+            const uint4* qtile = s_q + qt * KS * 128 + lane;
             const bool edge = t < lo || t + 32 > least;  // some column does not attend to all 32
             // ---- scores
             f32x16 s;
@@ -619,16 +660,12 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
                 for (int x = 0; x < 16; x++) vsc[x] = ((const float*)&tl.vs[x >> 2])[x & 3];
             }
-            // the next tile's ids and K
-            const int tn = t + dt;
-            const bool go = i + 1 < jend && tn < kend;
-            if (TURNS) {
-                load_v(t);
-                if (go) ids(tn);
-            } else if (go) {
-                ids(tn);
-                load_k(tn);
-            }
+            // the next tile's ids and K (behind the last tile: its own again)
+            const bool go = i + 1 < jend && t + dt < kend;
+            const int tn = go ? t + dt : t;
+            if (TURNS) load_v(t);
+            ids(tn);
+            if (!TURNS) load_k(tn);
 
             // ---- softmax: register x is position t + 16 (x / 8) + 8 half + x % 8
             float mt = -INFINITY;
@@ -729,15 +766,21 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     // An infinity or NaN in V times a weight of 0 is NaN, in columns that do not attend to it.
                     // Tiles that hold one: NaN to the outputs of the columns that do (a product of indicators
                     // counts them), then zeros in its place.
-                    auto value = [&](int d, int b, int k) {
-                        if constexpr (F32) return tl.v[8 * b + k][d];
-                        else return (float)__builtin_bit_cast(f16x8, tl.v[d][b])[k];
-                    };
+                    // the fp16 halves of a dword that are not numbers, as 0x1 in each (their exponent is all ones)
+                    auto odd16 = [](uint32_t u) { return (((u & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u; };
                     bool bad = false;
 #pragma unroll
-                    for (int d = 0; d < DT; d++)
+                    for (int d = 0; d < DT; d++) {
+                        if constexpr (F32) {
 #pragma unroll
-                        for (int k = 0; k < 16; k++) bad |= !(fabsf(value(d, k >> 3, k & 7)) <= 3.4e38f);
+                            for (int k = 0; k < 16; k++) bad |= !(fabsf(tl.v[k][d]) <= 3.4e38f);
+                        } else {
+                            uint32_t any = 0;
+#pragma unroll
+                            for (int k = 0; k < 8; k++) any |= odd16(((const uint32_t*)&tl.v[d][k >> 2])[k & 3]);
+                            bad |= any != 0;
+                        }
+                    }
                     if (__any(bad)) {
                         f16x8 att[2];
 #pragma unroll
@@ -752,20 +795,27 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                             for (int x = 0; x < 16; x++) c[x] = 0.f;
 #pragma unroll
                             for (int b = 0; b < 2; b++) {
-                                f16x8 f;
+                                uint4 f;  // fp16 ones where V is no number
+                                uint32_t* fu = (uint32_t*)&f;
+                                if constexpr (F32) {
 #pragma unroll
-                                for (int k = 0; k < 8; k++)
-                                    f[k] = fabsf(value(d, b, k)) <= 3.4e38f ? (_Float16)0.f : (_Float16)1.f;
-                                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, att[b], c, 0, 0, 0);
+                                    for (int k = 0; k < 8; k++) {
+                                        const float v = tl.v[8 * b + k][d];
+                                        const bool good = fabsf(v) <= 3.4e38f;
+                                        const uint32_t one = good ? 0u : k & 1 ? 0x3C000000u : 0x3C00u;
+                                        fu[k >> 1] = k & 1 ? fu[k >> 1] | one : one;
+                                        tl.v[8 * b + k][d] = good ? v : 0.f;
+                                    }
+                                } else {
+                                    uint32_t* u = (uint32_t*)&tl.v[d][b];
 #pragma unroll
-                                for (int k = 0; k < 8; k++) {
-                                    if constexpr (F32) {
-                                        tl.v[8 * b + k][d] = f[k] > (_Float16)0.f ? 0.f : tl.v[8 * b + k][d];
-                                    } else {
-                                        uint32_t* u = (uint32_t*)&tl.v[d][b];
-                                        u[k >> 1] &= f[k] > (_Float16)0.f ? (k & 1 ? 0xFFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
+                                    for (int k = 0; k < 4; k++) {
+                                        const uint32_t w = odd16(u[k]);
+                                        fu[k] = w * 0x3C00u;
+                                        u[k] &= ~(w * 0xFFFFu);
                                     }
                                 }
+                                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), att[b], c, 0, 0, 0);
                             }
 #pragma unroll
                             for (int x = 0; x < 16; x++) o[d][x] = c[x] > 0.f ? NAN : o[d][x];
@@ -795,83 +845,111 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b], o[d], 0, 0, 0);
                     }
                 }
-            if (go) {
-                if (TURNS) load_k(tn);
-                else load_v(tn);
-            }
+            if (TURNS) load_k(tn);
+            else load_v(tn);
             more = go;
             i++;
             t = tn;
         }
 
         // ---- join the waves of a column
-        __syncthreads();  // q's operands lie where the outputs go
+        lanes_again();
+        lds_sync();  // q's operands lie where the outputs go
         l = over_halves(l, [](float x, float y) { return x + y; });
         if (half == 0) {
             s_m[wave][col] = m;
             s_l[wave][col] = l;
         }
         const float unit = F16 ? 1.f : ldexpf(1.f, -vexp);
-        {
-            float* row = s_o + (wave * 32 + col) * OS;
+        if (qt * 32 + col < cols) {
+            float4* row = (float4*)(s_o + (wave * 32 + col) * HD);
+            const int x = col & 15;
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 if constexpr (F32) {  // register 4 b + c of tile d: dim DT * (8 b + 4 half + c) + d
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int c = 0; c < 4; c += 4 / DT) {
+                        float v[4];
 #pragma unroll
-                        for (int d = 0; d < DT; d++) row[DT * (8 * b + 4 * half + c) + d] = o[d][4 * b + c] * unit;
+                        for (int k = 0; k < 4; k++) v[k] = o[k % DT][4 * b + c + k / DT] * unit;
+                        row[(DT * (8 * b + 4 * half + c) >> 2) ^ x] = make_float4(v[0], v[1], v[2], v[3]);
+                    }
                 } else {  // dim 32 d + 8 b + 4 half + c
 #pragma unroll
                     for (int d = 0; d < DT; d++)
-                        *(float4*)(row + 32 * d + 8 * b + 4 * half) = float4{
-                            o[d][4 * b] * unit, o[d][4 * b + 1] * unit, o[d][4 * b + 2] * unit, o[d][4 * b + 3] * unit};
+                        row[(8 * d + 2 * b + half) ^ x] = make_float4(o[d][4 * b] * unit, o[d][4 * b + 1] * unit,
+                                                                      o[d][4 * b + 2] * unit, o[d][4 * b + 3] * unit);
                 }
             }
         }
-        __syncthreads();
-        const size_t slot0 = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + colbase + (size_t)BLK * w;
-        for (int e = tid; e < cols * (HD / 4); e += GTH) {
-            const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-            const int cq = c >> 5, ci = c & 31;
-            float M = -INFINITY;
-            for (int k = 0; k < wk; k++) M = fmaxf(M, s_m[cq + wq * k][ci]);
+        lds_sync();
+        // per column: the waves' factors, and where the joined output goes
+        if (kw == 0 && half == 0 && qt * 32 + col < cols) {
+            float mv[GW], lv[GW], M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int k = 0; k < GW; k++) {
+                const int v = min(qt + wq * k, GW - 1);
+                mv[k] = k < wk ? s_m[v][col] : -INFINITY;
+                lv[k] = k < wk ? s_l[v][col] : 0.f;
+                M = fmaxf(M, mv[k]);
+            }
             const float mu = M == -INFINITY ? 0.f : M;
-            float L = 0.f;
-            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < wk; k++) {
-                const int v = cq + wq * k;
-                const float f = __builtin_amdgcn_exp2f(s_m[v][ci] - mu);
-                const float4 x = *(const float4*)(s_o + (v * 32 + ci) * OS + d);
-                L = __builtin_fmaf(s_l[v][ci], f, L);
-                if (f > 0.f || f != f) {
-                    O.x = __builtin_fmaf(x.x, f, O.x);
-                    O.y = __builtin_fmaf(x.y, f, O.y);
-                    O.z = __builtin_fmaf(x.z, f, O.z);
-                    O.w = __builtin_fmaf(x.w, f, O.w);
-                }
+#pragma unroll
+            for (int k = 0; k < GW; k++) {
+                const float f = __builtin_amdgcn_exp2f(mv[k] - mu);
+                L = __builtin_fmaf(lv[k], f, L);
+                if (k < wk) s_m[qt + wq * k][col] = f;
             }
-            const int cab = colbase + c, cr = cab / G, hh = cab - cr * G;
-            const int cctx = row_ctx(a, cr);
-            const bool any_pre = min(cctx, pre) > 0, any_tail = cctx > pre;
-            if (whole && (tail ? !any_pre : any_pre && !any_tail)) {
-                *(float4*)(a.out + ((size_t)cr * a.H + kvh * G + hh) * HD + d) =
-                    make_float4(O.x / L, O.y / L, O.z / L, O.w / L);
-            } else if (tail || any_pre) {
-                *(float4*)(a.part_o + (slot0 + c) * HD + d) = O;
-                if (d == 0) a.part_ml[slot0 + c] = make_float2(M, L);
-            }
+            const bool any_pre = min(ctx, pre) > 0, any_tail = ctx > pre;
+            const bool alone = whole && (tail ? !any_pre : any_pre && !any_tail);
+            const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab + (size_t)BLK * w;
+            const bool part = !alone && (tail || any_pre);
+            s_to[qt * 32 + col] = alone ? a.out + (qrow - a.q) : part ? a.part_o + slot * HD : nullptr;
+            s_by[qt * 32 + col] = alone ? 1.f / L : 1.f;
+            if (part) a.part_ml[slot] = make_float2(M, L);
         }
-        __syncthreads();  // s_o, s_m, s_l are written again
+        lanes_again();
+        lds_sync();
+        auto join = [&](auto wk_c) {
+            constexpr int WK = decltype(wk_c)::value, WQ = GW / WK;
+#pragma unroll 2
+            for (int e = tid; e < cols * (HD / 4); e += GTH) {
+                const int c = e / (HD / 4), d = e % (HD / 4) * 4, cq = c >> 5, ci = c & 31;
+                float4 x[WK];
+                float f[WK];
+#pragma unroll
+                for (int k = 0; k < WK; k++) {
+                    x[k] = *(const float4*)(s_o + ((cq + WQ * k) * 32 + ci) * HD + (d ^ 4 * (ci & 15)));
+                    f[k] = s_m[cq + WQ * k][ci];
+                }
+                float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < WK; k++) {  // (a wave without positions holds zeros)
+                    O.x = __builtin_fmaf(x[k].x, f[k], O.x);
+                    O.y = __builtin_fmaf(x[k].y, f[k], O.y);
+                    O.z = __builtin_fmaf(x[k].z, f[k], O.z);
+                    O.w = __builtin_fmaf(x[k].w, f[k], O.w);
+                }
+                float* to = s_to[c];
+                const float by = s_by[c];
+                if (to) *(float4*)(to + d) = make_float4(O.x * by, O.y * by, O.z * by, O.w * by);
+            }
+        };
+        if (wk == 2) join(std::integral_constant<int, 2>());
+        else if (wk == 4) join(std::integral_constant<int, 4>());
+        else join(std::integral_constant<int, 8>());
+        lds_sync();  // s_o, s_m, s_l are written again
     }
 }
 
 // The parts of a column, joined in order: one wave per (row, query head).  A row
 // whose one part was the output itself is left; one without any is zero.
 template <int HD>
-__global__ __launch_bounds__(64) void group_merge_kernel(GroupArgs a, int gx) {
+__global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a, int gx) {
     constexpr int DPL = HD / 64;
-    const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / a.G, hh = h - kvh * a.G;
+    const int r = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (h >= a.H) return;
+    const int lane = threadIdx.x & 63, kvh = h / a.G, hh = h - kvh * a.G;
     const int pos = a.plan[2 + 2 * r], any_pre = a.plan[3 + 2 * r];
     if (pos < 0) return;  // outside every group
     const int T = a.plan[0], np = a.plan[1], shares = min(gx, T);
@@ -955,19 +1033,19 @@ static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
     return z;
 }
 static size_t group_lds(int hd, int n, int groups, int job_cap) {
-    return (size_t)GW * 32 * (hd + 4) * 4 + (size_t)(job_cap + n + 1 + 2 * (groups + 1)) * 4;
+    return (size_t)GW * 32 * hd * 4 + (size_t)(job_cap + 2 * n + 3 * (groups + 1)) * 4;
 }
 // shapes of the tiles (their LDS bounds what few very wide layouts would need)
 static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
     const int G = H / Hkv;
     return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 &&
-           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd).job_cap) + 3072 <= 160 * 1024;
+           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd).job_cap) + 5120 <= 160 * 1024;
 }
 
 int group_attention_init() {
 #define QH_GROUP_LDS(HDv, KVv)                                                         \
     QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv>,    \
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, 157 * 1024));
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024));
     QH_GROUP_LDS(64, DT_F32) QH_GROUP_LDS(64, DT_F16) QH_GROUP_LDS(64, DT_I8)
     QH_GROUP_LDS(128, DT_F32) QH_GROUP_LDS(128, DT_F16) QH_GROUP_LDS(128, DT_I8)
 #undef QH_GROUP_LDS
@@ -1036,8 +1114,8 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
         QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)
 #undef QH_GROUP_TILE
         QH_CHECK_HIP(hipGetLastError());
-        if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, H), dim3(64), 0, st, a, gx);
-        else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, H), dim3(64), 0, st, a, gx);
+        if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a, gx);
+        else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a, gx);
         QH_CHECK_HIP(hipGetLastError());
         return QRAF_HIP_OK;
     }
