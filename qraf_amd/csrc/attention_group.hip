@@ -304,35 +304,25 @@ __device__ __forceinline__ int wave_last_at(const int* v, int n, int x) {
     i = b + lane;
     return b + __popcll(__ballot(lane < step && i < n && v[min(i, n - 1)] <= x)) - 1;
 }
-// v[0..n) to its exclusive prefix sums, v[n] the sum; a barrier before and behind
-__device__ void prefix_sum(int* v, int n, int* s_wave) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (n + GTH - 1) / GTH, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    lds_sync();
+// v[0..n) to its exclusive prefix sums, v[n] the sum, by one wave
+__device__ __forceinline__ void wave_prefix_sum(int* v, int n) {
+    const int lane = threadIdx.x & 63, per = (n + 63) >> 6, i0 = min(n, lane * per), i1 = min(n, i0 + per);
     int sum = 0;
     for (int i = i0; i < i1; i++) sum += v[i];
-    int inc = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(inc, o);
-        if (lane >= o) inc += x;
-    }
-    if (lane == 63) s_wave[wave] = inc;
-    lds_sync();
-    int run = inc - sum, all = 0;
-#pragma unroll
-    for (int w = 0; w < GW; w++) {
-        const int x = s_wave[w];
-        run += w < wave ? x : 0;
-        all += x;
-    }
+    int inc = sum;  // over the lanes: rows of 16, then rows 1 and 3, then 2 and 3
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xF, 0xF, false);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xF, 0xF, false);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xF, 0xF, false);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xF, 0xF, false);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xA, 0xF, false);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xC, 0xF, false);
+    int run = inc - sum;
     for (int i = i0; i < i1; i++) {
         const int x = v[i];
         v[i] = run;
         run += x;
     }
-    if (tid == 0) v[n] = all;
-    lds_sync();
+    if (lane == 63) v[n] = inc;
 }
 // waves of a job of `cols` columns side by side along them (the others along the positions)
 __device__ __forceinline__ int waves_over(int cols) { return cols > 64 ? 4 : cols > 32 ? 2 : 1; }
@@ -344,33 +334,34 @@ __device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return ma
 // a tail begins with the 16 positions that hold the prefix's end, one page's
 __device__ __forceinline__ int tail_base(int prefix) { return prefix & ~15; }
 
-__device__ void group_plan(const GroupArgs& a, GroupPlan& p, int* s_wave) {
+__device__ void group_plan(const GroupArgs& a, GroupPlan& p) {
     const int tid = threadIdx.x;
     for (int i = tid; i < max(a.n, a.groups + 1); i += GTH) {  // (all requested at once)
-        const int c = row_ctx(a, min(i, a.n - 1)), s = group_start(a, min(i, a.groups)), e = prefix_len(a, min(i, a.groups - 1));
+        const int c = row_ctx(a, min(i, a.n - 1)), s = group_start(a, min(i, a.groups)),
+                  t = group_start(a, min(i + 1, a.groups)), e = prefix_len(a, min(i, a.groups - 1));
         if (i < a.n) p.ctx[i] = c;
         if (i <= a.groups) p.gs[i] = s;
-        if (i < a.groups) p.pre[i] = e;
+        if (i < a.groups) {
+            p.pre[i] = e;
+            p.jb[i] = (max(0, t - s) * a.G + BLK - 1) / BLK;
+        }
     }
+    for (int j = tid; j < a.job_cap + a.n; j += GTH) p.pref[j] = 0;
     lds_sync();
-    for (int g = tid; g < a.groups; g += GTH) p.jb[g] = (max(0, p.gs[g + 1] - p.gs[g]) * a.G + BLK - 1) / BLK;
-    prefix_sum(p.jb, a.groups, s_wave);
+    if (tid < 64) wave_prefix_sum(p.jb, a.groups);
+    lds_sync();
     p.np = min(p.jb[a.groups], a.job_cap);
-    for (int j = tid; j < p.np + a.n; j += GTH) p.pref[j] = 0;
-    lds_sync();
     for (int r = tid; r < a.n; r += GTH) {
         if (r < p.gs[0] || r >= p.gs[a.groups]) continue;
-        const int g = last_at(p.gs, a.groups, r), ctx = p.ctx[r], pre = p.pre[g];
-        const int c0 = (r - p.gs[g]) * a.G, j0 = p.jb[g] + c0 / BLK, j1 = p.jb[g] + (c0 + a.G - 1) / BLK;
-        for (int j = j0; j <= j1 && j < p.np; j++) atomicMax(&p.pref[j], min(ctx, pre));
+        const int g = last_at(p.gs, a.groups, r), ctx = p.ctx[r], pre = p.pre[g], all = (p.gs[g + 1] - p.gs[g]) * a.G;
+        const int c0 = (r - p.gs[g]) * a.G, b1 = (c0 + a.G - 1) / BLK;
+        for (int b = c0 / BLK; b <= b1 && p.jb[g] + b < p.np; b++)
+            atomicMax(&p.pref[p.jb[g] + b], tiles_of(min(ctx, pre), min(BLK, all - BLK * b)));
         if (ctx > pre) p.pref[p.np + r] = tiles_of(ctx - tail_base(pre), a.G);
     }
     lds_sync();
-    for (int j = tid; j < p.np; j += GTH) {
-        const int g = last_at(p.jb, a.groups, j);
-        p.pref[j] = tiles_of(p.pref[j], min(BLK, (p.gs[g + 1] - p.gs[g]) * a.G - BLK * (j - p.jb[g])));
-    }
-    prefix_sum(p.pref, p.np + a.n, s_wave);
+    if (tid < 64) wave_prefix_sum(p.pref, p.np + a.n);
+    lds_sync();
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         const int jobs = p.np + a.n;
         for (int j = tid; j <= jobs; j += GTH) a.plan[2 + 2 * a.n + j] = p.pref[j];
@@ -413,9 +404,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
     extern __shared__ __align__(16) float s_dyn[];
-    __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK];
+    __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK], s_qs[BLK];
     __shared__ float* s_to[BLK];
-    __shared__ int s_wave[GW];
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
     // c ^ (column % 16), which spreads a wave's writes over the banks
     float* s_o = s_dyn;
@@ -439,7 +429,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     };
     const int kvh = blockIdx.y, w = blockIdx.x, G = a.G, psl = a.ps_log2, psm = (1 << psl) - 1;
 
-    group_plan(a, plan, s_wave);
+    group_plan(a, plan);
     const int jobs = plan.np + a.n, T = plan.pref[jobs], shares = min((int)gridDim.x, T);
     if (w >= shares) return;
     const int t0 = (int)(((long long)w * T) / shares), t1 = (int)(((long long)(w + 1) * T) / shares);
@@ -480,14 +470,6 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         // behind the last position that some of the wave's columns attends to
         const int kend = __builtin_amdgcn_readfirstlane(over_wave(lim, imax2)), klast = max(kend - 1, 0);
         const int least = __builtin_amdgcn_readfirstlane(over_wave(lim, imin2));
-
-        float4 qraw[2 * KS];
-#pragma unroll
-        for (int kk = 0; kk < KS; kk++) {
-            const int d = I8 ? 32 * (kk >> 1) + 16 * half + 8 * (kk & 1) : 16 * kk + 8 * half;
-            qraw[2 * kk] = *(const float4*)(qrow + d);
-            qraw[2 * kk + 1] = *(const float4*)(qrow + d + 4);
-        }
 
         // ---- loads of the tile at position t
         GroupTile<HD, KV> tl;
@@ -557,17 +539,23 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         int i = ja, t = __builtin_amdgcn_readfirstlane(base + (i * wk + kw) * 32);  // the wave's tiles: every wk-th 32 positions
         const int dt = 32 * wk;
         bool more = i < jend && t < kend;
-        // No load depends on a branch, here and below: where paths with more and with fewer loads behind one meet,
-        // a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
         ids(more ? t : 0);
+        // No load of K and V depends on a branch, here and below: where paths with more and with fewer loads behind
+        // one meet, a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
         pg0 = more ? pg0 : 0;
         pg1 = more ? pg1 : 0;
         load_k(more ? t : 0);
 
-        // ---- q as fp16 hi + lo, scaled per column (waves of the same columns write the same)
-        float qs;
-        uint4* qop = s_q + qt * KS * 128 + lane;
-        {
+        // ---- q of 32 columns as fp16 hi + lo, scaled per column, by one wave for all that share them
+        if (kw == 0) {
+            float4 qraw[2 * KS];
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++) {
+                const int d = I8 ? 32 * (kk >> 1) + 16 * half + 8 * (kk & 1) : 16 * kk + 8 * half;
+                qraw[2 * kk] = *(const float4*)(qrow + d);
+                qraw[2 * kk + 1] = *(const float4*)(qrow + d + 4);
+            }
+            uint4* qop = s_q + qt * KS * 128 + lane;
             float mx = 0.f;
 #pragma unroll
             for (int k = 0; k < 2 * KS; k++)
@@ -575,21 +563,20 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             mx = over_halves(mx, fmax2);
             const int e = mx <= 3.0e38f ? unit_exp(mx) : 0;
             const float sg = ldexpf(1.f, e);
-            if (kw == 0) {
 #pragma unroll
-                for (int kk = 0; kk < KS; kk++) {
-                    const float4 x = qraw[2 * kk], y = qraw[2 * kk + 1];
-                    const float v[8] = {x.x * sg, x.y * sg, x.z * sg, x.w * sg, y.x * sg, y.y * sg, y.z * sg, y.w * sg};
-                    f16x8 hi, lw;
-                    split8(v, hi, lw);
-                    qop[128 * kk] = __builtin_bit_cast(uint4, hi);
-                    qop[128 * kk + 64] = __builtin_bit_cast(uint4, lw);
-                }
+            for (int kk = 0; kk < KS; kk++) {
+                const float4 x = qraw[2 * kk], y = qraw[2 * kk + 1];
+                const float v[8] = {x.x * sg, x.y * sg, x.z * sg, x.w * sg, y.x * sg, y.y * sg, y.z * sg, y.w * sg};
+                f16x8 hi, lw;
+                split8(v, hi, lw);
+                qop[128 * kk] = __builtin_bit_cast(uint4, hi);
+                qop[128 * kk + 64] = __builtin_bit_cast(uint4, lw);
             }
-            qs = ldexpf(a.scale * 1.44269504088896340736f, -e);  // scores in powers of two
+            if (half == 0) s_qs[qt * 32 + col] = ldexpf(a.scale * 1.44269504088896340736f, -e);
         }
         if (!TURNS) load_v(more ? t : 0);  // (behind q: their registers)
         lds_sync();
+        const float qs = s_qs[qt * 32 + col];  // scores in powers of two
 
         float m = -INFINITY, l = 0.f;  // running maximum; sum of the lane's own positions, times 2^14
         int vexp = 110;                // V's unit: outputs are held times 2^vexp (f32, int8)
@@ -978,39 +965,37 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a, int gx) {
         return i < count[0] ? column + (size_t)BLK * (first[0] + i)
                             : column + (size_t)a.n * a.G + (size_t)BLK * (first[1] + i - count[0]);
     };
-    float M = -INFINITY;
-    for (int i = lane; i < all; i += 64) M = fmaxf(M, a.part_ml[slot(i)].x);
-    M = over_wave(M, fmax2);
-    const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O[DPL];
+    float m = -INFINITY, l = 0.f, O[DPL];  // running, as in the tiles
 #pragma unroll
     for (int k = 0; k < DPL; k++) O[k] = 0.f;
-    for (int i0 = 0; i0 < all; i0 += 64) {
-        float wgt = 0.f, lw = 0.f;
-        if (i0 + lane < all) {
-            const float2 ml = a.part_ml[slot(i0 + lane)];
-            wgt = __builtin_amdgcn_exp2f(ml.x - mu);
-            lw = ml.y * wgt;
+    for (int i0 = 0; i0 < all; i0 += 8) {  // 8 parts in flight
+        float v[8][DPL];
+        float2 ml[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const size_t at = slot(min(i0 + u, all - 1));
+            ml[u] = a.part_ml[at];
+#pragma unroll
+            for (int k = 0; k < DPL; k++) v[u][k] = a.part_o[at * HD + lane + 64 * k];
         }
-        L += over_wave(lw, [](float x, float y) { return x + y; });
-        const int n = min(64, all - i0);
-        for (int u0 = 0; u0 < n; u0 += 8) {  // 8 parts' loads in flight
-            float v[8][DPL];
+        float mn = m;
 #pragma unroll
-            for (int u = 0; u < 8; u++)
+        for (int u = 0; u < 8; u++) mn = i0 + u < all ? fmaxf(mn, ml[u].x) : mn;
+        const float mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
+        l *= alpha;
 #pragma unroll
-                for (int k = 0; k < DPL; k++) v[u][k] = a.part_o[slot(i0 + min(u0 + u, n - 1)) * HD + lane + 64 * k];
+        for (int k = 0; k < DPL; k++) O[k] *= alpha;
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float f = __shfl(wgt, u0 + u);
-                if (u0 + u < n && (f > 0.f || f != f))
+        for (int u = 0; u < 8; u++) {
+            const float f = i0 + u < all ? __builtin_amdgcn_exp2f(ml[u].x - mu) : 0.f;
+            l = __builtin_fmaf(ml[u].y, f, l);
 #pragma unroll
-                    for (int k = 0; k < DPL; k++) O[k] = __builtin_fmaf(v[u][k], f, O[k]);
-            }
+            for (int k = 0; k < DPL; k++) O[k] = i0 + u < all ? __builtin_fmaf(v[u][k], f, O[k]) : O[k];
         }
+        m = mn;
     }
 #pragma unroll
-    for (int k = 0; k < DPL; k++) out[lane + 64 * k] = O[k] / L;
+    for (int k = 0; k < DPL; k++) out[lane + 64 * k] = O[k] / l;
 }
 
 // workgroups per KV head: as many as are resident at once, one per CU, whose
