@@ -182,9 +182,9 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
 // the second: nothing moves between lanes.  32 columns and not 16: half the
 // operand reads per product, and the reads are what bounds it.
 //
-// q, p and f32 K and V enter as fp16 hi + lo pairs (22 bits; q scaled per column,
-// f32 K per tile and V per wave by powers of two, p by 2^14, so that neither
-// half leaves fp16's range: what is smaller than 2^-39 of the largest may be lost),
+// q, p and f32 K and V enter as fp16 hi + lo pairs (23 bits; q scaled per column,
+// f32 K per tile and V per wave by powers of two, p by 2^13 to 2^15, so that neither
+// half leaves fp16's range: what is smaller than 2^-38 of the largest may be lost),
 // fp16 K and V as they are, int8 widened; a product of two pairs is three
 // matrix products (lo x lo is below 2^-22).  int8 scales: K's on the scores, V's
 // on p.  Sums in fp32.
@@ -199,7 +199,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int GW = 8, GTH = 64 * GW;  // waves and threads of a workgroup
 constexpr int BLK = 128;              // columns of a block: 4 waves of 32
-constexpr float P_UNIT = 14.f;        // p is held times 2^14
+// p is held times 2^13 of the running maximum it was taken against, which follows the largest score only
+// when that has grown by more than 2^2: outputs and sums are rescaled then, a few times a job and not at
+// every tile (some of 32 columns finds a larger score nearly always)
+constexpr float P_UNIT = 13.f, GROWTH = 2.f;
 
 template <int CTRL>
 __device__ __forceinline__ int gdpp(int x) {
@@ -241,10 +244,13 @@ __device__ __forceinline__ int unit_exp(float mx) {
     frexpf(mx, &e);
     return max(-110, min(15 - e, 110));
 }
-// two values as fp16 hi + lo
+// two values as fp16 hi + lo, each to the nearest: 23 bits
 __device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
-    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
-    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x - (float)hi[0], y - (float)hi[1]));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    hi = __builtin_convertvector((f32x2{x, y}), f16x2);
+    // (x - hi as a multiply-add: one instruction with the conversion inside)
+    lo = __builtin_convertvector(
+        (f32x2{__builtin_fmaf((float)hi[0], -1.f, x), __builtin_fmaf((float)hi[1], -1.f, y)}), f16x2);
 }
 __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
 #pragma unroll
@@ -562,7 +568,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(qraw[k].x), fabsf(qraw[k].y)), fmaxf(fabsf(qraw[k].z), fabsf(qraw[k].w))));
             mx = over_halves(mx, fmax2);
             const int e = mx <= 3.0e38f ? unit_exp(mx) : 0;
-            const float sg = ldexpf(1.f, e);
+            const float sg = copysignf(ldexpf(1.f, e), a.scale);  // (scores take the scale's magnitude)
 #pragma unroll
             for (int kk = 0; kk < KS; kk++) {
                 const float4 x = qraw[2 * kk], y = qraw[2 * kk + 1];
@@ -572,13 +578,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 qop[128 * kk] = __builtin_bit_cast(uint4, hi);
                 qop[128 * kk + 64] = __builtin_bit_cast(uint4, lw);
             }
-            if (half == 0) s_qs[qt * 32 + col] = ldexpf(a.scale * 1.44269504088896340736f, -e);
+            if (half == 0) s_qs[qt * 32 + col] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e);
         }
         if (!TURNS) load_v(more ? t : 0);  // (behind q: their registers)
         lds_sync();
         const float qs = s_qs[qt * 32 + col];  // scores in powers of two
 
-        float m = -INFINITY, l = 0.f;  // running maximum; sum of the lane's own positions, times 2^14
+        float m = -INFINITY, l = 0.f;  // running maximum; sum of the lane's own positions, times 2^13
         int vexp = 110;                // V's unit: outputs are held times 2^vexp (f32, int8)
         f32x16 o[DT];
 #pragma unroll
@@ -660,21 +666,16 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
                     const int pos = t + 16 * (x >> 3) + 8 * half + (x & 7);
-                    s[x] = pos >= lo && pos < lim ? s[x] * fs : -INFINITY;
+                    s[x] = pos >= lo && pos < lim ? s[x] : -INFINITY;
                     if constexpr (I8) vsc[x] = pos < kend ? vsc[x] : 0.f;
-                    mt = fmaxf(mt, s[x]);
-                }
-            } else {
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    s[x] *= fs;
-                    mt = fmaxf(mt, s[x]);
                 }
             }
+#pragma unroll
+            for (int x = 0; x < 16; x++) mt = fmaxf(mt, s[x]);
             mt = over_halves(mt, fmax2);
-            const float mn = fmaxf(m, mt);
-            if (__any(mn > m)) {
-                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            mt = mt == -INFINITY ? mt : mt * fs;
+            if (__any(mt > m + GROWTH)) {
+                const float mn = fmaxf(m, mt), alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
@@ -682,11 +683,12 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     for (int x = 0; x < 16; x++) o[d][x] *= alpha;
                 m = mn;
             }
-            const float sub = (mn == -INFINITY ? 0.f : mn) - P_UNIT;
+            const float sub = P_UNIT - (m == -INFINITY ? 0.f : m);
             float p[16];
 #pragma unroll
             for (int x = 0; x < 16; x++) {
-                p[x] = __builtin_amdgcn_exp2f(s[x] - sub);
+                p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], fs, sub));
+                if (edge) p[x] = s[x] == -INFINITY ? 0.f : p[x];  // (a factor of 0 times it)
                 l += p[x];
             }
             // V's unit, as small as the largest V so far needs
