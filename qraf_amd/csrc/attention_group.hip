@@ -6,15 +6,16 @@
 //
 // The work of one KV head is a list of jobs: per group its query vectors (rows x
 // the G query heads of the KV head, "columns") in blocks of up to 128 over the
-// positions below the prefix that some row of the block attends to, and per row
-// its G columns over its own positions behind the prefix.  A job is cut into
-// tiles of 32 positions per wave, and the tiles of all jobs, in order, into
-// equal shares for the workgroups (group_tile_kernel), all from the
-// device-resident lengths: a long prefix of few columns spreads over the chip,
-// and ragged lengths balance.  A share that holds all there is of a column
-// writes the output; the others write (max, sum, unnormalised output) parts,
-// which group_merge_kernel joins in position order.  group_any_kernel takes the
-// shapes that the tiles do not.
+// positions below the prefix that some row of the block attends to, and the rows,
+// four to a job, over their own positions behind the prefix.  Long jobs are cut
+// along the positions into pieces of equal length, as many as there are
+// workgroups at once (group_tile_kernel), all from the device-resident lengths:
+// a long prefix of few columns spreads over the chip, ragged lengths balance, and
+// a workgroup has one piece, or as few as may be (what a piece costs beside its
+// tiles, q to stage and outputs to join, is what 5 of them take).  A piece that
+// holds all there is of a column writes the output; the others write (max, sum,
+// unnormalised output) parts, which group_merge_kernel joins in position order.
+// group_any_kernel takes the shapes that the tiles do not.
 #include <math.h>
 
 #include <algorithm>
@@ -35,10 +36,11 @@ struct GroupArgs {
     float* out;                 // [n][H][HD]
     float* part_o;              // [Hkv][slots][HD] unnormalised outputs of parts
     float2* part_ml;            // [Hkv][slots] their maxima (in powers of two) and sums
-    int* plan;                  // for the merge: tiles, prefix jobs, {column, any of the prefix} of each row, tile prefix
+    int* plan;                  // for the merge: prefix jobs, {column, which parts} of each row, pieces of the jobs
     int n, groups, H, Hkv, G, page_size, max_pages, max_ctx;
     float scale;
     int ps_log2, job_cap;       // page_size = 1 << ps_log2; prefix jobs at most
+    int tail_rows, tails;       // rows of a tail job; tail jobs
     long long slots;            // part slots of a KV head
 };
 
@@ -283,9 +285,10 @@ __device__ __forceinline__ void lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// ---- the plan: jobs and tiles, from the device-resident lengths, by every workgroup
+// ---- the plan: jobs and their pieces, from the device-resident lengths, by every workgroup
 struct GroupPlan {
-    int* pref;   // [jobs + 1] first tile of each job: prefix blocks, then a tail per row
+    int* tiles;  // [jobs] tiles of each job: prefix blocks, then tails
+    int* upto;   // [jobs + 1] pieces ahead of each job, and from bit 16 on jobs with tiles ahead of it
     int* jb;     // [groups + 1] first prefix job of each group
     int* gs;     // [groups + 1] group starts
     int* pre;    // [groups] prefix lengths
@@ -302,13 +305,13 @@ __device__ __forceinline__ int last_at(const int* v, int n, int x) {
     }
     return lo;
 }
-// the same by a whole wave, n <= 4096: two reads instead of one per halving
-__device__ __forceinline__ int wave_last_at(const int* v, int n, int x) {
+// the same by a whole wave, n <= 4096, of entries' bits in `mask`: two reads instead of one per halving
+__device__ __forceinline__ int wave_last_at(const int* v, int n, int x, int mask = -1) {
     const int lane = threadIdx.x & 63, step = (n + 63) >> 6;
     int i = lane * step;
-    const int b = (__popcll(__ballot(i < n && v[min(i, n - 1)] <= x)) - 1) * step;
+    const int b = (__popcll(__ballot(i < n && (v[min(i, n - 1)] & mask) <= x)) - 1) * step;
     i = b + lane;
-    return b + __popcll(__ballot(lane < step && i < n && v[min(i, n - 1)] <= x)) - 1;
+    return b + __popcll(__ballot(lane < step && i < n && (v[min(i, n - 1)] & mask) <= x)) - 1;
 }
 // v[0..n) to its exclusive prefix sums, v[n] the sum, by one wave
 __device__ __forceinline__ void wave_prefix_sum(int* v, int n) {
@@ -340,7 +343,20 @@ __device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return ma
 // a tail begins with the 16 positions that hold the prefix's end, one page's
 __device__ __forceinline__ int tail_base(int prefix) { return prefix & ~15; }
 
-__device__ void group_plan(const GroupArgs& a, GroupPlan& p) {
+// a wave's sum of f(i) over i < n
+template <typename F>
+__device__ __forceinline__ int wave_sum(int n, F f) {
+    int x = 0;
+    for (int i = threadIdx.x & 63; i < n; i += 64) x += f(i);
+    return over_wave(x, [](int u, int v) { return u + v; });
+}
+// pieces of a job of `tiles` tiles, at most about `most` each; per_most = 1 / most
+__device__ __forceinline__ int pieces_of(int tiles, int most, float per_most) {
+    return tiles ? max(1, (int)((float)(tiles + most - 1) * per_most)) : 0;
+}
+constexpr int LEAST = 2;  // tiles that are not worth a piece of their own and a merge
+
+__device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     const int tid = threadIdx.x;
     for (int i = tid; i < max(a.n, a.groups + 1); i += GTH) {  // (all requested at once)
         const int c = row_ctx(a, min(i, a.n - 1)), s = group_start(a, min(i, a.groups)),
@@ -352,35 +368,52 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p) {
             p.jb[i] = (max(0, t - s) * a.G + BLK - 1) / BLK;
         }
     }
-    for (int j = tid; j < a.job_cap + a.n; j += GTH) p.pref[j] = 0;
+    for (int j = tid; j < a.job_cap + a.tails; j += GTH) p.tiles[j] = 0;
     lds_sync();
     if (tid < 64) wave_prefix_sum(p.jb, a.groups);
     lds_sync();
     p.np = min(p.jb[a.groups], a.job_cap);
+    const int jobs = p.np + a.tails;
     for (int r = tid; r < a.n; r += GTH) {
         if (r < p.gs[0] || r >= p.gs[a.groups]) continue;
         const int g = last_at(p.gs, a.groups, r), ctx = p.ctx[r], pre = p.pre[g], all = (p.gs[g + 1] - p.gs[g]) * a.G;
         const int c0 = (r - p.gs[g]) * a.G, b1 = (c0 + a.G - 1) / BLK;
         for (int b = c0 / BLK; b <= b1 && p.jb[g] + b < p.np; b++)
-            atomicMax(&p.pref[p.jb[g] + b], tiles_of(min(ctx, pre), min(BLK, all - BLK * b)));
-        if (ctx > pre) p.pref[p.np + r] = tiles_of(ctx - tail_base(pre), a.G);
+            atomicMax(&p.tiles[p.jb[g] + b], tiles_of(min(ctx, pre), min(BLK, all - BLK * b)));
+        if (ctx > pre) atomicMax(&p.tiles[p.np + r / a.tail_rows], tiles_of(ctx - tail_base(pre), BLK));
     }
     lds_sync();
-    if (tid < 64) wave_prefix_sum(p.pref, p.np + a.n);
+    if (tid < 64) {
+        // the shortest piece of which there are at most `shares`, or as many times that as there are jobs
+        const int full = wave_sum(jobs, [&](int j) { return p.tiles[j] > 0 ? 1 : 0; });
+        const int room = shares * max(1, (full + shares - 1) / shares);
+        int most = 0;
+        for (int j = tid; j < jobs; j += 64) most = max(most, p.tiles[j]);
+        most = over_wave(most, imax2);
+        int lo = min(LEAST, max(1, most)), hi = max(lo, most);
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            const float per = 1.f / (float)mid;
+            if (wave_sum(jobs, [&](int j) { return pieces_of(p.tiles[j], mid, per); }) <= room) hi = mid;
+            else lo = mid + 1;
+        }
+        const float per = 1.f / (float)lo;
+        for (int j = tid; j < jobs; j += 64) {
+            const int x = pieces_of(p.tiles[j], lo, per);
+            p.upto[j] = x | (x ? 1 << 16 : 0);
+        }
+        wave_prefix_sum(p.upto, jobs);
+    }
     lds_sync();
     if (blockIdx.x == 0 && blockIdx.y == 0) {
-        const int jobs = p.np + a.n;
-        for (int j = tid; j <= jobs; j += GTH) a.plan[2 + 2 * a.n + j] = p.pref[j];
+        for (int j = tid; j <= jobs; j += GTH) a.plan[1 + 2 * a.n + j] = p.upto[j];
         for (int r = tid; r < a.n; r += GTH) {
             const bool in = r >= p.gs[0] && r < p.gs[a.groups];
             const int g = in ? last_at(p.gs, a.groups, r) : 0;
-            a.plan[2 + 2 * r] = in ? p.jb[g] * BLK + (r - p.gs[g]) * a.G : -1;
-            a.plan[3 + 2 * r] = in && min(p.ctx[r], p.pre[g]) > 0;
+            a.plan[1 + 2 * r] = in ? p.jb[g] * BLK + (r - p.gs[g]) * a.G : -1;
+            a.plan[2 + 2 * r] = (min(p.ctx[r], p.pre[g]) > 0 ? 1 : 0) | (p.ctx[r] > p.pre[g] ? 2 : 0);
         }
-        if (tid == 0) {
-            a.plan[0] = p.pref[jobs];
-            a.plan[1] = p.np;
-        }
+        if (tid == 0) a.plan[0] = p.np;
     }
 }
 
@@ -417,8 +450,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     float* s_o = s_dyn;
     uint4* s_q = (uint4*)s_dyn;   // [4][KS][2][64] q's operands lane by lane, during them
     GroupPlan plan;
-    plan.pref = (int*)(s_dyn + GW * 32 * HD);
-    plan.jb = plan.pref + a.job_cap + a.n + 1;
+    plan.tiles = (int*)(s_dyn + GW * 32 * HD);
+    plan.upto = plan.tiles + a.job_cap + a.tails;
+    plan.jb = plan.upto + a.job_cap + a.tails + 1;
     plan.gs = plan.jb + a.groups + 1;
     plan.pre = plan.gs + a.groups + 1;
     plan.ctx = plan.pre + a.groups;
@@ -435,44 +469,52 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     };
     const int kvh = blockIdx.y, w = blockIdx.x, G = a.G, psl = a.ps_log2, psm = (1 << psl) - 1;
 
-    group_plan(a, plan);
-    const int jobs = plan.np + a.n, T = plan.pref[jobs], shares = min((int)gridDim.x, T);
-    if (w >= shares) return;
-    const int t0 = (int)(((long long)w * T) / shares), t1 = (int)(((long long)(w + 1) * T) / shares);
+    group_plan(a, plan, gridDim.x);
+    const int jobs = plan.np + a.tails, pieces = plan.upto[jobs] & 0xFFFF;
 
-    for (int j = wave_last_at(plan.pref, jobs, t0); j < jobs; j++) {
-        const int p0 = plan.pref[j], p1 = plan.pref[j + 1];
-        if (p0 >= t1) break;
-        if (p0 == p1) continue;
+    for (int piece = w; piece < pieces; piece += gridDim.x) {
         lanes_again();
-        const int ja = max(t0, p0) - p0, jend = min(t1, p1) - p0;  // the segment: tiles [ja, jend) of the job
-        const bool whole = ja == 0 && jend == p1 - p0;
+        const int j = __builtin_amdgcn_readfirstlane(wave_last_at(plan.upto, jobs, piece, 0xFFFF));
+        const int here = __builtin_amdgcn_readfirstlane(plan.upto[j]), next = __builtin_amdgcn_readfirstlane(plan.upto[j + 1]);
+        const int tiles = __builtin_amdgcn_readfirstlane(plan.tiles[j]);
+        const int i_of = piece - (here & 0xFFFF), n_of = (next & 0xFFFF) - (here & 0xFFFF);
+        const int ja = (int)((long long)i_of * tiles / n_of), jend = (int)((long long)(i_of + 1) * tiles / n_of);
+        const bool whole = n_of == 1;  // tiles [ja, jend) of the job
 
-        // ---- the job
+        // ---- the wave's place: qt of wq waves side by side along the job's columns, kw of wk along the positions
         const bool tail = j >= plan.np;
-        int g, colbase, cols, trow;
-        if (tail) {
-            trow = j - plan.np;
-            g = wave_last_at(plan.gs, a.groups, trow);
-            colbase = trow * G;
-            cols = G;
+        int g, trow, first, cols, wq;  // group; the row whose table is read; first column (among all rows'), columns
+        if (tail) {                    // a row's columns are 1, 2 or 4 waves'
+            wq = 4;
+            const int side = 4 / a.tail_rows, c0 = 32 * (wave & (side - 1));
+            const int row = (j - plan.np) * a.tail_rows + (wave & 3) / side;
+            const bool in = row < a.n && row >= plan.gs[0] && row < plan.gs[a.groups];
+            trow = min(row, a.n - 1);
+            g = in ? wave_last_at(plan.gs, a.groups, trow) : 0;
+            first = trow * G + c0;
+            cols = in && plan.ctx[trow] > plan.pre[g] ? min(32, G - c0) : 0;
         } else {
             g = wave_last_at(plan.jb, a.groups, j);
             const int b = j - plan.jb[g];
             trow = plan.gs[g];
-            colbase = trow * G + BLK * b;
             cols = min(BLK, (plan.gs[g + 1] - trow) * G - BLK * b);
+            wq = waves_over(cols);
+            const int c0 = 32 * (wave & (wq - 1));
+            first = trow * G + BLK * b + c0;
+            cols = min(32, cols - c0);
         }
-        const int pre = plan.pre[g], lo = tail ? pre : 0, base = tail ? tail_base(pre) : 0;
-        const int wq = waves_over(cols), wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
+        wq = __builtin_amdgcn_readfirstlane(wq);
+        cols = __builtin_amdgcn_readfirstlane(max(cols, 0));
+        const int wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
+        const int pre = __builtin_amdgcn_readfirstlane(plan.pre[g]), lo = tail ? pre : 0, base = tail ? tail_base(pre) : 0;
         // the page table through scalar loads: an id does not wait for vector loads ahead of it
         typedef const __attribute__((address_space(4))) int32_t ConstInt;
         ConstInt* ptab = (ConstInt*)(uintptr_t)(a.page_table + (size_t)__builtin_amdgcn_readfirstlane(trow) * a.max_pages);
 
-        // ---- the lane's column (past the block's end: its last, not written)
-        const int ab = colbase + min(qt * 32 + col, cols - 1), r = ab / G;
+        // ---- the lane's column (past the last: that again, not written), row and limit
+        const int ab = min(first + min(col, max(cols - 1, 0)), a.n * G - 1), r = ab / G;
         const float* qrow = a.q + ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
-        const int ctx = plan.ctx[r], lim = tail ? ctx : min(ctx, pre);
+        const int ctx = plan.ctx[r], lim = cols == 0 ? 0 : tail ? ctx : min(ctx, pre);
         // behind the last position that some of the wave's columns attends to
         const int kend = __builtin_amdgcn_readfirstlane(over_wave(lim, imax2)), klast = max(kend - 1, 0);
         const int least = __builtin_amdgcn_readfirstlane(over_wave(lim, imin2));
@@ -850,7 +892,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             s_l[wave][col] = l;
         }
         const float unit = F16 ? 1.f : ldexpf(1.f, -vexp);
-        if (qt * 32 + col < cols) {
+        if (col < cols) {
             float4* row = (float4*)(s_o + (wave * 32 + col) * HD);
             const int x = col & 15;
 #pragma unroll
@@ -873,7 +915,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         }
         lds_sync();
         // per column: the waves' factors, and where the joined output goes
-        if (kw == 0 && half == 0 && qt * 32 + col < cols) {
+        if (kw == 0 && half == 0) {
             float mv[GW], lv[GW], M = -INFINITY, L = 0.f;
 #pragma unroll
             for (int k = 0; k < GW; k++) {
@@ -891,9 +933,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             }
             const bool any_pre = min(ctx, pre) > 0, any_tail = ctx > pre;
             const bool alone = whole && (tail ? !any_pre : any_pre && !any_tail);
-            const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab + (size_t)BLK * w;
-            const bool part = !alone && (tail || any_pre);
-            s_to[qt * 32 + col] = alone ? a.out + (qrow - a.q) : part ? a.part_o + slot * HD : nullptr;
+            // (pieces ahead, less one for each of their jobs: a job's columns are at most 128, so slots stay apart)
+            const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab +
+                                (size_t)BLK * ((here & 0xFFFF) - (here >> 16) + i_of);
+            const bool mine = col < cols, part = mine && !alone && (tail || any_pre);
+            s_to[qt * 32 + col] = mine && alone ? a.out + (qrow - a.q) : part ? a.part_o + slot * HD : nullptr;
             s_by[qt * 32 + col] = alone ? 1.f / L : 1.f;
             if (part) a.part_ml[slot] = make_float2(M, L);
         }
@@ -902,8 +946,10 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         auto join = [&](auto wk_c) {
             constexpr int WK = decltype(wk_c)::value, WQ = GW / WK;
 #pragma unroll 2
-            for (int e = tid; e < cols * (HD / 4); e += GTH) {
+            for (int e = tid; e < WQ * 32 * (HD / 4); e += GTH) {
                 const int c = e / (HD / 4), d = e % (HD / 4) * 4, cq = c >> 5, ci = c & 31;
+                float* to = s_to[c];
+                if (!to) continue;
                 float4 x[WK];
                 float f[WK];
 #pragma unroll
@@ -919,9 +965,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     O.z = __builtin_fmaf(x[k].z, f[k], O.z);
                     O.w = __builtin_fmaf(x[k].w, f[k], O.w);
                 }
-                float* to = s_to[c];
                 const float by = s_by[c];
-                if (to) *(float4*)(to + d) = make_float4(O.x * by, O.y * by, O.z * by, O.w * by);
+                *(float4*)(to + d) = make_float4(O.x * by, O.y * by, O.z * by, O.w * by);
             }
         };
         if (wk == 2) join(std::integral_constant<int, 2>());
@@ -934,25 +979,22 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 // The parts of a column, joined in order: one wave per (row, query head).  A row
 // whose one part was the output itself is left; one without any is zero.
 template <int HD>
-__global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a, int gx) {
+__global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
     constexpr int DPL = HD / 64;
     const int r = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (h >= a.H) return;
     const int lane = threadIdx.x & 63, kvh = h / a.G, hh = h - kvh * a.G;
-    const int pos = a.plan[2 + 2 * r], any_pre = a.plan[3 + 2 * r];
+    const int np = a.plan[0], pos = a.plan[1 + 2 * r], which = a.plan[2 + 2 * r];
     if (pos < 0) return;  // outside every group
-    const int T = a.plan[0], np = a.plan[1], shares = min(gx, T);
-    const int* pref = a.plan + 2 + 2 * a.n;
-    // (first share, parts) of the prefix and of the tail: tile x lies in share ((x + 1) shares - 1) / T
+    const int* upto = a.plan + 1 + 2 * a.n;
+    // (first slot, parts) of the prefix and of the tail
     int first[2] = {0, 0}, count[2] = {0, 0};
-    const int jobs[2] = {(pos + hh) / BLK, np + r};
+    const int jobs[2] = {(pos + hh) / BLK, np + r / a.tail_rows};
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        if (k == 0 && !any_pre) continue;
-        const long long x0 = pref[jobs[k]], x1 = pref[jobs[k] + 1];
-        if (x1 <= x0) continue;
-        first[k] = (int)(((x0 + 1) * shares - 1) / T);
-        count[k] = (int)((x1 * shares - 1) / T) - first[k] + 1;
+        const int x = upto[jobs[k]], y = upto[jobs[k] + 1];
+        first[k] = (x & 0xFFFF) - (x >> 16);
+        count[k] = which >> k & 1 ? (y & 0xFFFF) - (x & 0xFFFF) : 0;
     }
     const int all = count[0] + count[1];
     float* out = a.out + ((size_t)r * a.H + h) * HD;
@@ -1005,7 +1047,7 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a, int gx) {
 static int group_grid(int Hkv) { return std::max(1, 256 / Hkv); }
 
 struct GroupSizes {
-    int job_cap;
+    int job_cap, tail_rows, tails;
     long long slots;
     size_t plan_bytes, ml_bytes, o_bytes;
 };
@@ -1013,20 +1055,22 @@ static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
     const int G = H / Hkv;
     GroupSizes z;
     z.job_cap = (int)((long long)n * G / BLK) + groups;
+    z.tail_rows = G <= 32 ? 4 : G <= 64 ? 2 : 1;
+    z.tails = (n + z.tail_rows - 1) / z.tail_rows;
     z.slots = 2ll * n * G + (long long)BLK * group_grid(Hkv);
-    z.plan_bytes = ((size_t)(2 + 2 * n + z.job_cap + n + 1) * 4 + 255) / 256 * 256;
+    z.plan_bytes = ((size_t)(2 + 2 * n + z.job_cap + z.tails) * 4 + 255) / 256 * 256;
     z.ml_bytes = ((size_t)Hkv * z.slots * sizeof(float2) + 255) / 256 * 256;
     z.o_bytes = (size_t)Hkv * z.slots * hd * 4;
     return z;
 }
-static size_t group_lds(int hd, int n, int groups, int job_cap) {
-    return (size_t)GW * 32 * hd * 4 + (size_t)(job_cap + 2 * n + 3 * (groups + 1)) * 4;
+static size_t group_lds(int hd, int n, int groups, const GroupSizes& z) {
+    return (size_t)GW * 32 * hd * 4 + (size_t)(2 * (z.job_cap + z.tails) + 1 + 3 * groups + 2 + n) * 4;
 }
 // shapes of the tiles (their LDS bounds what few very wide layouts would need)
 static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
     const int G = H / Hkv;
     return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 &&
-           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd).job_cap) + 5120 <= 160 * 1024;
+           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
 }
 
 int group_attention_init() {
@@ -1061,6 +1105,7 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
                "group attention: head_dim %d (16, 32, 64 or 128 supported)", hd);
     QH_REQUIRE(page_size > 0 && max_pages > 0 && max_ctx > 0 && max_ctx <= (long long)max_pages * page_size,
                QRAF_HIP_ERR_INVALID, "group attention: bad page geometry");
+    QH_REQUIRE(max_ctx <= 1 << 30, QRAF_HIP_ERR_INVALID, "group attention: max_ctx %d over 2^30", max_ctx);
     QH_REQUIRE(kv_dtype == DT_F32 || kv_dtype == DT_F16 || kv_dtype == DT_I8, QRAF_HIP_ERR_DTYPE,
                "group attention: KV dtype %u", kv_dtype);
     QH_REQUIRE(ws_bytes >= group_attention_workspace_bytes(n, groups, H, Hkv, hd, max_ctx), QRAF_HIP_ERR_INVALID,
@@ -1087,13 +1132,15 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
     if (group_tiles(n, groups, H, Hkv, hd, page_size)) {
         const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
         a.job_cap = z.job_cap;
+        a.tail_rows = z.tail_rows;
+        a.tails = z.tails;
         a.slots = z.slots;
         while ((1 << a.ps_log2) < page_size) a.ps_log2++;
         a.plan = (int*)ws;
         a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
         a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
         const int gx = group_grid(Hkv);
-        const size_t lds = group_lds(hd, n, groups, z.job_cap);
+        const size_t lds = group_lds(hd, n, groups, z);
 #define QH_GROUP_TILE(HDv, KVv)   \
     if (hd == HDv && kv_dtype == KVv) \
         hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv>), dim3(gx, Hkv), dim3(GTH), lds, st, a);
@@ -1101,8 +1148,8 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
         QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)
 #undef QH_GROUP_TILE
         QH_CHECK_HIP(hipGetLastError());
-        if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a, gx);
-        else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a, gx);
+        if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a);
         QH_CHECK_HIP(hipGetLastError());
         return QRAF_HIP_OK;
     }
