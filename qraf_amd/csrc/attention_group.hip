@@ -354,8 +354,6 @@ __device__ __forceinline__ int wave_sum(int n, F f) {
 __device__ __forceinline__ int pieces_of(int tiles, int most, float per_most) {
     return tiles ? max(1, (int)((float)(tiles + most - 1) * per_most)) : 0;
 }
-constexpr int LEAST = 2;  // tiles that are not worth a piece of their own and a merge
-
 __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     const int tid = threadIdx.x;
     for (int i = tid; i < max(a.n, a.groups + 1); i += GTH) {  // (all requested at once)
@@ -387,10 +385,9 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
         // the shortest piece of which there are at most `shares`, or as many times that as there are jobs
         const int full = wave_sum(jobs, [&](int j) { return p.tiles[j] > 0 ? 1 : 0; });
         const int room = shares * max(1, (full + shares - 1) / shares);
-        int most = 0;
-        for (int j = tid; j < jobs; j += 64) most = max(most, p.tiles[j]);
-        most = over_wave(most, imax2);
-        int lo = min(LEAST, max(1, most)), hi = max(lo, most);
+        const int all = wave_sum(jobs, [&](int j) { return p.tiles[j]; });
+        // (pieces of x tiles are at least all / x, and fewer than all / x + full)
+        int lo = max(1, (all + room - 1) / room), hi = room > full ? max(lo, (all + room - full - 1) / (room - full)) : max(lo, all);
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             const float per = 1.f / (float)mid;
@@ -528,15 +525,17 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         };
         const size_t blk = (size_t)a.page_size * (I8 ? HD + 4 : F16 ? 2 * HD : 4 * HD);  // bytes of a (page, KV head)
         auto block = [&](const void* pool, int pg) { return (const char*)pool + ((size_t)pg * a.Hkv + kvh) * blk; };
-        auto load_k = [&](int t) {
+        // (real false: one address for all lanes, a load that nothing uses)
+        auto load_k = [&](int t, bool real = true) {
             const int pc = min(t + key_of(col), klast);  // (past the end: the last position's, masked below)
-            const char* kp = pc >= t + 16 ? block(a.kc, pg1) : block(a.kc, pg0);
+            const char* kp = pc >= t + 16 && real ? block(a.kc, pg1) : block(a.kc, pg0);
+            const uint32_t on = real ? 0xFFFFFFFFu : 0u;
             if constexpr (F16) {
-                const uint32_t o = (uint32_t)((pc & psm) * HD + 8 * half) * 2u;
+                const uint32_t o = ((uint32_t)((pc & psm) * HD + 8 * half) * 2u) & on;
 #pragma unroll
                 for (int kk = 0; kk < KS; kk++) tl.k[kk] = *(const f16x8*)(kp + (o + 32u * kk));
             } else if constexpr (I8) {
-                const uint32_t o = (uint32_t)((pc & psm) * HD + 16 * half);
+                const uint32_t o = (uint32_t)((pc & psm) * HD + 16 * half) & on;
 #pragma unroll
                 for (int kk = 0; kk < KS / 2; kk++) tl.k[kk] = *(const uint4*)(kp + (o + 32u * kk));
 #pragma unroll
@@ -546,7 +545,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     tl.ks[2 * b + 1] = *(const float4*)(sp + 16);
                 }
             } else {
-                const uint32_t o = (uint32_t)((pc & psm) * HD + 8 * half) * 4u;
+                const uint32_t o = ((uint32_t)((pc & psm) * HD + 8 * half) * 4u) & on;
 #pragma unroll
                 for (int kk = 0; kk < KS; kk++) {
                     tl.k[2 * kk] = *(const float4*)(kp + (o + 64u * kk));
@@ -554,7 +553,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 }
             }
         };
-        auto load_v = [&](int t) {
+        auto load_v = [&](int t, bool real = true) {
+            const uint32_t on = real ? 0xFFFFFFFFu : 0u;
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 const char* vp = block(a.vc, b ? pg1 : pg0);
@@ -562,11 +562,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 if constexpr (F16) {
 #pragma unroll
                     for (int d = 0; d < DT; d++)
-                        tl.v[d][b] = *(const uint4*)(vp + (uint32_t)((32 * d + col) * a.page_size + off) * 2u);
+                        tl.v[d][b] = *(const uint4*)(vp + (((uint32_t)((32 * d + col) * a.page_size + off) * 2u) & on));
                 } else if constexpr (I8) {
 #pragma unroll
                     for (int d = 0; d < DT; d++)
-                        tl.v[d][b] = *(const uint2*)(vp + (uint32_t)((32 * d + col) * a.page_size + off));
+                        tl.v[d][b] = *(const uint2*)(vp + ((uint32_t)((32 * d + col) * a.page_size + off) & on));
                     const char* sp = vp + (size_t)a.page_size * HD + 4 * off;
                     tl.vs[2 * b] = *(const float4*)sp;
                     tl.vs[2 * b + 1] = *(const float4*)(sp + 16);
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         const int pc = min(t + 16 * b + 8 * half + i, klast);
                         const char* xp = pc >= t + 16 ? block(a.vc, pg1) : block(a.vc, pg0);
                         tl.v[8 * b + i] = *(const typename GroupTile<HD, (int)DT_F32>::vrow*)(
-                            xp + (uint32_t)((pc & psm) * HD + DT * col) * 4u);
+                            xp + (((uint32_t)((pc & psm) * HD + DT * col) * 4u) & on));
                     }
                 }
             }
@@ -592,7 +592,6 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         // one meet, a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
         pg0 = more ? pg0 : 0;
         pg1 = more ? pg1 : 0;
-        load_k(more ? t : 0);
 
         // ---- q of 32 columns as fp16 hi + lo, scaled per column, by one wave for all that share them
         if (kw == 0) {
@@ -603,6 +602,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 qraw[2 * kk] = *(const float4*)(qrow + d);
                 qraw[2 * kk + 1] = *(const float4*)(qrow + d + 4);
             }
+            load_k(more ? t : 0);  // (behind q, which is waited for alone)
             uint4* qop = s_q + qt * KS * 128 + lane;
             float mx = 0.f;
 #pragma unroll
@@ -621,6 +621,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 qop[128 * kk + 64] = __builtin_bit_cast(uint4, lw);
             }
             if (half == 0) s_qs[qt * 32 + col] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e);
+        } else {
+            load_k(more ? t : 0);
         }
         if (!TURNS) load_v(more ? t : 0);  // (behind q: their registers)
         lds_sync();
@@ -695,12 +697,12 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
                 for (int x = 0; x < 16; x++) vsc[x] = ((const float*)&tl.vs[x >> 2])[x & 3];
             }
-            // the next tile's ids and K (behind the last tile: its own again)
+            // the next tile's ids and K
             const bool go = i + 1 < jend && t + dt < kend;
             const int tn = go ? t + dt : t;
             if (TURNS) load_v(t);
             ids(tn);
-            if (!TURNS) load_k(tn);
+            if (!TURNS) load_k(tn, go);
 
             // ---- softmax: register x is position t + 16 (x / 8) + 8 half + x % 8
             float mt = -INFINITY;
@@ -876,8 +878,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b], o[d], 0, 0, 0);
                     }
                 }
-            if (TURNS) load_k(tn);
-            else load_v(tn);
+            if (TURNS) load_k(tn, go);
+            else load_v(tn, go);
             more = go;
             i++;
             t = tn;
