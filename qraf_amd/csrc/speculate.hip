@@ -11,12 +11,27 @@
 //   p_i = w_i / sum_{j in N} w_j for i in N, 0 elsewhere.
 // The kept set is one threshold: the order-preserving key of its smallest
 // logit and the number of equal logits it takes, lowest indices first.  It is
-// found by radix select over the keys, with counts for top_k and weights for
-// top_p.  Weights are summed as integers (w times a power of two that keeps the
-// row's sum below 2^62, from a 64-bit exponential): integer sums do not depend
-// on the order of the atomics, so results repeat bit for bit, and the border
-// of a nucleus whose tokens weigh 1e-6 of the row each is the one of the sums in
-// 64-bit floating point.
+// Weights are summed as integers there (w times a power of two that keeps the
+// row's sum below 2^62, from a 64-bit exponential): integer sums do not depend on
+// the order of the atomics, so results repeat bit for bit, and the border of a
+// nucleus whose tokens weigh 1e-6 of the row each is the one of the sums in 64-bit
+// floating point.
+//
+// A row of 152K logits is read by many workgroups (one alone reads 600 KB in
+// 10 us), in launches that follow one another:
+//   stats   per split the largest and smallest logit and, where nothing is cut
+//           off, the weight; for a short top_k also the largest of every thread's
+//           E logits (a sub-range)
+//   select  short top_k: one workgroup per row.  The top_k-th largest of the
+//           sub-ranges' maxima bounds the top_k-th largest logit from below;
+//           only sub-ranges whose maximum reaches it are read again
+//           (probs_topk_kernel)
+//           nucleus of the whole row: weights by bins of the logits' distance from
+//           the largest (probs_bins_kernel), the logits of the bin in which top_p
+//           is reached (probs_gather_kernel), those in order (probs_border_kernel)
+//           else, and where such a list overflows (flat rows): radix select over
+//           the keys by one workgroup
+//   write   w_i / sum in 32 bits, w by a two-part exponent
 //
 // qraf_hip_verify_draft_dev: row j of a sequence is the target's distribution
 // behind its first j drafted tokens.  Draft x_j, drawn from q_j, is accepted
@@ -51,29 +66,89 @@ __device__ __forceinline__ double weight64(float l, float m, double T) {
     return exp(((double)l - (double)m) / T);
 }
 
-__global__ __launch_bounds__(PNT) void probs_rows_kernel(const float* __restrict__ logits, int V, float T, int cutoff,
-                                                         float top_p, float* __restrict__ probs) {
-    const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float* l = logits + (size_t)row * V;
-    float* p = probs + (size_t)row * V;
-    __shared__ float s_f[16];
-    __shared__ int s_i[16];
-    __shared__ unsigned long long s_hist[256];
-    __shared__ unsigned long long s_sum;
-    __shared__ uint32_t s_key;
-    __shared__ unsigned long long s_need;
-    __shared__ int s_cut, s_cnt[PNT];
+// the same in 32 bits, off by at most 3 units of the last place: the exponent's
+// rounding errors (of l - m, of its product with log2(e) / T) as a factor behind it
+struct Weight32 {
+    float m, c, c_lo;
+    __device__ __forceinline__ Weight32(float m_, double T) : m(m_) {
+        const double k = 1.4426950408889634074 / T;
+        c = (float)k;
+        c_lo = (float)(k - (double)c);
+    }
+    __device__ __forceinline__ float operator()(float l) const {
+        const float d = l - m, bb = d + m;                  // l - m = d + err (Knuth's two-sum)
+        const float err = (l - bb) + (m - (bb - d));
+        const float h = d * c;
+        const float e = __builtin_fmaf(d, c, -h) + __builtin_fmaf(d, c_lo, err * c);
+        const float w = __builtin_amdgcn_exp2f(h);
+        return l == m ? 1.f : h > -160.f ? __builtin_fmaf(w, e * 0.693147180559945f, w) : 0.f;  // (-inf, NaN: 0)
+    }
+};
 
-    // ---- the largest logit and its first index
-    float m = -INFINITY;
-    int mi = V;
-    for (int i = tid; i < V; i += PNT) {
-        const float v = clean_logit(l[i]);
-        if (v > m) {
-            m = v;
-            mi = i;
+constexpr int STH = 256;       // threads of a split
+constexpr int TOPK_MAX = 512;  // largest top_k by sub-range maxima
+constexpr int SUB_REGS = 20;   // sub-range maxima a thread of the selection holds
+constexpr int LIST = 4096;     // candidates in order at most
+constexpr int BINS = 2048;
+
+struct SplitStats {
+    float m, s, least;  // the largest logit, the split's weight against it, the smallest above -inf
+    int mi;             // the first index of m
+};
+struct RowSel {  // what is kept: keys above `key`, and of those equal to it the logits before index `cut`
+    double inv;  // 1 / their weight
+    float m;
+    uint32_t key;
+    int cut;
+};
+struct ProbsArgs {
+    const float* logits;
+    float* probs;
+    SplitStats* stats;         // [rows][S]
+    float* sub;                // [rows][S * STH] sub-range maxima
+    unsigned long long* bins;  // [rows][BINS]
+    unsigned long long* list;  // [rows][LIST] (key, ~index)
+    int* count;                // [rows]
+    RowSel* sel;               // [rows]
+    int V, S, cutoff;
+    float T, top_p;
+};
+
+// logits of a split: thread's element u of E, its index; VEC: in float4s, of rows aligned to them
+template <int E, bool VEC>
+__device__ __forceinline__ int split_index(int split, int u) {
+    const int b = split * STH * E;
+    return VEC ? b + 4 * (threadIdx.x + STH * (u >> 2)) + (u & 3) : b + (int)threadIdx.x + STH * u;
+}
+// element u of sub-range (split, thread)
+template <int E, bool VEC>
+__device__ __forceinline__ int sub_index(int sub, int u) {
+    const int b = sub / STH * STH * E, t = sub % STH;
+    return VEC ? b + 4 * (t + STH * (u >> 2)) + (u & 3) : b + t + STH * u;
+}
+template <int E, bool VEC>
+__device__ __forceinline__ void load_split(const float* l, int V, int split, float (&v)[E]) {
+    if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < E / 4; j++) {
+            const int i = split_index<E, VEC>(split, 4 * j);
+            const float4 x = *(const float4*)(l + min(i, V - 4));
+            const bool in = i < V;
+            v[4 * j] = in ? x.x : -INFINITY, v[4 * j + 1] = in ? x.y : -INFINITY;
+            v[4 * j + 2] = in ? x.z : -INFINITY, v[4 * j + 3] = in ? x.w : -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < E; u++) {
+            const int i = split_index<E, VEC>(split, u);
+            const float x = l[min(i, V - 1)];
+            v[u] = i < V ? x : -INFINITY;
         }
     }
+}
+
+// the first of the largest over a workgroup's waves, in every thread (s_f, s_i: an entry for each wave)
+__device__ __forceinline__ void block_first_max(float& m, int& mi, float* s_f, int* s_i, int waves) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
         const float om = __shfl_xor(m, o);
@@ -83,55 +158,146 @@ __global__ __launch_bounds__(PNT) void probs_rows_kernel(const float* __restrict
             mi = oi;
         }
     }
-    if (lane == 0) {
-        s_f[wave] = m;
-        s_i[wave] = mi;
+    if ((threadIdx.x & 63) == 0) {
+        s_f[threadIdx.x >> 6] = m;
+        s_i[threadIdx.x >> 6] = mi;
     }
     __syncthreads();
-    for (int w = 0; w < 16; w++)
+    for (int w = 0; w < waves; w++)
         if (s_f[w] > m || (s_f[w] == m && s_i[w] < mi)) {
             m = s_f[w];
             mi = s_i[w];
         }
-    if (m == -INFINITY || !(T > 0.f)) {  // no token, or the first of the largest
-        for (int i = tid; i < V; i += PNT) p[i] = i == mi ? 1.f : 0.f;
-        return;
+}
+
+enum : int { STATS_SUM = 0, STATS_SUB = 1, STATS_BINS = 2 };  // what follows: the write, top_k, the nucleus' bins
+
+template <int E, bool VEC>
+__global__ __launch_bounds__(STH) void probs_stats_kernel(ProbsArgs a, int what) {
+    __shared__ float s_f[4], s_least[4], s_sum[4];
+    __shared__ int s_i[4];
+    const int split = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float v[E];
+    load_split<E, VEC>(a.logits + (size_t)row * a.V, a.V, split, v);
+    float m = -INFINITY, least = INFINITY;
+    int mi = a.V;
+#pragma unroll
+    for (int u = 0; u < E; u++) {
+        v[u] = clean_logit(v[u]);
+        if (v[u] > m) {  // (increasing index)
+            m = v[u];
+            mi = split_index<E, VEC>(split, u);
+        }
+        least = v[u] > -INFINITY ? fminf(least, v[u]) : least;
     }
+    if (what == STATS_SUB) a.sub[((size_t)row * a.S + split) * STH + tid] = m;
+    block_first_max(m, mi, s_f, s_i, 4);
+    float sum = 0.f;
+    if (what == STATS_SUM && m > -INFINITY) {
+        const Weight32 weight(m, a.T);
+#pragma unroll
+        for (int u = 0; u < E; u++) sum += weight(v[u]);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        least = fminf(least, __shfl_xor(least, o));
+        sum += __shfl_xor(sum, o);
+    }
+    if (lane == 0) {
+        s_least[wave] = least;
+        s_sum[wave] = sum;
+    }
+    __syncthreads();
+    if (tid == 0)
+        a.stats[(size_t)row * a.S + split] =
+            SplitStats{m, (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]),
+                       fminf(fminf(s_least[0], s_least[1]), fminf(s_least[2], s_least[3])), mi};
+    if (what == STATS_BINS) {  // cleared for what follows
+        for (int i = split * STH + tid; i < BINS; i += a.S * STH) a.bins[(size_t)row * BINS + i] = 0;
+        if (split == 0 && tid == 0) a.count[row] = 0;
+    }
+}
 
-    const double t64 = T;
-    const double unit = ldexp(1.0, 62 - (32 - __clz(V)));
-    auto weigh = [&](float v) { return (unsigned long long)(weight64(v, m, t64) * unit + 0.5); };
+// the row's largest logit, its first index, its smallest above -inf and its weight, from its splits, by each wave
+struct RowStats {
+    float m, least;
+    int mi;
+    double s;
+};
+__device__ __forceinline__ RowStats row_stats(const ProbsArgs& a, int row) {
+    const SplitStats* st = a.stats + (size_t)row * a.S;
+    RowStats r{-INFINITY, INFINITY, a.V, 0.0};
+    for (int i = threadIdx.x & 63; i < a.S; i += 64) {
+        const SplitStats x = st[i];
+        if (x.m > r.m) {
+            r.m = x.m;
+            r.mi = x.mi;
+        }
+        r.least = fminf(r.least, x.least);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const float om = __shfl_xor(r.m, o);
+        const int oi = __shfl_xor(r.mi, o);
+        if (om > r.m || (om == r.m && oi < r.mi)) {
+            r.m = om;
+            r.mi = oi;
+        }
+        r.least = fminf(r.least, __shfl_xor(r.least, o));
+    }
+    for (int i = threadIdx.x & 63; i < a.S; i += 64) r.s += (double)st[i].s * weight64(st[i].m, r.m, a.T);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) r.s += __shfl_xor(r.s, o);
+    return r;
+}
 
-    // the kept set: keys above `key`, and of the logits at it those before index `cut`
-    uint32_t key = 0;
+// integer weights: the power of two that keeps a row's sum below 2^62
+__device__ __forceinline__ double weight_unit(int V) { return ldexp(1.0, 62 - (32 - __clz(V))); }
+__device__ __forceinline__ unsigned long long weigh(float l, float m, double T, double unit) {
+    return (unsigned long long)(weight64(l, m, T) * unit + 0.5);
+}
+// weight that the nucleus has to reach
+__device__ __forceinline__ unsigned long long nucleus_need(unsigned long long z, float top_p) {
+    return max(1ull, (unsigned long long)ceil((double)z * (double)top_p));
+}
+
+// ---- radix select, one workgroup: any row and parameters
+struct RadixShared {
+    unsigned long long hist[256], sum, need;
+    uint32_t key;
+    int cut, cnt[PNT];
+};
+__device__ void radix_select(const ProbsArgs& a, const float* l, float m, RadixShared& sh, RowSel* out) {
+    const int tid = threadIdx.x, V = a.V;
+    const double t64 = a.T, unit = weight_unit(V);
+    uint32_t key = 0;  // the kept set so far
     int cut = V;
-    // among the kept logits, the largest prefix-closed set that falls short of
-    // `need` (counts, or weights), as a key and the need left at it
+    // the kept set's largest logits that reach `need` (a count, or a weight)
     auto select = [&](bool by_weight, unsigned long long need) {
         uint32_t prefix = 0, mask = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s_hist[tid] = 0;
+            if (tid < 256) sh.hist[tid] = 0;
             __syncthreads();
             for (int i = tid; i < V; i += PNT) {
                 const float v = clean_logit(l[i]);
                 const uint32_t k = logit_key(v);
                 if ((k & mask) != prefix || k < key || (k == key && i >= cut)) continue;
-                atomicAdd(&s_hist[(k >> shift) & 255u], by_weight ? weigh(v) : 1ull);
+                atomicAdd(&sh.hist[(k >> shift) & 255u], by_weight ? weigh(v, m, t64, unit) : 1ull);
             }
             __syncthreads();
             if (tid == 0) {
                 unsigned long long acc = 0;
                 int d = 255;
                 for (; d > 0; d--) {
-                    if (acc + s_hist[d] >= need) break;
-                    acc += s_hist[d];
+                    if (acc + sh.hist[d] >= need) break;
+                    acc += sh.hist[d];
                 }
-                s_key = prefix | ((uint32_t)d << shift);
-                s_need = need - acc;
+                sh.key = prefix | ((uint32_t)d << shift);
+                sh.need = need - acc;
             }
             __syncthreads();
-            prefix = s_key;
-            need = s_need;
+            prefix = sh.key;
+            need = sh.need;
             mask |= 255u << shift;
             __syncthreads();
         }
@@ -139,73 +305,420 @@ __global__ __launch_bounds__(PNT) void probs_rows_kernel(const float* __restrict
         unsigned long long ties = need;
         if (by_weight) {
             const uint32_t b = (prefix & 0x80000000u) ? (prefix & 0x7FFFFFFFu) : ~prefix;
-            const unsigned long long w = weigh(__uint_as_float(b));
+            const unsigned long long w = weigh(__uint_as_float(b), m, t64, unit);
             ties = w ? (need + w - 1) / w : (unsigned long long)V;
         }
         // the index behind the ties-th of them
         const int ch = (V + PNT - 1) / PNT, i0 = min(V, tid * ch), i1 = min(V, i0 + ch);
         int c = 0;
         for (int i = i0; i < i1; i++) c += logit_key(clean_logit(l[i])) == prefix;
-        s_cnt[tid] = c;
-        if (tid == 0) s_cut = V;
+        sh.cnt[tid] = c;
+        if (tid == 0) sh.cut = V;
         __syncthreads();
         unsigned long long before = 0;
-        for (int t = 0; t < tid; t++) before += s_cnt[t];
+        for (int t = 0; t < tid; t++) before += sh.cnt[t];
         if (before < ties && before + c >= ties) {
             int i = i0;
             for (; before < ties; i++) before += logit_key(clean_logit(l[i])) == prefix;
-            s_cut = i;
+            sh.cut = i;
         }
         __syncthreads();
-        cut = prefix == key ? min(cut, s_cut) : s_cut;
+        cut = prefix == key ? min(cut, sh.cut) : sh.cut;
         key = prefix;
         __syncthreads();
     };
     auto total = [&]() {  // the kept set's weight
-        if (tid == 0) s_sum = 0;
+        if (tid == 0) sh.sum = 0;
         __syncthreads();
         unsigned long long z = 0;
         for (int i = tid; i < V; i += PNT) {
             const float v = clean_logit(l[i]);
             const uint32_t k = logit_key(v);
-            if (k > key || (k == key && i < cut)) z += weigh(v);
+            if (k > key || (k == key && i < cut)) z += weigh(v, m, t64, unit);
         }
-        atomicAdd(&s_sum, z);
+        atomicAdd(&sh.sum, z);
         __syncthreads();
-        z = s_sum;
+        z = sh.sum;
         __syncthreads();
         return z;
     };
-    if (cutoff < V) select(false, (unsigned long long)cutoff);
+    if (a.cutoff < V) select(false, (unsigned long long)a.cutoff);
     unsigned long long z = total();
-    if (top_p > 0.f && top_p < 1.f) {
-        const double need = ceil((double)z * (double)top_p);
-        select(true, max(1ull, (unsigned long long)need));
+    if (a.top_p > 0.f && a.top_p < 1.f) {
+        select(true, nucleus_need(z, a.top_p));
         z = total();
     }
-    const double inv = unit / (double)z;
-    for (int i = tid; i < V; i += PNT) {
-        const float v = clean_logit(l[i]);
-        const uint32_t k = logit_key(v);
-        p[i] = k > key || (k == key && i < cut) ? (float)(weight64(v, m, t64) * inv) : 0.f;
+    if (tid == 0) *out = RowSel{unit / (double)z, m, key, cut};
+}
+
+__global__ __launch_bounds__(PNT) void probs_radix_kernel(ProbsArgs a) {
+    __shared__ RadixShared sh;
+    const int row = blockIdx.x;
+    const RowStats r = row_stats(a, row);
+    if (r.m == -INFINITY) return;  // (the write looks at the row's stats)
+    radix_select(a, a.logits + (size_t)row * a.V, r.m, sh, &a.sel[row]);
+}
+
+// ---- candidates in order: n <= LIST entries (key, ~index) of `in`, the largest first, to `sorted`
+__device__ __forceinline__ void rank_sort(const unsigned long long* in, unsigned long long* sorted, int n) {
+    for (int i = threadIdx.x; i < n; i += PNT) {
+        const unsigned long long x = in[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; j++) rank += in[j] > x;
+        sorted[rank] = x;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ float key_logit(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+}
+// The first nc of `sorted`, or (nucleus) as many of them as bring the weight `above` them to need(all), to *out.
+// (s_w: a word for each thread)
+template <typename F>
+__device__ void keep_prefix(const ProbsArgs& a, const unsigned long long* sorted, int nc, float m, bool nucleus,
+                            unsigned long long above, F need_of, unsigned long long* s_w, RowSel* out) {
+    const int tid = threadIdx.x;
+    const double unit = weight_unit(a.V);
+    const int per = (nc + PNT - 1) / PNT, i0 = min(nc, tid * per), i1 = min(nc, i0 + per);
+    unsigned long long w = 0;
+    for (int i = i0; i < i1; i++) w += weigh(key_logit((uint32_t)(sorted[i] >> 32)), m, a.T, unit);
+    s_w[tid] = w;
+    __syncthreads();
+    for (int o = 1; o < PNT; o <<= 1) {  // inclusive sums
+        const unsigned long long x = tid >= o ? s_w[tid - o] : 0;
+        __syncthreads();
+        s_w[tid] += x;
+        __syncthreads();
+    }
+    auto keep = [&](int i, unsigned long long sum) {
+        const unsigned long long last = sorted[i];
+        *out = RowSel{unit / (double)sum, m, (uint32_t)(last >> 32), (int)(0xFFFFFFFFu - (uint32_t)last) + 1};
+    };
+    const unsigned long long all = above + s_w[PNT - 1], need = need_of(all);
+    if (!nucleus) {
+        if (tid == 0) keep(nc - 1, all);
+        return;
+    }
+    unsigned long long sum = above + s_w[tid] - w;
+    if (sum < need && sum + w >= need) {
+        int i = i0;
+        for (;; i++) {
+            sum += weigh(key_logit((uint32_t)(sorted[i] >> 32)), m, a.T, unit);
+            if (sum >= need || i + 1 >= i1) break;
+        }
+        keep(i, sum);
     }
 }
 
+// ---- short top_k
+template <int E, bool VEC>
+__global__ __launch_bounds__(PNT) void probs_topk_kernel(ProbsArgs a) {
+    __shared__ RadixShared sh;
+    __shared__ unsigned long long s_list[LIST], s_sorted[LIST], s_w[PNT];
+    __shared__ int s_subs[PNT], s_cnt[3][8], s_n, s_ns;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, V = a.V, n_sub = a.S * STH, k = a.cutoff;
+    const float* l = a.logits + (size_t)row * V;
+    const RowStats r = row_stats(a, row);
+    if (r.m == -INFINITY) return;
+    const float* sub = a.sub + (size_t)row * n_sub;
+    uint32_t mine[SUB_REGS];
+#pragma unroll
+    for (int u = 0; u < SUB_REGS; u++) {
+        const int i = tid + PNT * u;
+        mine[u] = i < n_sub ? logit_key(sub[min(i, n_sub - 1)]) : 0u;
+    }
+    if (tid < 24) s_cnt[tid >> 3][tid & 7] = 0;
+    if (tid == 0) s_n = s_ns = 0;
+    __syncthreads();
+    // a bound that at least k, and not many more, maxima reach: 8 thresholds at a time.  (All rows of one
+    // value, or masked ones, end with a list that overflows.)
+    uint32_t lo = logit_key(-INFINITY), hi = logit_key(r.m);
+    const int enough = k + (k >> 2) + 8;
+    int reach = n_sub;
+    for (int pass = 0; pass < 12 && reach > enough && lo < hi; pass++) {
+        uint32_t th[8];
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            th[j] = lo + (uint32_t)(((unsigned long long)(hi - lo) * (j + 1)) >> 3);
+            int x = 0;
+#pragma unroll
+            for (int u = 0; u < SUB_REGS; u++) x += __popcll(__ballot(mine[u] >= th[j]));
+            c = lane == j ? x : c;
+        }
+        if (lane < 8 && c) atomicAdd(&s_cnt[pass % 3][lane], c);
+        __syncthreads();
+        uint32_t nlo = lo, nhi = hi;
+        int nr = reach;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int x = s_cnt[pass % 3][j];
+            if (x >= k) {
+                nlo = th[j];
+                nr = x;
+            } else if (th[j] < nhi) {
+                nhi = th[j];
+            }
+        }
+        if (tid < 8) s_cnt[(pass + 2) % 3][tid] = 0;  // last read before this pass's barrier
+        if (nlo == lo && nhi == hi) break;
+        lo = nlo, hi = nhi, reach = nr;
+    }
+    // sub-ranges that reach it, then their logits that do
+#pragma unroll
+    for (int u = 0; u < SUB_REGS; u++)
+        if (mine[u] >= lo && tid + PNT * u < n_sub) {
+            const int x = atomicAdd(&s_ns, 1);
+            if (x < PNT) s_subs[x] = tid + PNT * u;
+        }
+    __syncthreads();
+    const int ns = s_ns;
+    if (ns <= PNT) {
+        for (int i = tid; i < ns * E; i += PNT) {
+            const int at = sub_index<E, VEC>(s_subs[i / E], i % E);
+            if (at >= V) continue;
+            const uint32_t key = logit_key(clean_logit(l[at]));
+            if (key >= lo) {
+                const int x = atomicAdd(&s_n, 1);
+                if (x < LIST) s_list[x] = (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)at);
+            }
+        }
+    }
+    __syncthreads();
+    const int n = s_n;
+    if (ns > PNT || n > LIST || n < k) {  // (n < k: fewer logits than sub-ranges' places)
+        radix_select(a, l, r.m, sh, &a.sel[row]);
+        return;
+    }
+    rank_sort(s_list, s_sorted, n);
+    keep_prefix(a, s_sorted, min(n, k), r.m, a.top_p > 0.f && a.top_p < 1.f, 0,
+                [&](unsigned long long z) { return nucleus_need(z, a.top_p); }, s_w, &a.sel[row]);
+}
+
+// ---- nucleus of the whole row: bin of a logit by its distance from the largest, up to 32 T or the smallest
+__device__ __forceinline__ float bin_scale(const RowStats& r, float T) {
+    const float d = fminf((r.m - r.least) / T, 32.f);
+    return (float)(BINS - 1) / (fmaxf(d, 1e-30f) * T);
+}
+__device__ __forceinline__ int bin_of(float l, float m, float scale) {  // monotone in l
+    return l == m ? 0 : (int)fminf((m - l) * scale, (float)(BINS - 1));
+}
+// whether rows of infinities, or of T that leaves the range, have bins at all
+__device__ __forceinline__ bool has_bins(const RowStats& r, float scale) {
+    return r.m < INFINITY && scale > 0.f && scale < INFINITY;
+}
+
+template <int E, bool VEC>
+__global__ __launch_bounds__(STH) void probs_bins_kernel(ProbsArgs a, int per_wg) {
+    __shared__ unsigned long long s_bin[BINS];
+    const int row = blockIdx.y, tid = threadIdx.x;
+    const RowStats r = row_stats(a, row);
+    const float scale = bin_scale(r, a.T);
+    if (r.m == -INFINITY || !has_bins(r, scale)) return;
+    for (int i = tid; i < BINS; i += STH) s_bin[i] = 0;
+    __syncthreads();
+    const double unit = weight_unit(a.V);
+    const int s1 = min(a.S, ((int)blockIdx.x + 1) * per_wg);
+    for (int split = blockIdx.x * per_wg; split < s1; split++) {
+        float v[E];
+        load_split<E, VEC>(a.logits + (size_t)row * a.V, a.V, split, v);
+#pragma unroll 4
+        for (int u = 0; u < E; u++) {
+            const float x = clean_logit(v[u]);
+            if (x > -INFINITY) atomicAdd(&s_bin[bin_of(x, r.m, scale)], weigh(x, r.m, a.T, unit));
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < BINS; i += STH)
+        if (s_bin[i]) atomicAdd(&a.bins[(size_t)row * BINS + i], s_bin[i]);
+}
+
+// the bin in which the nucleus ends, the weight ahead of it and the weight needed, from a row's bins, by a
+// workgroup of NT threads (s_w: a word for each thread)
+struct Border {
+    int bin;
+    unsigned long long above, need;
+};
+template <int NT>
+__device__ Border find_border(const ProbsArgs& a, int row, unsigned long long* s_w, Border* s_b) {
+    constexpr int PER = BINS / NT;
+    const int tid = threadIdx.x;
+    unsigned long long x[PER], w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        x[i] = a.bins[(size_t)row * BINS + tid * PER + i];
+        w += x[i];
+    }
+    s_w[tid] = w;
+    __syncthreads();
+    for (int o = 1; o < NT; o <<= 1) {
+        const unsigned long long y = tid >= o ? s_w[tid - o] : 0;
+        __syncthreads();
+        s_w[tid] += y;
+        __syncthreads();
+    }
+    const unsigned long long need = nucleus_need(s_w[NT - 1], a.top_p);
+    unsigned long long sum = s_w[tid] - w;
+    if (sum < need && sum + w >= need) {
+        int i = 0;
+        for (; i + 1 < PER && sum + x[i] < need; i++) sum += x[i];
+        *s_b = Border{tid * PER + i, sum, need};
+    }
+    __syncthreads();
+    return *s_b;
+}
+
+template <int E, bool VEC>
+__global__ __launch_bounds__(STH) void probs_gather_kernel(ProbsArgs a) {
+    __shared__ unsigned long long s_w[STH];
+    __shared__ Border s_b;
+    const int split = blockIdx.x, row = blockIdx.y;
+    float v[E];
+    load_split<E, VEC>(a.logits + (size_t)row * a.V, a.V, split, v);
+    const RowStats r = row_stats(a, row);
+    const float scale = bin_scale(r, a.T);
+    if (r.m == -INFINITY || !has_bins(r, scale)) return;
+    const Border b = find_border<STH>(a, row, s_w, &s_b);
+#pragma unroll
+    for (int u = 0; u < E; u++) {
+        const float x = clean_logit(v[u]);
+        if (x > -INFINITY && bin_of(x, r.m, scale) == b.bin) {
+            const int at = atomicAdd(&a.count[row], 1);
+            if (at < LIST)
+                a.list[(size_t)row * LIST + at] =
+                    (unsigned long long)logit_key(x) << 32 | (0xFFFFFFFFu - (uint32_t)split_index<E, VEC>(split, u));
+        }
+    }
+}
+
+__global__ __launch_bounds__(PNT) void probs_border_kernel(ProbsArgs a) {
+    __shared__ RadixShared sh;
+    __shared__ unsigned long long s_list[LIST], s_sorted[LIST], s_w[PNT];
+    __shared__ Border s_b;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const RowStats r = row_stats(a, row);
+    if (r.m == -INFINITY) return;
+    const int n = a.count[row];
+    if (!has_bins(r, bin_scale(r, a.T)) || n > LIST) {
+        radix_select(a, a.logits + (size_t)row * a.V, r.m, sh, &a.sel[row]);
+        return;
+    }
+    const Border b = find_border<PNT>(a, row, s_w, &s_b);
+    for (int i = tid; i < n; i += PNT) s_list[i] = a.list[(size_t)row * LIST + i];
+    __syncthreads();
+    rank_sort(s_list, s_sorted, n);
+    keep_prefix(a, s_sorted, n, r.m, true, b.above, [&](unsigned long long) { return b.need; }, s_w, &a.sel[row]);
+}
+
+// ---- the probabilities
+enum : int { WRITE_ALL = 0, WRITE_SEL = 1, WRITE_FIRST = 2 };  // no cut, the selection's, temperature 0
+
+template <int E, bool VEC>
+__global__ __launch_bounds__(STH) void probs_write_kernel(ProbsArgs a, int what) {
+    const int split = blockIdx.x, row = blockIdx.y;
+    float v[E];
+    load_split<E, VEC>(a.logits + (size_t)row * a.V, a.V, split, v);
+    const RowStats r = row_stats(a, row);
+    float* p = a.probs + (size_t)row * a.V;
+    RowSel sel{0.0, r.m, 0u, a.V};
+    if (what == WRITE_SEL && r.m > -INFINITY) sel = a.sel[row];
+    const float inv = (float)(what == WRITE_SEL ? sel.inv : 1.0 / r.s);
+    const Weight32 weight(r.m, a.T);
+#pragma unroll
+    for (int u = 0; u < E; u++) {
+        const int i = split_index<E, VEC>(split, u);
+        const float x = clean_logit(v[u]);
+        const uint32_t k = logit_key(x);
+        const bool in = what == WRITE_FIRST ? i == r.mi : k > sel.key || (k == sel.key && i < sel.cut);
+        v[u] = !in || r.m == -INFINITY ? 0.f : what == WRITE_FIRST ? 1.f : weight(x) * inv;
+    }
+    if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < E / 4; j++) {
+            const int i = split_index<E, VEC>(split, 4 * j);
+            if (i < a.V) *(float4*)(p + i) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < E; u++) {
+            const int i = split_index<E, VEC>(split, u);
+            if (i < a.V) p[i] = v[u];
+        }
+    }
+}
+
+// Logits of a thread's sub-range: 32 where that still gives every CU a workgroup, else 8 (4 rows x 49152:
+// 24 workgroups of 32, 96 of 8).
+static int probs_e(int rows, int V) { return V >= 65536 && (long long)rows * V >= 256ll * STH * 32 ? 32 : 8; }
+static int probs_splits(int rows, int V) {
+    const int e = STH * probs_e(rows, V);
+    return (V + e - 1) / e;
+}
+struct ProbsSizes {
+    size_t stats, sub, bins, list, count, sel;
+};
+static ProbsSizes probs_sizes(int rows, int V) {
+    const size_t S = probs_splits(rows, V), n = rows;
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    return ProbsSizes{up(n * S * sizeof(SplitStats)), up(n * S * STH * 4), up(n * BINS * 8), up(n * LIST * 8),
+                      up(n * 4), up(n * sizeof(RowSel))};
+}
 size_t sample_probs_workspace_bytes(int rows, int V) {
-    (void)rows;
-    (void)V;
-    return 16;
+    const ProbsSizes z = probs_sizes(rows, V);
+    return z.stats + z.sub + z.bins + z.list + z.count + z.sel;
 }
 
 int launch_sample_probs(float* logits, int rows, int V, const qraf_sampling_params& sp, const uint32_t* recent,
                         const int32_t* counts, int stride, float* probs, void* ws, size_t ws_bytes, hipStream_t s) {
     QH_REQUIRE(logits && probs && ws && rows > 0 && V > 0, QRAF_HIP_ERR_INVALID, "sample_probs: bad arguments");
+    QH_REQUIRE(V <= 1 << 30, QRAF_HIP_ERR_INVALID, "sample_probs: vocabulary %d over 2^30", V);
+    QH_REQUIRE(rows <= 65535, QRAF_HIP_ERR_INVALID, "sample_probs: %d rows over 65535", rows);
     QH_REQUIRE(ws_bytes >= sample_probs_workspace_bytes(rows, V), QRAF_HIP_ERR_INVALID,
                "sample_probs: workspace of %zu bytes, %zu needed", ws_bytes, sample_probs_workspace_bytes(rows, V));
     QH_TRY(launch_penalty(logits, rows, V, sp.repetition_penalty, recent, counts, stride, s));
-    const int cutoff = (sp.top_k > 0 && sp.top_k < V) ? sp.top_k : V;
-    hipLaunchKernelGGL(probs_rows_kernel, dim3(rows), dim3(PNT), 0, s, logits, V, sp.temperature, cutoff, sp.top_p,
-                       probs);
+    const ProbsSizes z = probs_sizes(rows, V);
+    ProbsArgs a{};
+    a.logits = logits;
+    a.probs = probs;
+    uint8_t* w = (uint8_t*)ws;
+    a.stats = (SplitStats*)w;
+    a.sub = (float*)(w += z.stats);
+    a.bins = (unsigned long long*)(w += z.sub);
+    a.list = (unsigned long long*)(w += z.bins);
+    a.count = (int*)(w += z.list);
+    a.sel = (RowSel*)(w += z.count);
+    a.V = V;
+    a.S = probs_splits(rows, V);
+    a.cutoff = (sp.top_k > 0 && sp.top_k < V) ? sp.top_k : V;
+    a.T = sp.temperature;
+    a.top_p = sp.top_p;
+    const bool greedy = !(sp.temperature > 0.f), cut_p = sp.top_p > 0.f && sp.top_p < 1.f;
+    const bool cuts = !greedy && (a.cutoff < V || cut_p);
+    const bool topk = cuts && a.cutoff < V && a.cutoff <= TOPK_MAX && a.S * STH <= SUB_REGS * PNT;
+    const bool bins = cuts && a.cutoff == V;
+    const bool vec = V % 4 == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)probs & 15) == 0;
+    const int e = probs_e(rows, V);
+    const dim3 grid(a.S, rows);
+#define QH_PROBS(Ev, Vv)                                                                                            \
+    if (e == Ev && vec == Vv) {                                                                                     \
+        hipLaunchKernelGGL((probs_stats_kernel<Ev, Vv>), grid, dim3(STH), 0, s, a,                                  \
+                           topk ? STATS_SUB : bins ? STATS_BINS : STATS_SUM);                                       \
+        if (topk) {                                                                                                 \
+            hipLaunchKernelGGL((probs_topk_kernel<Ev, Vv>), dim3(rows), dim3(PNT), 0, s, a);                        \
+        } else if (bins) {                                                                                          \
+            const int per = std::max(1, a.S * rows / 1024); /* splits of a workgroup, which has bins of its own */  \
+            hipLaunchKernelGGL((probs_bins_kernel<Ev, Vv>), dim3((a.S + per - 1) / per, rows), dim3(STH), 0, s, a, per); \
+            hipLaunchKernelGGL((probs_gather_kernel<Ev, Vv>), grid, dim3(STH), 0, s, a);                            \
+            hipLaunchKernelGGL(probs_border_kernel, dim3(rows), dim3(PNT), 0, s, a);                                \
+        } else if (cuts) {                                                                                          \
+            hipLaunchKernelGGL(probs_radix_kernel, dim3(rows), dim3(PNT), 0, s, a);                                 \
+        }                                                                                                           \
+        hipLaunchKernelGGL((probs_write_kernel<Ev, Vv>), grid, dim3(STH), 0, s, a,                                  \
+                           greedy ? WRITE_FIRST : cuts ? WRITE_SEL : WRITE_ALL);                                    \
+    }
+    QH_PROBS(8, true) QH_PROBS(8, false) QH_PROBS(32, true) QH_PROBS(32, false)
+#undef QH_PROBS
     QH_CHECK_HIP(hipGetLastError());
     return QRAF_HIP_OK;
 }
