@@ -899,7 +899,7 @@ __device__ __forceinline__ void draw_weights(const VerifyArgs& a, size_t r, bool
 
 // sums of a split of STH x E tokens of each sequence's deciding row
 template <int E, bool VEC>
-__global__ __launch_bounds__(STH) void verify_sums_kernel(VerifyArgs a, double2* part) {
+__global__ __launch_bounds__(STH) void verify_sums_kernel(VerifyArgs a, double2* part, int* decides) {
     __shared__ double s_less[4], s_p[4];
     const int split = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     int r0, r1;
@@ -930,6 +930,7 @@ __global__ __launch_bounds__(STH) void verify_sums_kernel(VerifyArgs a, double2*
         s_p[tid >> 6] = sp;
     }
     __syncthreads();
+    if (tid == 0 && split == 0) decides[s] = r;
     if (tid == 0)
         part[(size_t)s * gridDim.x + split] =
             make_double2((s_less[0] + s_less[1]) + (s_less[2] + s_less[3]), (s_p[0] + s_p[1]) + (s_p[2] + s_p[3]));
@@ -943,7 +944,6 @@ __device__ __forceinline__ double block_scan(double w, double* s_w, double& all)
         const double x = __shfl_up(w, o);
         w += lane >= o ? x : 0.0;
     }
-    __syncthreads();
     if (lane == 63) s_w[wave] = w;
     __syncthreads();
     double before = 0.0;
@@ -956,12 +956,30 @@ __device__ __forceinline__ double block_scan(double w, double* s_w, double& all)
     return before + w;
 }
 
-// The draw: the split in which the running sum passes it, then the token; a workgroup for each sequence.  (A sum
-// rounds otherwise here than there: where none passes, the last with any weight.)
+// The first of a workgroup's threads whose inclusive sum passes the target, else the last that adds anything (a sum
+// rounds otherwise here than where the target was formed): -1 where none does.  (s_t: two words for each wave)
+__device__ __forceinline__ int passing_thread(double inc, double w, double target, int (*s_t)[2]) {
+    const int wave = threadIdx.x >> 6;
+    const unsigned long long pass = __ballot(w > 0.0 && inc > target), any = __ballot(w > 0.0);
+    if ((threadIdx.x & 63) == 0) {
+        s_t[wave][0] = pass ? 64 * wave + __builtin_ctzll(pass) : -1;
+        s_t[wave][1] = any ? 64 * wave + 63 - __builtin_clzll(any) : -1;
+    }
+    __syncthreads();
+    int first = -1, last = -1;
+#pragma unroll
+    for (int v = STH / 64 - 1; v >= 0; v--) {
+        first = s_t[v][0] >= 0 ? s_t[v][0] : first;
+        last = max(last, s_t[v][1]);
+    }
+    return first >= 0 ? first : last;
+}
+
+// The draw: the split in which the running sum passes it, then the token; a workgroup for each sequence
 template <int E, bool VEC>
-__global__ __launch_bounds__(STH) void verify_pick_kernel(VerifyArgs a, const double2* part, int S) {
-    __shared__ double s_w[STH / 64];
-    __shared__ int s_first, s_last;
+__global__ __launch_bounds__(STH) void verify_pick_kernel(VerifyArgs a, const double2* part, const int* decides, int S) {
+    __shared__ double s_w[2][STH / 64], s_ahead;
+    __shared__ int s_t[2][STH / 64][2], s_split, s_token;
     const int s = blockIdx.x, tid = threadIdx.x;
     int r0, r1;
     rows_of(a, s, r0, r1);
@@ -969,76 +987,58 @@ __global__ __launch_bounds__(STH) void verify_pick_kernel(VerifyArgs a, const do
         if (tid == 0) a.accepted[s] = 0;
         return;
     }
-    const int r = rejecting_row(a, r0, r1);
+    const int r = decides[s];
+    const uint32_t draft = a.draft[r];
     const double2* mine = part + (size_t)s * S;
-    double all = 0.0, all_p = 0.0;
-    for (int i = tid; i < S; i += STH) {
-        all += mine[i].x;
-        all_p += mine[i].y;
+    const int per = (S + STH - 1) / STH, i0 = min(S, tid * per), i1 = min(S, i0 + per);
+    double w = 0.0, w_p = 0.0, all;
+    for (int i = i0; i < i1; i++) {
+        w += mine[i].x;
+        w_p += mine[i].y;
     }
-    block_scan(all, s_w, all);
-    block_scan(all_p, s_w, all_p);
+    double inc = block_scan(w, s_w[0], all);
     const bool left = all > 0.0;  // else nothing is left of p: the target's own distribution
-    const bool missed = left && r < r1 - 1;
-    all = left ? all : all_p;
+    if (!left) {
+        w = w_p;
+        inc = block_scan(w, s_w[1], all);
+    }
     // a draw outside [0, 1) (or NaN) takes the nearest inside
     const double target = (double)fminf(fmaxf(a.v[s], 0.f), 0x1.fffffep-1f) * all;
-    auto pick = [&](int n, double before, auto weight) {  // in [0, n): the first whose sum passes, else the last of any weight
-        if (tid == 0) {
-            s_first = n;
-            s_last = 0;
-        }
-        const int per = (n + STH - 1) / STH, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-        double w = 0.0, sum;
-        for (int i = i0; i < i1; i++) w += weight(i);
-        double c = before + (block_scan(w, s_w, sum) - w);
-        for (int i = i0; i < i1; i++) {
-            const double x = weight(i);
+    if (tid == max(0, passing_thread(inc, w, target, s_t[0]))) {  // among the thread's splits
+        double c = inc - w;
+        int i = i0;
+        for (; i + 1 < i1; i++) {
+            const double x = left ? mine[i].x : mine[i].y;
+            if (c + x > target) break;
             c += x;
-            if (x > 0.0) {
-                atomicMax(&s_last, i);
-                if (c > target) {
-                    atomicMin(&s_first, i);
-                    break;
-                }
-            }
         }
-        __syncthreads();
-        return s_first < n ? s_first : s_last;
-    };
-    const int split = pick(S, 0.0, [&](int i) { return left ? mine[i].x : mine[i].y; });
-    // the sum ahead of the split, as its sums add up
-    double ahead = 0.0;
-    for (int i = tid; i < split; i += STH) ahead += left ? mine[i].x : mine[i].y;
-    block_scan(ahead, s_w, ahead);
+        s_split = i;
+        s_ahead = c;
+    }
+    __syncthreads();
+    const int split = min(s_split, S - 1);
     float p[E];
-    double less[E];
-    draw_weights<E, VEC>(a, r, missed, a.draft[r], split * STH * E + tid * E, p, less);
-    double w = 0.0, sum;
+    double less[E], sum;
+    draw_weights<E, VEC>(a, r, left && r < r1 - 1, draft, split * STH * E + tid * E, p, less);
+    w = 0.0;
 #pragma unroll
     for (int u = 0; u < E; u++) w += less[u];
-    if (tid == 0) {
-        s_first = STH * E;
-        s_last = 0;
-    }
-    double c = ahead + (block_scan(w, s_w, sum) - w);
-    int first = STH * E, last = 0;
+    double c = s_ahead + (block_scan(w, s_w[1], sum) - w);
+    if (tid == max(0, passing_thread(c + w, w, target, s_t[1]))) {
+        int first = -1, last = 0;
 #pragma unroll
-    for (int u = 0; u < E; u++) {
-        c += less[u];
-        if (less[u] > 0.0) {
-            last = tid * E + u;
-            if (c > target) first = min(first, tid * E + u);
+        for (int u = 0; u < E; u++) {
+            c += less[u];
+            last = less[u] > 0.0 ? u : last;
+            first = first < 0 && less[u] > 0.0 && c > target ? u : first;
         }
+        s_token = split * STH * E + tid * E + (first >= 0 ? first : last);
     }
-    if (first < STH * E) atomicMin(&s_first, first);
-    if (last) atomicMax(&s_last, last);
     __syncthreads();
     if (tid == 0) {
-        const int at = split * STH * E + (s_first < STH * E ? s_first : s_last);
         a.accepted[s] = r - r0;
         for (int i = r0; i < r; i++) a.tokens[i] = a.draft[i];
-        a.tokens[r] = at < a.V && all > 0.0 ? (uint32_t)at : 0u;
+        a.tokens[r] = s_token < a.V && all > 0.0 ? (uint32_t)s_token : 0u;
         for (int i = r + 1; i < r1; i++) a.tokens[i] = 0xFFFFFFFFu;
     }
 }
@@ -1050,7 +1050,9 @@ static int verify_splits(int n, int V) {
     return (V + e - 1) / e;
 }
 
-size_t verify_draft_workspace_bytes(int n, int V) { return (size_t)n * verify_splits(n, V) * sizeof(double2); }
+size_t verify_draft_workspace_bytes(int n, int V) {
+    return (size_t)n * verify_splits(n, V) * sizeof(double2) + (size_t)n * sizeof(int);
+}
 
 int launch_verify_draft(const float* probs, const float* draft_probs, const uint32_t* draft_tokens,
                         const int32_t* row_starts, int n, int n_rows, int V, const float* accept_uniforms,
@@ -1068,10 +1070,12 @@ int launch_verify_draft(const float* probs, const float* draft_probs, const uint
                        accepted, tokens, n, n_rows, V};
     const bool vec = V % 4 == 0 && ((uintptr_t)probs & 15) == 0 && ((uintptr_t)draft_probs & 15) == 0;
     const int e = verify_e(n, V), S = verify_splits(n, V);
+    double2* part = (double2*)ws;
+    int* decides = (int*)(part + (size_t)n * S);
 #define QH_VERIFY(Ev, Vv)                                                                                               \
     if (e == Ev && vec == Vv) {                                                                                         \
-        hipLaunchKernelGGL((verify_sums_kernel<Ev, Vv>), dim3(S, n), dim3(STH), 0, s, a, (double2*)ws);                 \
-        hipLaunchKernelGGL((verify_pick_kernel<Ev, Vv>), dim3(n), dim3(STH), 0, s, a, (const double2*)ws, S);           \
+        hipLaunchKernelGGL((verify_sums_kernel<Ev, Vv>), dim3(S, n), dim3(STH), 0, s, a, part, decides);                \
+        hipLaunchKernelGGL((verify_pick_kernel<Ev, Vv>), dim3(n), dim3(STH), 0, s, a, part, decides, S);                \
     }
     QH_VERIFY(8, true) QH_VERIFY(8, false) QH_VERIFY(32, true) QH_VERIFY(32, false)
 #undef QH_VERIFY
