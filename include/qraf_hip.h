@@ -239,12 +239,15 @@ uint64_t qraf_hip_attention_noalloc_max_bytes(void);
  * rows of one sequence in one step (drafted tokens, a prompt chunk) are a group
  * whose prefix is its whole cache, each row with its own ctx.  prefix 0 is plain
  * attention.  Rows outside every group are left as they were.
- * n_rows 1..1024, n_groups 1..n_rows; head_dim 16, 32, 64 or 128, any page_size
- * and any number of query heads per KV head.  The workspace (qraf_hip_group_attention_workspace_bytes, 16-byte
- * aligned) needs no initialisation; calls that share one must not overlap.
+ * n_rows 1..1024, n_groups 1..n_rows, max_ctx up to 2^30; head_dim 16, 32, 64
+ * or 128, any page_size and any number of query heads per KV head.  q, the
+ * caches, out and the workspace are 16-byte aligned.  The workspace
+ * (qraf_hip_group_attention_workspace_bytes) needs no initialisation; calls that
+ * share one must not overlap.
  * Results are within the attention tolerance of qraf_hip_paged_attention_dev's
- * on the same rows, and the same from call to call.  An infinity or NaN in the
- * K or V of a position reaches the rows that attend to it and no others.
+ * on the same rows, and the same from call to call; weights below 2^-37 of a
+ * row's largest may count as zero.  An infinity or NaN in the K or V of a
+ * position reaches the rows that attend to it and no others.
  * No counterpart in the reference, which runs one sequence at a time. */
 uint64_t qraf_hip_group_attention_workspace_bytes(int32_t n_rows, int32_t n_groups, int32_t n_heads,
                                                   int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx);
@@ -457,8 +460,9 @@ int qraf_hip_sample_dev(float* logits, int32_t rows, int32_t vocab, const qraf_s
                         const float* uniforms, uint32_t* tokens, void* stream);
 
 /* The distribution that qraf_hip_sample_dev draws from, as probabilities:
- * probs [rows][vocab] (may be logits itself) from logits [rows][vocab], for
- * verification against a draft (below).  With 64-bit weights w_i = exp((l_i -
+ * probs [rows][vocab] (logits itself, or not overlapping it) from logits
+ * [rows][vocab], rows up to 65535 and vocab up to 2^30, for verification against
+ * a draft (below).  With 64-bit weights w_i = exp((l_i -
  * max) / T): of the top_k largest logits (all when top_k <= 0 or >= vocab;
  * equal logits in index order) the shortest prefix whose weight reaches top_p
  * times theirs (all of them unless 0 < top_p < 1), w_i over their sum; 0 elsewhere.
@@ -494,7 +498,8 @@ int qraf_hip_sample_probs_dev(float* logits, int32_t rows, int32_t vocab, const 
  * target's own samples.
  *   accepted [n_seqs] drafts accepted;  tokens [n_rows]: at row_starts[s] the
  *   accepted drafts, then the next token, then 0xFFFFFFFF up to the last row.
- * A sequence without rows has accepted 0.  Workspace as above
+ * A sequence without rows has accepted 0; rows of no sequence get no tokens.
+ * n_seqs up to 65535, vocab up to 2^30.  Workspace as above
  * (qraf_hip_verify_draft_workspace_bytes).  No counterpart in the reference. */
 uint64_t qraf_hip_verify_draft_workspace_bytes(int32_t n_seqs, int32_t vocab);
 int qraf_hip_verify_draft_dev(const float* probs, const float* draft_probs, const uint32_t* draft_tokens,
@@ -585,6 +590,31 @@ int qraf_engine_set_keep_logits(qraf_engine* engine, int32_t keep);
 int qraf_engine_sample(qraf_engine* engine, int32_t row0, int32_t rows, const qraf_sampling_params* params,
                        const uint32_t* recent, const int32_t* recent_count, int32_t recent_stride,
                        const float* uniforms, uint32_t* tokens);
+/* qraf_hip_sample_probs_dev on the last step's logit rows where they lie in HBM
+ * (row0, rows, params and the host arrays of a repetition penalty as for
+ * qraf_engine_sample): their distributions to probs [rows][vocab], the caller's
+ * device memory, complete on return.  A repetition penalty changes the logit
+ * rows in place, so a further call on them passes 1.  What a draft model gives
+ * its target's qraf_engine_verify beside the tokens.  No reference counterpart. */
+int qraf_engine_probs(qraf_engine* engine, int32_t row0, int32_t rows, const qraf_sampling_params* params,
+                      const uint32_t* recent, const int32_t* recent_count, int32_t recent_stride, float* probs);
+/* Verification of drafted tokens on the last step's logit rows
+ * (qraf_hip_sample_probs_dev, then qraf_hip_verify_draft_dev).  Sequence i, of k
+ * drafted tokens, fed k + 1 rows in the step that asked for their logits: its
+ * last token and the drafts; row_counts [n_seqs] are those k + 1, and the rows
+ * lie one sequence behind another from logit row row0 on.  draft_tokens [rows]:
+ * the draft behind each row (a sequence's last row: any token); draft_probs
+ * [rows][vocab] on the device, or NULL; uniforms on the host (NULL when greedy:
+ * drafts are accepted while they are the argmax).  recent, recent_count and
+ * recent_stride [rows]: a row's history holds the drafts ahead of it.  accepted
+ * [n_seqs] and tokens [rows] as there.  The sequence's next step begins at the
+ * position behind its accepted drafts: feeding a position again overwrites it.
+ * No reference counterpart. */
+int qraf_engine_verify(qraf_engine* engine, int32_t row0, int32_t n_seqs, const int32_t* row_counts,
+                       const qraf_sampling_params* params, const uint32_t* recent, const int32_t* recent_count,
+                       int32_t recent_stride, const uint32_t* draft_tokens, const float* draft_probs,
+                       const float* accept_uniforms, const float* pick_uniforms, int32_t* accepted,
+                       uint32_t* tokens);
 /* The last step's logit rows row0 .. row0+rows-1 (the rows it returned
  * logits or argmax for, in order) copied from HBM to out [rows][vocab]: a
  * step can keep its logits on the device and a caller read back only the
@@ -625,8 +655,11 @@ int qraf_engine_set_row_padding(qraf_engine* engine, int32_t rows);
  * split, GEMM and reduction launches) on it, with the RMSNorm / SiLU-gate
  * formed in its staging; when the QKV and O projections qualify, the layer
  * runs projection by projection instead of as the split-K GEMM layer (fp32
- * products as at batch 1, summed in another order than the GEMM's).  No
- * reference counterpart (launch-count and traffic measures). */
+ * products as at batch 1, summed in another order than the GEMM's); bit 3
+ * (default off) = in steps that hold several rows of a sequence one behind
+ * another (drafted tokens, prompt chunks) attention reads the positions that
+ * those share once (qraf_hip_group_attention_dev: the same sums in another
+ * order).  No reference counterpart (launch-count and traffic measures). */
 int qraf_engine_set_fusion(qraf_engine* engine, int32_t flags);
 /* Repetition penalty on the device for one sequence, set before its first
  * step (QRAF_HIP_ERR_STATE after): from then on every token the sequence is

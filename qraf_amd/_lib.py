@@ -133,6 +133,9 @@ SIGNATURES.update({
     "qraf_hip_verify_draft_dev": (C.c_int, [vp, vp, vp, vp] + [C.c_int32] * 3 + [vp, vp, vp, vp, vp, C.c_uint64, vp]),
     "qraf_engine_sample": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), u32p, i32p, C.c_int32, fp,
                                      u32p]),
+    "qraf_engine_probs": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), u32p, i32p, C.c_int32, vp]),
+    "qraf_engine_verify": (C.c_int, [vp, C.c_int32, C.c_int32, i32p, C.POINTER(SamplingParams), u32p, i32p, C.c_int32,
+                                     u32p, vp, fp, fp, i32p, u32p]),
     "qraf_engine_create": (C.c_int, [C.POINTER(ModelConfig), C.POINTER(EngineOptions), C.POINTER(vp)]),
     "qraf_engine_destroy": (C.c_int, [vp]),
     "qraf_engine_set_tensor": (C.c_int, [vp, C.c_char_p, C.c_uint32, C.c_uint32, u32p, C.c_uint32, vp, C.c_uint64]),

@@ -33,7 +33,8 @@ struct GroupArgs {
     const int32_t* ctx;         // [n] positions attended
     const int32_t* starts;      // [groups + 1]
     const int32_t* prefix;      // [groups]
-    float* out;                 // [n][H][HD]
+    float* out;                 // [n][H][HD], or (out_hi != null) the planes a GEMM reads (qraf_hip_split_bf16_dev)
+    uint16_t *out_hi, *out_lo;
     float* part_o;              // [Hkv][slots][HD] unnormalised outputs of parts
     float2* part_ml;            // [Hkv][slots] their maxima (in powers of two) and sums
     int* plan;                  // for the merge: prefix jobs, {column, which parts} of each row, pieces of the jobs
@@ -43,6 +44,25 @@ struct GroupArgs {
     int tail_rows, tails;       // rows of a tail job; tail jobs
     long long slots;            // part slots of a KV head
 };
+
+// output elements i .. i + 3, i
+__device__ __forceinline__ void group_store4(const GroupArgs& a, size_t i, float4 v) {
+    if (a.out_hi) {
+        ushort4 h, l;
+        split_bf16(v.x, &h.x, &l.x);
+        split_bf16(v.y, &h.y, &l.y);
+        split_bf16(v.z, &h.z, &l.z);
+        split_bf16(v.w, &h.w, &l.w);
+        *(ushort4*)(a.out_hi + i) = h;
+        *(ushort4*)(a.out_lo + i) = l;
+    } else {
+        *(float4*)(a.out + i) = v;
+    }
+}
+__device__ __forceinline__ void group_store(const GroupArgs& a, size_t i, float v) {
+    if (a.out_hi) split_bf16(v, &a.out_hi[i], &a.out_lo[i]);
+    else a.out[i] = v;
+}
 
 // entries of the device-resident layout, taken into their ranges
 __device__ __forceinline__ int group_start(const GroupArgs& a, int g) { return max(0, min(a.starts[g], a.n)); }
@@ -165,7 +185,7 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
             O = __builtin_fmaf(s_o[w][d], e, O);
             L = __builtin_fmaf(s_l[w], e, L);
         }
-        a.out[base + d] = ctx ? O / L : 0.f;
+        group_store(a, base + d, ctx ? O / L : 0.f);
     }
 }
 
@@ -441,7 +461,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
     extern __shared__ __align__(16) float s_dyn[];
     __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK], s_qs[BLK];
-    __shared__ float* s_to[BLK];
+    __shared__ long long s_to[BLK];  // where a column's output goes: an element of out, or ~ one of part_o
+    constexpr long long NOWHERE = 1ll << 62;
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
     // c ^ (column % 16), which spreads a wave's writes over the banks
     float* s_o = s_dyn;
@@ -939,7 +960,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab +
                                 (size_t)BLK * ((here & 0xFFFF) - (here >> 16) + i_of);
             const bool mine = col < cols, part = mine && !alone && (tail || any_pre);
-            s_to[qt * 32 + col] = mine && alone ? a.out + (qrow - a.q) : part ? a.part_o + slot * HD : nullptr;
+            s_to[qt * 32 + col] = mine && alone ? (long long)(qrow - a.q) : part ? ~(long long)(slot * HD) : NOWHERE;
             s_by[qt * 32 + col] = alone ? 1.f / L : 1.f;
             if (part) a.part_ml[slot] = make_float2(M, L);
         }
@@ -950,8 +971,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll 2
             for (int e = tid; e < WQ * 32 * (HD / 4); e += GTH) {
                 const int c = e / (HD / 4), d = e % (HD / 4) * 4, cq = c >> 5, ci = c & 31;
-                float* to = s_to[c];
-                if (!to) continue;
+                const long long to = s_to[c];
+                if (to == NOWHERE) continue;
                 float4 x[WK];
                 float f[WK];
 #pragma unroll
@@ -968,7 +989,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     O.w = __builtin_fmaf(x[k].w, f[k], O.w);
                 }
                 const float by = s_by[c];
-                *(float4*)(to + d) = make_float4(O.x * by, O.y * by, O.z * by, O.w * by);
+                O = make_float4(O.x * by, O.y * by, O.z * by, O.w * by);
+                if (to < 0) *(float4*)(a.part_o + ~to + d) = O;
+                else group_store4(a, to + d, O);
             }
         };
         if (wk == 2) join(std::integral_constant<int, 2>());
@@ -999,10 +1022,10 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
         count[k] = which >> k & 1 ? (y & 0xFFFF) - (x & 0xFFFF) : 0;
     }
     const int all = count[0] + count[1];
-    float* out = a.out + ((size_t)r * a.H + h) * HD;
+    const size_t out = ((size_t)r * a.H + h) * HD;
     if (all == 0) {
 #pragma unroll
-        for (int k = 0; k < DPL; k++) out[lane + 64 * k] = 0.f;
+        for (int k = 0; k < DPL; k++) group_store(a, out + lane + 64 * k, 0.f);
         return;
     }
     if (all == 1) return;
@@ -1041,7 +1064,7 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
         m = mn;
     }
 #pragma unroll
-    for (int k = 0; k < DPL; k++) out[lane + 64 * k] = O[k] / l;
+    for (int k = 0; k < DPL; k++) group_store(a, out + lane + 64 * k, O[k] / l);
 }
 
 // workgroups per KV head: as many as are resident at once, one per CU, whose
@@ -1096,9 +1119,12 @@ size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd
 int launch_group_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype,
                            const int32_t* page_table, int max_pages, const int32_t* ctx, const int32_t* group_starts,
                            const int32_t* prefix, int n, int groups, int H, int Hkv, int hd, int page_size, float scale,
-                           int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st) {
-    QH_REQUIRE(q && kc && vc && page_table && ctx && group_starts && prefix && out && ws, QRAF_HIP_ERR_INVALID,
-               "group attention: null pointer");
+                           int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st, uint16_t* out_hi,
+                           uint16_t* out_lo) {
+    QH_REQUIRE(q && kc && vc && page_table && ctx && group_starts && prefix && (out || (out_hi && out_lo)) && ws,
+               QRAF_HIP_ERR_INVALID, "group attention: null pointer");
+    QH_REQUIRE((((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)out | (uintptr_t)ws) & 15) == 0,
+               QRAF_HIP_ERR_INVALID, "group attention: q, caches, out and workspace must be 16-byte aligned");
     QH_REQUIRE(n > 0 && n <= 1024, QRAF_HIP_ERR_INVALID, "group attention: %d rows outside 1..1024", n);
     QH_REQUIRE(groups > 0 && groups <= n, QRAF_HIP_ERR_INVALID, "group attention: %d groups of %d rows", groups, n);
     QH_REQUIRE(Hkv > 0 && H > 0 && H % Hkv == 0, QRAF_HIP_ERR_INVALID,
@@ -1122,6 +1148,8 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
     a.starts = group_starts;
     a.prefix = prefix;
     a.out = out;
+    a.out_hi = out_hi;
+    a.out_lo = out_lo;
     a.n = n;
     a.groups = groups;
     a.H = H;

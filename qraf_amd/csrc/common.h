@@ -225,7 +225,8 @@ size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd
 int launch_group_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype,
                            const int32_t* page_table, int max_pages, const int32_t* ctx, const int32_t* group_starts,
                            const int32_t* prefix, int n, int groups, int H, int Hkv, int hd, int page_size, float scale,
-                           int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st);
+                           int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st,
+                           uint16_t* out_hi = nullptr, uint16_t* out_lo = nullptr);
 int launch_rope_append(const float* qkv, const float* bias, int n, int H, int Hkv, int hd, const int32_t* pos,
                        const float* rope, float* q_out, void* kc, void* vc, uint32_t kv_dtype,
                        const int32_t* page_table, int max_pages, int page_size, hipStream_t st, int S = 1,

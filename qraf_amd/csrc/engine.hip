@@ -442,6 +442,7 @@ struct qraf_engine {
     bool fuse_rope = true;            // one-row steps: RoPE/append fused into the QKV matvec
     bool fuse_swiglu = true;          // steps over 256 rows: SiLU-gate in the gate/up GEMM's epilogue
     bool batch_mv = true;             // steps of 2-8 rows: projections on the multi-vector matvec
+    bool group_rows = false;          // steps with several rows of a sequence: their shared positions read once
     int32_t default_seq = -1;
     int last_logit_rows = 0;          // logit rows the last step left in `logits`
     bool keep_logits = true;          // false: greedy-only steps take the head's argmax without writing logits
@@ -459,6 +460,8 @@ struct qraf_engine {
     int pen_live = 0;                 // sequences with a slot
     uint8_t* samp = nullptr;          // sampling staging: recent tokens, counts, uniforms, tokens
     size_t samp_cap = 0;
+    void* spec = nullptr;             // probabilities: workspace; verification: that, the rows and the small arrays
+    size_t spec_cap = 0;
     void* sort_ws = nullptr;          // sampling sort storage (large top_k, flat whole-vocabulary rows)
     size_t sort_cap = 0;
 
@@ -469,7 +472,7 @@ struct qraf_engine {
     uint16_t *ah = nullptr, *al = nullptr;  // SwiGLU activation planes [max_batch][F] (fused gate/up epilogue)
     uint32_t* amax = nullptr;
     int32_t* d_in = nullptr;  // tokens | positions | ctx | logit rows | token sources | penalty slots | penalties |
-                              // page table rows
+                              // group prefixes | group starts | page table rows
     // Pinned staging, one slot per step in flight: a step's inputs are written
     // into slot `slot` while the previous step (the other slot) may still be
     // queued; its tokens come back into h_amax of the same slot.
@@ -484,6 +487,8 @@ struct qraf_engine {
     int n_pending = 0;
     void* attn_ws = nullptr;
     size_t attn_ws_bytes = 0;
+    void* group_ws = nullptr;  // attention by group (group_rows), allocated when that is first turned on
+    size_t group_ws_bytes = 0;
     void* gemm_ws = nullptr;  // split-K partial tiles of the batched projections
     size_t gemm_ws_bytes = 0;
     float* am_val = nullptr;  // argmax chunk winners [max_batch][32]
@@ -504,6 +509,7 @@ struct qraf_engine {
     struct StepGraph {
         int n = 0, n_logit_rows = 0, ctx = 0;
         int head = 0;  // 0: no head, 1: logits (and argmax), 2: argmax only
+        bool grouped = false;
         uint32_t gen = 0;
         hipGraphExec_t exec = nullptr;
         uint64_t used = 0;
@@ -654,7 +660,7 @@ int qraf_engine_create(const qraf_model_config* cfg, const qraf_engine_options* 
     A(e->am_idx, (size_t)B * ARGMAX_CHUNKS * 4);
     e->am_keys_bytes = qgemm_argmax_keys_bytes((int)V, (int)B);
     A(e->am_keys, e->am_keys_bytes);
-    e->in_words = (size_t)B * (7 + e->max_pages);
+    e->in_words = (size_t)B * (9 + e->max_pages) + 1;
     A(e->d_in, e->in_words * 4);
     e->attn_ws_bytes = attn_workspace_bytes(B, (int)c.num_heads, (int)kvh, hd, e->capacity);
     A(e->attn_ws, e->attn_ws_bytes);
@@ -1093,7 +1099,9 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     int32_t* src = lrows + n_pad;
     int32_t* pslot = src + n_pad;
     float* ppen = (float*)(pslot + n_pad);
-    int32_t* ptab = (int32_t*)(ppen + n_pad);
+    int32_t* gpre = (int32_t*)(ppen + n_pad);
+    int32_t* gstart = gpre + n_pad;
+    int32_t* ptab = gstart + n_pad + 1;
     // the rows' sequences and positions checked, their new pages taken from
     // the pool and their page-table rows written (nothing changes on failure);
     // step_ctx, the longest context of this step, sizes the attention grid
@@ -1121,6 +1129,26 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         ppen[i] = 1.f;
         for (int j = 0; j < MP; j++) ptab[(size_t)i * MP + j] = j == 0 ? e->scratch_page : 0;
     }
+    // Runs of rows of one sequence: a group that shares the positions up to its longest context, whose pages the
+    // group's first row has to name (its own table ends where its position did).  Pad rows are a group, unused
+    // entries empty ones.
+    bool grouped = false;
+    int groups = 0;
+    for (int i = 0; i < n_pad; i++) {
+        if (i > 0 && (i < n ? seq_ids[i] == seq_ids[i - 1] : i > n)) {
+            if (ctx[i] > gpre[groups - 1]) {
+                gpre[groups - 1] = ctx[i];
+                memcpy(ptab + (size_t)gstart[groups - 1] * MP, ptab + (size_t)i * MP, (size_t)MP * 4);
+            }
+            grouped |= i < n;
+        } else {
+            gpre[groups] = ctx[i];
+            gstart[groups++] = i;
+        }
+    }
+    for (int g = groups; g < n_pad; g++) gpre[g] = 0;
+    for (int g = groups; g <= n_pad; g++) gstart[g] = n_pad;
+    grouped = grouped && e->group_rows;
     const int n_logit_real = n_logit_rows;
     if (n_pad != n && n_logit_rows > 0) {
         const int nl = std::min((n_logit_rows + e->row_pad - 1) / e->row_pad * e->row_pad, n_pad);
@@ -1129,7 +1157,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     }
     n = n_pad;
     hipStream_t s = e->stream;
-    const size_t words = (size_t)n * (7 + MP);
+    const size_t words = (size_t)n * (9 + MP) + 1;
     const bool head = n_logit_rows > 0 && (logits || tok_out);
     // greedy-only step (no logits wanted, none kept): the head's argmax fused into its GEMM where it runs one
     const bool argmax_only = head && !logits && tok_out && !e->keep_logits && e->pen_live == 0;
@@ -1141,7 +1169,9 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     const int32_t* d_src = d_lrows + n;
     const int32_t* d_pslot = d_src + n;
     const float* d_ppen = (const float*)(d_pslot + n);
-    const int32_t* d_ptab = (const int32_t*)(d_ppen + n);
+    const int32_t* d_gpre = (const int32_t*)(d_ppen + n);
+    const int32_t* d_gstart = d_gpre + n;
+    const int32_t* d_ptab = d_gstart + n + 1;
 
     const int D = (int)c.hidden_size, F = (int)c.intermediate_size, V = (int)c.vocab_size;
     const int H = (int)c.num_heads, Hkv = (int)c.num_kv_heads, hd = e->hd;
@@ -1195,6 +1225,14 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         return launch_qgemm(Wt, dt, 32, N, K, e->xh, e->xl, rows, y, add, e->gemm_ws, e->gemm_ws_bytes, s, true);
     };
 
+    auto attention = [&](const uint8_t* kc, const uint8_t* vc, int ctx_grid, float* out, uint16_t* hi, uint16_t* lo) {
+        if (grouped)
+            return launch_group_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_ctx, d_gstart, d_gpre, n, n, H, Hkv, hd,
+                                          ps, scale, ctx_grid, out, e->group_ws, e->group_ws_bytes, s, hi, lo);
+        return launch_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_ctx, n, H, Hkv, hd, ps, scale, ctx_grid, out,
+                                e->attn_ws, e->attn_ws_bytes, s, hi, lo);
+    };
+
     // The step's launches, stream-ordered: embedding, layers, head and argmax.
     // ctx_grid >= every row's context sizes the attention grid.
     auto enqueue = [&](int ctx_grid) -> int {
@@ -1227,8 +1265,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
                                     e->part_ws_bytes, s, true, &S));
                 QH_TRY(launch_rope_append(P, L.has_bias ? L.bqkv : nullptr, n, H, Hkv, hd, d_pos, e->rope, e->q, kc, vc,
                                           e->o.kv_dtype, d_ptab, MP, ps, s, S, (size_t)n * e->qkvd));
-                QH_TRY(launch_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_ctx, n, H, Hkv, hd, ps, scale,
-                                        ctx_grid, nullptr, e->attn_ws, e->attn_ws_bytes, s, e->xh, e->xl));
+                QH_TRY(attention(kc, vc, ctx_grid, nullptr, e->xh, e->xl));
                 QH_TRY(launch_qgemm(L.wo_t, L.dt_attn, 32, D, e->qd, e->xh, e->xl, n, e->qkv, nullptr, P, e->part_ws_bytes,
                                     s, true, &S));
                 QH_TRY(launch_residual_norm_split(P, S, (size_t)n * D, e->h, L.fn, D, c.rms_norm_eps, e->xh, e->xl, n, s));
@@ -1277,8 +1314,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
             if (!fused)
                 QH_TRY(launch_rope_append(e->qkv, L.has_bias ? L.bqkv : nullptr, n, H, Hkv, hd, d_pos, e->rope, e->q,
                                           kc, vc, e->o.kv_dtype, d_ptab, MP, ps, s));
-            QH_TRY(launch_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_ctx, n, H, Hkv, hd, ps, scale, ctx_grid,
-                                    e->att, e->attn_ws, e->attn_ws_bytes, s));
+            QH_TRY(attention(kc, vc, ctx_grid, e->att, nullptr, nullptr));
             QH_TRY(proj(L.wo, L.wo_t, L.dt_attn, D, e->qd, e->att, n, e->h, e->h));  // + residual (transformer.cpp:593)
             const MvPrep ffn_norm{XP_NORM, L.fn, c.rms_norm_eps, e->xn};  // transformer.cpp:595
             QH_TRY(proj(L.wgu, L.wgu_t, L.dt_mlp, 2 * F, D, e->h, n, e->gu, nullptr, &ffn_norm));
@@ -1339,13 +1375,14 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         const uint32_t gen = tuning_generation();
         qraf_engine::StepGraph* g = nullptr;
         for (auto& sg : e->graphs)
-            if (sg.n == n && sg.n_logit_rows == n_logit_rows && sg.ctx == ctx_grid && sg.head == head_mode && sg.gen == gen)
+            if (sg.n == n && sg.n_logit_rows == n_logit_rows && sg.ctx == ctx_grid && sg.head == head_mode &&
+                sg.grouped == grouped && sg.gen == gen)
                 g = &sg;
         bool second = false;
         if (!g) {
             for (auto it = e->seen.begin(); it != e->seen.end(); ++it)
                 if (it->n == n && it->n_logit_rows == n_logit_rows && it->ctx == ctx_grid && it->head == head_mode &&
-                    it->gen == gen) {
+                    it->grouped == grouped && it->gen == gen) {
                     second = true;
                     e->seen.erase(it);
                     break;
@@ -1356,6 +1393,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
                 sg.n_logit_rows = n_logit_rows;
                 sg.ctx = ctx_grid;
                 sg.head = head_mode;
+                sg.grouped = grouped;
                 sg.gen = gen;
                 if (e->seen.size() >= 4 * MAX_STEP_GRAPHS) e->seen.erase(e->seen.begin());
                 e->seen.push_back(sg);
@@ -1394,6 +1432,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
             sg.n_logit_rows = n_logit_rows;
             sg.ctx = ctx_grid;
             sg.head = head_mode;
+            sg.grouped = grouped;
             sg.gen = gen;
             sg.exec = exec;
             e->graphs.push_back(sg);
@@ -1487,11 +1526,20 @@ int qraf_engine_read_logits(qraf_engine* e, int32_t row0, int32_t rows, float* o
 
 int qraf_engine_set_fusion(qraf_engine* e, int32_t flags) {
     clear_error();
-    QH_REQUIRE(e && (flags & ~7) == 0, QRAF_HIP_ERR_INVALID, "set_fusion: flags %d", flags);
+    QH_REQUIRE(e && (flags & ~15) == 0, QRAF_HIP_ERR_INVALID, "set_fusion: flags %d", flags);
     QH_CHECK_HIP(hipStreamSynchronize(e->stream));  // no captured step still in flight
+    if ((flags & 8) && !e->group_ws) {
+        size_t bytes = 0;
+        for (int n = 2; n <= (int)e->o.max_batch; n++)  // (not monotone: the largest batches take another form)
+            bytes = std::max(bytes, group_attention_workspace_bytes(n, n, (int)e->c.num_heads, (int)e->c.num_kv_heads,
+                                                                    e->hd, e->capacity));
+        if (bytes) QH_TRY(ealloc(e, &e->group_ws, bytes));
+        e->group_ws_bytes = bytes;
+    }
     e->fuse_rope = (flags & 1) != 0;
     e->fuse_swiglu = (flags & 2) != 0;
     e->batch_mv = (flags & 4) != 0;
+    e->group_rows = (flags & 8) != 0;
     e->drop_graphs();  // captured steps hold the other form
     return QRAF_HIP_OK;
 }
@@ -1552,6 +1600,115 @@ int qraf_engine_sample(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sa
     QH_TRY(launch_sample(e->logits + (size_t)row0 * e->c.vocab_size, rows, (int)e->c.vocab_size, *p,
                          pen ? d_rec : nullptr, pen ? d_cnt : nullptr, stride, greedy ? nullptr : d_uni, d_tok,
                          e->sort_ws, e->sort_cap, s));
+    QH_CHECK_HIP(hipMemcpyAsync(tokens, d_tok, (size_t)rows * 4, hipMemcpyDeviceToHost, s));
+    QH_CHECK_HIP(hipStreamSynchronize(s));
+    return QRAF_HIP_OK;
+}
+
+// `bytes` of the engine's storage for probabilities and verification.  It grows by a quarter more than it must (rows
+// of histories grow by a token a step), and the smaller one, idle since its call returned, goes.
+static int spec_storage(qraf_engine* e, size_t bytes) {
+    if (bytes <= e->spec_cap) return QRAF_HIP_OK;
+    if (e->spec) {
+        QH_CHECK_HIP(hipStreamSynchronize(e->stream));
+        e->allocs.erase(std::find(e->allocs.begin(), e->allocs.end(), e->spec));
+        hipFree(e->spec);
+        e->spec = nullptr;
+        e->spec_cap = 0;
+    }
+    bytes += bytes / 4;
+    QH_TRY(ealloc(e, &e->spec, bytes));
+    e->spec_cap = bytes;
+    return QRAF_HIP_OK;
+}
+// what probabilities and verification of the last step's logit rows have in common: those rows, and the recent
+// tokens of a repetition penalty (rounded sizes of the device copies: counts, tokens)
+static int spec_rows(qraf_engine* e, const char* what, int32_t row0, int32_t rows, const qraf_sampling_params* p,
+                     const uint32_t* recent, const int32_t* counts, int32_t stride, size_t* cnt, size_t* rec) {
+    QH_REQUIRE(e && p && rows > 0 && row0 >= 0, QRAF_HIP_ERR_INVALID, "%s: bad arguments", what);
+    QH_REQUIRE(rows <= e->last_logit_rows - row0, QRAF_HIP_ERR_STATE, "%s: rows %d..%lld, the last step left %d logit rows",
+               what, row0, (long long)row0 + rows - 1, e->last_logit_rows);
+    QH_REQUIRE(e->last_logits_kept, QRAF_HIP_ERR_STATE,
+               "%s: the last step was greedy-only and kept no logits (qraf_engine_set_keep_logits)", what);
+    const bool pen = p->repetition_penalty != 1.0f && recent;
+    QH_REQUIRE(!pen || (counts && stride > 0), QRAF_HIP_ERR_INVALID, "%s: recent tokens need counts", what);
+    *cnt = pen ? ((size_t)rows * 4 + 255) / 256 * 256 : 0;
+    *rec = pen ? ((size_t)rows * stride * 4 + 255) / 256 * 256 : 0;
+    return QRAF_HIP_OK;
+}
+
+// The distribution that qraf_engine_sample draws from, for rows of the last step, to the caller's device memory.
+int qraf_engine_probs(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sampling_params* p, const uint32_t* recent,
+                      const int32_t* counts, int32_t stride, float* probs) {
+    clear_error();
+    size_t cnt, rec;
+    QH_REQUIRE(probs, QRAF_HIP_ERR_INVALID, "probs: null pointer");
+    QH_TRY(spec_rows(e, "probs", row0, rows, p, recent, counts, stride, &cnt, &rec));
+    const int V = (int)e->c.vocab_size;
+    const size_t ws = (sample_probs_workspace_bytes(rows, V) + 255) / 256 * 256;
+    QH_TRY(spec_storage(e, ws + cnt + rec));
+    hipStream_t s = e->stream;
+    int32_t* d_cnt = (int32_t*)((uint8_t*)e->spec + ws);
+    uint32_t* d_rec = (uint32_t*)((uint8_t*)d_cnt + cnt);
+    if (rec) {
+        QH_CHECK_HIP(hipMemcpyAsync(d_cnt, counts, (size_t)rows * 4, hipMemcpyHostToDevice, s));
+        QH_CHECK_HIP(hipMemcpyAsync(d_rec, recent, (size_t)rows * stride * 4, hipMemcpyHostToDevice, s));
+    }
+    QH_TRY(launch_sample_probs(e->logits + (size_t)row0 * V, rows, V, *p, rec ? d_rec : nullptr, rec ? d_cnt : nullptr,
+                               stride, probs, e->spec, ws, s));
+    QH_CHECK_HIP(hipStreamSynchronize(s));
+    return QRAF_HIP_OK;
+}
+
+// Drafted tokens of several sequences against the last step's logit rows.
+int qraf_engine_verify(qraf_engine* e, int32_t row0, int32_t n_seqs, const int32_t* row_counts,
+                       const qraf_sampling_params* p, const uint32_t* recent, const int32_t* counts, int32_t stride,
+                       const uint32_t* draft_tokens, const float* draft_probs, const float* accept_uniforms,
+                       const float* pick_uniforms, int32_t* accepted, uint32_t* tokens) {
+    clear_error();
+    QH_REQUIRE(e && row_counts && draft_tokens && accepted && tokens && n_seqs > 0 && n_seqs <= (int32_t)e->o.max_batch,
+               QRAF_HIP_ERR_INVALID, "verify: bad arguments");
+    std::vector<int32_t> starts(n_seqs + 1, 0);
+    for (int i = 0; i < n_seqs; i++) {
+        QH_REQUIRE(row_counts[i] > 0 && row_counts[i] <= (int32_t)e->o.max_batch - starts[i], QRAF_HIP_ERR_INVALID,
+                   "verify: %d rows of sequence %d (max_batch %u)", row_counts[i], i, e->o.max_batch);
+        starts[i + 1] = starts[i] + row_counts[i];
+    }
+    const int rows = starts[n_seqs], V = (int)e->c.vocab_size;
+    size_t cnt, rec;
+    QH_TRY(spec_rows(e, "verify", row0, rows, p, recent, counts, stride, &cnt, &rec));
+    const bool greedy = !(p->temperature > 0.f);
+    QH_REQUIRE(greedy || (accept_uniforms && pick_uniforms), QRAF_HIP_ERR_INVALID, "verify: temperature %g needs uniforms",
+               p->temperature);
+    const std::vector<float> zeros(greedy ? rows : 0, 0.f);  // greedy rows hold one token: any draw takes it
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    const size_t ws = up(std::max(sample_probs_workspace_bytes(rows, V), verify_draft_workspace_bytes(n_seqs, V)));
+    const size_t pr = up((size_t)rows * V * 4), rb = up((size_t)rows * 4 + 4);
+    QH_TRY(spec_storage(e, ws + pr + 6 * rb + cnt + rec));
+    uint8_t* b = (uint8_t*)e->spec + ws;
+    float* d_probs = (float*)b;
+    int32_t* d_starts = (int32_t*)(b += pr);
+    uint32_t* d_draft = (uint32_t*)(b += rb);
+    float* d_u = (float*)(b += rb);
+    float* d_v = (float*)(b += rb);
+    int32_t* d_acc = (int32_t*)(b += rb);
+    uint32_t* d_tok = (uint32_t*)(b += rb);
+    int32_t* d_cnt = (int32_t*)(b += rb);
+    uint32_t* d_rec = (uint32_t*)(b += cnt);
+    hipStream_t s = e->stream;
+    QH_CHECK_HIP(hipMemcpyAsync(d_starts, starts.data(), (size_t)(n_seqs + 1) * 4, hipMemcpyHostToDevice, s));
+    QH_CHECK_HIP(hipMemcpyAsync(d_draft, draft_tokens, (size_t)rows * 4, hipMemcpyHostToDevice, s));
+    QH_CHECK_HIP(hipMemcpyAsync(d_u, greedy ? zeros.data() : accept_uniforms, (size_t)rows * 4, hipMemcpyHostToDevice, s));
+    QH_CHECK_HIP(hipMemcpyAsync(d_v, greedy ? zeros.data() : pick_uniforms, (size_t)n_seqs * 4, hipMemcpyHostToDevice, s));
+    if (rec) {
+        QH_CHECK_HIP(hipMemcpyAsync(d_cnt, counts, (size_t)rows * 4, hipMemcpyHostToDevice, s));
+        QH_CHECK_HIP(hipMemcpyAsync(d_rec, recent, (size_t)rows * stride * 4, hipMemcpyHostToDevice, s));
+    }
+    QH_TRY(launch_sample_probs(e->logits + (size_t)row0 * V, rows, V, *p, rec ? d_rec : nullptr, rec ? d_cnt : nullptr,
+                               stride, d_probs, e->spec, ws, s));
+    QH_TRY(launch_verify_draft(d_probs, draft_probs, d_draft, d_starts, n_seqs, rows, V, d_u, d_v, d_acc, d_tok, e->spec,
+                               ws, s));
+    QH_CHECK_HIP(hipMemcpyAsync(accepted, d_acc, (size_t)n_seqs * 4, hipMemcpyDeviceToHost, s));
     QH_CHECK_HIP(hipMemcpyAsync(tokens, d_tok, (size_t)rows * 4, hipMemcpyDeviceToHost, s));
     QH_CHECK_HIP(hipStreamSynchronize(s));
     return QRAF_HIP_OK;

@@ -779,6 +779,7 @@ int launch_sample_probs(float* logits, int rows, int V, const qraf_sampling_para
     QH_REQUIRE(logits && probs && ws && rows > 0 && V > 0, QRAF_HIP_ERR_INVALID, "sample_probs: bad arguments");
     QH_REQUIRE(V <= 1 << 30, QRAF_HIP_ERR_INVALID, "sample_probs: vocabulary %d over 2^30", V);
     QH_REQUIRE(rows <= 65535, QRAF_HIP_ERR_INVALID, "sample_probs: %d rows over 65535", rows);
+    QH_REQUIRE(((uintptr_t)ws & 15) == 0, QRAF_HIP_ERR_INVALID, "sample_probs: workspace not 16-byte aligned");
     QH_REQUIRE(ws_bytes >= sample_probs_workspace_bytes(rows, V), QRAF_HIP_ERR_INVALID,
                "sample_probs: workspace of %zu bytes, %zu needed", ws_bytes, sample_probs_workspace_bytes(rows, V));
     QH_TRY(launch_penalty(logits, rows, V, sp.repetition_penalty, recent, counts, stride, s));
@@ -1062,6 +1063,7 @@ int launch_verify_draft(const float* probs, const float* draft_probs, const uint
                QRAF_HIP_ERR_INVALID, "verify_draft: null pointer");
     QH_REQUIRE(n > 0 && n_rows > 0 && V > 0, QRAF_HIP_ERR_INVALID, "verify_draft: %d sequences, %d rows, vocabulary %d",
                n, n_rows, V);
+    QH_REQUIRE(((uintptr_t)ws & 15) == 0, QRAF_HIP_ERR_INVALID, "verify_draft: workspace not 16-byte aligned");
     QH_REQUIRE(ws_bytes >= verify_draft_workspace_bytes(n, V), QRAF_HIP_ERR_INVALID,
                "verify_draft: workspace of %zu bytes, %zu needed", ws_bytes, verify_draft_workspace_bytes(n, V));
     QH_REQUIRE(V <= 1 << 30 && n <= 65535, QRAF_HIP_ERR_INVALID,

@@ -127,6 +127,11 @@ class Engine:
         self.vocab = cfg.vocab_size
         return self
 
+    @property
+    def capacity(self) -> int:
+        """Positions a sequence can hold."""
+        return min(self.config.max_seq_len or 2048, 8192)
+
     def close(self):
         if getattr(self, "h", None):
             lib.qraf_engine_destroy(self.h)
@@ -248,7 +253,10 @@ class Engine:
         more than 256 rows run the gate/up GEMM with the SiLU-gate in its
         epilogue (default on; the same sums in another order).  Bit 2: steps
         of 2-8 rows run their projections on the multi-vector matvec where
-        it covers them (default on; batch-1 arithmetic instead of the GEMM's)."""
+        it covers them (default on; batch-1 arithmetic instead of the GEMM's).
+        Bit 3: steps with several rows of a sequence one behind another read
+        the positions that they share once (default off; the same sums in
+        another order)."""
         call("qraf_engine_set_fusion", self.h, int(flags))
 
     def set_row_padding(self, rows: int) -> None:
@@ -277,6 +285,48 @@ class Engine:
              cnt.ctypes.data_as(i32p) if cnt is not None else None, stride,
              uni.ctypes.data_as(fp) if uni is not None else None, out.ctypes.data_as(u32p))
         return out
+
+
+    def _penalty(self, params, recent):
+        """The recent lists of a call's rows as the host arrays of a repetition penalty: (tokens, counts, stride)."""
+        if recent is None or params.repetition_penalty == 1.0:
+            return None, None, 0
+        rec = np.zeros((len(recent), max(1, max(len(r) for r in recent))), np.uint32)
+        cnt = np.array([len(r) for r in recent], np.int32)
+        for i, r in enumerate(recent):
+            rec[i, :len(r)] = r
+        return rec, cnt, rec.shape[1]
+
+    def probs(self, params: SamplingParams, out: int, recent=None, row0=0, rows=1) -> None:
+        """The distributions that sample() draws from, for rows row0.. of the last step's logit rows, to the device
+        memory at `out` [rows][vocab] (qraf_engine_probs)."""
+        rec, cnt, stride = self._penalty(params, recent)
+        call("qraf_engine_probs", self.h, row0, rows, C.byref(params),
+             rec.ctypes.data_as(u32p) if rec is not None else None,
+             cnt.ctypes.data_as(i32p) if cnt is not None else None, stride, out)
+
+    def verify(self, params: SamplingParams, drafts, recent=None, draft_probs: int | None = None, uniforms=None,
+               picks=None, row0=0):
+        """Drafted tokens against the last step's logit rows (qraf_engine_verify).  drafts: per sequence its drafted
+        tokens, whose rows (one more than drafts) lie one sequence behind another from row0 on; recent: a list per
+        row; draft_probs: device address of [rows][vocab]; uniforms, picks: draws per row and per sequence (not
+        needed when greedy).  Per sequence the tokens it emits: its accepted drafts and the one behind them."""
+        counts = np.array([len(d) + 1 for d in drafts], np.int32)
+        tok = np.array([t for d in drafts for t in (*d, 0)], np.uint32)
+        rec, cnt, stride = self._penalty(params, recent)
+        uni = None if uniforms is None else np.ascontiguousarray(uniforms, dtype=np.float32)
+        pic = None if picks is None else np.ascontiguousarray(picks, dtype=np.float32)
+        for name, a, n in (("uniforms", uni, tok.size), ("picks", pic, counts.size), ("recent", cnt, tok.size)):
+            if a is not None and a.size != n:
+                raise ValueError(f"{name}: {a.size} for {n}")
+        accepted, out = np.empty(counts.size, np.int32), np.empty(tok.size, np.uint32)
+        call("qraf_engine_verify", self.h, row0, counts.size, counts.ctypes.data_as(i32p), C.byref(params),
+             rec.ctypes.data_as(u32p) if rec is not None else None,
+             cnt.ctypes.data_as(i32p) if cnt is not None else None, stride, tok.ctypes.data_as(u32p), draft_probs,
+             uni.ctypes.data_as(fp) if uni is not None else None, pic.ctypes.data_as(fp) if pic is not None else None,
+             accepted.ctypes.data_as(i32p), out.ctypes.data_as(u32p))
+        at = np.concatenate([[0], np.cumsum(counts)])
+        return [[int(t) for t in out[a:a + n + 1]] for a, n in zip(at, accepted)]
 
 
 class Transformer:
@@ -394,6 +444,55 @@ class InferenceEngine:
             e.seq_release(seq)
         return out
 
+    def generate_speculative(self, prompt_tokens, max_tokens=256, stop_tokens=(), sampling: SamplingConfig | None = None,
+                             drafts: int = 4, draft: Transformer | None = None, ngram: int = 3):
+        """generate_tokens with several tokens to a step: up to `drafts` drafted tokens are fed with the last token
+        and verified on the device against the target's distribution (qraf_engine_verify), so a step emits its
+        accepted drafts and one token more.  Greedy (the default, without a penalty) gives generate_tokens' tokens, as
+        far as rows of one step round as steps of one row do; sampled tokens are distributed as its tokens are, from
+        another order of draws.  draft: a smaller model with the same vocabulary that drafts them; without one they
+        are what followed the last `ngram` tokens (or fewer) where these occurred before.  The engine's max_batch has
+        to hold drafts + 1 rows."""
+        if len(prompt_tokens) == 0:
+            raise ValueError("empty prompt")
+        e = self.transformer.engine
+        if drafts < 0 or drafts + 1 > e.max_batch:
+            raise ValueError(f"{drafts} drafts and the last token need {drafts + 1} rows (max_batch {e.max_batch})")
+        if draft is not None and draft.engine.vocab != e.vocab:
+            raise ValueError("the draft model has another vocabulary")
+        if sampling is None:
+            sampling = SamplingConfig(temperature=0.0, top_k=0, top_p=1.0, repetition_penalty=1.0, deterministic=True)
+        sampler = Sampler(sampling) if not sampling.greedy else None
+        params = sampling.params()
+        stops = set(stop_tokens) | ({self.eos} if self.eos is not None else set())
+        self.transformer.reset()
+        seq = e.seq_create()
+        drafter = _Drafter(draft, e.vocab, drafts, params, sampler, ngram)
+        history, out = list(prompt_tokens), []
+        try:
+            for a in range(0, len(history) - 1, e.max_batch):  # the prompt but its last token
+                chunk = history[a:min(a + e.max_batch, len(history) - 1)]
+                e.step([seq] * len(chunk), chunk, range(a, a + len(chunk)), want_logits=[0] * len(chunk), argmax=False)
+            while len(out) < max_tokens:
+                pos = len(history) - 1  # of the last token, not fed yet
+                room = min(drafts, max_tokens - len(out) - 1, e.capacity - pos - 1)
+                guess, q = drafter.propose(history, max(room, 0))
+                rows = [history[-1], *guess]
+                e.step([seq] * len(rows), rows, range(pos, pos + len(rows)), logits=False, argmax=True)
+                recent = [history + guess[:j] for j in range(len(rows))]
+                uni = None if sampler is None else sampler.uniforms(len(rows) + 1)
+                got = e.verify(params, [guess], recent, q, None if uni is None else uni[:-1],
+                               None if uni is None else uni[-1:])[0]
+                for t in got:
+                    if t in stops:
+                        return out
+                    out.append(t)
+                    history.append(t)
+        finally:
+            e.seq_release(seq)
+            drafter.close()
+        return out
+
     @staticmethod
     def _penalised_greedy_pipelined(e, seq, prompt, max_tokens, stops, penalty):
         e.set_repetition_penalty(seq, penalty)
@@ -416,6 +515,55 @@ class InferenceEngine:
                 e.collect()
                 pending -= 1
         return out
+
+
+class _Drafter:
+    """Drafted tokens: a model's own samples with their distributions, or what followed the last tokens before."""
+
+    def __init__(self, model: Transformer | None, vocab, drafts, params, sampler, ngram):
+        self.model, self.vocab, self.params, self.sampler, self.ngram = model, vocab, params, sampler, ngram
+        self.seq, self.held, self.q = -1, [], None
+        if model is not None:
+            self.seq = model.engine.seq_create()
+            if sampler is not None:
+                from .backend import DeviceBuffer
+                self.q = DeviceBuffer((drafts + 1) * vocab * 4)  # row j: what draft j was drawn from; the last unused
+
+    def close(self):
+        if self.seq >= 0:
+            self.model.engine.seq_release(self.seq)
+            self.seq = -1
+
+    def propose(self, history, most):
+        """At most `most` tokens behind `history`, and the device address of their distributions or None."""
+        if most <= 0:
+            return [], None
+        if self.model is None:
+            for n in range(min(self.ngram, len(history) - 1), 0, -1):
+                tail = history[-n:]
+                for at in range(len(history) - n - 1, -1, -1):  # the latest occurrence
+                    if history[at:at + n] == tail:
+                        return history[at + n:at + n + most], None
+            return [], None
+        e, guess = self.model.engine, []
+        same = 0  # positions of the draft's cache that still hold this history
+        while same < min(len(self.held), len(history) - 1) and self.held[same] == history[same]:
+            same += 1
+        for a in range(same, len(history) - 1, e.max_batch):
+            chunk = history[a:min(a + e.max_batch, len(history) - 1)]
+            e.step([self.seq] * len(chunk), chunk, range(a, a + len(chunk)), want_logits=[0] * len(chunk), argmax=False)
+        for j in range(min(most, e.capacity - len(history) + 1)):
+            last = guess[-1] if guess else history[-1]
+            e.step([self.seq], [last], [len(history) - 1 + j], logits=False, argmax=True)
+            if self.sampler is None:
+                guess.append(int(e.sample(self.params, [history + guess], rows=1)[0]))
+                continue
+            # (the penalty, if any, is applied to the logits in place: once)
+            e.probs(self.params, self.q.ptr + j * self.vocab * 4, [history + guess])
+            once = SamplingParams(self.params.temperature, self.params.top_k, self.params.top_p, 1.0)
+            guess.append(int(e.sample(once, None, [self.sampler.uniform()], rows=1)[0]))
+        self.held = history + guess[:-1]
+        return guess, self.q.ptr if self.q is not None and guess else None
 
 
 @dataclass

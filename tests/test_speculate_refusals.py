@@ -25,6 +25,25 @@ def test_group_attention_refuses(change):
     assert rc == ERR_INVALID and msg.startswith(b"group attention"), msg
 
 
+@pytest.mark.parametrize("change", [dict(q=P + 4), dict(k=P + 8), dict(v=P + 2), dict(out=P + 4), dict(ws=P + 8),
+                                    dict(max_ctx=(1 << 30) + 1, max_pages=1 << 27)])
+def test_group_attention_refuses_alignments_and_lengths(change):
+    rc, msg = group(**change)
+    assert rc == ERR_INVALID and msg.startswith(b"group attention"), msg
+
+
+@pytest.mark.parametrize("change", [dict(ws=P + 4), dict(rows=65536), dict(vocab=(1 << 30) + 1)])
+def test_sample_probs_refuses_alignments_and_sizes(change):
+    rc, msg = probs(**change)
+    assert rc == ERR_INVALID and msg.startswith(b"sample_probs"), msg
+
+
+@pytest.mark.parametrize("change", [dict(ws=P + 8), dict(n=65536), dict(vocab=(1 << 30) + 1)])
+def test_verify_draft_refuses_alignments_and_sizes(change):
+    rc, msg = verify(**change)
+    assert rc == ERR_INVALID and msg.startswith(b"verify_draft"), msg
+
+
 def test_group_attention_refuses_other_pages():
     assert group(kv=10)[0] == ERR_DTYPE
 
