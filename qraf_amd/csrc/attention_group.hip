@@ -12,9 +12,10 @@
 // workgroups at once (group_tile_kernel), all from the device-resident lengths:
 // a long prefix of few columns spreads over the chip, ragged lengths balance, and
 // a workgroup has one piece, or as few as may be (what a piece costs beside its
-// tiles, q to stage and outputs to join, is what 5 of them take).  A piece that
+// tiles, q to stage and outputs to join, is what 3 to 5 of them take).  A piece that
 // holds all there is of a column writes the output; the others write (max, sum,
 // unnormalised output) parts, which group_merge_kernel joins in position order.
+// Small calls go without: a workgroup per (row, KV head) takes all its positions.
 // group_any_kernel takes the shapes that the tiles do not.
 #include <math.h>
 
@@ -220,6 +221,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int GW = 8, GTH = 64 * GW;  // waves and threads of a workgroup
+constexpr int DIRECT_ROWS = 256;      // rows of a call without a plan, at most
 constexpr int BLK = 128;              // columns of a block: 4 waves of 32
 // p is held times 2^13 of the running maximum it was taken against, which follows the largest score only
 // when that has grown by more than 2^2: outputs and sums are rescaled then, a few times a job and not at
@@ -251,6 +253,11 @@ __device__ __forceinline__ T over_wave(T x, F op) {
     x = op(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
     return over_halves(x, op);
 }
+// max(m, |x|, |y|) in one instruction (fmaxf quiets each operand first, in another one): a NaN may come of a NaN
+__device__ __forceinline__ float amax3(float m, float x, float y) {
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
+    return m;
+}
 __device__ __forceinline__ float fmax2(float x, float y) { return fmaxf(x, y); }
 __device__ __forceinline__ int imax2(int x, int y) { return max(x, y); }
 __device__ __forceinline__ int imin2(int x, int y) { return min(x, y); }
@@ -273,6 +280,21 @@ __device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
     // (x - hi as a multiply-add: one instruction with the conversion inside)
     lo = __builtin_convertvector(
         (f32x2{__builtin_fmaf((float)hi[0], -1.f, x), __builtin_fmaf((float)hi[1], -1.f, y)}), f16x2);
+}
+// 8 values times a power of two (the products inside the multiply-adds: 5 instructions a pair, 6 with them ahead)
+__device__ __forceinline__ void split8(const float (&x)[8], float by, f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        f16x2 h;
+        h[0] = (_Float16)__builtin_fmaf(x[i], by, 0.f);
+        h[1] = (_Float16)__builtin_fmaf(x[i + 1], by, 0.f);
+        uint32_t u = __builtin_bit_cast(uint32_t, h);
+        asm("" : "+v"(u));  // one register of two halves, as the products take them
+        h = __builtin_bit_cast(f16x2, u);
+        hi[i] = h[0], hi[i + 1] = h[1];
+        lo[i] = (_Float16)__builtin_fmaf(x[i], by, -(float)h[0]);
+        lo[i + 1] = (_Float16)__builtin_fmaf(x[i + 1], by, -(float)h[1]);
+    }
 }
 __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
 #pragma unroll
@@ -455,7 +477,8 @@ struct GroupTile<HD, (int)DT_F32> {
     vrow v[16];
 };
 
-template <int HD, int KV>
+// DIRECT: no plan; workgroup (r, KV head) takes row r alone, its prefix and its tail one behind the other.
+template <int HD, int KV, bool DIRECT>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
@@ -487,22 +510,63 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     };
     const int kvh = blockIdx.y, w = blockIdx.x, G = a.G, psl = a.ps_log2, psm = (1 << psl) - 1;
 
-    group_plan(a, plan, gridDim.x);
-    const int jobs = plan.np + a.tails, pieces = plan.upto[jobs] & 0xFFFF;
+    int jobs = 0, pieces = w + 1;
+    int d_ctx = 0, d_pre = 0, d_first = 0, d_tiles = 0;  // DIRECT: the row's context, prefix, group's first row; prefix tiles
+    if constexpr (DIRECT) {
+        static_assert(DIRECT_ROWS % 64 == 0, "rows by lane");
+        int s[DIRECT_ROWS / 64], e[DIRECT_ROWS / 64];
+#pragma unroll
+        for (int k = 0; k < DIRECT_ROWS / 64; k++) {  // (groups <= rows <= DIRECT_ROWS)
+            s[k] = group_start(a, min(lane + 64 * k, a.groups));
+            e[k] = prefix_len(a, min(lane + 64 * k, a.groups - 1));
+        }
+        d_ctx = row_ctx(a, w);
+        if (w < group_start(a, 0) || w >= group_start(a, a.groups)) return;  // outside every group
+        int g = -1;
+#pragma unroll
+        for (int k = 0; k < DIRECT_ROWS / 64; k++) g += __popcll(__ballot(lane + 64 * k < a.groups && s[k] <= w));
+#pragma unroll
+        for (int k = 0; k < DIRECT_ROWS / 64; k++)
+            if (g >> 6 == k) {
+                d_first = __builtin_amdgcn_readlane(s[k], g & 63);
+                d_pre = __builtin_amdgcn_readlane(e[k], g & 63);
+            }
+        d_tiles = (min(d_ctx, d_pre) + 31) >> 5;
+    } else {
+        group_plan(a, plan, gridDim.x);
+        jobs = plan.np + a.tails;
+        pieces = plan.upto[jobs] & 0xFFFF;
+    }
 
     for (int piece = w; piece < pieces; piece += gridDim.x) {
         lanes_again();
-        const int j = __builtin_amdgcn_readfirstlane(wave_last_at(plan.upto, jobs, piece, 0xFFFF));
-        const int here = __builtin_amdgcn_readfirstlane(plan.upto[j]), next = __builtin_amdgcn_readfirstlane(plan.upto[j + 1]);
-        const int tiles = __builtin_amdgcn_readfirstlane(plan.tiles[j]);
-        const int i_of = piece - (here & 0xFFFF), n_of = (next & 0xFFFF) - (here & 0xFFFF);
-        const int ja = (int)((long long)i_of * tiles / n_of), jend = (int)((long long)(i_of + 1) * tiles / n_of);
-        const bool whole = n_of == 1;  // tiles [ja, jend) of the job
+        int j = 0, here = 0, i_of = 0, ja = 0, jend = 0;
+        bool whole = true;  // tiles [ja, jend) of the job
+        if constexpr (!DIRECT) {
+            j = __builtin_amdgcn_readfirstlane(wave_last_at(plan.upto, jobs, piece, 0xFFFF));
+            here = __builtin_amdgcn_readfirstlane(plan.upto[j]);
+            const int next = __builtin_amdgcn_readfirstlane(plan.upto[j + 1]);
+            const int tiles = __builtin_amdgcn_readfirstlane(plan.tiles[j]);
+            const int n_of = (next & 0xFFFF) - (here & 0xFFFF);
+            i_of = piece - (here & 0xFFFF);
+            ja = (int)((long long)i_of * tiles / n_of);
+            jend = (int)((long long)(i_of + 1) * tiles / n_of);
+            whole = n_of == 1;
+        }
 
         // ---- the wave's place: qt of wq waves side by side along the job's columns, kw of wk along the positions
-        const bool tail = j >= plan.np;
+        bool tail = !DIRECT && j >= plan.np;
         int g, trow, first, cols, wq;  // group; the row whose table is read; first column (among all rows'), columns
-        if (tail) {                    // a row's columns are 1, 2 or 4 waves'
+        if constexpr (DIRECT) {
+            wq = 1;
+            first = w * G;
+            cols = G;
+            // tiles: the prefix's, then the tail's
+            jend = d_tiles + (d_ctx > d_pre ? (d_ctx - tail_base(d_pre) + 31) >> 5 : 0);
+            tail = wave >= d_tiles;
+            trow = tail ? w : d_first;
+            g = 0;
+        } else if (tail) {             // a row's columns are 1, 2 or 4 waves'
             wq = 4;
             const int side = 4 / a.tail_rows, c0 = 32 * (wave & (side - 1));
             const int row = (j - plan.np) * a.tail_rows + (wave & 3) / side;
@@ -524,18 +588,23 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         wq = __builtin_amdgcn_readfirstlane(wq);
         cols = __builtin_amdgcn_readfirstlane(max(cols, 0));
         const int wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
-        const int pre = __builtin_amdgcn_readfirstlane(plan.pre[g]), lo = tail ? pre : 0, base = tail ? tail_base(pre) : 0;
+        const int pre = __builtin_amdgcn_readfirstlane(DIRECT ? d_pre : plan.pre[g]), base = tail ? tail_base(pre) : 0;
+        int lo = tail ? pre : 0;
         // the page table through scalar loads: an id does not wait for vector loads ahead of it
         typedef const __attribute__((address_space(4))) int32_t ConstInt;
-        ConstInt* ptab = (ConstInt*)(uintptr_t)(a.page_table + (size_t)__builtin_amdgcn_readfirstlane(trow) * a.max_pages);
+        auto table_of = [&](int row) {
+            return (ConstInt*)(uintptr_t)(a.page_table + (size_t)__builtin_amdgcn_readfirstlane(row) * a.max_pages);
+        };
+        ConstInt* ptab = table_of(trow);
 
         // ---- the lane's column (past the last: that again, not written), row and limit
         const int ab = min(first + min(col, max(cols - 1, 0)), a.n * G - 1), r = ab / G;
         const float* qrow = a.q + ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
-        const int ctx = plan.ctx[r], lim = cols == 0 ? 0 : tail ? ctx : min(ctx, pre);
+        const int ctx = DIRECT ? d_ctx : plan.ctx[r];
+        int lim = cols == 0 ? 0 : tail ? ctx : min(ctx, pre);
         // behind the last position that some of the wave's columns attends to
-        const int kend = __builtin_amdgcn_readfirstlane(over_wave(lim, imax2)), klast = max(kend - 1, 0);
-        const int least = __builtin_amdgcn_readfirstlane(over_wave(lim, imin2));
+        int kend = __builtin_amdgcn_readfirstlane(DIRECT ? lim : over_wave(lim, imax2)), klast = max(kend - 1, 0);
+        int least = __builtin_amdgcn_readfirstlane(DIRECT ? lim : over_wave(lim, imin2));
 
         // ---- loads of the tile at position t
         GroupTile<HD, KV> tl;
@@ -605,9 +674,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 
         // f32 rows of 128 fill the registers: V is requested behind the scores, the next K behind the outputs
         constexpr bool TURNS = F32 && HD == 128;
-        int i = ja, t = __builtin_amdgcn_readfirstlane(base + (i * wk + kw) * 32);  // the wave's tiles: every wk-th 32 positions
+        // the wave's tiles: every wk-th 32 positions
+        int i = DIRECT ? wave : ja;
+        int t = __builtin_amdgcn_readfirstlane(DIRECT ? base + 32 * (i - (tail ? d_tiles : 0)) : base + (i * wk + kw) * 32);
         const int dt = 32 * wk;
-        bool more = i < jend && t < kend;
+        bool more = i < jend && (DIRECT || t < kend);
         ids(more ? t : 0);
         // No load of K and V depends on a branch, here and below: where paths with more and with fewer loads behind
         // one meet, a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
@@ -669,26 +740,24 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             if constexpr (F32) {
                 float mx = 0.f;
 #pragma unroll
-                for (int k = 0; k < 2 * KS; k++)
-                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(tl.k[k].x), fabsf(tl.k[k].y)), fmaxf(fabsf(tl.k[k].z), fabsf(tl.k[k].w))));
-                mx = over_wave(mx, fmax2);
-                if (mx > 3.0e38f) {  // an infinity: the unit of the others
+                for (int k = 0; k < 2 * KS; k++) mx = amax3(amax3(mx, tl.k[k].x, tl.k[k].y), tl.k[k].z, tl.k[k].w);
+                if (__any(!(mx <= 3.0e38f))) {  // an infinity or NaN: the unit of the others
                     mx = 0.f;
                     for (int k = 0; k < 2 * KS; k++) {
                         const float v[4] = {tl.k[k].x, tl.k[k].y, tl.k[k].z, tl.k[k].w};
                         for (int c = 0; c < 4; c++) mx = fabsf(v[c]) <= 3.0e38f ? fmaxf(mx, fabsf(v[c])) : mx;
                     }
-                    mx = over_wave(mx, fmax2);
                 }
+                mx = over_wave(mx, fmax2);
                 const int e = unit_exp(mx);
                 const float sg = ldexpf(1.f, e);
                 fs = ldexpf(qs, -e);
 #pragma unroll
                 for (int kk = 0; kk < KS; kk++) {
                     const float4 x = tl.k[2 * kk], y = tl.k[2 * kk + 1];
-                    const float v[8] = {x.x * sg, x.y * sg, x.z * sg, x.w * sg, y.x * sg, y.y * sg, y.z * sg, y.w * sg};
+                    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
                     f16x8 kh, kl;
-                    split8(v, kh, kl);
+                    split8(v, sg, kh, kl);
                     const f16x8 qh = __builtin_bit_cast(f16x8, qtile[128 * kk]);
                     const f16x8 ql = __builtin_bit_cast(f16x8, qtile[128 * kk + 64]);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh, s, 0, 0, 0);
@@ -719,9 +788,15 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 for (int x = 0; x < 16; x++) vsc[x] = ((const float*)&tl.vs[x >> 2])[x & 3];
             }
             // the next tile's ids and K
-            const bool go = i + 1 < jend && t + dt < kend;
-            const int tn = go ? t + dt : t;
+            const bool go = DIRECT ? i + GW < jend : i + 1 < jend && t + dt < kend;
+            int tn = go ? t + dt : t;
+            const bool turn = DIRECT && go && !tail && i + GW >= d_tiles;  // from the prefix to the tail
             if (TURNS) load_v(t);
+            if (turn) {
+                tn = tail_base(pre) + 32 * (i + GW - d_tiles);
+                ptab = table_of(w);
+                klast = ctx - 1;
+            }
             ids(tn);
             if (!TURNS) load_k(tn, go);
 
@@ -767,15 +842,14 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
                     for (int k = 0; k < 16; k++)
 #pragma unroll
-                        for (int c = 0; c < DT; c++) mx = fmaxf(mx, fabsf(tl.v[k][c]));
-                    mx = over_wave(mx, fmax2);
-                    if (mx > 3.0e38f) {
+                        for (int c = 0; c < DT; c += 2) mx = amax3(mx, tl.v[k][c], tl.v[k][c + 1]);
+                    if (__any(!(mx <= 3.0e38f))) {
                         mx = 0.f;
                         for (int k = 0; k < 16; k++)
                             for (int c = 0; c < DT; c++)
                                 mx = fabsf(tl.v[k][c]) <= 3.0e38f ? fmaxf(mx, fabsf(tl.v[k][c])) : mx;
-                        mx = over_wave(mx, fmax2);
                     }
+                    mx = over_wave(mx, fmax2);
                 }
                 const int e = __builtin_amdgcn_readfirstlane(I8 ? unit_exp(mx) - 15 : unit_exp(mx));
                 if (e < vexp) {
@@ -885,9 +959,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     if constexpr (F32) {  // dims DT * row + d
                         float x[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] = tl.v[8 * b + k][d] * vg;
+                        for (int k = 0; k < 8; k++) x[k] = tl.v[8 * b + k][d];
                         f16x8 vh, vl;
-                        split8(x, vh, vl);
+                        split8(x, vg, vh, vl);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[b], o[d], 0, 0, 0);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[b], o[d], 0, 0, 0);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[b], o[d], 0, 0, 0);
@@ -902,8 +976,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             if (TURNS) load_k(tn, go);
             else load_v(tn, go);
             more = go;
-            i++;
+            i += DIRECT ? GW : 1;
             t = tn;
+            if (turn) {
+                tail = true;
+                lo = pre;
+                lim = kend = least = ctx;
+            }
         }
 
         // ---- join the waves of a column
@@ -955,13 +1034,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 if (k < wk) s_m[qt + wq * k][col] = f;
             }
             const bool any_pre = min(ctx, pre) > 0, any_tail = ctx > pre;
-            const bool alone = whole && (tail ? !any_pre : any_pre && !any_tail);
+            const bool alone = DIRECT || (whole && (tail ? !any_pre : any_pre && !any_tail));
             // (pieces ahead, less one for each of their jobs: a job's columns are at most 128, so slots stay apart)
             const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab +
                                 (size_t)BLK * ((here & 0xFFFF) - (here >> 16) + i_of);
             const bool mine = col < cols, part = mine && !alone && (tail || any_pre);
             s_to[qt * 32 + col] = mine && alone ? (long long)(qrow - a.q) : part ? ~(long long)(slot * HD) : NOWHERE;
-            s_by[qt * 32 + col] = alone ? 1.f / L : 1.f;
+            s_by[qt * 32 + col] = DIRECT && ctx == 0 ? 0.f : alone ? 1.f / L : 1.f;
             if (part) a.part_ml[slot] = make_float2(M, L);
         }
         lanes_again();
@@ -1098,9 +1177,21 @@ static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size
            group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
 }
 
+// Small calls: one launch without a plan, a workgroup per (row, KV head), which saves the plan (3 us) and the launch
+// that joins parts (4) and costs 1 (fp16) to 5 us (f32, head_dim 128) per 256 positions, shared or not.  Planned against
+// direct, us: 5 rows of 40 / 300 / 600 / 1,000 positions, fp16, 16/2 heads of 128: 13.9 / 15.0 / 15.2 / 15.6 against
+// 8.1 / 9.8 / 11.9 / 15.8; int8 14.2 / 16.0 / 16.1 / 16.3 against 8.7 / 11.0 / 13.3 / 18.2; f32 16.8 / 19.3 / 19.6 /
+// 19.8 against 11.1 / 15.2 / 20.6 / 32.0.  250 workgroups of 300 / 600 positions, fp16: 18.5 / 19.5 against 13.3 / 17.7.
+static bool group_direct(int n, int H, int Hkv, uint32_t kv_dtype, int max_ctx) {
+    const int most = 256 * (kv_dtype == DT_F32 ? 2 : kv_dtype == DT_I8 ? 3 : 4);
+    return H / Hkv <= 32 && n <= DIRECT_ROWS && (long long)n * Hkv <= 256 && max_ctx <= (n * Hkv > 128 ? most / 2 : most);
+}
+
 int group_attention_init() {
 #define QH_GROUP_LDS(HDv, KVv)                                                         \
-    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv>,    \
+    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, false>, \
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024)); \
+    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, true>, \
                                      hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024));
     QH_GROUP_LDS(64, DT_F32) QH_GROUP_LDS(64, DT_F16) QH_GROUP_LDS(64, DT_I8)
     QH_GROUP_LDS(128, DT_F32) QH_GROUP_LDS(128, DT_F16) QH_GROUP_LDS(128, DT_I8)
@@ -1171,13 +1262,18 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
         a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
         const int gx = group_grid(Hkv);
         const size_t lds = group_lds(hd, n, groups, z);
-#define QH_GROUP_TILE(HDv, KVv)   \
-    if (hd == HDv && kv_dtype == KVv) \
-        hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv>), dim3(gx, Hkv), dim3(GTH), lds, st, a);
+        const bool direct = group_direct(n, H, Hkv, kv_dtype, max_ctx);
+#define QH_GROUP_TILE(HDv, KVv)                                                                                            \
+    if (hd == HDv && kv_dtype == KVv) {                                                                                    \
+        if (direct)                                                                                                        \
+            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true>), dim3(n, Hkv), dim3(GTH), GW * 32 * HDv * 4, st, a); \
+        else hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false>), dim3(gx, Hkv), dim3(GTH), lds, st, a);          \
+    }
         QH_GROUP_TILE(64, DT_F32) QH_GROUP_TILE(64, DT_F16) QH_GROUP_TILE(64, DT_I8)
         QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)
 #undef QH_GROUP_TILE
         QH_CHECK_HIP(hipGetLastError());
+        if (direct) return QRAF_HIP_OK;
         if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a);
         QH_CHECK_HIP(hipGetLastError());
