@@ -657,9 +657,9 @@ int qraf_engine_set_row_padding(qraf_engine* engine, int32_t rows);
  * runs projection by projection instead of as the split-K GEMM layer (fp32
  * products as at batch 1, summed in another order than the GEMM's); bit 3
  * (default off) = in steps that hold several rows of a sequence one behind
- * another (drafted tokens, prompt chunks) attention reads the positions that
- * those share once (qraf_hip_group_attention_dev: the same sums in another
- * order).  No reference counterpart (launch-count and traffic measures). */
+ * another (drafted tokens, prompt chunks), where those share enough positions
+ * for it to pay, attention reads them once (qraf_hip_group_attention_dev: the
+ * same sums in another order).  No reference counterpart (launch-count and traffic measures). */
 int qraf_engine_set_fusion(qraf_engine* engine, int32_t flags);
 /* Repetition penalty on the device for one sequence, set before its first
  * step (QRAF_HIP_ERR_STATE after): from then on every token the sequence is

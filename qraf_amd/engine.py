@@ -255,8 +255,8 @@ class Engine:
         of 2-8 rows run their projections on the multi-vector matvec where
         it covers them (default on; batch-1 arithmetic instead of the GEMM's).
         Bit 3: steps with several rows of a sequence one behind another read
-        the positions that they share once (default off; the same sums in
-        another order)."""
+        the positions that they share once, where that pays (default off;
+        the same sums in another order)."""
         call("qraf_engine_set_fusion", self.h, int(flags))
 
     def set_row_padding(self, rows: int) -> None:

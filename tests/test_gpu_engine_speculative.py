@@ -78,6 +78,38 @@ def test_steps_by_group_over_int8_pages_of_one_layer(hip, name):
         check_logits(b, a, name)
 
 
+@pytest.mark.parametrize("kv", [po.F32, po.F16, 102], ids=["f32", "f16", "i8"])
+@pytest.mark.parametrize("name", ["q4_gqa8_hd128", "q8_hd64_gqa3"])
+def test_long_steps_by_group(hip, name, kv):
+    """Steps whose rows share enough positions for attention by group (24 million keys' elements): prompt chunks up
+    to 1,900 positions of two sequences, drafts behind them, eager, captured and replayed, and single rows again.
+    One layer, so that int8 pages hold the same bytes either way."""
+    kw = SMALL[name][0]
+    toks = tokens(np.random.default_rng(9), kw, 2048)
+    heads, got = kw["kv_heads"] * (kw["hidden"] // kw["heads"]), []
+    for flags in (7, 15):
+        tf, _ = transformer(name, kv, max_batch=128, layers=1, max_seq=2048)
+        e = tf.engine
+        e.set_fusion(flags)
+        seqs, res = [e.seq_create(), e.seq_create()], []
+        def step(base, k):
+            rows = [(s, base + i + 7 * j) for j, s in enumerate(seqs) for i in range(k)]
+            pos = [p - 7 * (s == seqs[1]) for s, p in rows]
+            res.append(e.step([s for s, _ in rows], [toks[p] for _, p in rows], pos, logits=True)[0])
+        for at in range(0, 1900, 61):
+            step(at, 61)
+        assert 2 * 60 * 1891 * heads >= 24000000
+        for _ in range(3):
+            step(1952, 60)
+        step(2012, 1)
+        step(2013, 5)
+        got.append(res)
+        e.close()
+    assert not all(np.array_equal(a, b) for a, b in zip(*got))  # both forms ran
+    for a, b in zip(*got):
+        check_logits(b, a, name)
+
+
 def test_many_rows_by_group(hip):
     """Steps of the batched layers, whose attention writes the next product's planes."""
     rng = np.random.default_rng(2)
