@@ -38,11 +38,11 @@ struct GroupArgs {
     uint16_t *out_hi, *out_lo;
     float* part_o;              // [Hkv][slots][HD] unnormalised outputs of parts
     float2* part_ml;            // [Hkv][slots] their maxima (in powers of two) and sums
-    int* plan;                  // for the merge: prefix jobs, {column, which parts} of each row, pieces of the jobs
+    int4* plan;                 // for the merge: [n][2] where each row's parts lie (group_plan)
     int n, groups, H, Hkv, G, page_size, max_pages, max_ctx;
     float scale;
     int ps_log2, job_cap;       // page_size = 1 << ps_log2; prefix jobs at most
-    int tail_rows, tails;       // rows of a tail job; tail jobs
+    int tail_log2, tails;       // a tail job is 1 << tail_log2 rows; tail jobs
     long long slots;            // part slots of a KV head
 };
 
@@ -240,18 +240,25 @@ __device__ __forceinline__ T over_halves(T x, F op) {
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return op(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
 }
+// (16 neighbouring lanes; lanes l and l ^ 16)
 template <typename T, typename F>
-__device__ __forceinline__ T over_wave(T x, F op) {
+__device__ __forceinline__ T over_row(T x, F op) {
     auto in = [](T v) { return __builtin_bit_cast(int, v); };
     auto back = [](int v) { return __builtin_bit_cast(T, v); };
     x = op(x, back(gdpp<GDPP_XOR1>(in(x))));
     x = op(x, back(gdpp<GDPP_XOR2>(in(x))));
     x = op(x, back(gdpp<GDPP_ROR4>(in(x))));
-    x = op(x, back(gdpp<GDPP_ROR8>(in(x))));
+    return op(x, back(gdpp<GDPP_ROR8>(in(x))));
+}
+template <typename T, typename F>
+__device__ __forceinline__ T over_rows(T x, F op) {
     const unsigned u = __builtin_bit_cast(unsigned, x);
     const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    x = op(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
-    return over_halves(x, op);
+    return op(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
+}
+template <typename T, typename F>
+__device__ __forceinline__ T over_wave(T x, F op) {
+    return over_halves(over_rows(over_row(x, op), op), op);
 }
 // max(m, |x|, |y|) in one instruction (fmaxf quiets each operand first, in another one): a NaN may come of a NaN
 __device__ __forceinline__ float amax3(float m, float x, float y) {
@@ -378,8 +385,8 @@ __device__ __forceinline__ void wave_prefix_sum(int* v, int n) {
 // waves of a job of `cols` columns side by side along them (the others along the positions)
 __device__ __forceinline__ int waves_over(int cols) { return cols > 64 ? 4 : cols > 32 ? 2 : 1; }
 __device__ __forceinline__ int tiles_of(int positions, int cols) {
-    const int step = 32 * (GW / waves_over(cols));
-    return (positions + step - 1) / step;
+    const int s = cols > 64 ? 6 : cols > 32 ? 7 : 8;  // 32 positions times GW / waves_over(cols)
+    return (positions + (1 << s) - 1) >> s;
 }
 __device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return max(0, min(a.prefix[g], a.max_ctx)); }
 // a tail begins with the 16 positions that hold the prefix's end, one page's
@@ -420,7 +427,7 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
         const int c0 = (r - p.gs[g]) * a.G, b1 = (c0 + a.G - 1) / BLK;
         for (int b = c0 / BLK; b <= b1 && p.jb[g] + b < p.np; b++)
             atomicMax(&p.tiles[p.jb[g] + b], tiles_of(min(ctx, pre), min(BLK, all - BLK * b)));
-        if (ctx > pre) atomicMax(&p.tiles[p.np + r / a.tail_rows], tiles_of(ctx - tail_base(pre), BLK));
+        if (ctx > pre) atomicMax(&p.tiles[p.np + (r >> a.tail_log2)], tiles_of(ctx - tail_base(pre), BLK));
     }
     lds_sync();
     if (tid < 64) {
@@ -445,14 +452,16 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     }
     lds_sync();
     if (blockIdx.x == 0 && blockIdx.y == 0) {
-        for (int j = tid; j <= jobs; j += GTH) a.plan[1 + 2 * a.n + j] = p.upto[j];
+        // {first column among the prefix jobs' (-1: outside every group), pieces ahead of its block, of the next, of
+        // the one behind}, {which parts, pieces ahead of its tail, behind it}; a row's columns are in two blocks at most
         for (int r = tid; r < a.n; r += GTH) {
             const bool in = r >= p.gs[0] && r < p.gs[a.groups];
             const int g = in ? last_at(p.gs, a.groups, r) : 0;
-            a.plan[1 + 2 * r] = in ? p.jb[g] * BLK + (r - p.gs[g]) * a.G : -1;
-            a.plan[2 + 2 * r] = (min(p.ctx[r], p.pre[g]) > 0 ? 1 : 0) | (p.ctx[r] > p.pre[g] ? 2 : 0);
+            const int pos = p.jb[g] * BLK + (r - p.gs[g]) * a.G, b = in ? pos / BLK : 0, t = p.np + (r >> a.tail_log2);
+            a.plan[2 * r] = make_int4(in ? pos : -1, p.upto[min(b, jobs)], p.upto[min(b + 1, jobs)], p.upto[min(b + 2, jobs)]);
+            a.plan[2 * r + 1] = make_int4((min(p.ctx[r], p.pre[g]) > 0 ? 1 : 0) | (p.ctx[r] > p.pre[g] ? 2 : 0), p.upto[t],
+                                          p.upto[t + 1], 0);
         }
-        if (tid == 0) a.plan[0] = p.np;
     }
 }
 
@@ -489,7 +498,10 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
     // c ^ (column % 16), which spreads a wave's writes over the banks
     float* s_o = s_dyn;
-    uint4* s_q = (uint4*)s_dyn;   // [4][KS][2][64] q's operands lane by lane, during them
+    // q's operands, during them: [4 tiles of 32 columns][hi, lo][KS][2 halves][33] 16-byte pieces of 8 dims, the 33rd
+    // unused (a column's pieces, which neighbouring lanes write, are in banks of their own)
+    uint4* s_q = (uint4*)s_dyn;
+    constexpr int QB = 33, QLO = 2 * KS * QB, QT = 2 * QLO;
     GroupPlan plan;
     plan.tiles = (int*)(s_dyn + GW * 32 * HD);
     plan.upto = plan.tiles + a.job_cap + a.tails;
@@ -509,6 +521,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         half = lane >> 5;
     };
     const int kvh = blockIdx.y, w = blockIdx.x, G = a.G, psl = a.ps_log2, psm = (1 << psl) - 1;
+    const float inv_g = 1.f / (float)G;
 
     int jobs = 0, pieces = w + 1;
     int d_ctx = 0, d_pre = 0, d_first = 0, d_tiles = 0;  // DIRECT: the row's context, prefix, group's first row; prefix tiles
@@ -549,18 +562,20 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             const int tiles = __builtin_amdgcn_readfirstlane(plan.tiles[j]);
             const int n_of = (next & 0xFFFF) - (here & 0xFFFF);
             i_of = piece - (here & 0xFFFF);
-            ja = (int)((long long)i_of * tiles / n_of);
-            jend = (int)((long long)(i_of + 1) * tiles / n_of);
+            const int each = (int)((unsigned)tiles / (unsigned)n_of), odd = tiles - each * n_of;  // `odd` pieces of one more
+            ja = i_of * each + min(i_of, odd);
+            jend = ja + each + (i_of < odd ? 1 : 0);
             whole = n_of == 1;
         }
 
         // ---- the wave's place: qt of wq waves side by side along the job's columns, kw of wk along the positions
         bool tail = !DIRECT && j >= plan.np;
         int g, trow, first, cols, wq;  // group; the row whose table is read; first column (among all rows'), columns
+        int bfirst = 0, bcols = 0;     // those of the workgroup (of a prefix)
         if constexpr (DIRECT) {
             wq = 1;
-            first = w * G;
-            cols = G;
+            first = bfirst = w * G;
+            cols = bcols = G;
             // tiles: the prefix's, then the tail's
             jend = d_tiles + (d_ctx > d_pre ? (d_ctx - tail_base(d_pre) + 31) >> 5 : 0);
             tail = wave >= d_tiles;
@@ -568,8 +583,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             g = 0;
         } else if (tail) {             // a row's columns are 1, 2 or 4 waves'
             wq = 4;
-            const int side = 4 / a.tail_rows, c0 = 32 * (wave & (side - 1));
-            const int row = (j - plan.np) * a.tail_rows + (wave & 3) / side;
+            const int side = 4 >> a.tail_log2, c0 = 32 * (wave & (side - 1));
+            const int row = ((j - plan.np) << a.tail_log2) + ((wave & 3) >> (2 - a.tail_log2));
             const bool in = row < a.n && row >= plan.gs[0] && row < plan.gs[a.groups];
             trow = min(row, a.n - 1);
             g = in ? wave_last_at(plan.gs, a.groups, trow) : 0;
@@ -579,10 +594,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             g = wave_last_at(plan.jb, a.groups, j);
             const int b = j - plan.jb[g];
             trow = plan.gs[g];
-            cols = min(BLK, (plan.gs[g + 1] - trow) * G - BLK * b);
+            cols = bcols = min(BLK, (plan.gs[g + 1] - trow) * G - BLK * b);
             wq = waves_over(cols);
             const int c0 = 32 * (wave & (wq - 1));
-            first = trow * G + BLK * b + c0;
+            bfirst = trow * G + BLK * b;
+            first = bfirst + c0;
             cols = min(32, cols - c0);
         }
         wq = __builtin_amdgcn_readfirstlane(wq);
@@ -598,8 +614,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         ConstInt* ptab = table_of(trow);
 
         // ---- the lane's column (past the last: that again, not written), row and limit
-        const int ab = min(first + min(col, max(cols - 1, 0)), a.n * G - 1), r = ab / G;
-        const float* qrow = a.q + ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
+        const int ab = min(first + min(col, max(cols - 1, 0)), a.n * G - 1);
+        const int r = DIRECT ? w : (int)(((float)ab + 0.5f) * inv_g);  // (ab < 2^17: exact)
+        const size_t orow = ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
         const int ctx = DIRECT ? d_ctx : plan.ctx[r];
         int lim = cols == 0 ? 0 : tail ? ctx : min(ctx, pre);
         // behind the last position that some of the wave's columns attends to
@@ -685,37 +702,49 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         pg0 = more ? pg0 : 0;
         pg1 = more ? pg1 : 0;
 
-        // ---- q of 32 columns as fp16 hi + lo, scaled per column, by one wave for all that share them
-        if (kw == 0) {
-            float4 qraw[2 * KS];
+        // ---- q as fp16 hi + lo, scaled per column: 32 (HD 128) or 16 neighbouring lanes to a column, 16 bytes each,
+        // all waves (a lane to a column, as the products take it, is a line of memory per lane and load: 2 us more)
+        auto stage_q = [&](auto tiles_c) {
+            constexpr int NQ = decltype(tiles_c)::value * 32 * HD / (4 * GTH), CPL = 256 / HD;
+            const int d0 = 4 * (lane % (HD / 4)), c0 = wave * NQ * CPL + lane / (HD / 4);
+            float4 x[NQ];
 #pragma unroll
-            for (int kk = 0; kk < KS; kk++) {
-                const int d = I8 ? 32 * (kk >> 1) + 16 * half + 8 * (kk & 1) : 16 * kk + 8 * half;
-                qraw[2 * kk] = *(const float4*)(qrow + d);
-                qraw[2 * kk + 1] = *(const float4*)(qrow + d + 4);
+            for (int u = 0; u < NQ; u++) {
+                const int c = c0 + u * CPL;
+                int row, h;
+                if (!DIRECT && tail) {
+                    const int per = 7 - a.tail_log2;  // BLK columns over the rows
+                    row = min(((j - plan.np) << a.tail_log2) + (c >> per), a.n - 1);
+                    h = min(c & ((1 << per) - 1), G - 1);
+                } else {
+                    const int at = bfirst + min(c, bcols - 1);
+                    row = DIRECT ? w : (int)(((float)at + 0.5f) * inv_g);
+                    h = at - row * G;
+                }
+                x[u] = *(const float4*)(a.q + (uint32_t)((row * a.H + kvh * G + h) * HD + d0));
             }
             load_k(more ? t : 0);  // (behind q, which is waited for alone)
-            uint4* qop = s_q + qt * KS * 128 + lane;
-            float mx = 0.f;
+            const int kk = I8 ? 2 * (d0 >> 5) + ((d0 >> 3) & 1) : d0 >> 4, hf = I8 ? (d0 >> 4) & 1 : (d0 >> 3) & 1;
 #pragma unroll
-            for (int k = 0; k < 2 * KS; k++)
-                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(qraw[k].x), fabsf(qraw[k].y)), fmaxf(fabsf(qraw[k].z), fabsf(qraw[k].w))));
-            mx = over_halves(mx, fmax2);
-            const int e = mx <= 3.0e38f ? unit_exp(mx) : 0;
-            const float sg = copysignf(ldexpf(1.f, e), a.scale);  // (scores take the scale's magnitude)
-#pragma unroll
-            for (int kk = 0; kk < KS; kk++) {
-                const float4 x = qraw[2 * kk], y = qraw[2 * kk + 1];
-                const float v[8] = {x.x * sg, x.y * sg, x.z * sg, x.w * sg, y.x * sg, y.y * sg, y.z * sg, y.w * sg};
-                f16x8 hi, lw;
-                split8(v, hi, lw);
-                qop[128 * kk] = __builtin_bit_cast(uint4, hi);
-                qop[128 * kk + 64] = __builtin_bit_cast(uint4, lw);
+            for (int u = 0; u < NQ; u++) {
+                const int c = c0 + u * CPL;
+                float mx = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
+                mx = over_row(mx, fmax2);
+                if (HD == 128) mx = over_rows(mx, fmax2);
+                const int e = mx <= 3.0e38f ? unit_exp(mx) : 0;
+                const float sg = copysignf(ldexpf(1.f, e), a.scale);  // (scores take the scale's magnitude)
+                f16x2 h0, l0, h1, l1;
+                split2(x[u].x * sg, x[u].y * sg, h0, l0);
+                split2(x[u].z * sg, x[u].w * sg, h1, l1);
+                uint2* to = (uint2*)(s_q + (c >> 5) * QT + (2 * kk + hf) * QB + (c & 31)) + ((d0 >> 2) & 1);
+                to[0] = make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1));
+                to[2 * QLO] = make_uint2(__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1));
+                if (d0 == 0) s_qs[c] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e);
             }
-            if (half == 0) s_qs[qt * 32 + col] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e);
-        } else {
-            load_k(more ? t : 0);
-        }
+        };
+        if (DIRECT || wq == 1) stage_q(std::integral_constant<int, 1>());
+        else if (wq == 2) stage_q(std::integral_constant<int, 2>());
+        else stage_q(std::integral_constant<int, 4>());
         if (!TURNS) load_v(more ? t : 0);  // (behind q: their registers)
         lds_sync();
         const float qs = s_qs[qt * 32 + col];  // scores in powers of two
@@ -730,7 +759,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 
         while (more) {
             lanes_again();
-            const uint4* qtile = s_q + qt * KS * 128 + lane;
+            const uint4* qtile = s_q + qt * QT + half * QB + col;
             const bool edge = t < lo || t + 32 > least;  // some column does not attend to all 32
             // ---- scores
             f32x16 s;
@@ -758,8 +787,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
                     f16x8 kh, kl;
                     split8(v, sg, kh, kl);
-                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[128 * kk]);
-                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[128 * kk + 64]);
+                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[2 * QB * kk]);
+                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[QLO + 2 * QB * kk]);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh, s, 0, 0, 0);
@@ -774,8 +803,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     } else {
                         kf = tl.k[kk];
                     }
-                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[128 * kk]);
-                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[128 * kk + 64]);
+                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[2 * QB * kk]);
+                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[QLO + 2 * QB * kk]);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh, s, 0, 0, 0);
                 }
@@ -1039,7 +1068,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab +
                                 (size_t)BLK * ((here & 0xFFFF) - (here >> 16) + i_of);
             const bool mine = col < cols, part = mine && !alone && (tail || any_pre);
-            s_to[qt * 32 + col] = mine && alone ? (long long)(qrow - a.q) : part ? ~(long long)(slot * HD) : NOWHERE;
+            s_to[qt * 32 + col] = mine && alone ? (long long)orow : part ? ~(long long)(slot * HD) : NOWHERE;
             s_by[qt * 32 + col] = DIRECT && ctx == 0 ? 0.f : alone ? 1.f / L : 1.f;
             if (part) a.part_ml[slot] = make_float2(M, L);
         }
@@ -1047,7 +1076,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         lds_sync();
         auto join = [&](auto wk_c) {
             constexpr int WK = decltype(wk_c)::value, WQ = GW / WK;
-#pragma unroll 2
+#pragma unroll 4
             for (int e = tid; e < WQ * 32 * (HD / 4); e += GTH) {
                 const int c = e / (HD / 4), d = e % (HD / 4) * 4, cq = c >> 5, ci = c & 31;
                 const long long to = s_to[c];
@@ -1088,17 +1117,16 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
     const int r = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (h >= a.H) return;
     const int lane = threadIdx.x & 63, kvh = h / a.G, hh = h - kvh * a.G;
-    const int np = a.plan[0], pos = a.plan[1 + 2 * r], which = a.plan[2 + 2 * r];
-    if (pos < 0) return;  // outside every group
-    const int* upto = a.plan + 1 + 2 * a.n;
+    const int4 at0 = a.plan[2 * r], at1 = a.plan[2 * r + 1];
+    if (at0.x < 0) return;  // outside every group
     // (first slot, parts) of the prefix and of the tail
     int first[2] = {0, 0}, count[2] = {0, 0};
-    const int jobs[2] = {(pos + hh) / BLK, np + r / a.tail_rows};
+    const bool second = (at0.x + hh) / BLK != at0.x / BLK;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const int x = upto[jobs[k]], y = upto[jobs[k] + 1];
+        const int x = k ? at1.y : second ? at0.z : at0.y, y = k ? at1.z : second ? at0.w : at0.z;
         first[k] = (x & 0xFFFF) - (x >> 16);
-        count[k] = which >> k & 1 ? (y & 0xFFFF) - (x & 0xFFFF) : 0;
+        count[k] = at1.x >> k & 1 ? (y & 0xFFFF) - (x & 0xFFFF) : 0;
     }
     const int all = count[0] + count[1];
     const size_t out = ((size_t)r * a.H + h) * HD;
@@ -1151,7 +1179,7 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
 static int group_grid(int Hkv) { return std::max(1, 256 / Hkv); }
 
 struct GroupSizes {
-    int job_cap, tail_rows, tails;
+    int job_cap, tail_log2, tails;
     long long slots;
     size_t plan_bytes, ml_bytes, o_bytes;
 };
@@ -1159,10 +1187,10 @@ static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
     const int G = H / Hkv;
     GroupSizes z;
     z.job_cap = (int)((long long)n * G / BLK) + groups;
-    z.tail_rows = G <= 32 ? 4 : G <= 64 ? 2 : 1;
-    z.tails = (n + z.tail_rows - 1) / z.tail_rows;
+    z.tail_log2 = G <= 32 ? 2 : G <= 64 ? 1 : 0;
+    z.tails = (n + (1 << z.tail_log2) - 1) >> z.tail_log2;
     z.slots = 2ll * n * G + (long long)BLK * group_grid(Hkv);
-    z.plan_bytes = ((size_t)(2 + 2 * n + z.job_cap + z.tails) * 4 + 255) / 256 * 256;
+    z.plan_bytes = ((size_t)n * 32 + 255) / 256 * 256;
     z.ml_bytes = ((size_t)Hkv * z.slots * sizeof(float2) + 255) / 256 * 256;
     z.o_bytes = (size_t)Hkv * z.slots * hd * 4;
     return z;
@@ -1174,7 +1202,7 @@ static size_t group_lds(int hd, int n, int groups, const GroupSizes& z) {
 static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
     const int G = H / Hkv;
     return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 &&
-           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
+           (long long)n * H * hd <= 1 << 30 && group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
 }
 
 // Small calls: one launch without a plan, a workgroup per (row, KV head), which saves the plan (3 us) and the launch
@@ -1253,11 +1281,11 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
     if (group_tiles(n, groups, H, Hkv, hd, page_size)) {
         const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
         a.job_cap = z.job_cap;
-        a.tail_rows = z.tail_rows;
+        a.tail_log2 = z.tail_log2;
         a.tails = z.tails;
         a.slots = z.slots;
         while ((1 << a.ps_log2) < page_size) a.ps_log2++;
-        a.plan = (int*)ws;
+        a.plan = (int4*)ws;
         a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
         a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
         const int gx = group_grid(Hkv);
