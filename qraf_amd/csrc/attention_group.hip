@@ -312,6 +312,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo
         lo[i] = l[0], lo[i + 1] = l[1];
     }
 }
+// the fp16 halves of a dword that are not numbers, as 0x1 in each (their exponent is all ones)
+__device__ __forceinline__ uint32_t odd16(uint32_t u) { return (((u & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u; }
 // 4 int8 (one dword) -> 4 fp16, exactly: the biased byte q + 128 under the
 // exponent of 1024, less 1152
 __device__ __forceinline__ uint2 widen4(uint32_t w) {
@@ -487,23 +489,28 @@ struct GroupTile<HD, (int)DT_F32> {
 };
 
 // DIRECT: no plan; workgroup (r, KV head) takes row r alone, its prefix and its tail one behind the other.
+// LDS floats for the tiles: the waves' outputs, [GW][32][hd]; before them q, and two f32 tiles that waves share
+constexpr int tile_floats(int hd) { return GW * 32 * hd; }
+
 template <int HD, int KV, bool DIRECT>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
     extern __shared__ __align__(16) float s_dyn[];
     __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK], s_qs[BLK];
+    __shared__ float s_ku[2][4];  // f32 tiles that four waves share: one over K's units, V's, of 8 positions each
+    __shared__ int s_vu[2][4];
     __shared__ long long s_to[BLK];  // where a column's output goes: an element of out, or ~ one of part_o
     constexpr long long NOWHERE = 1ll << 62;
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
     // c ^ (column % 16), which spreads a wave's writes over the banks
     float* s_o = s_dyn;
-    // q's operands, during them: [4 tiles of 32 columns][hi, lo][KS][2 halves][33] 16-byte pieces of 8 dims, the 33rd
+    // q's operands, during them: [lo, hi][4 tiles of 32 columns][KS][2 halves][33] 16-byte pieces of 8 dims, the 33rd
     // unused (a column's pieces, which neighbouring lanes write, are in banks of their own)
-    uint4* s_q = (uint4*)s_dyn;
-    constexpr int QB = 33, QLO = 2 * KS * QB, QT = 2 * QLO;
+    constexpr int QB = 33, QT = 2 * KS * QB, QHI = 4 * QT;
+    uint4 *s_qlo = (uint4*)s_dyn, *s_qhi = s_qlo + QHI;
     GroupPlan plan;
-    plan.tiles = (int*)(s_dyn + GW * 32 * HD);
+    plan.tiles = (int*)(s_dyn + tile_floats(HD));
     plan.upto = plan.tiles + a.job_cap + a.tails;
     plan.jb = plan.upto + a.job_cap + a.tails + 1;
     plan.gs = plan.jb + a.groups + 1;
@@ -695,6 +702,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         int i = DIRECT ? wave : ja;
         int t = __builtin_amdgcn_readfirstlane(DIRECT ? base + 32 * (i - (tail ? d_tiles : 0)) : base + (i * wk + kw) * 32);
         const int dt = 32 * wk;
+        const bool shared = F32 && !DIRECT && !tail && wq == 4;
         bool more = i < jend && (DIRECT || t < kend);
         ids(more ? t : 0);
         // No load of K and V depends on a branch, here and below: where paths with more and with fewer loads behind
@@ -736,9 +744,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 f16x2 h0, l0, h1, l1;
                 split2(x[u].x * sg, x[u].y * sg, h0, l0);
                 split2(x[u].z * sg, x[u].w * sg, h1, l1);
-                uint2* to = (uint2*)(s_q + (c >> 5) * QT + (2 * kk + hf) * QB + (c & 31)) + ((d0 >> 2) & 1);
-                to[0] = make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1));
-                to[2 * QLO] = make_uint2(__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1));
+                uint2* to = (uint2*)(s_qlo + (c >> 5) * QT + (2 * kk + hf) * QB + (c & 31)) + ((d0 >> 2) & 1);
+                to[0] = make_uint2(__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1));
+                to[2 * QHI] = make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1));
                 if (d0 == 0) s_qs[c] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e);
             }
         };
@@ -757,9 +765,248 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
             for (int x = 0; x < 16; x++) o[d][x] = 0.f;
 
-        while (more) {
+        if constexpr (F32 && !DIRECT) {
+            // f32 tiles of more than 64 columns: the four waves side by side load and split a quarter of a tile each, 8
+            // positions, for all of them (alone each would split it all, and a lane to a position reads a line of memory
+            // per lane).  The tiles lie where q's hi halves were, which stay in registers.  K's and V's powers of two are
+            // those of the 8 positions; V's enter through p, over the running one.
+            if (shared) {
+                constexpr int NP = HD / 64, PCS = HD / 8, RP = 64 / PCS;  // K: passes, pieces of a row, rows of a pass
+                constexpr int KP = 2 * QT, TP = KP + 2 * 2 * 64 * DT;      // 16-byte pieces of K (hi, lo), of a tile
+                static_assert((QHI + 2 * TP) * 16 <= 4 * tile_floats(HD), "q's lo halves and a tile of each kw");
+                uint4* tile = s_qhi + kw * TP;
+                f16x8 qh[KS];
+#pragma unroll
+                for (int kk = 0; kk < KS; kk++) qh[kk] = __builtin_bit_cast(f16x8, s_qhi[qt * QT + half * QB + col + 2 * QB * kk]);
+                // behind the last position that some column of the block attends to
+                int kl = 0;
+#pragma unroll
+                for (int c = 0; c < BLK; c += 64)
+                    kl = max(kl, plan.ctx[(int)(((float)(bfirst + min(lane + c, bcols - 1)) + 0.5f) * inv_g)]);
+                kl = max(min(__builtin_amdgcn_readfirstlane(over_wave(kl, imax2)), pre), 1) - 1;
+                float kx[NP][8];
+                typedef float vpart __attribute__((ext_vector_type(NP)));
+                vpart vx[8];
+                auto id_of = [&](int at) { return ptab[min(at + 8 * qt, kl) >> psl]; };
+                auto request = [&](int at, int id) {
+                    const char *kp = block(a.kc, id), *vp = block(a.vc, id);
+                    lanes_again();
+#pragma unroll
+                    for (int u = 0; u < NP; u++) {
+                        const int pc = min(at + 8 * qt + u * RP + lane / PCS, kl) & psm;
+                        const uint32_t off = (uint32_t)(pc * HD + 8 * (lane % PCS)) * 4u;
+                        const float4 x = *(const float4*)(kp + off), y = *(const float4*)(kp + (off + 16u));
+                        kx[u][0] = x.x, kx[u][1] = x.y, kx[u][2] = x.z, kx[u][3] = x.w;
+                        kx[u][4] = y.x, kx[u][5] = y.y, kx[u][6] = y.z, kx[u][7] = y.w;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        vx[k] = *(const vpart*)(vp + (uint32_t)(((min(at + 8 * qt + k, kl) & psm) * HD + NP * lane) * 4));
+                };
+                // the power of two for values of which |.| is at most mx, or (some are no numbers) as `find` says
+                auto unit_of = [&](float mx, auto find) {
+                    if (__any(!(mx <= 3.0e38f))) mx = find();
+                    return __builtin_amdgcn_readfirstlane(unit_exp(over_wave(mx, fmax2)));
+                };
+                t = __builtin_amdgcn_readfirstlane(t);
+                request(t, id_of(t));
+                int id = id_of(t + dt);
+                for (; i < jend; i++, t += dt) {
+                    lds_sync();  // what lay there is read
+                    // ---- this wave's quarter
+                    {
+                        float mx = 0.f;
+#pragma unroll
+                        for (int u = 0; u < NP; u++)
+#pragma unroll
+                            for (int k = 0; k < 8; k += 2) mx = amax3(mx, kx[u][k], kx[u][k + 1]);
+                        const int e = unit_of(mx, [&] {
+                            float y = 0.f;
+                            for (int u = 0; u < NP; u++)
+                                for (int k = 0; k < 8; k++) y = fabsf(kx[u][k]) <= 3.0e38f ? fmaxf(y, fabsf(kx[u][k])) : y;
+                            return y;
+                        });
+                        const float sg = ldexpf(1.f, e);
+                        lanes_again();
+#pragma unroll
+                        for (int u = 0; u < NP; u++) {
+                            f16x8 h, lw;
+                            split8(kx[u], sg, h, lw);
+                            const int p = 8 * qt + u * RP + lane / PCS;  // of A's row with key_of(row) = p
+                            uint4* to = tile + (lane % PCS) * QB + ((p & 0x13) | (p >> 1 & 4) | (p << 1 & 8));
+                            to[0] = __builtin_bit_cast(uint4, h);
+                            to[QT] = __builtin_bit_cast(uint4, lw);
+                        }
+                        mx = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2)
+#pragma unroll
+                            for (int c = 0; c < NP; c++) mx = amax3(mx, vx[k][c], vx[k + 1][c]);
+                        const int ev = unit_of(mx, [&] {
+                            float y = 0.f;
+                            for (int k = 0; k < 8; k++)
+                                for (int c = 0; c < NP; c++) y = fabsf(vx[k][c]) <= 3.0e38f ? fmaxf(y, fabsf(vx[k][c])) : y;
+                            return y;
+                        });
+                        const float vg = ldexpf(1.f, ev);
+                        lanes_again();
+#pragma unroll
+                        for (int c = 0; c < NP; c++) {
+                            float x[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) x[k] = vx[k][c];
+                            f16x8 h, lw;
+                            split8(x, vg, h, lw);
+                            const int dim = NP * lane + c;
+                            uint4* to = tile + KP + (dim % DT * 2 + (qt >> 1)) * 64 + (qt & 1) * 32 + dim / DT;
+                            to[0] = __builtin_bit_cast(uint4, h);
+                            to[2 * 64 * DT] = __builtin_bit_cast(uint4, lw);
+                        }
+                        if (lane == 0) {
+                            s_ku[kw][qt] = ldexpf(1.f, -e);
+                            s_vu[kw][qt] = ev;
+                        }
+                    }
+                    lds_sync();
+                    request(t + dt, id);
+                    id = id_of(t + 2 * dt);
+                    if (t >= kend) continue;
+                    const bool edge = t + 32 > least;
+                    // ---- scores
+                    lanes_again();
+                    f32x16 s;
+#pragma unroll
+                    for (int x = 0; x < 16; x++) s[x] = 0.f;
+                    const uint4 *kt = tile + half * QB + col, *qtile = s_qlo + qt * QT + half * QB + col;
+                    uint4 kf[2][3];  // a product ahead, and no more of them: registers
+                    kf[0][0] = kt[0], kf[0][1] = kt[QT], kf[0][2] = qtile[0];
+#pragma unroll
+                    for (int kk = 0; kk < KS; kk++) {
+                        if (kk + 1 < KS) {
+                            kf[(kk + 1) & 1][0] = kt[2 * QB * (kk + 1)];
+                            kf[(kk + 1) & 1][1] = kt[QT + 2 * QB * (kk + 1)];
+                            kf[(kk + 1) & 1][2] = qtile[2 * QB * (kk + 1)];
+                        }
+                        const f16x8 kh = __builtin_bit_cast(f16x8, kf[kk & 1][0]), klo = __builtin_bit_cast(f16x8, kf[kk & 1][1]);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(klo, qh[kk], s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, __builtin_bit_cast(f16x8, kf[kk & 1][2]), s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[kk], s, 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    const float fs[2] = {qs * s_ku[kw][half], qs * s_ku[kw][2 + half]};
+                    const int e0 = s_vu[kw][half], e1 = s_vu[kw][2 + half];
+                    const int e = __builtin_amdgcn_readfirstlane(over_halves(min(e0, e1), imin2));
+                    if (e < vexp) {
+                        const float f = ldexpf(1.f, max(e - vexp, -126));
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int x = 0; x < 16; x++) o[d][x] *= f;
+                        vexp = e;
+                    }
+                    // ---- softmax
+                    if (edge) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            s[x] = t + 16 * (x >> 3) + 8 * half + (x & 7) < lim ? s[x] : -INFINITY;
+                    }
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        m0 = fmaxf(m0, s[x]);
+                        m1 = fmaxf(m1, s[x + 8]);
+                    }
+                    float mt = fmaxf(m0 == -INFINITY ? m0 : m0 * fs[0], m1 == -INFINITY ? m1 : m1 * fs[1]);
+                    mt = over_halves(mt, fmax2);
+                    if (__any(mt > m + GROWTH)) {
+                        const float mn = fmaxf(m, mt), alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                        l *= alpha;
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int x = 0; x < 16; x++) o[d][x] *= alpha;
+                        m = mn;
+                    }
+                    const float sub = P_UNIT - (m == -INFINITY ? 0.f : m);
+                    const float vf[2] = {ldexpf(1.f, max(vexp - e0, -126)), ldexpf(1.f, max(vexp - e1, -126))};
+                    f16x8 ph[2], pl[2];
+#pragma unroll
+                    for (int b2 = 0; b2 < 2; b2++) {
+                        float p[8];
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {
+                            p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * b2 + x], fs[b2], sub));
+                            if (edge) p[x] = s[8 * b2 + x] == -INFINITY ? 0.f : p[x];
+                            l += p[x];
+                        }
+                        split8(p, vf[b2], ph[b2], pl[b2]);
+                    }
+                    // ---- outputs
+                    const uint4* vt = tile + KP + half * 32 + col;
+                    bool bad = false;
+                    if (edge) {  // (an infinity or NaN where some columns do not attend, as below)
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (int d = 0; d < 2 * DT; d++) {
+                            const uint4 u = vt[64 * d];
+                            odd |= odd16(u.x) | odd16(u.y) | odd16(u.z) | odd16(u.w);
+                        }
+                        bad = __any(odd != 0);
+                    }
+                    if (bad) {
+                        f16x8 att[2];
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            att[x >> 3][x & 7] = t + 16 * (x >> 3) + 8 * half + (x & 7) < lim ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            f32x16 c;
+#pragma unroll
+                            for (int x = 0; x < 16; x++) c[x] = 0.f;
+#pragma unroll
+                            for (int b2 = 0; b2 < 2; b2++) {
+                                uint4 f = vt[64 * (2 * d + b2)];
+                                f = make_uint4(odd16(f.x) * 0x3C00u, odd16(f.y) * 0x3C00u, odd16(f.z) * 0x3C00u, odd16(f.w) * 0x3C00u);
+                                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), att[b2], c, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int x = 0; x < 16; x++) o[d][x] = c[x] > 0.f ? NAN : o[d][x];
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        uint4 uh[2], ul[2];
+#pragma unroll
+                        for (int b2 = 0; b2 < 2; b2++) {
+                            uh[b2] = vt[64 * (2 * d + b2)];
+                            ul[b2] = vt[2 * 64 * DT + 64 * (2 * d + b2)];
+                        }
+                        if (bad) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                uint32_t *hu = (uint32_t*)&uh[k >> 2] + (k & 3), *lu = (uint32_t*)&ul[k >> 2] + (k & 3);
+                                const uint32_t keep = ~(odd16(*hu) * 0xFFFFu);
+                                *hu &= keep;
+                                *lu &= keep;
+                            }
+                        }
+#pragma unroll
+                        for (int b2 = 0; b2 < 2; b2++) {
+                            const f16x8 vh = __builtin_bit_cast(f16x8, uh[b2]), vl = __builtin_bit_cast(f16x8, ul[b2]);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[b2], o[d], 0, 0, 0);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[b2], o[d], 0, 0, 0);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[b2], o[d], 0, 0, 0);
+                        }
+                        if (d & 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                tl = {};  // (nothing of it is held across the loop)
+            }
+        }
+        if (!shared) while (more) {
             lanes_again();
-            const uint4* qtile = s_q + qt * QT + half * QB + col;
+            const uint4* qtile = s_qlo + qt * QT + half * QB + col;
             const bool edge = t < lo || t + 32 > least;  // some column does not attend to all 32
             // ---- scores
             f32x16 s;
@@ -787,8 +1034,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
                     f16x8 kh, kl;
                     split8(v, sg, kh, kl);
-                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[2 * QB * kk]);
-                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[QLO + 2 * QB * kk]);
+                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[QHI + 2 * QB * kk]);
+                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[2 * QB * kk]);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh, s, 0, 0, 0);
@@ -803,8 +1050,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     } else {
                         kf = tl.k[kk];
                     }
-                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[2 * QB * kk]);
-                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[QLO + 2 * QB * kk]);
+                    const f16x8 qh = __builtin_bit_cast(f16x8, qtile[QHI + 2 * QB * kk]);
+                    const f16x8 ql = __builtin_bit_cast(f16x8, qtile[2 * QB * kk]);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh, s, 0, 0, 0);
                 }
@@ -923,8 +1170,6 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     // An infinity or NaN in V times a weight of 0 is NaN, in columns that do not attend to it.
                     // Tiles that hold one: NaN to the outputs of the columns that do (a product of indicators
                     // counts them), then zeros in its place.
-                    // the fp16 halves of a dword that are not numbers, as 0x1 in each (their exponent is all ones)
-                    auto odd16 = [](uint32_t u) { return (((u & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u; };
                     bool bad = false;
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
@@ -1196,7 +1441,7 @@ static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
     return z;
 }
 static size_t group_lds(int hd, int n, int groups, const GroupSizes& z) {
-    return (size_t)GW * 32 * hd * 4 + (size_t)(2 * (z.job_cap + z.tails) + 1 + 3 * groups + 2 + n) * 4;
+    return (size_t)tile_floats(hd) * 4 + (size_t)(2 * (z.job_cap + z.tails) + 1 + 3 * groups + 2 + n) * 4;
 }
 // shapes of the tiles (their LDS bounds what few very wide layouts would need)
 static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
@@ -1294,7 +1539,7 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
 #define QH_GROUP_TILE(HDv, KVv)                                                                                            \
     if (hd == HDv && kv_dtype == KVv) {                                                                                    \
         if (direct)                                                                                                        \
-            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true>), dim3(n, Hkv), dim3(GTH), GW * 32 * HDv * 4, st, a); \
+            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true>), dim3(n, Hkv), dim3(GTH), tile_floats(HDv) * 4, st, a); \
         else hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false>), dim3(gx, Hkv), dim3(GTH), lds, st, a);          \
     }
         QH_GROUP_TILE(64, DT_F32) QH_GROUP_TILE(64, DT_F16) QH_GROUP_TILE(64, DT_I8)
