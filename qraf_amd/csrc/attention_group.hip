@@ -212,9 +212,15 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
 // matrix products (lo x lo is below 2^-22).  int8 scales: K's on the scores, V's
 // on p.  Sums in fp32.
 //
-// K of the next tile is requested behind this tile's scores, V behind its
-// outputs, straight into registers (a wave shares no tile with others but through the
-// caches): two waves per SIMD cover each other's waits.
+// Up to 64 columns, tails and int8: K of the next tile is requested behind this
+// tile's scores, V behind its outputs, straight into the wave's registers; two waves
+// per SIMD cover each other's waits.  More columns: four waves share tiles in LDS.
+// Measured (16/2 heads of 128, us): 48 sequences of 5 rows at 128..4,096 fp16 positions
+// 40, of which the tiles 34 (108 MB at 5 TB/s of HBM while they run, beside 6 of plan
+// and prologue); 128 rows behind 2,048 shared and 512 own ones 28, half of it plan,
+// prologue and join; 4 chunks of 128 rows at 400..2,000 f32 positions 43; 256 rows of
+// 32,768: fp16 197 (348 TFLOP/s of products with q and p in 22 bits: 697 of the
+// matrix cores'), int8 248, f32 280.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -702,7 +708,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         int i = DIRECT ? wave : ja;
         int t = __builtin_amdgcn_readfirstlane(DIRECT ? base + 32 * (i - (tail ? d_tiles : 0)) : base + (i * wk + kw) * 32);
         const int dt = 32 * wk;
-        const bool shared = F32 && !DIRECT && !tail && wq == 4;
+        const bool shared = !DIRECT && !I8 && !tail && wq == 4;
         bool more = i < jend && (DIRECT || t < kend);
         ids(more ? t : 0);
         // No load of K and V depends on a branch, here and below: where paths with more and with fewer loads behind
@@ -765,14 +771,16 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
             for (int x = 0; x < 16; x++) o[d][x] = 0.f;
 
-        if constexpr (F32 && !DIRECT) {
-            // f32 tiles of more than 64 columns: the four waves side by side load and split a quarter of a tile each, 8
-            // positions, for all of them (alone each would split it all, and a lane to a position reads a line of memory
-            // per lane).  The tiles lie where q's hi halves were, which stay in registers.  K's and V's powers of two are
-            // those of the 8 positions; V's enter through p, over the running one.
+        if constexpr (!DIRECT && !I8) {
+            // Tiles of more than 64 columns: the four waves side by side load a quarter of a tile each, 8 positions, and
+            // write it as operands for all of them, f32 split (alone each would load and split it all, and a lane to a
+            // position reads a line of memory per lane).  The tiles lie where q's hi halves were, which stay in
+            // registers.  f32: K's and V's powers of two are those of the 8 positions; V's enter through p, over the
+            // running one.  256 rows of 32,768 positions, 16/2 heads of 128: f32 280 us for 444, fp16 197 for 221; int8
+            // gained nothing (254 for 253) and goes on alone.
             if (shared) {
                 constexpr int NP = HD / 64, PCS = HD / 8, RP = 64 / PCS;  // K: passes, pieces of a row, rows of a pass
-                constexpr int KP = 2 * QT, TP = KP + 2 * 2 * 64 * DT;      // 16-byte pieces of K (hi, lo), of a tile
+                constexpr int HL = F32 ? 2 : 1, KP = HL * QT, VP = 2 * 64 * DT, TP = KP + HL * VP;  // 16-byte pieces: hi, lo
                 static_assert((QHI + 2 * TP) * 16 <= 4 * tile_floats(HD), "q's lo halves and a tile of each kw");
                 uint4* tile = s_qhi + kw * TP;
                 f16x8 qh[KS];
@@ -784,24 +792,32 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 for (int c = 0; c < BLK; c += 64)
                     kl = max(kl, plan.ctx[(int)(((float)(bfirst + min(lane + c, bcols - 1)) + 0.5f) * inv_g)]);
                 kl = max(min(__builtin_amdgcn_readfirstlane(over_wave(kl, imax2)), pre), 1) - 1;
-                float kx[NP][8];
                 typedef float vpart __attribute__((ext_vector_type(NP)));
-                vpart vx[8];
+                std::conditional_t<F32, float[NP][8], int> kx;
+                std::conditional_t<F32, vpart[8], int> vx;
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                std::conditional_t<F16, u32x4[NP], int> kr, vr;  // 8 dims of K, 8 positions of V
                 auto id_of = [&](int at) { return ptab[min(at + 8 * qt, kl) >> psl]; };
                 auto request = [&](int at, int id) {
                     const char *kp = block(a.kc, id), *vp = block(a.vc, id);
                     lanes_again();
 #pragma unroll
                     for (int u = 0; u < NP; u++) {
-                        const int pc = min(at + 8 * qt + u * RP + lane / PCS, kl) & psm;
-                        const uint32_t off = (uint32_t)(pc * HD + 8 * (lane % PCS)) * 4u;
-                        const float4 x = *(const float4*)(kp + off), y = *(const float4*)(kp + (off + 16u));
-                        kx[u][0] = x.x, kx[u][1] = x.y, kx[u][2] = x.z, kx[u][3] = x.w;
-                        kx[u][4] = y.x, kx[u][5] = y.y, kx[u][6] = y.z, kx[u][7] = y.w;
+                        const uint32_t off = (uint32_t)((min(at + 8 * qt + u * RP + lane / PCS, kl) & psm) * HD + 8 * (lane % PCS));
+                        if constexpr (F32) {
+                            const float4 x = *(const float4*)(kp + 4u * off), y = *(const float4*)(kp + (4u * off + 16u));
+                            kx[u][0] = x.x, kx[u][1] = x.y, kx[u][2] = x.z, kx[u][3] = x.w;
+                            kx[u][4] = y.x, kx[u][5] = y.y, kx[u][6] = y.z, kx[u][7] = y.w;
+                        } else {
+                            kr[u] = *(const u32x4*)(kp + 2u * off);
+                            vr[u] = *(const u32x4*)(vp + 2u * (uint32_t)((64 * u + lane) * a.page_size + ((at + 8 * qt) & psm)));
+                        }
                     }
+                    if constexpr (F32) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        vx[k] = *(const vpart*)(vp + (uint32_t)(((min(at + 8 * qt + k, kl) & psm) * HD + NP * lane) * 4));
+                        for (int k = 0; k < 8; k++)
+                            vx[k] = *(const vpart*)(vp + (uint32_t)(((min(at + 8 * qt + k, kl) & psm) * HD + NP * lane) * 4));
+                    }
                 };
                 // the power of two for values of which |.| is at most mx, or (some are no numbers) as `find` says
                 auto unit_of = [&](float mx, auto find) {
@@ -814,7 +830,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 for (; i < jend; i++, t += dt) {
                     lds_sync();  // what lay there is read
                     // ---- this wave's quarter
-                    {
+                    if constexpr (F32) {
                         float mx = 0.f;
 #pragma unroll
                         for (int u = 0; u < NP; u++)
@@ -860,11 +876,24 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                             const int dim = NP * lane + c;
                             uint4* to = tile + KP + (dim % DT * 2 + (qt >> 1)) * 64 + (qt & 1) * 32 + dim / DT;
                             to[0] = __builtin_bit_cast(uint4, h);
-                            to[2 * 64 * DT] = __builtin_bit_cast(uint4, lw);
+                            to[VP] = __builtin_bit_cast(uint4, lw);
                         }
                         if (lane == 0) {
                             s_ku[kw][qt] = ldexpf(1.f, -e);
                             s_vu[kw][qt] = ev;
+                        }
+                    } else {
+                        lanes_again();
+                        const int valid = kl + 1 - (t + 8 * qt);  // positions of the 8 that are any (V behind: zeros)
+#pragma unroll
+                        for (int u = 0; u < NP; u++) {
+                            const int p = 8 * qt + u * RP + lane / PCS, dim = 64 * u + lane;
+                            auto keep = [&](uint32_t x, int k) {
+                                return x & (valid >= 2 * k + 2 ? 0xFFFFFFFFu : valid == 2 * k + 1 ? 0xFFFFu : 0u);
+                            };
+                            const uint4 vv = make_uint4(keep(vr[u][0], 0), keep(vr[u][1], 1), keep(vr[u][2], 2), keep(vr[u][3], 3));
+                            tile[lane % PCS * QB + ((p & 0x13) | (p >> 1 & 4) | (p << 1 & 8))] = __builtin_bit_cast(uint4, kr[u]);
+                            tile[KP + ((dim >> 5) * 2 + (qt >> 1)) * 64 + (qt & 1) * 32 + (dim & 31)] = vv;
                         }
                     }
                     lds_sync();
@@ -879,30 +908,38 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     for (int x = 0; x < 16; x++) s[x] = 0.f;
                     const uint4 *kt = tile + half * QB + col, *qtile = s_qlo + qt * QT + half * QB + col;
                     uint4 kf[2][3];  // a product ahead, and no more of them: registers
-                    kf[0][0] = kt[0], kf[0][1] = kt[QT], kf[0][2] = qtile[0];
+                    kf[0][0] = kt[0], kf[0][2] = qtile[0];
+                    if (F32) kf[0][1] = kt[QT];
 #pragma unroll
                     for (int kk = 0; kk < KS; kk++) {
                         if (kk + 1 < KS) {
                             kf[(kk + 1) & 1][0] = kt[2 * QB * (kk + 1)];
-                            kf[(kk + 1) & 1][1] = kt[QT + 2 * QB * (kk + 1)];
+                            if (F32) kf[(kk + 1) & 1][1] = kt[QT + 2 * QB * (kk + 1)];
                             kf[(kk + 1) & 1][2] = qtile[2 * QB * (kk + 1)];
                         }
-                        const f16x8 kh = __builtin_bit_cast(f16x8, kf[kk & 1][0]), klo = __builtin_bit_cast(f16x8, kf[kk & 1][1]);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(klo, qh[kk], s, 0, 0, 0);
+                        const f16x8 kh = __builtin_bit_cast(f16x8, kf[kk & 1][0]);
+                        if constexpr (F32)
+                            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, kf[kk & 1][1]), qh[kk], s, 0, 0, 0);
                         s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, __builtin_bit_cast(f16x8, kf[kk & 1][2]), s, 0, 0, 0);
                         s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[kk], s, 0, 0, 0);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    const float fs[2] = {qs * s_ku[kw][half], qs * s_ku[kw][2 + half]};
-                    const int e0 = s_vu[kw][half], e1 = s_vu[kw][2 + half];
-                    const int e = __builtin_amdgcn_readfirstlane(over_halves(min(e0, e1), imin2));
-                    if (e < vexp) {
-                        const float f = ldexpf(1.f, max(e - vexp, -126));
+                    float fs[2] = {qs, qs};
+                    int e0 = 0, e1 = 0;
+                    if constexpr (F32) {
+                        fs[0] *= s_ku[kw][half];
+                        fs[1] *= s_ku[kw][2 + half];
+                        e0 = t + 8 * half < kend ? s_vu[kw][half] : 110;  // (the wave's columns end ahead of them: no part)
+                        e1 = t + 16 + 8 * half < kend ? s_vu[kw][2 + half] : 110;
+                        const int e = __builtin_amdgcn_readfirstlane(over_halves(min(e0, e1), imin2));
+                        if (e < vexp) {
+                            const float f = ldexpf(1.f, max(e - vexp, -126));
 #pragma unroll
-                        for (int d = 0; d < DT; d++)
+                            for (int d = 0; d < DT; d++)
 #pragma unroll
-                            for (int x = 0; x < 16; x++) o[d][x] *= f;
-                        vexp = e;
+                                for (int x = 0; x < 16; x++) o[d][x] *= f;
+                            vexp = e;
+                        }
                     }
                     // ---- softmax
                     if (edge) {
@@ -928,7 +965,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         m = mn;
                     }
                     const float sub = P_UNIT - (m == -INFINITY ? 0.f : m);
-                    const float vf[2] = {ldexpf(1.f, max(vexp - e0, -126)), ldexpf(1.f, max(vexp - e1, -126))};
+                    const float vf[2] = {ldexpf(1.f, max(vexp - e0, -126)), ldexpf(1.f, max(vexp - e1, -126))};  // (f32)
                     f16x8 ph[2], pl[2];
 #pragma unroll
                     for (int b2 = 0; b2 < 2; b2++) {
@@ -939,7 +976,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                             if (edge) p[x] = s[8 * b2 + x] == -INFINITY ? 0.f : p[x];
                             l += p[x];
                         }
-                        split8(p, vf[b2], ph[b2], pl[b2]);
+                        if (F32) split8(p, vf[b2], ph[b2], pl[b2]);
+                        else split8(p, ph[b2], pl[b2]);
                     }
                     // ---- outputs
                     const uint4* vt = tile + KP + half * 32 + col;
@@ -976,25 +1014,26 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     }
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
-                        uint4 uh[2], ul[2];
+                        uint4 uh[2], ul[2];  // (fp16: no lo)
 #pragma unroll
                         for (int b2 = 0; b2 < 2; b2++) {
                             uh[b2] = vt[64 * (2 * d + b2)];
-                            ul[b2] = vt[2 * 64 * DT + 64 * (2 * d + b2)];
+                            if (F32) ul[b2] = vt[VP + 64 * (2 * d + b2)];
                         }
                         if (bad) {
 #pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                uint32_t *hu = (uint32_t*)&uh[k >> 2] + (k & 3), *lu = (uint32_t*)&ul[k >> 2] + (k & 3);
-                                const uint32_t keep = ~(odd16(*hu) * 0xFFFFu);
-                                *hu &= keep;
-                                *lu &= keep;
+                            for (int b2 = 0; b2 < 2; b2++) {
+                                auto good = [](uint32_t u) { return ~(odd16(u) * 0xFFFFu); };
+                                const uint4 k = make_uint4(good(uh[b2].x), good(uh[b2].y), good(uh[b2].z), good(uh[b2].w));
+                                uh[b2] = make_uint4(uh[b2].x & k.x, uh[b2].y & k.y, uh[b2].z & k.z, uh[b2].w & k.w);
+                                if (F32) ul[b2] = make_uint4(ul[b2].x & k.x, ul[b2].y & k.y, ul[b2].z & k.z, ul[b2].w & k.w);
                             }
                         }
 #pragma unroll
                         for (int b2 = 0; b2 < 2; b2++) {
-                            const f16x8 vh = __builtin_bit_cast(f16x8, uh[b2]), vl = __builtin_bit_cast(f16x8, ul[b2]);
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[b2], o[d], 0, 0, 0);
+                            const f16x8 vh = __builtin_bit_cast(f16x8, uh[b2]);
+                            if constexpr (F32)
+                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, ul[b2]), ph[b2], o[d], 0, 0, 0);
                             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[b2], o[d], 0, 0, 0);
                             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[b2], o[d], 0, 0, 0);
                         }
