@@ -466,10 +466,10 @@ class InferenceEngine:
         params = sampling.params()
         stops = set(stop_tokens) | ({self.eos} if self.eos is not None else set())
         self.transformer.reset()
-        seq = e.seq_create()
         drafter = _Drafter(draft, e.vocab, drafts, params, sampler, ngram)
-        history, out = list(prompt_tokens), []
+        history, out, seq = list(prompt_tokens), [], -1
         try:
+            seq = e.seq_create()
             for a in range(0, len(history) - 1, e.max_batch):  # the prompt but its last token
                 chunk = history[a:min(a + e.max_batch, len(history) - 1)]
                 e.step([seq] * len(chunk), chunk, range(a, a + len(chunk)), want_logits=[0] * len(chunk), argmax=False)
@@ -489,7 +489,8 @@ class InferenceEngine:
                     out.append(t)
                     history.append(t)
         finally:
-            e.seq_release(seq)
+            if seq >= 0:
+                e.seq_release(seq)
             drafter.close()
         return out
 
@@ -546,6 +547,8 @@ class _Drafter:
                         return history[at + n:at + n + most], None
             return [], None
         e, guess = self.model.engine, []
+        if len(history) > e.capacity:
+            return [], None  # the draft model's cache ends here
         same = 0  # positions of the draft's cache that still hold this history
         while same < min(len(self.held), len(history) - 1) and self.held[same] == history[same]:
             same += 1

@@ -238,6 +238,21 @@ def test_greedy_generation_stops_and_ends(hip):
     tf.engine.close()
 
 
+def test_a_draft_model_with_a_shorter_cache(hip):
+    """Past the draft model's last position the target goes on alone; no sequence stays behind."""
+    from qraf_amd.engine import InferenceEngine
+    tf, kw = transformer("q8_llama")
+    short, _ = transformer("q8_llama", max_batch=4, max_seq=24)
+    prompt = tokens(np.random.default_rng(10), kw, 6)
+    want, sure = reference_stream(tf, prompt, 40)
+    free = tf.engine.free_pages(), short.engine.free_pages()
+    got = InferenceEngine(tf, eos_token=None).generate_speculative(prompt, 40, drafts=5, draft=short)
+    assert len(got) == 40 and got[:sure] == want[:sure]
+    assert (tf.engine.free_pages(), short.engine.free_pages()) == free
+    short.engine.close()
+    tf.engine.close()
+
+
 def test_greedy_generation_with_a_penalty(hip):
     from qraf_amd.engine import InferenceEngine, SamplingConfig, apply_repetition_penalty
     tf, kw = transformer("q8_hd64_gqa3")
