@@ -102,7 +102,7 @@ __device__ __forceinline__ float any_v(const GroupArgs& a, size_t block, int off
 template <int HD, int KV>
 __device__ __forceinline__ float any_scale(const GroupArgs& a, const void* pool, size_t block, int off) {
     if (KV != DT_I8) return 1.f;
-    return *(const float*)((const int8_t*)pool + block * a.page_size * (HD + 4) + (size_t)a.page_size * HD + 4 * off);
+    return *(const float*)((const int8_t*)pool + block * a.page_size * (HD + 4) + (size_t)a.page_size * HD + 4 * (size_t)off);
 }
 
 template <int HD, int KV>
@@ -1482,10 +1482,11 @@ static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
 static size_t group_lds(int hd, int n, int groups, const GroupSizes& z) {
     return (size_t)tile_floats(hd) * 4 + (size_t)(2 * (z.job_cap + z.tails) + 1 + 3 * groups + 2 + n) * 4;
 }
-// shapes of the tiles (their LDS bounds what few very wide layouts would need)
+// shapes of the tiles (their LDS bounds what few very wide layouts would need; offsets inside a page, and of q, are
+// held in 32 bits)
 static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
     const int G = H / Hkv;
-    return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 &&
+    return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 && (long long)page_size * hd <= 1 << 29 &&
            (long long)n * H * hd <= 1 << 30 && group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
 }
 

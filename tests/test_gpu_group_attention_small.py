@@ -44,3 +44,33 @@ def test_query_heads_of_one_kv_head(hip, kv, H):
     c = calls.Cache(rng, [(50, [48, 49, 50]), (20, [77, 20])], 1, 64, 32, kv)
     q = calls.queries(rng, c.n, H, 64)
     calls.check(c, calls.Call(hip, c, q, H).run(), q, H)
+
+
+@pytest.mark.parametrize("log2", [23, 25])
+def test_pages_of_many_positions(hip, log2):
+    """One page of 2^23 and of 2^25 positions (offsets inside it pass 2^31 bytes): keys of zero but for the last, which
+    takes all the weight (2^25 e^-60 of it is left to the others), so each row's output is the V of its last position."""
+    from qraf_amd.backend import DeviceBuffer
+    hd, ps = 64, 1 << log2
+    k, v = (DeviceBuffer(ps * hd * 2) for _ in range(2))
+    k.zero()
+    v.zero()
+    rng = np.random.default_rng(log2)
+    q = np.ones((3, 2, hd), np.float32)
+    ctx = np.array([ps, ps - 1, 5], np.int32)
+    want = rng.standard_normal((3, hd)).astype(np.float16)
+    for r, c in enumerate(ctx):
+        # scores 60, 120 and 180, the longest row's last one the largest
+        k.upload(np.full(hd, 60.0 * (3 - r) / np.sqrt(hd), np.float16), int(c - 1) * hd * 2)
+        for d in range(hd):
+            v.upload(want[r, d:d + 1], (d * ps + int(c) - 1) * 2)
+    up = DeviceBuffer.from_array
+    bufs = [up(q), up(np.zeros((3, 1), np.int32)), up(ctx), up(np.array([0, 3], np.int32)), up(np.array([ps], np.int32))]
+    size = hip.lib.qraf_hip_group_attention_workspace_bytes(3, 1, 2, 1, hd, ps)
+    ws, out = DeviceBuffer(max(size, 16)), up(np.zeros((3, 2, hd), np.float32))
+    hip._lib.call("qraf_hip_group_attention_dev", bufs[0].ptr, k.ptr, v.ptr, calls.F16, bufs[1].ptr, 1,
+                  bufs[2].ptr, bufs[3].ptr, bufs[4].ptr, 3, 1, 2, 1, hd, ps, np.float32(1 / np.sqrt(hd)), ps, out.ptr,
+                  ws.ptr, size, None)
+    hip._lib.call("qraf_hip_stream_synchronize", None)
+    got = out.download(np.float32, 6 * hd).reshape(3, 2, hd)
+    assert np.all(np.abs(got - want[:, None]) <= 1e-5 * np.abs(want[:, None]) + 1e-6)
