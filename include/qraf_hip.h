@@ -245,9 +245,11 @@ uint64_t qraf_hip_attention_noalloc_max_bytes(void);
  * (qraf_hip_group_attention_workspace_bytes) needs no initialisation; calls that
  * share one must not overlap.
  * Results are within the attention tolerance of qraf_hip_paged_attention_dev's
- * on the same rows, and the same from call to call; weights below 2^-37 of a
- * row's largest may count as zero.  An infinity or NaN in the K or V of a
- * position reaches the rows that attend to it and no others.
+ * on the same rows, and the same from call to call.  (f32 pages: an element of
+ * a q, K or V vector is held to 2^-22 of itself and 2^-25 of the vector's
+ * largest; a weighted V, of int8 pages too, to 2^-20 of the row's largest.)
+ * Values of positions that a row does not attend to do not reach it, an infinity
+ * or NaN among them, nor do the words of a row's own pages below the prefix.
  * No counterpart in the reference, which runs one sequence at a time. */
 uint64_t qraf_hip_group_attention_workspace_bytes(int32_t n_rows, int32_t n_groups, int32_t n_heads,
                                                   int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx);

@@ -205,12 +205,18 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
 // the second: nothing moves between lanes.  32 columns and not 16: half the
 // operand reads per product, and the reads are what bounds it.
 //
-// q, p and f32 K and V enter as fp16 hi + lo pairs (23 bits; q scaled per column,
-// f32 K per tile and V per wave by powers of two, p by 2^13 to 2^15, so that neither
-// half leaves fp16's range: what is smaller than 2^-38 of the largest may be lost),
-// fp16 K and V as they are, int8 widened; a product of two pairs is three
-// matrix products (lo x lo is below 2^-22).  int8 scales: K's on the scores, V's
-// on p.  Sums in fp32.
+// q, p and f32 K and V enter as fp16 hi + lo pairs (23 bits), fp16 K and V as they
+// are, int8 widened; a product of two pairs is three matrix products (lo x lo is
+// below 2^-22).  int8 scales: K's on the scores, V's on p.  Sums in fp32.  So that
+// neither half leaves fp16's range,
+//   q     is over a power of two of its column,
+//   K, V  (f32) over one of their tile's, in [2^14, 2^15) at its largest, or, where the
+//         positions of a tile lie further apart than SPREAD, each over its own: a
+//         position that some row does not attend to costs it no bits of the others;
+//   p     of f32 and int8 V takes V's powers of two in, over one of the column's own,
+//         which follows the largest weighted V of the tiles so far: what is lost of a
+//         weighted V is below 2^-34 of that (2^-20 next to f32 V of no weight just
+//         within SPREAD), however large a V of no weight is.
 //
 // Up to 64 columns, tails and int8: K of the next tile is requested behind this
 // tile's scores, V behind its outputs, straight into the wave's registers; two waves
@@ -232,13 +238,17 @@ constexpr int BLK = 128;              // columns of a block: 4 waves of 32
 // p is held times 2^13 of the running maximum it was taken against, which follows the largest score only
 // when that has grown by more than 2^2: outputs and sums are rescaled then, a few times a job and not at
 // every tile (some of 32 columns finds a larger score nearly always)
+// (int8: times 1, and brought into fp16's range with V's scale)
 constexpr float P_UNIT = 13.f, GROWTH = 2.f;
+// f32 positions whose largest value lies this far below the tile's get powers of two of their own.  Nearer ones lose
+// at most 14 of the 38 bits between the tile's largest and fp16's least step.
+constexpr float SPREAD = 0x1p-14f;
 
 template <int CTRL>
 __device__ __forceinline__ int gdpp(int x) {
     return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, true);
 }
-enum : int { GDPP_XOR1 = 0xB1, GDPP_XOR2 = 0x4E, GDPP_ROR4 = 0x124, GDPP_ROR8 = 0x128 };
+enum : int { GDPP_XOR1 = 0xB1, GDPP_XOR2 = 0x4E, GDPP_ROR4 = 0x124, GDPP_ROR8 = 0x128, GDPP_HALF_MIRROR = 0x141 };
 // op over all lanes / over lanes l and l ^ 32, in every lane
 template <typename T, typename F>
 __device__ __forceinline__ T over_halves(T x, F op) {
@@ -256,6 +266,21 @@ __device__ __forceinline__ T over_row(T x, F op) {
     x = op(x, back(gdpp<GDPP_ROR4>(in(x))));
     return op(x, back(gdpp<GDPP_ROR8>(in(x))));
 }
+// (2, 4, 8 neighbouring lanes)
+template <typename F>
+__device__ __forceinline__ float over_pair(float x, F op) {
+    return op(x, __int_as_float(gdpp<GDPP_XOR1>(__float_as_int(x))));
+}
+template <typename F>
+__device__ __forceinline__ float over_quad(float x, F op) {
+    x = over_pair(x, op);
+    return op(x, __int_as_float(gdpp<GDPP_XOR2>(__float_as_int(x))));
+}
+template <typename F>
+__device__ __forceinline__ float over_8(float x, F op) {
+    x = over_quad(x, op);
+    return op(x, __int_as_float(gdpp<GDPP_HALF_MIRROR>(__float_as_int(x))));
+}
 template <typename T, typename F>
 __device__ __forceinline__ T over_rows(T x, F op) {
     const unsigned u = __builtin_bit_cast(unsigned, x);
@@ -266,11 +291,21 @@ template <typename T, typename F>
 __device__ __forceinline__ T over_wave(T x, F op) {
     return over_halves(over_rows(over_row(x, op), op), op);
 }
-// max(m, |x|, |y|) in one instruction (fmaxf quiets each operand first, in another one): a NaN may come of a NaN
+// max(m, |x|, |y|) and max(|x|, |y|) in one instruction; a NaN among them, of either kind, gives a NaN (fmaxf, v_max3_f32
+// drop a quiet one, and what a signalling one was compared with)
 __device__ __forceinline__ float amax3(float m, float x, float y) {
-    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
+    asm("v_maximum3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x), "v"(y));
     return m;
 }
+__device__ __forceinline__ float amax2(float x, float y) {
+    float m;
+    asm("v_maximum3_f32 %0, |%1|, |%2|, |%2|" : "=v"(m) : "v"(x), "v"(y));
+    return m;
+}
+// some lane's condition, seldom true: its code lies behind the kernel, and registers are spilled there
+__device__ __forceinline__ bool seldom(bool x) { return __builtin_expect(__any(x), 0); }
+// |x|, or 0 of an infinity or NaN
+__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 __device__ __forceinline__ float fmax2(float x, float y) { return fmaxf(x, y); }
 __device__ __forceinline__ int imax2(int x, int y) { return max(x, y); }
 __device__ __forceinline__ int imin2(int x, int y) { return min(x, y); }
@@ -279,13 +314,30 @@ __device__ __forceinline__ int imin2(int x, int y) { return min(x, y); }
 __device__ __forceinline__ int key_of(int rho) {
     return 16 * ((rho >> 4) & 1) + 8 * ((rho >> 2) & 1) + 4 * ((rho >> 3) & 1) + (rho & 3);
 }
-// power of two that brings a largest magnitude into [2^14, 2^15), as its exponent
+// the row of the first product's A that holds position p of a tile: key_of(row_of(p)) = p
+__device__ __forceinline__ int row_of(int p) { return (p & 0x13) | (p >> 1 & 4) | (p << 1 & 8); }
+// power of two that brings a largest magnitude into [2^14, 2^15), as its exponent: -113 (fp32's largest) .. 110
 __device__ __forceinline__ int unit_exp(float mx) {
     if (!(mx > 0.f)) return 110;
     int e;
     frexpf(mx, &e);
-    return max(-110, min(15 - e, 110));
+    return min(15 - e, 110);
 }
+// floor(x), at most 1000 (of a NaN, an infinity)
+__device__ __forceinline__ int floor_to(float x) { return (int)floorf(fminf(x, 1000.f)); }
+// of magnitudes the largest (a NaN of a NaN) and the least
+struct Spread {
+    float most = 0.f;
+    uint32_t least = 0x7F800000u;
+    __device__ __forceinline__ void add(float x, float y) {
+        most = amax3(most, x, y);
+        least = min(least, min(__float_as_uint(x), __float_as_uint(y)));
+    }
+    // whether values of the lane may lie too far below `all`, the largest of all lanes, or are no numbers
+    __device__ __forceinline__ bool apart(float all) const { return !(most < INFINITY) || __uint_as_float(least) < all * SPREAD; }
+};
+// and whether they do (y, of a position; 0 has no bits to lose)
+__device__ __forceinline__ bool far_below(float y, float all) { return y > 0.f && y < all * SPREAD; }
 // two values as fp16 hi + lo, each to the nearest: 23 bits
 __device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -294,20 +346,25 @@ __device__ __forceinline__ void split2(float x, float y, f16x2& hi, f16x2& lo) {
     lo = __builtin_convertvector(
         (f32x2{__builtin_fmaf((float)hi[0], -1.f, x), __builtin_fmaf((float)hi[1], -1.f, y)}), f16x2);
 }
-// 8 values times a power of two (the products inside the multiply-adds: 5 instructions a pair, 6 with them ahead)
-__device__ __forceinline__ void split8(const float (&x)[8], float by, f16x8& hi, f16x8& lo) {
+// 8 values, value i times by(i), a power of two (the products inside the multiply-adds: 5 instructions a pair, 6 with
+// them ahead)
+template <typename F>
+__device__ __forceinline__ void split8_by(const float (&x)[8], F by, f16x8& hi, f16x8& lo) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         f16x2 h;
-        h[0] = (_Float16)__builtin_fmaf(x[i], by, 0.f);
-        h[1] = (_Float16)__builtin_fmaf(x[i + 1], by, 0.f);
+        h[0] = (_Float16)__builtin_fmaf(x[i], by(i), 0.f);
+        h[1] = (_Float16)__builtin_fmaf(x[i + 1], by(i + 1), 0.f);
         uint32_t u = __builtin_bit_cast(uint32_t, h);
         asm("" : "+v"(u));  // one register of two halves, as the products take them
         h = __builtin_bit_cast(f16x2, u);
         hi[i] = h[0], hi[i + 1] = h[1];
-        lo[i] = (_Float16)__builtin_fmaf(x[i], by, -(float)h[0]);
-        lo[i + 1] = (_Float16)__builtin_fmaf(x[i + 1], by, -(float)h[1]);
+        lo[i] = (_Float16)__builtin_fmaf(x[i], by(i), -(float)h[0]);
+        lo[i + 1] = (_Float16)__builtin_fmaf(x[i + 1], by(i + 1), -(float)h[1]);
     }
+}
+__device__ __forceinline__ void split8(const float (&x)[8], float by, f16x8& hi, f16x8& lo) {
+    split8_by(x, [by](int) { return by; }, hi, lo);
 }
 __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
 #pragma unroll
@@ -504,8 +561,12 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
     extern __shared__ __align__(16) float s_dyn[];
     __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK], s_qs[BLK];
-    __shared__ float s_ku[2][4];  // f32 tiles that four waves share: one over K's units, V's, of 8 positions each
-    __shared__ int s_vu[2][4];
+    // f32 tiles that four waves share: the exponents of K's and V's powers of two, of 8 positions each, or (OWN) of each,
+    // where the waves' maxima and sums lie behind the tiles
+    int(*const s_kx)[32] = (int(*)[32])s_m;
+    int(*const s_vx)[32] = (int(*)[32])s_l;
+    constexpr int OWN = -(1 << 20);  // (scores over it are infinite)
+    __shared__ int s_ku[2][4], s_vu[2][4];
     __shared__ long long s_to[BLK];  // where a column's output goes: an element of out, or ~ one of part_o
     constexpr long long NOWHERE = 1ll << 62;
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
@@ -747,7 +808,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 float mx = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
                 mx = over_row(mx, fmax2);
                 if (HD == 128) mx = over_rows(mx, fmax2);
-                const int e = mx <= 3.0e38f ? unit_exp(mx) : 0;
+                const int e = mx < INFINITY ? unit_exp(mx) : 0;
                 const float sg = copysignf(ldexpf(1.f, e), a.scale);  // (scores take the scale's magnitude)
                 f16x2 h0, l0, h1, l1;
                 split2(x[u].x * sg, x[u].y * sg, h0, l0);
@@ -766,19 +827,48 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         const float qs = s_qs[qt * 32 + col];  // scores in powers of two
 
         float m = -INFINITY, l = 0.f;  // running maximum; sum of the lane's own positions, times 2^13
-        int vexp = 110;                // V's unit: outputs are held times 2^vexp (f32, int8)
+        int vexp = 110;                // f32, int8: the column's outputs are held times 2^vexp
         f32x16 o[DT];
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int x = 0; x < 16; x++) o[d][x] = 0.f;
 
+        // the running maximum to that of a tile, mt, if it has grown (f32, int8: a whole number, so that outputs keep
+        // their bits: they and the column's power of two go along)
+        auto follow = [&](float mt) {
+            if (!__any(mt > m + GROWTH)) return;
+            const float mn = fmaxf(m, F16 ? mt : ceilf(mt));
+            float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+            if constexpr (!F16) {
+                const int up = min(floor_to(mn - m), 110 - vexp);
+                vexp += up;
+                alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn + (float)up);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[d][x] *= alpha;
+            m = mn;
+        };
+        // the column's power of two to `lim`, the one that a tile's weighted V need, if it is more than GROWTH above
+        auto hold = [&](int lim) {
+            if (!__any(vexp > lim + (int)GROWTH)) return;
+            const int down = vexp > lim + (int)GROWTH ? lim - vexp : 0;
+            const float f = ldexpf(1.f, down);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[d][x] *= f;
+            vexp += down;
+        };
+
         if constexpr (!DIRECT && !I8) {
             // Tiles of more than 64 columns: the four waves side by side load a quarter of a tile each, 8 positions, and
             // write it as operands for all of them, f32 split (alone each would load and split it all, and a lane to a
             // position reads a line of memory per lane).  The tiles lie where q's hi halves were, which stay in
-            // registers.  f32: K's and V's powers of two are those of the 8 positions; V's enter through p, over the
-            // running one.  256 rows of 32,768 positions, 16/2 heads of 128: f32 280 us for 444, fp16 197 for 221; int8
+            // registers.  f32: K's and V's powers of two are those of the 8 positions, or each position's.  256 rows of 32,768 positions, 16/2 heads of 128: f32 280 us for 444, fp16 197 for 221; int8
             // gained nothing (254 for 253) and goes on alone.
             if (shared) {
                 constexpr int NP = HD / 64, PCS = HD / 8, RP = 64 / PCS;  // K: passes, pieces of a row, rows of a pass
@@ -821,11 +911,6 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                             vx[k] = *(const vpart*)(vp + (uint32_t)(((min(at + 8 * qt + k, kl) & psm) * HD + NP * lane) * 4));
                     }
                 };
-                // the power of two for values of which |.| is at most mx, or (some are no numbers) as `find` says
-                auto unit_of = [&](float mx, auto find) {
-                    if (__any(!(mx <= 3.0e38f))) mx = find();
-                    return __builtin_amdgcn_readfirstlane(unit_exp(over_wave(mx, fmax2)));
-                };
                 t = __builtin_amdgcn_readfirstlane(t);
                 request(t, id_of(t));
                 int id = id_of(t + dt);
@@ -833,41 +918,83 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     lds_sync();  // what lay there is read
                     // ---- this wave's quarter
                     if constexpr (F32) {
-                        float mx = 0.f;
+                        Spread sp;
+                        float y[NP];  // (a row's 8 values of this lane for the row)
 #pragma unroll
-                        for (int u = 0; u < NP; u++)
+                        for (int u = 0; u < NP; u++) {
+                            y[u] = amax2(kx[u][0], kx[u][1]);
 #pragma unroll
-                            for (int k = 0; k < 8; k += 2) mx = amax3(mx, kx[u][k], kx[u][k + 1]);
-                        const int e = unit_of(mx, [&] {
-                            float y = 0.f;
-                            for (int u = 0; u < NP; u++)
-                                for (int k = 0; k < 8; k++) y = fabsf(kx[u][k]) <= 3.0e38f ? fmaxf(y, fabsf(kx[u][k])) : y;
-                            return y;
-                        });
-                        const float sg = ldexpf(1.f, e);
+                            for (int k = 2; k < 8; k += 2) y[u] = amax3(y[u], kx[u][k], kx[u][k + 1]);
+                        }
+                        sp.add(y[0], y[NP - 1]);
+                        float most = over_wave(sp.most, fmax2);
+                        bool k_own = false, v_own = false;
+                        if (seldom(sp.apart(most))) {
+                            most = 0.f;
+#pragma unroll
+                            for (int u = 0; u < NP; u++) {
+                                y[u] = 0.f;
+#pragma unroll
+                                for (int k = 0; k < 8; k++) y[u] = fmaxf(y[u], finite_abs(kx[u][k]));
+                                y[u] = PCS == 16 ? over_row(y[u], fmax2) : over_8(y[u], fmax2);
+                                most = fmaxf(most, y[u]);
+                            }
+                            most = over_wave(most, fmax2);
+#pragma unroll
+                            for (int u = 0; u < NP; u++) k_own = k_own || __any(far_below(y[u], most));
+                        }
+                        const int e = __builtin_amdgcn_readfirstlane(unit_exp(most));
                         lanes_again();
 #pragma unroll
                         for (int u = 0; u < NP; u++) {
+                            const int p = 8 * qt + u * RP + lane / PCS;
+                            int eu = e;
+                            if (__builtin_expect(k_own, 0)) {
+                                eu = unit_exp(y[u]);
+                                s_kx[kw][p] = eu;
+                            }
                             f16x8 h, lw;
-                            split8(kx[u], sg, h, lw);
-                            const int p = 8 * qt + u * RP + lane / PCS;  // of A's row with key_of(row) = p
-                            uint4* to = tile + (lane % PCS) * QB + ((p & 0x13) | (p >> 1 & 4) | (p << 1 & 8));
+                            split8(kx[u], ldexpf(1.f, eu), h, lw);
+                            uint4* to = tile + (lane % PCS) * QB + row_of(p);
                             to[0] = __builtin_bit_cast(uint4, h);
                             to[QT] = __builtin_bit_cast(uint4, lw);
                         }
-                        mx = 0.f;
+                        sp = Spread();
+                        float z[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k += 2)
+                        for (int k = 0; k < 8; k++) {
+                            if constexpr (NP == 1) z[k] = fabsf(vx[k][0]);
+                            else z[k] = amax2(vx[k][0], vx[k][1]);
+                            if (NP == 1) z[k] = over_pair(z[k], amax2);  // (of 2 dims: one alone is often small)
+                            if (k & 1) sp.add(z[k - 1], z[k]);
+                        }
+                        most = over_wave(sp.most, fmax2);
+                        if (seldom(sp.apart(most))) {
+                            most = 0.f;
 #pragma unroll
-                            for (int c = 0; c < NP; c++) mx = amax3(mx, vx[k][c], vx[k + 1][c]);
-                        const int ev = unit_of(mx, [&] {
-                            float y = 0.f;
-                            for (int k = 0; k < 8; k++)
-                                for (int c = 0; c < NP; c++) y = fabsf(vx[k][c]) <= 3.0e38f ? fmaxf(y, fabsf(vx[k][c])) : y;
-                            return y;
-                        });
-                        const float vg = ldexpf(1.f, ev);
+                            for (int k = 0; k < 8; k++) {
+                                z[k] = 0.f;
+#pragma unroll
+                                for (int c = 0; c < NP; c++) z[k] = fmaxf(z[k], finite_abs(vx[k][c]));
+                                z[k] = over_wave(z[k], fmax2);
+                                most = fmaxf(most, z[k]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 8; k++) v_own = v_own || __any(far_below(z[k], most));
+                        }
+                        const int ev = __builtin_amdgcn_readfirstlane(unit_exp(most));
+                        float vg = ldexpf(1.f, ev);
                         lanes_again();
+                        if (__builtin_expect(v_own, 0)) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                const int ek = __builtin_amdgcn_readfirstlane(unit_exp(z[k]));
+#pragma unroll
+                                for (int c = 0; c < NP; c++) vx[k][c] = ldexpf(vx[k][c], ek);
+                                if (lane == 0) s_vx[kw][8 * qt + k] = ek;
+                            }
+                            vg = 1.f;
+                        }
 #pragma unroll
                         for (int c = 0; c < NP; c++) {
                             float x[8];
@@ -881,8 +1008,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                             to[VP] = __builtin_bit_cast(uint4, lw);
                         }
                         if (lane == 0) {
-                            s_ku[kw][qt] = ldexpf(1.f, -e);
-                            s_vu[kw][qt] = ev;
+                            s_ku[kw][qt] = k_own ? OWN : e;
+                            s_vu[kw][qt] = v_own ? OWN : ev;
                         }
                     } else {
                         lanes_again();
@@ -894,7 +1021,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                                 return x & (valid >= 2 * k + 2 ? 0xFFFFFFFFu : valid == 2 * k + 1 ? 0xFFFFu : 0u);
                             };
                             const uint4 vv = make_uint4(keep(vr[u][0], 0), keep(vr[u][1], 1), keep(vr[u][2], 2), keep(vr[u][3], 3));
-                            tile[lane % PCS * QB + ((p & 0x13) | (p >> 1 & 4) | (p << 1 & 8))] = __builtin_bit_cast(uint4, kr[u]);
+                            tile[lane % PCS * QB + row_of(p)] = __builtin_bit_cast(uint4, kr[u]);
                             tile[KP + ((dim >> 5) * 2 + (qt >> 1)) * 64 + (qt & 1) * 32 + (dim & 31)] = vv;
                         }
                     }
@@ -926,22 +1053,27 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[kk], s, 0, 0, 0);
                         __builtin_amdgcn_sched_barrier(0);
                     }
+                    // f32: scores and outputs over the positions' powers of two (half's 8 of a quarter of the tile)
                     float fs[2] = {qs, qs};
-                    int e0 = 0, e1 = 0;
+                    int ve[2] = {0, 0};
+                    bool v_own = false;
                     if constexpr (F32) {
-                        fs[0] *= s_ku[kw][half];
-                        fs[1] *= s_ku[kw][2 + half];
-                        e0 = t + 8 * half < kend ? s_vu[kw][half] : 110;  // (the wave's columns end ahead of them: no part)
-                        e1 = t + 16 + 8 * half < kend ? s_vu[kw][2 + half] : 110;
-                        const int e = __builtin_amdgcn_readfirstlane(over_halves(min(e0, e1), imin2));
-                        if (e < vexp) {
-                            const float f = ldexpf(1.f, max(e - vexp, -126));
+                        const int k0 = s_ku[kw][half], k1 = s_ku[kw][2 + half];
+                        fs[0] = ldexpf(qs, -k0);
+                        fs[1] = ldexpf(qs, -k1);
+                        if (seldom(!(fmaxf(fs[0], fs[1]) < INFINITY))) {
+                            int qe;
+                            const float qm = frexpf(qs, &qe);
 #pragma unroll
-                            for (int d = 0; d < DT; d++)
-#pragma unroll
-                                for (int x = 0; x < 16; x++) o[d][x] *= f;
-                            vexp = e;
+                            for (int x = 0; x < 16; x++) {
+                                const int k = x < 8 ? k0 : k1, e = k == OWN ? s_kx[kw][16 * (x >> 3) + 8 * half + (x & 7)] : k;
+                                s[x] = ldexpf(s[x] * qm, qe - e);
+                            }
+                            fs[0] = fs[1] = 1.f;
                         }
+                        ve[0] = t + 8 * half < kend ? s_vu[kw][half] : 110;  // (the wave's columns end ahead of them: no part)
+                        ve[1] = t + 16 + 8 * half < kend ? s_vu[kw][2 + half] : 110;
+                        v_own = seldom(min(ve[0], ve[1]) == OWN);
                     }
                     // ---- softmax
                     if (edge) {
@@ -955,19 +1087,28 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         m0 = fmaxf(m0, s[x]);
                         m1 = fmaxf(m1, s[x + 8]);
                     }
-                    float mt = fmaxf(m0 == -INFINITY ? m0 : m0 * fs[0], m1 == -INFINITY ? m1 : m1 * fs[1]);
-                    mt = over_halves(mt, fmax2);
-                    if (__any(mt > m + GROWTH)) {
-                        const float mn = fmaxf(m, mt), alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                        l *= alpha;
-#pragma unroll
-                        for (int d = 0; d < DT; d++)
-#pragma unroll
-                            for (int x = 0; x < 16; x++) o[d][x] *= alpha;
-                        m = mn;
-                    }
+                    m0 = m0 == -INFINITY ? m0 : m0 * fs[0];
+                    m1 = m1 == -INFINITY ? m1 : m1 * fs[1];
+                    follow(over_halves(fmaxf(m0, m1), fmax2));
                     const float sub = P_UNIT - (m == -INFINITY ? 0.f : m);
-                    const float vf[2] = {ldexpf(1.f, max(vexp - e0, -126)), ldexpf(1.f, max(vexp - e1, -126))};  // (f32)
+                    float vf[2] = {1.f, 1.f};  // V's powers of two over the column's
+                    if constexpr (F32) {
+                        int lim = 1000;
+                        if (__builtin_expect(v_own, 0)) {
+#pragma unroll
+                            for (int x = 0; x < 16; x++) {
+                                const int k = ve[x >> 3], e = k == OWN ? s_vx[kw][16 * (x >> 3) + 8 * half + (x & 7)] : k;
+                                lim = min(lim, e + floor_to(m - s[x] * fs[x >> 3]));
+                            }
+                        } else {
+                            lim = min(ve[0] + floor_to(m - m0), ve[1] + floor_to(m - m1));
+                        }
+                        hold(over_halves(lim, imin2));
+                        if (__builtin_expect(!v_own, 1)) {
+                            vf[0] = ldexpf(1.f, min(vexp - ve[0], 100));
+                            vf[1] = ldexpf(1.f, min(vexp - ve[1], 100));
+                        }
+                    }
                     f16x8 ph[2], pl[2];
 #pragma unroll
                     for (int b2 = 0; b2 < 2; b2++) {
@@ -977,6 +1118,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                             p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * b2 + x], fs[b2], sub));
                             if (edge) p[x] = s[8 * b2 + x] == -INFINITY ? 0.f : p[x];
                             l += p[x];
+                        }
+                        if (__builtin_expect(F32 && v_own, 0)) {
+#pragma unroll
+                            for (int x = 0; x < 8; x++)
+                                p[x] = ldexpf(p[x], min(vexp - (ve[b2] == OWN ? s_vx[kw][16 * b2 + 8 * half + x] : ve[b2]), 100));
                         }
                         if (F32) split8(p, vf[b2], ph[b2], pl[b2]);
                         else split8(p, ph[b2], pl[b2]);
@@ -1055,20 +1201,31 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             for (int x = 0; x < 16; x++) s[x] = 0.f;
             float fs = qs;
             if constexpr (F32) {
-                float mx = 0.f;
+                float mx = 0.f;  // of the lane's position
 #pragma unroll
                 for (int k = 0; k < 2 * KS; k++) mx = amax3(amax3(mx, tl.k[k].x, tl.k[k].y), tl.k[k].z, tl.k[k].w);
-                if (__any(!(mx <= 3.0e38f))) {  // an infinity or NaN: the unit of the others
-                    mx = 0.f;
+                const bool odd = !(mx < INFINITY);
+                mx = over_halves(mx, fmax2);
+                float most = over_rows(over_row(mx, fmax2), fmax2);
+                int e = unit_exp(most);
+                fs = ldexpf(qs, -e);
+                bool own = false;
+                if (seldom(odd || mx < most * SPREAD || !(fs < INFINITY))) {
+                    mx = 0.f;  // without infinities and NaN
+#pragma unroll
                     for (int k = 0; k < 2 * KS; k++) {
                         const float v[4] = {tl.k[k].x, tl.k[k].y, tl.k[k].z, tl.k[k].w};
-                        for (int c = 0; c < 4; c++) mx = fabsf(v[c]) <= 3.0e38f ? fmaxf(mx, fabsf(v[c])) : mx;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) mx = fmaxf(mx, finite_abs(v[c]));
                     }
+                    mx = over_halves(mx, fmax2);
+                    most = over_rows(over_row(mx, fmax2), fmax2);
+                    e = unit_exp(most);
+                    fs = ldexpf(qs, -e);
+                    own = __any(far_below(mx, most) || !(fs < INFINITY));
+                    if (own) e = unit_exp(mx);
                 }
-                mx = over_wave(mx, fmax2);
-                const int e = unit_exp(mx);
                 const float sg = ldexpf(1.f, e);
-                fs = ldexpf(qs, -e);
 #pragma unroll
                 for (int kk = 0; kk < KS; kk++) {
                     const float4 x = tl.k[2 * kk], y = tl.k[2 * kk + 1];
@@ -1080,6 +1237,14 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql, s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh, s, 0, 0, 0);
+                }
+                if (__builtin_expect(own, 0)) {
+                    int qe;
+                    const float qm = frexpf(qs, &qe);
+#pragma unroll
+                    for (int x = 0; x < 16; x++)
+                        s[x] = ldexpf(s[x] * qm, qe - __shfl(e, row_of(16 * (x >> 3) + 8 * half + (x & 7))));
+                    fs = 1.f;
                 }
             } else {
 #pragma unroll
@@ -1131,16 +1296,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             for (int x = 0; x < 16; x++) mt = fmaxf(mt, s[x]);
             mt = over_halves(mt, fmax2);
             mt = mt == -INFINITY ? mt : mt * fs;
-            if (__any(mt > m + GROWTH)) {
-                const float mn = fmaxf(m, mt), alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int x = 0; x < 16; x++) o[d][x] *= alpha;
-                m = mn;
-            }
-            const float sub = P_UNIT - (m == -INFINITY ? 0.f : m);
+            follow(mt);
+            const float sub = (I8 ? 0.f : P_UNIT) - (m == -INFINITY ? 0.f : m);
             float p[16];
 #pragma unroll
             for (int x = 0; x < 16; x++) {
@@ -1148,39 +1305,70 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 if (edge) p[x] = s[x] == -INFINITY ? 0.f : p[x];  // (a factor of 0 times it)
                 l += p[x];
             }
-            // V's unit, as small as the largest V so far needs
-            if constexpr (F32 || I8) {
+            float vf = 1.f, vg = 1.f;  // V's powers of two over the column's, and those (f32)
+            bool v_own = false;
+            if constexpr (I8) {
                 float mx = 0.f;
-                if constexpr (I8) {
 #pragma unroll
-                    for (int x = 0; x < 16; x++) mx = fabsf(vsc[x]) <= 3.0e38f ? fmaxf(mx, fabsf(vsc[x])) : mx;
-                    mx = over_halves(mx, fmax2);
-                } else {
+                for (int x = 0; x < 16; x++) {
+                    p[x] = !edge || s[x] > -INFINITY ? p[x] * vsc[x] : 0.f;
+                    mx = fmaxf(mx, fabsf(p[x]));
+                }
+                hold(unit_exp(over_halves(mx, fmax2)) - (int)GROWTH);
+                vf = ldexpf(1.f, vexp);
+            }
+            if constexpr (F32) {
+                Spread sp;  // of positions, DT dims of each
 #pragma unroll
-                    for (int k = 0; k < 16; k++)
+                for (int k = 0; k < 16; k += 2) {
+                    float x = amax2(tl.v[k][0], tl.v[k][1]), y = amax2(tl.v[k + 1][0], tl.v[k + 1][1]);
 #pragma unroll
-                        for (int c = 0; c < DT; c += 2) mx = amax3(mx, tl.v[k][c], tl.v[k][c + 1]);
-                    if (__any(!(mx <= 3.0e38f))) {
-                        mx = 0.f;
-                        for (int k = 0; k < 16; k++)
-                            for (int c = 0; c < DT; c++)
-                                mx = fabsf(tl.v[k][c]) <= 3.0e38f ? fmaxf(mx, fabsf(tl.v[k][c])) : mx;
+                    for (int c = 2; c < DT; c += 2) {
+                        x = amax3(x, tl.v[k][c], tl.v[k][c + 1]);
+                        y = amax3(y, tl.v[k + 1][c], tl.v[k + 1][c + 1]);
                     }
-                    mx = over_wave(mx, fmax2);
+                    sp.add(x, y);
                 }
-                const int e = __builtin_amdgcn_readfirstlane(I8 ? unit_exp(mx) - 15 : unit_exp(mx));
-                if (e < vexp) {
-                    const float f = ldexpf(1.f, max(e - vexp, -126));
+                float most = over_wave(sp.most, fmax2);
+                if (seldom(sp.apart(most))) {
+                    most = 0.f;
+                    float least = INFINITY;
 #pragma unroll
-                    for (int d = 0; d < DT; d++)
+                    for (int k = 0; k < 16; k++) {  // (the lanes of a half hold its position)
+                        float y = 0.f;
 #pragma unroll
-                        for (int x = 0; x < 16; x++) o[d][x] *= f;
-                    vexp = e;
+                        for (int c = 0; c < DT; c++) y = fmaxf(y, finite_abs(tl.v[k][c]));
+                        y = over_rows(over_row(y, fmax2), fmax2);
+                        most = fmaxf(most, y);
+                        least = y > 0.f ? fminf(least, y) : least;
+                        s_m[wave][16 * half + k] = y;
+                        __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
+                    }
+                    most = over_halves(most, fmax2);
+                    v_own = __any(far_below(least, most));
                 }
-                if constexpr (I8) {
-                    const float f = ldexpf(1.f, vexp);
+                int e = unit_exp(most), lim = e + floor_to(m - mt);
+                if (__builtin_expect(v_own, 0)) {
+                    int top = -1000;  // log2 of the largest weighted magnitude, at most
 #pragma unroll
-                    for (int x = 0; x < 16; x++) p[x] = !edge || s[x] > -INFINITY ? p[x] * (vsc[x] * f) : 0.f;
+                    for (int k = 0; k < 16; k++) {
+                        e = unit_exp(s_m[wave][16 * half + k]);
+                        top = max(top, p[k] > 0.f ? __builtin_amdgcn_frexp_expf(p[k]) - e : -1000);
+                        s_m[wave][16 * half + k] = ldexpf(1.f, e);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    lim = (int)P_UNIT - over_halves(top, imax2);
+                }
+                hold(lim);
+                if (__builtin_expect(v_own, 0)) {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        p[k] = ldexpf(p[k], min(vexp + 1 - __builtin_amdgcn_frexp_expf(s_m[wave][16 * half + k]), 100));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+                    s_m[wave][col] = ldexpf(1.f, e);
+                    vf = ldexpf(1.f, min(vexp - e, 100));
                 }
             }
             f16x8 ph[2], pl[2];
@@ -1188,7 +1376,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             for (int b = 0; b < 2; b++) {
                 const float v[8] = {p[8 * b], p[8 * b + 1], p[8 * b + 2], p[8 * b + 3],
                                     p[8 * b + 4], p[8 * b + 5], p[8 * b + 6], p[8 * b + 7]};
-                split8(v, ph[b], pl[b]);
+                if constexpr (F16) split8(v, ph[b], pl[b]);
+                else split8(v, vf, ph[b], pl[b]);
             }
 
             // ---- outputs
@@ -1216,7 +1405,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     for (int d = 0; d < DT; d++) {
                         if constexpr (F32) {
 #pragma unroll
-                            for (int k = 0; k < 16; k++) bad |= !(fabsf(tl.v[k][d]) <= 3.4e38f);
+                            for (int k = 0; k < 16; k++) bad |= !(fabsf(tl.v[k][d]) < INFINITY);
                         } else {
                             uint32_t any = 0;
 #pragma unroll
@@ -1244,7 +1433,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
                                     for (int k = 0; k < 8; k++) {
                                         const float v = tl.v[8 * b + k][d];
-                                        const bool good = fabsf(v) <= 3.4e38f;
+                                        const bool good = fabsf(v) < INFINITY;
                                         const uint32_t one = good ? 0u : k & 1 ? 0x3C000000u : 0x3C00u;
                                         fu[k >> 1] = k & 1 ? fu[k >> 1] | one : one;
                                         tl.v[8 * b + k][d] = good ? v : 0.f;
@@ -1266,28 +1455,34 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     }
                 }
             }
-            const float vg = F32 ? ldexpf(1.f, vexp) : 1.f;
+            // dims DT * row + d of tile d (f32), 32 d + row
+            auto product = [&](int d, int b, auto by) {
+                if constexpr (F32) {
+                    float x[8];
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    if constexpr (F32) {  // dims DT * row + d
-                        float x[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] = tl.v[8 * b + k][d];
-                        f16x8 vh, vl;
-                        split8(x, vg, vh, vl);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[b], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[b], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[b], o[d], 0, 0, 0);
-                    } else {  // dims 32 d + row
-                        f16x8 vf;
-                        if constexpr (I8) vf = widen8(tl.v[d][b].x, tl.v[d][b].y);
-                        else vf = __builtin_bit_cast(f16x8, tl.v[d][b]);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b], o[d], 0, 0, 0);
-                    }
+                    for (int k = 0; k < 8; k++) x[k] = tl.v[8 * b + k][d];
+                    f16x8 vh, vl;
+                    split8_by(x, by, vh, vl);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[b], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[b], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[b], o[d], 0, 0, 0);
+                } else {
+                    f16x8 vf;
+                    if constexpr (I8) vf = widen8(tl.v[d][b].x, tl.v[d][b].y);
+                    else vf = __builtin_bit_cast(f16x8, tl.v[d][b]);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b], o[d], 0, 0, 0);
                 }
+            };
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                float by[8];  // (f32: a half's 8 positions; 8 at a time: registers)
+#pragma unroll
+                for (int k = 0; k < 8; k++) by[k] = F32 ? s_m[wave][16 * half + 8 * b + k] : 1.f;
+#pragma unroll
+                for (int d = 0; d < DT; d++) product(d, b, [&](int k) { return by[k]; });
+                if (F32) __builtin_amdgcn_sched_barrier(0);
+            }
             if (TURNS) load_k(tn, go);
             else load_v(tn, go);
             more = go;
@@ -1304,11 +1499,12 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         lanes_again();
         lds_sync();  // q's operands lie where the outputs go
         l = over_halves(l, [](float x, float y) { return x + y; });
+        if (F32) l = ldexpf(l, -(int)P_UNIT);  // weights of 1 again: V next to fp32's largest stay in it
         if (half == 0) {
             s_m[wave][col] = m;
             s_l[wave][col] = l;
         }
-        const float unit = F16 ? 1.f : ldexpf(1.f, -vexp);
+        const float unit = F16 ? 1.f : ldexpf(1.f, -vexp - (F32 ? (int)P_UNIT : 0));
         if (col < cols) {
             float4* row = (float4*)(s_o + (wave * 32 + col) * HD);
             const int x = col & 15;
