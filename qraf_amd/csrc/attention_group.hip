@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "group_pieces.h"
 
 namespace qraf_hip {
 
@@ -464,10 +465,6 @@ __device__ __forceinline__ int wave_sum(int n, F f) {
     for (int i = threadIdx.x & 63; i < n; i += 64) x += f(i);
     return over_wave(x, [](int u, int v) { return u + v; });
 }
-// pieces of a job of `tiles` tiles, at most about `most` each; per_most = 1 / most
-__device__ __forceinline__ int pieces_of(int tiles, int most, float per_most) {
-    return tiles ? max(1, (int)((float)(tiles + most - 1) * per_most)) : 0;
-}
 __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     const int tid = threadIdx.x;
     for (int i = tid; i < max(a.n, a.groups + 1); i += GTH) {  // (all requested at once)
@@ -497,20 +494,23 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     lds_sync();
     if (tid < 64) {
         // the shortest piece of which there are at most `shares`, or as many times that as there are jobs
-        const int full = wave_sum(jobs, [&](int j) { return p.tiles[j] > 0 ? 1 : 0; });
-        const int room = shares * max(1, (full + shares - 1) / shares);
-        const int all = wave_sum(jobs, [&](int j) { return p.tiles[j]; });
-        // (pieces of x tiles are at least all / x, and fewer than all / x + full)
-        int lo = max(1, (all + room - 1) / room), hi = room > full ? max(lo, (all + room - full - 1) / (room - full)) : max(lo, all);
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            const float per = 1.f / (float)mid;
-            if (wave_sum(jobs, [&](int j) { return pieces_of(p.tiles[j], mid, per); }) <= room) hi = mid;
-            else lo = mid + 1;
+        // (from bit 16 on those of LONG_JOB tiles: where there is none, all of the at most 4,096 fit 32 bits)
+        const int jobs_full = wave_sum(jobs, [&](int j) { return p.tiles[j] > 0 ? 1 + (p.tiles[j] >= LONG_JOB ? 1 << 16 : 0) : 0; });
+        const int full = jobs_full & 0xFFFF, room = piece_room(full, shares);
+        const bool longs = __builtin_amdgcn_readfirstlane(jobs_full >> 16) != 0;
+        uint64_t all = (unsigned)wave_sum(jobs, [&](int j) { return p.tiles[j]; });
+        if (longs) {
+            all = (unsigned)wave_sum(jobs, [&](int j) { return p.tiles[j] & 0xFFFF; });
+            all += (uint64_t)wave_sum(jobs, [&](int j) { return p.tiles[j] >> 16; }) << 16;
         }
+        const int lo = shortest_piece(all, full, room, [&](int most) {
+            const float per = 1.f / (float)most;
+            if (longs) return wave_sum(jobs, [&](int j) { return pieces_of_long(p.tiles[j], most); });
+            return wave_sum(jobs, [&](int j) { return pieces_of(p.tiles[j], most, per); });
+        });
         const float per = 1.f / (float)lo;
         for (int j = tid; j < jobs; j += 64) {
-            const int x = pieces_of(p.tiles[j], lo, per);
+            const int x = longs ? pieces_of_long(p.tiles[j], lo) : pieces_of(p.tiles[j], lo, per);
             p.upto[j] = x | (x ? 1 << 16 : 0);
         }
         wave_prefix_sum(p.upto, jobs);
