@@ -1005,16 +1005,19 @@ __global__ __launch_bounds__(STH) void verify_pick_kernel(VerifyArgs a, const do
     }
     // a draw outside [0, 1) (or NaN) takes the nearest inside
     const double target = (double)fminf(fmaxf(a.v[s], 0.f), 0x1.fffffep-1f) * all;
-    if (tid == max(0, passing_thread(inc, w, target, s_t[0]))) {  // among the thread's splits
+    if (tid == max(0, passing_thread(inc, w, target, s_t[0]))) {  // among the thread's splits, as among the threads
         double c = inc - w;
-        int i = i0;
-        for (; i + 1 < i1; i++) {
+        s_split = i0;
+        s_ahead = c;
+        for (int i = i0; i < i1; i++) {
             const double x = left ? mine[i].x : mine[i].y;
-            if (c + x > target) break;
+            if (x > 0.0) {
+                s_split = i;
+                s_ahead = c;
+                if (c + x > target) break;
+            }
             c += x;
         }
-        s_split = i;
-        s_ahead = c;
     }
     __syncthreads();
     const int split = min(s_split, S - 1);

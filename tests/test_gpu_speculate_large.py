@@ -5,7 +5,7 @@ are those of test_gpu_speculate."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_speculate import check_probs, check_verify, device_probs, drafted, model_logits, ref_probs
+from tests.test_gpu_speculate import check_probs, check_verify, device_probs, device_verify, drafted, model_logits, ref_probs
 
 pytestmark = pytest.mark.gpu
 PARAMS = [(0.7, 0, 1.0), (0.0, 0, 1.0), (0.8, 40, 0.9), (1.0, 0, 0.95), (1.0, 512, 0.8), (1.0, 700, 0.999), (2.0, 0, 0.3)]
@@ -72,3 +72,33 @@ def test_verify_with_several_splits_a_thread(hip, n, V):
     starts = np.arange(n + 1).astype(np.int32)
     for v in (0.0, 1e-4, 0.3, 0.7, 0.9999999):
         check_verify(hip, p, None, np.zeros(n, np.uint32), starts, np.zeros(n, np.float32), np.full(n, v, np.float32))
+
+
+# (seed, a tail's second value): the target lies within a rounding of the running sum behind a thread's first split, and
+# its second split is empty (found with the device's order of sums, on the CPU)
+BORDERS = [(9, "0x1.f04daep-45"), (31, "0x1.d30e94p-45"), (53, "0x1.d7c288p-45"), (85, "0x1.d7b0a2p-45"),
+           (91, "0x1.d80e26p-45"), (92, "0x1.ef4c38p-45")]
+
+
+def test_a_draw_next_to_a_split_of_nothing_takes_a_token_of_some_weight(hip):
+    V, split = 600000, 2048
+    v = np.float32(1 - 2.0 ** -24)
+    for a in range(0, len(BORDERS), 3):
+        p = np.zeros((3, V), np.float32)
+        for row, (seed, last) in zip(p, BORDERS[a:a + 3]):
+            rng = np.random.default_rng(seed)
+            w = np.zeros(-(-V // split), np.float32)
+            j = rng.integers(40, 120)
+            w[0] = 0.9
+            for t in range(1, j + 1):
+                w[2 * t] = rng.random() * 1e-9
+            tail = 2 * j + 2 + 2 * rng.integers(1, 6, 1)[0]
+            w[tail] = float(np.sum(w.astype(np.float64))) / (2 ** 24 - 1) * (1 - 1e-6)
+            w[tail + 2] = float.fromhex(last)
+            row[np.arange(w.size) * split] = w
+        _, tok = device_verify(hip, p, None, np.zeros(3, np.uint32), np.arange(4), np.zeros(3, np.float32), np.full(3, v))
+        for row, t in zip(p, tok):
+            assert row[t] > 0, t
+            before = row[:t].astype(np.float64).sum()  # a border of the draw's, to a few roundings
+            target = row.astype(np.float64).sum() * float(v)
+            assert before - 1e-12 <= target <= before + float(row[t]) + 1e-12
