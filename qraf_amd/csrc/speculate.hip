@@ -80,17 +80,18 @@ __device__ __forceinline__ double weight64(float l, float m, double T) {
 }
 
 // the same in 32 bits, off by at most 3 units of the last place: the exponent's
-// rounding errors (of l - m, of its product with log2(e) / T) as a factor behind it
+// rounding errors (of l - m, of its product with log2(e) / T) as a factor behind it.
+// l and m by halves: their difference may leave fp32's range where T brings it back
 struct Weight32 {
-    float m, c, c_lo;
-    __device__ __forceinline__ Weight32(float m_, double T) : m(m_) {
-        const double k = 1.4426950408889634074 / T;
+    float m, mh, c, c_lo;
+    __device__ __forceinline__ Weight32(float m_, double T) : m(m_), mh(0.5f * m_) {
+        const double k = 2 * 1.4426950408889634074 / T;
         c = (float)k;
         c_lo = (float)(k - (double)c);
     }
     __device__ __forceinline__ float operator()(float l) const {
-        const float d = l - m, bb = d + m;                  // l - m = d + err (Knuth's two-sum)
-        const float err = (l - bb) + (m - (bb - d));
+        const float d = __builtin_fmaf(l, 0.5f, -mh), bb = d + mh;  // (l - m) / 2 = d + err (Knuth's two-sum)
+        const float err = __builtin_fmaf(l, 0.5f, -bb) + (mh - (bb - d));
         const float h = d * c;
         const float e = __builtin_fmaf(d, c, -h) + __builtin_fmaf(d, c_lo, err * c);
         const float w = __builtin_amdgcn_exp2f(h);

@@ -52,6 +52,15 @@ def test_probs_of_equal_masked_and_infinite_rows(hip):
         check_probs(device_probs(hip, x, T, k, p), ref_probs(x, T, k, p))
 
 
+@pytest.mark.parametrize("V", [1000, 4099, 151936])
+def test_probs_of_logits_further_apart_than_fp32(hip, V):
+    """Differences past fp32's largest, over a temperature that brings them back: -6.6 at the most."""
+    rng = np.random.default_rng(V)
+    x = rng.uniform(-3.3e38, 3.3e38, (14, V)).astype(np.float32)
+    for T, k, p in ((1e38, 0, 1.0), (1e38, 40, 1.0), (1e38, 0, 0.95), (2e38, 700, 0.9), (3e38, 0, 1.0)):
+        check_probs(device_probs(hip, x, T, k, p), ref_probs(x, T, k, p))
+
+
 @pytest.mark.parametrize("given", [True, False], ids=["model", "ngram"])
 @pytest.mark.parametrize("n,V", [(13, 151936), (14, 151936), (16, 151937), (40, 52429), (4, 524289)])
 def test_verify(hip, n, V, given):
