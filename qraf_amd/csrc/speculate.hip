@@ -1010,7 +1010,7 @@ __global__ __launch_bounds__(STH) void verify_pick_kernel(VerifyArgs a, const do
         double c = inc - w;
         s_split = i0;
         s_ahead = c;
-        for (int i = i0; i < i1; i++) {
+        for (int i = i0; per > 1 && i < i1; i++) {
             const double x = left ? mine[i].x : mine[i].y;
             if (x > 0.0) {
                 s_split = i;
