@@ -660,9 +660,18 @@ int qraf_engine_set_row_padding(qraf_engine* engine, int32_t rows);
  * products as at batch 1, summed in another order than the GEMM's); bit 3
  * (default off) = in steps that hold several rows of a sequence one behind
  * another (drafted tokens, prompt chunks), where those share enough positions
- * for it to pay, attention reads them once (qraf_hip_group_attention_dev: the
- * same sums in another order).  No reference counterpart (launch-count and traffic measures). */
+ * for it to pay (below), attention reads them once: qraf_hip_group_attention_dev,
+ * whose f32 operands keep 22 bits; head_dim 64 or 128, pages of 16 positions and
+ * more, elsewhere attention goes on by row.  No reference counterpart
+ * (launch-count and traffic measures). */
 int qraf_engine_set_fusion(qraf_engine* engine, int32_t flags);
+/* With bit 3: the least that a step has to share for it, in positions (each row
+ * of a sequence but its last counts those it attends to) times KV heads times
+ * head_dim.  Default 24,000,000, where it measured faster; 0: every step with
+ * several rows of a sequence.  qraf_engine_group_steps: steps so far that went
+ * by group.  No reference counterpart. */
+int qraf_engine_set_group_least(qraf_engine* engine, int64_t least);
+int qraf_engine_group_steps(qraf_engine* engine, uint64_t* steps);
 /* Repetition penalty on the device for one sequence, set before its first
  * step (QRAF_HIP_ERR_STATE after): from then on every token the sequence is
  * fed (prompt rows, decode rows, tokens taken on the device from a previous

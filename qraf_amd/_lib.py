@@ -153,6 +153,8 @@ SIGNATURES.update({
     "qraf_engine_set_keep_logits": (C.c_int, [vp, C.c_int32]),
     "qraf_engine_set_row_padding": (C.c_int, [vp, C.c_int32]),
     "qraf_engine_set_fusion": (C.c_int, [vp, C.c_int32]),
+    "qraf_engine_set_group_least": (C.c_int, [vp, C.c_int64]),
+    "qraf_engine_group_steps": (C.c_int, [vp, C.POINTER(C.c_uint64)]),
     "qraf_engine_set_repetition_penalty": (C.c_int, [vp, C.c_int32, C.c_float]),
     "qraf_engine_forward": (C.c_int, [vp, C.c_uint32, C.c_int32, fp]),
     "qraf_engine_read_logits": (C.c_int, [vp, C.c_int32, C.c_int32, fp]),

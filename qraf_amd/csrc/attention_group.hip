@@ -1682,7 +1682,7 @@ static size_t group_lds(int hd, int n, int groups, const GroupSizes& z) {
 }
 // shapes of the tiles (their LDS bounds what few very wide layouts would need; offsets inside a page, and of q, are
 // held in 32 bits)
-static bool group_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
+bool group_attention_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
     const int G = H / Hkv;
     return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 && (long long)page_size * hd <= 1 << 29 &&
            (long long)n * H * hd <= 1 << 30 && group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
@@ -1713,7 +1713,7 @@ int group_attention_init() {
 // (of any page size: one that the tiles do not take needs less)
 size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd, int max_ctx) {
     (void)max_ctx;
-    if (H % Hkv || !group_tiles(n, groups, H, Hkv, hd, 16)) return 16;
+    if (H % Hkv || !group_attention_tiles(n, groups, H, Hkv, hd, 16)) return 16;
     const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
     return z.plan_bytes + z.ml_bytes + z.o_bytes;
 }
@@ -1761,7 +1761,7 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
     a.max_pages = max_pages;
     a.max_ctx = max_ctx;
     a.scale = scale;
-    if (group_tiles(n, groups, H, Hkv, hd, page_size)) {
+    if (group_attention_tiles(n, groups, H, Hkv, hd, page_size)) {
         const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
         a.job_cap = z.job_cap;
         a.tail_log2 = z.tail_log2;

@@ -443,6 +443,13 @@ struct qraf_engine {
     bool fuse_swiglu = true;          // steps over 256 rows: SiLU-gate in the gate/up GEMM's epilogue
     bool batch_mv = true;             // steps of 2-8 rows: projections on the multi-vector matvec
     bool group_rows = false;          // steps with several rows of a sequence: their shared positions read once
+    // ... where that spares enough, in positions times KV heads times dimensions: attention by row takes about as long
+    // for a position as it has of those, whatever the pages.  A layer by row less the same by group, 2 heads of 128,
+    // f32 / fp16 / int8: 5 rows at 4,000 positions (16,000 spared) -5 / -7 / -6 us, 128 at 512 (73,000) -6 / -9 / -7,
+    // 16 sequences of 5 at 2,000 (128,000) +18 / +2 / +3, 64 of 4 at 1,000 (192,000) +25 / +8 / +11, 4 of 128 at 1,024
+    // (553,000) +73 / +41 / +56.
+    int64_t group_least = 24000000;
+    uint64_t group_steps = 0;         // steps issued that way
     int32_t default_seq = -1;
     int last_logit_rows = 0;          // logit rows the last step left in `logits`
     bool keep_logits = true;          // false: greedy-only steps take the head's argmax without writing logits
@@ -1132,12 +1139,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     // Runs of rows of one sequence: a group that shares the positions up to its longest context, whose pages the
     // group's first row has to name (its own table ends where its position did).  Pad rows are a group, unused
     // entries empty ones.
-    // By group when that spares enough: attention by row takes about as long for a position as it has KV heads times
-    // dimensions, whatever the pages.  A layer by row less the same by group, 2 heads of 128, f32 / fp16 / int8:
-    // 5 rows at 4,000 positions (16,000 spared) -5 / -7 / -6 us, 128 at 512 (73,000) -6 / -9 / -7, 16 sequences of 5
-    // at 2,000 (128,000) +18 / +2 / +3, 64 of 4 at 1,000 (192,000) +25 / +8 / +11, 4 of 128 at 1,024 (553,000)
-    // +73 / +41 / +56.
-    constexpr long long GROUP_LEAST = 24000000;
+    // By group when that spares enough (group_least), in shapes that it reads shared positions of once.
     int groups = 0;
     long long spared = 0;  // positions
     for (int i = 0; i < n_pad; i++) {
@@ -1154,7 +1156,9 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     }
     for (int g = groups; g < n_pad; g++) gpre[g] = 0;
     for (int g = groups; g <= n_pad; g++) gstart[g] = n_pad;
-    const bool grouped = e->group_rows && spared * (long long)(c.num_kv_heads * e->hd) >= GROUP_LEAST;
+    const bool grouped = e->group_rows && spared > 0 && spared * (long long)(c.num_kv_heads * e->hd) >= e->group_least &&
+                         group_attention_tiles(n_pad, n_pad, (int)c.num_heads, (int)c.num_kv_heads, e->hd, ps);
+    e->group_steps += grouped;
     const int n_logit_real = n_logit_rows;
     if (n_pad != n && n_logit_rows > 0) {
         const int nl = std::min((n_logit_rows + e->row_pad - 1) / e->row_pad * e->row_pad, n_pad);
@@ -1547,6 +1551,20 @@ int qraf_engine_set_fusion(qraf_engine* e, int32_t flags) {
     e->batch_mv = (flags & 4) != 0;
     e->group_rows = (flags & 8) != 0;
     e->drop_graphs();  // captured steps hold the other form
+    return QRAF_HIP_OK;
+}
+
+int qraf_engine_set_group_least(qraf_engine* e, int64_t least) {
+    clear_error();
+    QH_REQUIRE(e && least >= 0, QRAF_HIP_ERR_INVALID, "set_group_least: least %lld", (long long)least);
+    e->group_least = least;
+    return QRAF_HIP_OK;
+}
+
+int qraf_engine_group_steps(qraf_engine* e, uint64_t* steps) {
+    clear_error();
+    QH_REQUIRE(e && steps, QRAF_HIP_ERR_INVALID, "group_steps: null argument");
+    *steps = e->group_steps;
     return QRAF_HIP_OK;
 }
 

@@ -256,8 +256,19 @@ class Engine:
         it covers them (default on; batch-1 arithmetic instead of the GEMM's).
         Bit 3: steps with several rows of a sequence one behind another read
         the positions that they share once, where that pays (default off;
-        the same sums in another order)."""
+        f32 operands in 22 bits)."""
         call("qraf_engine_set_fusion", self.h, int(flags))
+
+    def set_group_least(self, least: int) -> None:
+        """With fusion bit 3: what a step has to share at least, in positions
+        times KV heads times head_dim (default 24,000,000; 0: any)."""
+        call("qraf_engine_set_group_least", self.h, int(least))
+
+    def group_steps(self) -> int:
+        """Steps so far whose attention read shared positions once."""
+        n = C.c_uint64()
+        call("qraf_engine_group_steps", self.h, C.byref(n))
+        return n.value
 
     def set_row_padding(self, rows: int) -> None:
         """Steps of more than 8 rows run padded to a multiple of `rows` (with
