@@ -53,6 +53,55 @@ PLAN = [[(0, 0, 40), (1, 0, 3)], [(0, 40, 21), (1, 3, 19)], [(0, 61, 1), (1, 22,
         [(1, 27, 5)], [(0, 71, 4), (1, 32, 9)], [(0, 71, 4), (1, 32, 9)], [(0, 71, 4), (1, 32, 9)], [(0, 75, 50)]]
 
 
+@KINDS
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("layers", [1, 3])
+@pytest.mark.parametrize("name", TILES)
+def test_steps_by_group(hip, name, layers, page, kv):
+    toks = tokens(np.random.default_rng(1), SMALL[name][0], 300)
+    got = []
+    for flags in (7, 15):
+        tf = engine(name, kv, 64, page, flags, layers=layers)
+        got.append(run(tf.engine, toks, PLAN))
+        assert tf.engine.group_steps() == (0 if flags == 7 else len(PLAN) - 1)  # all but the one of single rows
+        assert flags == 7 or tf.engine.stats()["pad_rows"] > 0
+        tf.engine.close()
+    compare(*got, kv, layers)
+
+
+@KINDS
+def test_many_rows_by_group(hip, kv):
+    """Steps of the batched layers, whose attention writes the next product's planes."""
+    toks = tokens(np.random.default_rng(2), SMALL["q4_gqa8_hd128"][0], 300)
+    plan = [[(s, at, 15) for s in range(8)] for at in (0, 15, 30)] + [[(0, 45, 100), (1, 45, 28)]]
+    got = []
+    for flags in (7, 15):
+        tf = engine("q4_gqa8_hd128", kv, 128, 16, flags)
+        got.append(run(tf.engine, toks, plan))
+        assert tf.engine.group_steps() == (flags == 15) * len(plan)
+        tf.engine.close()
+    compare(*got, kv, 3)
+
+
+@pytest.mark.parametrize("kv", [po.F32, po.F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("name", TILES)
+def test_greedy_generation_by_group(hip, name, kv):
+    """n-gram drafts and a model's drafts give the greedy tokens."""
+    from qraf_amd.engine import InferenceEngine
+    tf, other = engine(name, kv, 16), engine(name, kv, 8)
+    prompt = tokens(np.random.default_rng(4), SMALL[name][0], 7) * 3
+    want, sure = reference_stream(tf, prompt, 30)
+    gen = InferenceEngine(tf, eos_token=None)
+    for draft in (None, other):
+        for drafts in (1, 4, 15):
+            before = tf.engine.group_steps()
+            got = gen.generate_speculative(prompt, max_tokens=30, drafts=drafts, draft=draft)
+            assert len(got) == 30 and got[:sure] == want[:sure], (drafts, draft is not None)
+            assert tf.engine.group_steps() > before
+    other.engine.close()
+    tf.engine.close()
+
+
 @pytest.mark.parametrize("name,page,kv", [("q8_llama", 16, po.F32), ("q4_qwen2_tied_bias", 16, po.F16),
                                           ("q8_hd64_gqa3", 8, po.F16), ("q4_gqa8_hd128", 4, po.F32),
                                           ("q4_gqa8_hd128", 8, I8)])
