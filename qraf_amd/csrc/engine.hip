@@ -1136,28 +1136,34 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         ppen[i] = 1.f;
         for (int j = 0; j < MP; j++) ptab[(size_t)i * MP + j] = j == 0 ? e->scratch_page : 0;
     }
-    // Runs of rows of one sequence: a group that shares the positions up to its longest context, whose pages the
-    // group's first row has to name (its own table ends where its position did).  Pad rows are a group, unused
-    // entries empty ones.
-    // By group when that spares enough (group_least), in shapes that it reads shared positions of once.
-    int groups = 0;
-    long long spared = 0;  // positions
-    for (int i = 0; i < n_pad; i++) {
-        if (i > 0 && (i < n ? seq_ids[i] == seq_ids[i - 1] : i > n)) {
-            if (ctx[i] > gpre[groups - 1]) {
-                gpre[groups - 1] = ctx[i];
-                memcpy(ptab + (size_t)gstart[groups - 1] * MP, ptab + (size_t)i * MP, (size_t)MP * 4);
+    // Runs of rows of one sequence: a group that shares the positions up to its longest context.  Pad rows are a group,
+    // unused entries empty ones.  By group when that spares enough (group_least), in shapes that it reads shared
+    // positions of once.
+    bool grouped = false;
+    if (e->group_rows) {
+        int groups = 0;
+        long long spared = 0;  // positions
+        for (int i = 0; i < n_pad; i++) {
+            if (i > 0 && (i < n ? seq_ids[i] == seq_ids[i - 1] : i > n)) {
+                gpre[groups - 1] = std::max(gpre[groups - 1], ctx[i]);
+                spared += ctx[i - 1];
+            } else {
+                gpre[groups] = ctx[i];
+                gstart[groups++] = i;
             }
-            spared += ctx[i - 1];
-        } else {
-            gpre[groups] = ctx[i];
-            gstart[groups++] = i;
         }
+        for (int g = groups; g < n_pad; g++) gpre[g] = 0;
+        for (int g = groups; g <= n_pad; g++) gstart[g] = n_pad;
+        grouped = spared > 0 && spared * (long long)(c.num_kv_heads * e->hd) >= e->group_least &&
+                  group_attention_tiles(n_pad, n_pad, (int)c.num_heads, (int)c.num_kv_heads, e->hd, ps);
+        // a group's pages are read through its first row's, whose own ended where its position did
+        for (int g = 0; grouped && g < groups; g++)
+            for (int i = gstart[g]; i < gstart[g + 1]; i++)
+                if (ctx[i] == gpre[g]) {
+                    if (i > gstart[g]) memcpy(ptab + (size_t)gstart[g] * MP, ptab + (size_t)i * MP, (size_t)MP * 4);
+                    break;
+                }
     }
-    for (int g = groups; g < n_pad; g++) gpre[g] = 0;
-    for (int g = groups; g <= n_pad; g++) gstart[g] = n_pad;
-    const bool grouped = e->group_rows && spared > 0 && spared * (long long)(c.num_kv_heads * e->hd) >= e->group_least &&
-                         group_attention_tiles(n_pad, n_pad, (int)c.num_heads, (int)c.num_kv_heads, e->hd, ps);
     e->group_steps += grouped;
     const int n_logit_real = n_logit_rows;
     if (n_pad != n && n_logit_rows > 0) {
