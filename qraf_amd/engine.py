@@ -298,10 +298,12 @@ class Engine:
         return out
 
 
-    def _penalty(self, params, recent):
+    def _penalty(self, params, recent, rows):
         """The recent lists of a call's rows as the host arrays of a repetition penalty: (tokens, counts, stride)."""
         if recent is None or params.repetition_penalty == 1.0:
             return None, None, 0
+        if len(recent) != rows:
+            raise ValueError(f"recent: {len(recent)} for {rows}")
         rec = np.zeros((len(recent), max(1, max(len(r) for r in recent))), np.uint32)
         cnt = np.array([len(r) for r in recent], np.int32)
         for i, r in enumerate(recent):
@@ -311,7 +313,7 @@ class Engine:
     def probs(self, params: SamplingParams, out: int, recent=None, row0=0, rows=1) -> None:
         """The distributions that sample() draws from, for rows row0.. of the last step's logit rows, to the device
         memory at `out` [rows][vocab] (qraf_engine_probs)."""
-        rec, cnt, stride = self._penalty(params, recent)
+        rec, cnt, stride = self._penalty(params, recent, rows)
         call("qraf_engine_probs", self.h, row0, rows, C.byref(params),
              rec.ctypes.data_as(u32p) if rec is not None else None,
              cnt.ctypes.data_as(i32p) if cnt is not None else None, stride, out)
@@ -324,10 +326,10 @@ class Engine:
         needed when greedy).  Per sequence the tokens it emits: its accepted drafts and the one behind them."""
         counts = np.array([len(d) + 1 for d in drafts], np.int32)
         tok = np.array([t for d in drafts for t in (*d, 0)], np.uint32)
-        rec, cnt, stride = self._penalty(params, recent)
+        rec, cnt, stride = self._penalty(params, recent, tok.size)
         uni = None if uniforms is None else np.ascontiguousarray(uniforms, dtype=np.float32)
         pic = None if picks is None else np.ascontiguousarray(picks, dtype=np.float32)
-        for name, a, n in (("uniforms", uni, tok.size), ("picks", pic, counts.size), ("recent", cnt, tok.size)):
+        for name, a, n in (("uniforms", uni, tok.size), ("picks", pic, counts.size)):
             if a is not None and a.size != n:
                 raise ValueError(f"{name}: {a.size} for {n}")
         accepted, out = np.empty(counts.size, np.int32), np.empty(tok.size, np.uint32)
