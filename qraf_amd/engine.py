@@ -541,7 +541,11 @@ class _Drafter:
             self.seq = model.engine.seq_create()
             if sampler is not None:
                 from .backend import DeviceBuffer
-                self.q = DeviceBuffer((drafts + 1) * vocab * 4)  # row j: what draft j was drawn from; the last unused
+                try:
+                    self.q = DeviceBuffer((drafts + 1) * vocab * 4)  # row j: what draft j was drawn from; the last unused
+                except BaseException:
+                    self.close()
+                    raise
 
     def close(self):
         if self.seq >= 0:
