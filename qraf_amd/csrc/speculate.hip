@@ -191,8 +191,9 @@ __device__ __forceinline__ void block_first_max(float& m, int& mi, float* s_f, i
         }
 }
 
-// what follows: the write, top_k (clear: and the probabilities are zeroed for it), the nucleus' bins
-enum : int { STATS_SUM = 0, STATS_SUB = 1, STATS_BINS = 2 };
+// what follows: the write of whole rows, top_k (clear: and the probabilities are zeroed for it), the nucleus' bins, or
+// what needs the largest logit alone
+enum : int { STATS_SUM = 0, STATS_SUB = 1, STATS_BINS = 2, STATS_MAX = 3 };
 
 template <int E, bool VEC>
 __device__ __forceinline__ void store_split(float* p, int V, int split, const float (&v)[E]) {
@@ -815,7 +816,7 @@ int launch_sample_probs(float* logits, int rows, int V, const qraf_sampling_para
 #define QH_PROBS(Ev, Vv)                                                                                            \
     if (e == Ev && vec == Vv) {                                                                                     \
         hipLaunchKernelGGL((probs_stats_kernel<Ev, Vv>), grid, dim3(STH), 0, s, a,                                  \
-                           topk ? STATS_SUB : bins ? STATS_BINS : STATS_SUM, (int)scatter);                         \
+                           topk ? STATS_SUB : bins ? STATS_BINS : cuts || greedy ? STATS_MAX : STATS_SUM, (int)scatter);                         \
         if (topk) {                                                                                                 \
             hipLaunchKernelGGL((probs_topk_kernel<Ev, Vv>), dim3(rows), dim3(PNT), 0, s, a, (int)scatter);          \
         } else if (bins) {                                                                                          \
