@@ -245,11 +245,17 @@ uint64_t qraf_hip_attention_noalloc_max_bytes(void);
  * (qraf_hip_group_attention_workspace_bytes) needs no initialisation; calls that
  * share one must not overlap.
  * Results are within the attention tolerance of qraf_hip_paged_attention_dev's
- * on the same rows, and the same from call to call.  (f32 pages: an element of
- * a q, K or V vector is held to 2^-22 of itself and 2^-25 of the vector's
- * largest; a weighted V, of int8 pages too, to 2^-20 of the row's largest.)
+ * on the same rows, and the same from call to call.  By row f32 operands are
+ * fp32; here q, weights and f32 K and V are two fp16 halves: an element of a
+ * vector is held to 2^-22 of itself and 2^-25 of the vector's largest (and 2^-135),
+ * a weighted V of f32 and int8 pages to 2^-20 of the row's largest, a weight over
+ * fp16 pages to 2^-38 of the row's largest.
  * Values of positions that a row does not attend to do not reach it, an infinity
  * or NaN among them, nor do the words of a row's own pages below the prefix.
+ * Shared positions are read once by blocks of 128 query vectors (head_dim 64 and
+ * 128, page_size a power of two from 16, up to 128 query heads per KV head); in
+ * small calls (a workgroup per row and KV head) and all other shapes each row
+ * reads them.
  * No counterpart in the reference, which runs one sequence at a time. */
 uint64_t qraf_hip_group_attention_workspace_bytes(int32_t n_rows, int32_t n_groups, int32_t n_heads,
                                                   int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx);
@@ -464,10 +470,12 @@ int qraf_hip_sample_dev(float* logits, int32_t rows, int32_t vocab, const qraf_s
 /* The distribution that qraf_hip_sample_dev draws from, as probabilities:
  * probs [rows][vocab] (logits itself, or not overlapping it) from logits
  * [rows][vocab], rows up to 65535 and vocab up to 2^30, for verification against
- * a draft (below).  With 64-bit weights w_i = exp((l_i -
- * max) / T): of the top_k largest logits (all when top_k <= 0 or >= vocab;
- * equal logits in index order) the shortest prefix whose weight reaches top_p
- * times theirs (all of them unless 0 < top_p < 1), w_i over their sum; 0 elsewhere.
+ * a draft (below).  With w_i = exp((l_i - max) / T): of the top_k largest logits
+ * (all when top_k <= 0 or >= vocab; equal logits in index order) the shortest
+ * prefix whose weight reaches top_p times theirs (all of them unless 0 < top_p <
+ * 1), w_i over their sum; 0 elsewhere.  What is kept is decided by 64-bit
+ * exponentials, summed in steps of 2^-62 times the power of two above vocab; the
+ * probabilities are 32-bit and within 8 * 2^-24 of their values.
  * temperature <= 0: 1 at the first of the largest logits (Sampler::argmax,
  * sampler.cpp:25-35).  repetition_penalty, recent, recent_count and
  * recent_stride as for qraf_hip_sample_dev (the logits are penalised in place).
@@ -611,7 +619,8 @@ int qraf_engine_probs(qraf_engine* engine, int32_t row0, int32_t rows, const qra
  * recent_stride [rows]: a row's history holds the drafts ahead of it.  accepted
  * [n_seqs] and tokens [rows] as there.  The sequence's next step begins at the
  * position behind its accepted drafts: feeding a position again overwrites it.
- * No reference counterpart. */
+ * (The counts of qraf_engine_set_repetition_penalty keep rejected drafts: here
+ * the penalty comes with the call.)  No reference counterpart. */
 int qraf_engine_verify(qraf_engine* engine, int32_t row0, int32_t n_seqs, const int32_t* row_counts,
                        const qraf_sampling_params* params, const uint32_t* recent, const int32_t* recent_count,
                        int32_t recent_stride, const uint32_t* draft_tokens, const float* draft_probs,

@@ -206,10 +206,12 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
 // the second: nothing moves between lanes.  32 columns and not 16: half the
 // operand reads per product, and the reads are what bounds it.
 //
-// q, p and f32 K and V enter as fp16 hi + lo pairs (23 bits), fp16 K and V as they
+// q, p and f32 K and V enter as fp16 hi + lo pairs (22 bits), fp16 K and V as they
 // are, int8 widened; a product of two pairs is three matrix products (lo x lo is
-// below 2^-22).  int8 scales: K's on the scores, V's on p.  Sums in fp32.  So that
-// neither half leaves fp16's range,
+// below 2^-22).  A choice for speed: three of them run at 383 TFLOP/s where fp32
+// matrix products run at 154, and outputs come within 2.8e-7 to 3.5e-7 of 64-bit ones
+// (fp32 products: 2.2e-7 to 4.7e-7).  int8 scales: K's on the scores, V's on p.  Sums
+// in fp32.  So that neither half leaves fp16's range,
 //   q     is over a power of two of its column,
 //   K, V  (f32) over one of their tile's, in [2^14, 2^15) at its largest, or, where the
 //         positions of a tile lie further apart than SPREAD, each over its own: a
@@ -223,11 +225,13 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
 // tile's scores, V behind its outputs, straight into the wave's registers; two waves
 // per SIMD cover each other's waits.  More columns: four waves share tiles in LDS.
 // Measured (16/2 heads of 128, us): 48 sequences of 5 rows at 128..4,096 fp16 positions
-// 40, of which the tiles 34 (108 MB at 5 TB/s of HBM while they run, beside 6 of plan
-// and prologue); 128 rows behind 2,048 shared and 512 own ones 28, half of it plan,
-// prologue and join; 4 chunks of 128 rows at 400..2,000 f32 positions 43; 256 rows of
-// 32,768: fp16 197 (348 TFLOP/s of products with q and p in 22 bits: 697 of the
-// matrix cores'), int8 248, f32 280.
+// 41, of which the tiles 34 (117 MB read in the 28 beside 6 of plan and prologue: the
+// rate of a plain read); 128 rows behind 2,048 shared and 512 own ones 27, half of it
+// plan, prologue and join; 4 chunks of 128 rows at 400..2,000 f32 positions 46 (matrix
+// cores 18% busy, VALU 44%, 23% of the waves' time waiting for an instruction's turn);
+// 256 rows of 32,768: fp16 154 (446 TFLOP/s of products with q and p in 22 bits: 893
+// of the matrix cores'), int8 198, f32 266.  Powers of two by position and column cost
+// f32 3 to 4% over one for a tile and a running one, and int8 nothing.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -868,8 +872,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             // Tiles of more than 64 columns: the four waves side by side load a quarter of a tile each, 8 positions, and
             // write it as operands for all of them, f32 split (alone each would load and split it all, and a lane to a
             // position reads a line of memory per lane).  The tiles lie where q's hi halves were, which stay in
-            // registers.  f32: K's and V's powers of two are those of the 8 positions, or each position's.  256 rows of 32,768 positions, 16/2 heads of 128: f32 280 us for 444, fp16 197 for 221; int8
-            // gained nothing (254 for 253) and goes on alone.
+            // registers.  f32: K's and V's powers of two are those of the 8 positions, or each position's.  256 rows of
+            // 32,768 positions, 16/2 heads of 128: f32 in 0.63 and fp16 in 0.89 of the time of waves alone; int8 gained
+            // nothing and goes on alone.
             if (shared) {
                 constexpr int NP = HD / 64, PCS = HD / 8, RP = 64 / PCS;  // K: passes, pieces of a row, rows of a pass
                 constexpr int HL = F32 ? 2 : 1, KP = HL * QT, VP = 2 * 64 * DT, TP = KP + HL * VP;  // 16-byte pieces: hi, lo

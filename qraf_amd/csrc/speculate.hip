@@ -11,11 +11,16 @@
 //   p_i = w_i / sum_{j in N} w_j for i in N, 0 elsewhere.
 // The kept set is one threshold: the order-preserving key of its smallest
 // logit and the number of equal logits it takes, lowest indices first.  It is
-// Weights are summed as integers there (w times a power of two that keeps the
-// row's sum below 2^62, from a 64-bit exponential): integer sums do not depend on
-// the order of the atomics, so results repeat bit for bit, and the border of a
+// found from a short list of candidates in order, or by a radix select over all
+// keys.  Weights are summed as integers there (w times a power of two that keeps
+// the row's sum below 2^62, from a 64-bit exponential): integer sums do not depend
+// on the order of the atomics, so results repeat bit for bit, and the border of a
 // nucleus whose tokens weigh 1e-6 of the row each is the one of the sums in 64-bit
-// floating point.
+// floating point.  (Steps of 2^-62 times the next power of two above the
+// vocabulary: 2^-44 of the largest weight for 151,936 tokens.)  The probabilities
+// themselves are 32-bit products, w by a two-part exponent, sums of whole rows in
+// 32 bits within a split and in 64 over the splits: within 8 * 2^-24 of a value, which
+// a 32-bit result has room for and the draw (64-bit sums of them) takes as it is.
 //
 // A row of 152K logits is read by many workgroups (one alone reads 600 KB in
 // 10 us), in launches that follow one another:
@@ -29,9 +34,10 @@
 //           nucleus of the whole row: weights by bins of the logits' distance from
 //           the largest (probs_bins_kernel), the logits of the bin in which top_p
 //           is reached (probs_gather_kernel), those in order (probs_border_kernel)
-//           else, and where such a list overflows (flat rows): radix select over
-//           the keys by one workgroup
-//   write   w_i / sum in 32 bits, w by a two-part exponent
+//           else (top_k over 512, or of more sub-ranges than the workgroup holds:
+//           from 163,841 logits by 8, 655,361 by 32), and where such a list
+//           overflows (flat rows): radix select over the keys by one workgroup
+//   write   w_i / sum in 32 bits
 //
 // qraf_hip_verify_draft_dev: row j of a sequence is the target's distribution
 // behind its first j drafted tokens.  Draft x_j, drawn from q_j, is accepted
