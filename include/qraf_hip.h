@@ -265,6 +265,36 @@ int qraf_hip_group_attention_dev(const float* q, const void* k_cache, const void
                                  int32_t n_groups, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                  int32_t page_size, float scale, int32_t max_ctx, float* out, void* workspace,
                                  uint64_t workspace_bytes, void* stream);
+/* Attention of trees of drafted tokens: sequence s has rows row_starts[s] ..
+ * row_starts[s+1]-1, the nodes of its tree, and base_lens[s] positions of cache
+ * ahead of them.  A row attends to all of its sequence's cache and, of the
+ * positions behind it, to those that its mask names.  The batch of
+ * qraf_hip_paged_attention_dev (its caches, page types, scale and out), but:
+ *   page_table [n_seqs][max_pages_per_seq], a row for each sequence
+ *   row_starts [n_seqs + 1] ascending (a sequence may have no rows)
+ *   base_lens [n_seqs] positions that every row of the sequence attends to
+ *   masks [n_rows]: bit b set: the row attends to position base_lens[s] + b
+ * (All of them on the device; entries are taken into 0 .. n_rows, 0 .. max_ctx,
+ * and a bit at or past max_ctx names nothing.)  For a tree whose node i lies at
+ * position base + i (qraf_hip_tree_append_dev) a row's mask is its parent's with
+ * its own bit; any other mask will do.  A row that attends to nothing is zero;
+ * rows of no sequence are left as they were.
+ * n_rows 1..1024, n_seqs 1..n_rows, max_ctx up to 2^30; head_dim 16, 32, 64 or
+ * 128, any page_size and any number of query heads per KV head.  q, the caches,
+ * out and the workspace are 16-byte, masks 8-byte aligned.  The workspace
+ * (qraf_hip_tree_attention_workspace_bytes) needs no initialisation; calls that
+ * share one must not overlap.  The same from call to call; what is held of each
+ * operand is as for qraf_hip_group_attention_dev, whose shapes and blocks these
+ * are: a sequence's positions are read once by each 128 query vectors.  Values of
+ * positions that a row does not attend to do not reach it, an infinity or NaN
+ * among them.  No counterpart in the reference, which has no drafts. */
+uint64_t qraf_hip_tree_attention_workspace_bytes(int32_t n_rows, int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
+                                                 int32_t head_dim, int32_t max_ctx);
+int qraf_hip_tree_attention_dev(const float* q, const void* k_cache, const void* v_cache, uint32_t kv_dtype,
+                                const int32_t* page_table, int32_t max_pages_per_seq, const int32_t* base_lens,
+                                const int32_t* row_starts, const uint64_t* masks, int32_t n_rows, int32_t n_seqs,
+                                int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t page_size, float scale,
+                                int32_t max_ctx, float* out, void* workspace, uint64_t workspace_bytes, void* stream);
 /* RoPE angle table, RopeCache::init (ops.cpp:179-193) computed on the host
  * with the host libm: table[pos*head_dim + i] = cos(pos*f_i),
  * table[pos*head_dim + i + 1] = sin(pos*f_i), f_i = 1/powf(theta, i/head_dim)
@@ -283,6 +313,30 @@ int qraf_hip_rope_append_dev(const float* qkv, const float* bias, int32_t n_seqs
                              int32_t n_kv_heads, int32_t head_dim, const int32_t* positions, const float* rope_table,
                              float* q_out, void* k_cache, void* v_cache, uint32_t kv_dtype, const int32_t* page_table,
                              int32_t max_pages_per_seq, int32_t page_size, void* stream);
+
+/* qraf_hip_rope_append_dev for the nodes of trees, whose place in the cache is not
+ * the position that they are rotated for (nodes of one depth share a position):
+ * row i is rotated for positions[i] and its K and V go to position slots[i] of
+ * row row_seqs[i] of the page table ([n_seqs][max_pages_per_seq], as
+ * qraf_hip_tree_attention_dev takes it).  No two rows share a place. */
+int qraf_hip_tree_append_dev(const float* qkv, const float* bias, int32_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                             int32_t head_dim, const int32_t* positions, const int32_t* slots, const int32_t* row_seqs,
+                             const float* rope_table, float* q_out, void* k_cache, void* v_cache, uint32_t kv_dtype,
+                             const int32_t* page_table, int32_t max_pages_per_seq, int32_t page_size, void* stream);
+/* The accepted path of a tree to the positions where its sequence goes on: the K
+ * and V of position base_lens[s] + j become those of base_lens[s] + path[r + j],
+ * r = row_starts[s], for j = 0, 1, .. while the path's entries ascend and are nodes
+ * of the tree (below its number of rows; -1 ends a path: qraf_hip_tree_accept_dev).
+ * In every layer: k_cache and v_cache are n_layers caches of the layouts above,
+ * layer_bytes apart (a multiple of 4).  page_table as for
+ * qraf_hip_tree_attention_dev; entries of a path past max_pages_per_seq pages end
+ * it.  Positions behind the path keep their contents.  n_rows is the number of
+ * entries of path, n_seqs up to 65535, head_dim 16, 32, 64 or 128.  No counterpart
+ * in the reference. */
+int qraf_hip_kv_compact_dev(void* k_cache, void* v_cache, uint32_t kv_dtype, int32_t n_layers, uint64_t layer_bytes,
+                            const int32_t* page_table, int32_t max_pages_per_seq, const int32_t* base_lens,
+                            const int32_t* row_starts, const int32_t* path, int32_t n_seqs, int32_t n_rows,
+                            int32_t n_kv_heads, int32_t head_dim, int32_t page_size, void* stream);
 
 /* ------------------------------------------------- batched quantized GEMM */
 
@@ -516,6 +570,52 @@ int qraf_hip_verify_draft_dev(const float* probs, const float* draft_probs, cons
                               const int32_t* row_starts, int32_t n_seqs, int32_t n_rows, int32_t vocab,
                               const float* accept_uniforms, const float* pick_uniforms, int32_t* accepted,
                               uint32_t* tokens, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* The accepted path of trees of drafted tokens, many sequences at once, on the
+ * device.  Sequence s has rows row_starts[s] .. row_starts[s+1]-1 (row_starts
+ * [n_seqs + 1] ascending, on the device, entries taken into 0 .. n_rows): node 0
+ * the root, its last token that is certain, every other node a draft.
+ *   parents [n_rows] each node's parent, as a node of its sequence, lower than it
+ *            (a node whose parent is not is never reached; a root's: not read)
+ *   draft_tokens [n_rows] each node's token (a root's: not read)
+ *   picks [n_rows] the token sampled from the target's distribution behind each
+ *            node (qraf_hip_sample_dev of the step's logit rows)
+ * From the root, the walk goes from a node to the lowest of its children whose
+ * draft is the node's pick; where there is none, the pick is the next token.  For
+ * drafts that are given, not drawn (a drafter's top alternatives, n-grams), the
+ * emitted tokens are distributed as the target's own samples.
+ *   accepted [n_seqs] drafts accepted;  path [n_rows]: at row_starts[s] the nodes
+ *   of the path, 0 first, then -1 up to the last row;  tokens [n_rows]: there the
+ *   accepted drafts, then the next token, then 0xFFFFFFFF.
+ * A sequence without rows has accepted 0; rows of no sequence get nothing.  n_seqs
+ * up to 65535; a tree may have any number of nodes.  Outputs overlap no input.  No
+ * counterpart in the reference. */
+int qraf_hip_tree_accept_dev(const uint32_t* picks, const uint32_t* draft_tokens, const int32_t* parents,
+                             const int32_t* row_starts, int32_t n_seqs, int32_t n_rows, int32_t* accepted,
+                             int32_t* path, uint32_t* tokens, void* stream);
+
+/* What is said about a token beside it, of rows of logits [rows][vocab] (rows up to
+ * 65535, vocab up to 2^30), device pointers, stream-ordered.  Tokens are in the
+ * order of their logits, equal ones by index; l is a row, m its largest logit:
+ *   logprobs [rows]  ln softmax(l) of the row's token tokens[row]
+ *   ranks [rows]     how many tokens are ahead of it (0: Sampler::argmax)
+ *   entropies [rows] - sum p ln p of p = softmax(l)
+ *   top_tokens, top_logprobs [rows][top]  the first `top` tokens (0..64, at most
+ *            vocab), in order, and their log probabilities
+ * Outputs that are NULL are not wanted (top_tokens and top_logprobs go together;
+ * tokens NULL: no logprobs, no ranks).  A token outside the vocabulary has log
+ * probability -inf and rank -1.  A NaN counts as -inf; of infinite logits each has
+ * the same probability; a row without a logit above -inf has log probabilities of
+ * -inf and entropy 0.  The logits are as the model left them (temperature 1, no
+ * penalty).  Exponentials in 32 bits, sums of whole rows and logarithms in 64:
+ * log probabilities and entropies are within 2^-19 of (1 + their size).  The
+ * workspace (qraf_hip_token_logprobs_workspace_bytes, 16-byte aligned) needs no
+ * initialisation; calls that share one must not overlap.  The same from call to
+ * call.  No counterpart in the reference. */
+uint64_t qraf_hip_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top);
+int qraf_hip_token_logprobs_dev(const float* logits, int32_t rows, int32_t vocab, const uint32_t* tokens,
+                                float* logprobs, int32_t* ranks, float* entropies, int32_t top, uint32_t* top_tokens,
+                                float* top_logprobs, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* QRAF file -> HBM.  The file layout of include/qraf/format.h:26-132 is
  * checked as validate_header (src/qraf/header.cpp:8-45) and get_string

@@ -131,6 +131,17 @@ SIGNATURES.update({
                                             vp, C.c_uint64, vp]),
     "qraf_hip_verify_draft_workspace_bytes": (C.c_uint64, [C.c_int32] * 2),
     "qraf_hip_verify_draft_dev": (C.c_int, [vp, vp, vp, vp] + [C.c_int32] * 3 + [vp, vp, vp, vp, vp, C.c_uint64, vp]),
+    "qraf_hip_tree_attention_workspace_bytes": (C.c_uint64, [C.c_int32] * 6),
+    "qraf_hip_tree_attention_dev": (C.c_int, [vp, vp, vp, C.c_uint32, vp, C.c_int32, vp, vp, vp] + [C.c_int32] * 6 +
+                                    [C.c_float, C.c_int32, vp, vp, C.c_uint64, vp]),
+    "qraf_hip_tree_append_dev": (C.c_int, [vp, vp] + [C.c_int32] * 4 + [vp] * 7 + [C.c_uint32, vp, C.c_int32, C.c_int32,
+                                                                                vp]),
+    "qraf_hip_tree_accept_dev": (C.c_int, [vp, vp, vp, vp, C.c_int32, C.c_int32, vp, vp, vp, vp]),
+    "qraf_hip_kv_compact_dev": (C.c_int, [vp, vp, C.c_uint32, C.c_int32, C.c_uint64, vp, C.c_int32, vp, vp, vp] +
+                                [C.c_int32] * 5 + [vp]),
+    "qraf_hip_token_logprobs_workspace_bytes": (C.c_uint64, [C.c_int32] * 3),
+    "qraf_hip_token_logprobs_dev": (C.c_int, [vp, C.c_int32, C.c_int32, vp, vp, vp, vp, C.c_int32, vp, vp, vp,
+                                              C.c_uint64, vp]),
     "qraf_engine_sample": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), u32p, i32p, C.c_int32, fp,
                                      u32p]),
     "qraf_engine_probs": (C.c_int, [vp, C.c_int32, C.c_int32, C.POINTER(SamplingParams), u32p, i32p, C.c_int32, vp]),

@@ -1859,7 +1859,7 @@ __global__ void rope_append_kernel(const float* __restrict__ qkv, const float* _
                                    int hd, const int32_t* __restrict__ pos, const float* __restrict__ rope,
                                    float* __restrict__ q_out, KT* __restrict__ kc, KT* __restrict__ vc,
                                    const int32_t* __restrict__ page_table, int max_pages, int page_size, int n, int S,
-                                   size_t slice) {
+                                   size_t slice, const int32_t* __restrict__ slots, const int32_t* __restrict__ seqs) {
     const int qd = H * hd, kvd = Hkv * hd, row = qd + 2 * kvd;
     const int per = (qd + kvd) / 2 + kvd;  // work elements per sequence
     for (size_t w = (size_t)blockIdx.x * blockDim.x + threadIdx.x; w < (size_t)n * per;
@@ -1889,7 +1889,8 @@ __global__ void rope_append_kernel(const float* __restrict__ qkv, const float* _
     float a = ld(i0), b = ld(i1);
     const float* bp = bias ? bias : qkv;  // without a bias these loads read qkv and are not used
     const float ba = bp[bias ? i0 : 0], bb = bp[bias ? i1 : 0];
-    const int page = page_table[(size_t)s * max_pages + p / page_size], off = p % page_size;
+    const int at = slots ? slots[s] : p;
+    const int page = page_table[(size_t)(seqs ? seqs[s] : s) * max_pages + at / page_size], off = at % page_size;
     const int i = rot ? i0 % hd : 0;  // even index inside the head
     const float* cs = rope + (size_t)p * hd + i;  // (cos, sin) of pair i/2
     const float c = cs[0], sn = cs[1];
@@ -1936,7 +1937,9 @@ __global__ __launch_bounds__(256) void rope_append_i8_kernel(const float* __rest
                                                              const float* __restrict__ rope, float* __restrict__ q_out,
                                                              int8_t* __restrict__ kc, int8_t* __restrict__ vc,
                                                              const int32_t* __restrict__ page_table, int max_pages,
-                                                             int page_size, int S, size_t slice) {
+                                                             int page_size, int S, size_t slice,
+                                                             const int32_t* __restrict__ slots,
+                                                             const int32_t* __restrict__ seqs) {
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int qd = H * hd, kvd = Hkv * hd;
     // blockIdx.y 0: the K and V heads; y >= 1: q pairs (y-1)*256 + tid, ...
@@ -1946,7 +1949,8 @@ __global__ __launch_bounds__(256) void rope_append_i8_kernel(const float* __rest
         return bias ? __fadd_rn(x, bias[i]) : x;
     };
     const int p = pos[s];
-    const int page = page_table[(size_t)s * max_pages + p / page_size], off = p % page_size;
+    const int at = slots ? slots[s] : p;
+    const int page = page_table[(size_t)(seqs ? seqs[s] : s) * max_pages + at / page_size], off = at % page_size;
     const float* cs = rope + (size_t)p * hd;
     // rotated pair (i0, i0 + 1) of the q|k part, as rope_append_kernel
     auto rot = [&](int i0, float& ra, float& rb) {
@@ -2001,7 +2005,8 @@ __global__ __launch_bounds__(256) void rope_append_i8_kernel(const float* __rest
 
 int launch_rope_append(const float* qkv, const float* bias, int n, int H, int Hkv, int hd, const int32_t* pos,
                        const float* rope, float* q_out, void* kc, void* vc, uint32_t kv_dtype,
-                       const int32_t* page_table, int max_pages, int page_size, hipStream_t st, int S, size_t slice) {
+                       const int32_t* page_table, int max_pages, int page_size, hipStream_t st, int S, size_t slice,
+                       const int32_t* slots, const int32_t* seqs) {
     QH_REQUIRE(qkv && pos && rope && q_out && kc && vc && page_table && n > 0 && hd % 2 == 0 && S >= 1,
                QRAF_HIP_ERR_INVALID, "rope_append: bad arguments");
     if (kv_dtype == DT_I8) {
@@ -2009,7 +2014,8 @@ int launch_rope_append(const float* qkv, const float* bias, int n, int H, int Hk
                    "rope_append: int8 pages need head_dim <= 128 (multiple of 4) and page_size %% 4 == 0");
         const int qblocks = std::min(8, (H * hd / 2 + 255) / 256);
         hipLaunchKernelGGL(rope_append_i8_kernel, dim3(n, 1 + qblocks), dim3(256), 0, st, qkv, bias, H, Hkv, hd, pos,
-                           rope, q_out, (int8_t*)kc, (int8_t*)vc, page_table, max_pages, page_size, S, slice);
+                           rope, q_out, (int8_t*)kc, (int8_t*)vc, page_table, max_pages, page_size, S, slice,
+                           slots, seqs);
         QH_CHECK_HIP(hipGetLastError());
         return QRAF_HIP_OK;
     }
@@ -2018,7 +2024,7 @@ int launch_rope_append(const float* qkv, const float* bias, int n, int H, int Hk
     if (kv_dtype != DT_F32 && kv_dtype != DT_F16) return set_error(QRAF_HIP_ERR_DTYPE, "rope_append: KV dtype %u", kv_dtype);
 #define QH_RA(KTv, SCv)                                                                                              \
     hipLaunchKernelGGL((rope_append_kernel<KTv, SCv>), dim3(grid), dim3(256), 0, st, qkv, bias, H, Hkv, hd, pos, rope, \
-                       q_out, (KTv*)kc, (KTv*)vc, page_table, max_pages, page_size, n, S, slice)
+                       q_out, (KTv*)kc, (KTv*)vc, page_table, max_pages, page_size, n, S, slice, slots, seqs)
 #define QH_RA_S(KTv)                  \
     switch (S) {                      \
         case 1: QH_RA(KTv, 1); break; \
@@ -2152,6 +2158,20 @@ int qraf_hip_rope_append_dev(const float* qkv, const float* bias, int32_t n_seqs
     return qraf_hip::launch_rope_append(qkv, bias, n_seqs, n_heads, n_kv_heads, head_dim, positions, rope_table, q_out,
                                         k_cache, v_cache, kv_dtype, page_table, max_pages_per_seq, page_size,
                                         qraf_hip::as_stream(stream));
+}
+
+int qraf_hip_tree_append_dev(const float* qkv, const float* bias, int32_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                             int32_t head_dim, const int32_t* positions, const int32_t* slots, const int32_t* row_seqs,
+                             const float* rope_table, float* q_out, void* k_cache, void* v_cache, uint32_t kv_dtype,
+                             const int32_t* page_table, int32_t max_pages_per_seq, int32_t page_size, void* stream) {
+    qraf_hip::clear_error();
+    QH_REQUIRE(slots && row_seqs, QRAF_HIP_ERR_INVALID, "tree_append: null pointer");
+    QH_REQUIRE(n_heads > 0 && n_kv_heads > 0 && head_dim > 0 && max_pages_per_seq > 0 && page_size > 0,
+               QRAF_HIP_ERR_INVALID, "tree_append: %d heads, %d kv heads of %d, pages of %d", n_heads, n_kv_heads,
+               head_dim, page_size);
+    return qraf_hip::launch_rope_append(qkv, bias, n_rows, n_heads, n_kv_heads, head_dim, positions, rope_table, q_out,
+                                        k_cache, v_cache, kv_dtype, page_table, max_pages_per_seq, page_size,
+                                        qraf_hip::as_stream(stream), 1, 0, slots, row_seqs);
 }
 
 }  // extern "C"

@@ -45,6 +45,8 @@ struct GroupArgs {
     int ps_log2, job_cap;       // page_size = 1 << ps_log2; prefix jobs at most
     int tail_log2, tails;       // a tail job is 1 << tail_log2 rows; tail jobs
     long long slots;            // part slots of a KV head
+    // Trees: groups are sequences, page_table is [groups][max_pages], prefix their caches' lengths, ctx unused.
+    const unsigned long long* masks;  // [n] positions prefix + bit that a row attends to beside its cache
 };
 
 // output elements i .. i + 3, i
@@ -79,6 +81,13 @@ __device__ __forceinline__ int group_of(const GroupArgs& a, int r) {
     return lo;
 }
 __device__ __forceinline__ int row_ctx(const GroupArgs& a, int r) { return max(0, min(a.ctx[r], a.max_ctx)); }
+__device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return max(0, min(a.prefix[g], a.max_ctx)); }
+// trees: row r's mask behind a cache of `base` positions, below max_ctx; the end of what it attends to
+__device__ __forceinline__ unsigned long long row_mask(const GroupArgs& a, int r, int base) {
+    const int room = a.max_ctx - base;
+    return room >= 64 ? a.masks[r] : a.masks[r] & ((1ull << room) - 1);
+}
+__device__ __forceinline__ int mask_end(unsigned long long mask, int base) { return mask ? base + 64 - __clzll(mask) : base; }
 
 // ---------------------------------------------------------------------------
 // Any head layout and page size: a workgroup per (row, query head), its four
@@ -106,7 +115,7 @@ __device__ __forceinline__ float any_scale(const GroupArgs& a, const void* pool,
     return *(const float*)((const int8_t*)pool + block * a.page_size * (HD + 4) + (size_t)a.page_size * HD + 4 * (size_t)off);
 }
 
-template <int HD, int KV>
+template <int HD, int KV, bool TREE>
 __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
     constexpr int DPL = HD > 64 ? HD / 64 : 1;  // dimensions per lane of P.V
     constexpr int NP = HD < 64 ? 64 / HD : 1;   // positions side by side
@@ -118,7 +127,10 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
     const int r = blockIdx.x, h = blockIdx.y, kvh = h / a.G;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (r < group_start(a, 0) || r >= group_start(a, a.groups)) return;  // outside every group
-    const int ctx = row_ctx(a, r), g = group_of(a, r), prefix = a.prefix[g], r0 = group_start(a, g);
+    const int g = group_of(a, r), prefix = TREE ? prefix_len(a, g) : a.prefix[g], r0 = TREE ? g : group_start(a, g);
+    const unsigned long long mask = TREE ? row_mask(a, r, prefix) : 0;
+    const int ctx = TREE ? mask_end(mask, prefix) : row_ctx(a, r);
+    auto attends = [&](int t) { return t < ctx && (!TREE || t < prefix || (mask >> (t - prefix) & 1)); };
     const size_t base = ((size_t)r * a.H + h) * HD;
     for (int d = tid; d < HD; d += 256) s_q[d] = a.q[base + d];
     __syncthreads();
@@ -131,9 +143,10 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
         const int t0 = it * 256 + wave * 64, t = t0 + lane;
         float sc = -INFINITY, vs = 0.f;
         size_t block = 0;
-        int off = 0;
-        if (t < ctx) {
-            const int pg = a.page_table[(size_t)(t < prefix ? r0 : r) * a.max_pages + t / a.page_size];
+        int off = TREE ? -1 : 0;  // (of a position that the row does not attend to: no value of it is read)
+        const bool in = attends(t);
+        if (in) {
+            const int pg = a.page_table[(size_t)(TREE || t < prefix ? r0 : r) * a.max_pages + t / a.page_size];
             block = (size_t)pg * a.Hkv + kvh;
             off = t % a.page_size;
             float acc = 0.f;
@@ -147,7 +160,7 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
         for (int s = 32; s >= 1; s >>= 1) mt = fmaxf(mt, __shfl_xor(mt, s));
         const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
         const float alpha = expf(m - mu);
-        const float p = t < ctx ? expf(sc - mu) : 0.f;
+        const float p = in ? expf(sc - mu) : 0.f;
         float lt = p;
 #pragma unroll
         for (int s = 32; s >= 1; s >>= 1) lt += __shfl_xor(lt, s);
@@ -162,6 +175,7 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
         const int here = min(64, ctx - t0);
         for (int k = pl; k < here; k += NP) {
             const float pk = s_p[wave][k];
+            if (TREE && s_off[wave][k] < 0) continue;
 #pragma unroll
             for (int j = 0; j < DPL; j++)
                 o[j] = __builtin_fmaf(pk, any_v<HD, KV>(a, s_block[wave][k], s_off[wave][k], dl + 64 * j), o[j]);
@@ -458,7 +472,6 @@ __device__ __forceinline__ int tiles_of(int positions, int cols) {
     const int s = cols > 64 ? 6 : cols > 32 ? 7 : 8;  // 32 positions times GW / waves_over(cols)
     return (positions + (1 << s) - 1) >> s;
 }
-__device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return max(0, min(a.prefix[g], a.max_ctx)); }
 // a tail begins with the 16 positions that hold the prefix's end, one page's
 __device__ __forceinline__ int tail_base(int prefix) { return prefix & ~15; }
 
@@ -1723,6 +1736,23 @@ size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd
     return z.plan_bytes + z.ml_bytes + z.o_bytes;
 }
 
+// the plain form, of every shape
+template <bool TREE>
+static int group_any(const GroupArgs& a, uint32_t kv_dtype, int hd, hipStream_t st) {
+    const dim3 grid(a.n, a.H);
+#define QH_GROUP_ANY(HDv, KVv)                                                                     \
+    if (hd == HDv && kv_dtype == KVv) {                                                            \
+        hipLaunchKernelGGL((group_any_kernel<HDv, (int)KVv, TREE>), grid, dim3(256), 0, st, a);    \
+        QH_CHECK_HIP(hipGetLastError());                                                           \
+        return QRAF_HIP_OK;                                                                        \
+    }
+#define QH_GROUP_ANYS(HDv) QH_GROUP_ANY(HDv, DT_F32) QH_GROUP_ANY(HDv, DT_F16) QH_GROUP_ANY(HDv, DT_I8)
+    QH_GROUP_ANYS(16) QH_GROUP_ANYS(32) QH_GROUP_ANYS(64) QH_GROUP_ANYS(128)
+#undef QH_GROUP_ANYS
+#undef QH_GROUP_ANY
+    return QRAF_HIP_OK;
+}
+
 int launch_group_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype,
                            const int32_t* page_table, int max_pages, const int32_t* ctx, const int32_t* group_starts,
                            const int32_t* prefix, int n, int groups, int H, int Hkv, int hd, int page_size, float scale,
@@ -1795,18 +1825,60 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
         QH_CHECK_HIP(hipGetLastError());
         return QRAF_HIP_OK;
     }
-    const dim3 grid(n, H);
-#define QH_GROUP_ANY(HDv, KVv)                                                                     \
-    if (hd == HDv && kv_dtype == KVv) {                                                            \
-        hipLaunchKernelGGL((group_any_kernel<HDv, (int)KVv>), grid, dim3(256), 0, st, a);          \
-        QH_CHECK_HIP(hipGetLastError());                                                           \
-        return QRAF_HIP_OK;                                                                        \
-    }
-#define QH_GROUP_ANYS(HDv) QH_GROUP_ANY(HDv, DT_F32) QH_GROUP_ANY(HDv, DT_F16) QH_GROUP_ANY(HDv, DT_I8)
-    QH_GROUP_ANYS(16) QH_GROUP_ANYS(32) QH_GROUP_ANYS(64) QH_GROUP_ANYS(128)
-#undef QH_GROUP_ANYS
-#undef QH_GROUP_ANY
-    return QRAF_HIP_OK;
+    return group_any<false>(a, kv_dtype, hd, st);
+}
+
+size_t tree_attention_workspace_bytes(int n, int seqs, int H, int Hkv, int hd, int max_ctx) {
+    (void)n, (void)seqs, (void)H, (void)Hkv, (void)hd, (void)max_ctx;
+    return 16;
+}
+
+int launch_tree_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype, const int32_t* page_table,
+                          int max_pages, const int32_t* base, const int32_t* row_starts, const uint64_t* masks, int n,
+                          int seqs, int H, int Hkv, int hd, int page_size, float scale, int max_ctx, float* out,
+                          void* ws, size_t ws_bytes, hipStream_t st, uint16_t* out_hi, uint16_t* out_lo) {
+    QH_REQUIRE(q && kc && vc && page_table && base && row_starts && masks && (out || (out_hi && out_lo)) && ws,
+               QRAF_HIP_ERR_INVALID, "tree attention: null pointer");
+    QH_REQUIRE((((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)out | (uintptr_t)ws) & 15) == 0 &&
+                   ((uintptr_t)masks & 7) == 0,
+               QRAF_HIP_ERR_INVALID,
+               "tree attention: q, caches, out and workspace must be 16-byte, masks 8-byte aligned");
+    QH_REQUIRE(n > 0 && n <= 1024, QRAF_HIP_ERR_INVALID, "tree attention: %d rows outside 1..1024", n);
+    QH_REQUIRE(seqs > 0 && seqs <= n, QRAF_HIP_ERR_INVALID, "tree attention: %d sequences of %d rows", seqs, n);
+    QH_REQUIRE(Hkv > 0 && H > 0 && H % Hkv == 0, QRAF_HIP_ERR_INVALID,
+               "tree attention: %d heads not a multiple of %d kv heads", H, Hkv);
+    QH_REQUIRE(H <= 65535, QRAF_HIP_ERR_INVALID, "tree attention: %d heads over 65535", H);
+    QH_REQUIRE(hd == 16 || hd == 32 || hd == 64 || hd == 128, QRAF_HIP_ERR_INVALID,
+               "tree attention: head_dim %d (16, 32, 64 or 128 supported)", hd);
+    QH_REQUIRE(page_size > 0 && max_pages > 0 && max_ctx > 0 && max_ctx <= (long long)max_pages * page_size,
+               QRAF_HIP_ERR_INVALID, "tree attention: bad page geometry");
+    QH_REQUIRE(max_ctx <= 1 << 30, QRAF_HIP_ERR_INVALID, "tree attention: max_ctx %d over 2^30", max_ctx);
+    QH_REQUIRE(kv_dtype == DT_F32 || kv_dtype == DT_F16 || kv_dtype == DT_I8, QRAF_HIP_ERR_DTYPE,
+               "tree attention: KV dtype %u", kv_dtype);
+    const size_t need = tree_attention_workspace_bytes(n, seqs, H, Hkv, hd, max_ctx);
+    QH_REQUIRE(ws_bytes >= need, QRAF_HIP_ERR_INVALID, "tree attention: workspace of %zu bytes, %zu needed", ws_bytes,
+               need);
+    GroupArgs a{};
+    a.q = q;
+    a.kc = kc;
+    a.vc = vc;
+    a.page_table = page_table;
+    a.starts = row_starts;
+    a.prefix = base;
+    a.masks = (const unsigned long long*)masks;
+    a.out = out;
+    a.out_hi = out_hi;
+    a.out_lo = out_lo;
+    a.n = n;
+    a.groups = seqs;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.G = H / Hkv;
+    a.page_size = page_size;
+    a.max_pages = max_pages;
+    a.max_ctx = max_ctx;
+    a.scale = scale;
+    return group_any<true>(a, kv_dtype, hd, st);
 }
 
 }  // namespace qraf_hip
@@ -1831,6 +1903,23 @@ int qraf_hip_group_attention_dev(const float* q, const void* k_cache, const void
     return launch_group_attention(q, k_cache, v_cache, kv_dtype, page_table, max_pages_per_seq, ctx_lens, group_starts,
                                   prefix_lens, n_rows, n_groups, n_heads, n_kv_heads, head_dim, page_size, scale,
                                   max_ctx, out, workspace, workspace_bytes, as_stream(stream));
+}
+
+uint64_t qraf_hip_tree_attention_workspace_bytes(int32_t n_rows, int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
+                                                 int32_t head_dim, int32_t max_ctx) {
+    if (n_rows <= 0 || n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || max_ctx <= 0) return 0;
+    return tree_attention_workspace_bytes(n_rows, n_seqs, n_heads, n_kv_heads, head_dim, max_ctx);
+}
+
+int qraf_hip_tree_attention_dev(const float* q, const void* k_cache, const void* v_cache, uint32_t kv_dtype,
+                                const int32_t* page_table, int32_t max_pages_per_seq, const int32_t* base_lens,
+                                const int32_t* row_starts, const uint64_t* masks, int32_t n_rows, int32_t n_seqs,
+                                int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t page_size, float scale,
+                                int32_t max_ctx, float* out, void* workspace, uint64_t workspace_bytes, void* stream) {
+    clear_error();
+    return launch_tree_attention(q, k_cache, v_cache, kv_dtype, page_table, max_pages_per_seq, base_lens, row_starts,
+                                 masks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, scale, max_ctx, out,
+                                 workspace, workspace_bytes, as_stream(stream), nullptr, nullptr);
 }
 
 }  // extern "C"

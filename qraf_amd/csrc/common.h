@@ -126,6 +126,17 @@ __device__ __forceinline__ void split_bf16(float v, uint16_t* hi, uint16_t* lo) 
 // SiLU-gate of one gate/up pair (ops.cpp:218-222 then :275-279): silu(g) * u
 __device__ __forceinline__ float silu_gate(float g, float u) { return __fmul_rn(g / (1.0f + expf(-g)), u); }
 
+// a logit as it is ordered and weighed: NaN counts as -inf, -0 as +0
+__device__ __forceinline__ float clean_logit(float l) { return l == l ? l + 0.0f : -INFINITY; }
+
+__device__ __forceinline__ uint32_t logit_key(float f) {  // a < b  <=>  key(a) < key(b)
+    const uint32_t b = __float_as_uint(f);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_logit(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+}
+
 // element e of S slices (GEMM split-K partials) of `slice` floats, summed in
 // slice order.  Up to 8 slices: every load issued before the first add (one
 // round trip); beyond, 8 slices per round trip.
@@ -183,6 +194,12 @@ int launch_verify_draft(const float* probs, const float* draft_probs, const uint
                         const float* pick_uniforms, int32_t* accepted, uint32_t* tokens, void* ws, size_t ws_bytes,
                         hipStream_t s);
 
+// what is said about a token: log probability, rank, the row's entropy and its top alternatives (logprobs.hip)
+size_t token_logprobs_workspace_bytes(int rows, int V, int top);
+int launch_token_logprobs(const float* logits, int rows, int V, const uint32_t* tokens, float* logprobs, int32_t* ranks,
+                          float* entropies, int top, uint32_t* top_tokens, float* top_logprobs, void* ws,
+                          size_t ws_bytes, hipStream_t s);
+
 // x may be S slices of `slice` floats each (GEMM partials), summed in slice order
 int launch_split_bf16(const float* x, uint16_t* hi, uint16_t* lo, int M, int K, int op, float* xout, hipStream_t s,
                       int S = 1, size_t slice = 0);
@@ -229,10 +246,25 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
                            const int32_t* prefix, int n, int groups, int H, int Hkv, int hd, int page_size, float scale,
                            int max_ctx, float* out, void* ws, size_t ws_bytes, hipStream_t st,
                            uint16_t* out_hi = nullptr, uint16_t* out_lo = nullptr);
+// a tree's nodes attend to their sequence's cache and to the positions behind it that their masks name; page_table
+// has a row for each sequence (attention_group.hip)
+size_t tree_attention_workspace_bytes(int n, int seqs, int H, int Hkv, int hd, int max_ctx);
+int launch_tree_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype, const int32_t* page_table,
+                          int max_pages, const int32_t* base, const int32_t* row_starts, const uint64_t* masks, int n,
+                          int seqs, int H, int Hkv, int hd, int page_size, float scale, int max_ctx, float* out,
+                          void* ws, size_t ws_bytes, hipStream_t st, uint16_t* out_hi = nullptr,
+                          uint16_t* out_lo = nullptr);
+// the accepted path of each tree, and its keys and values moved together (tree.hip)
+int launch_tree_accept(const uint32_t* picks, const uint32_t* drafts, const int32_t* parents, const int32_t* starts,
+                       int seqs, int rows, int32_t* accepted, int32_t* path, uint32_t* tokens, hipStream_t st);
+int launch_kv_compact(void* kc, void* vc, uint32_t kv_dtype, int layers, size_t layer_bytes, const int32_t* table,
+                      int max_pages, const int32_t* base, const int32_t* starts, const int32_t* path, int seqs, int rows,
+                      int Hkv, int hd, int page_size, hipStream_t st);
+// slots, seqs (trees): row i's K and V go to position slots[i] of page table row seqs[i], not to pos[i] of row i
 int launch_rope_append(const float* qkv, const float* bias, int n, int H, int Hkv, int hd, const int32_t* pos,
                        const float* rope, float* q_out, void* kc, void* vc, uint32_t kv_dtype,
                        const int32_t* page_table, int max_pages, int page_size, hipStream_t st, int S = 1,
-                       size_t slice = 0);
+                       size_t slice = 0, const int32_t* slots = nullptr, const int32_t* seqs = nullptr);
 int launch_gen_weights(void* dst, uint32_t dtype, uint64_t count, uint64_t seed, uint64_t stream_id, float stddev,
                        hipStream_t s);
 int launch_quantize(const float* src, uint64_t count, uint32_t dtype, void* dst, hipStream_t s);

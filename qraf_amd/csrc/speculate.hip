@@ -57,14 +57,6 @@ namespace qraf_hip {
 
 constexpr int PNT = 1024;  // threads per row
 
-// a logit as it is ordered and weighed: NaN counts as -inf, -0 as +0
-__device__ __forceinline__ float clean_logit(float l) { return l == l ? l + 0.0f : -INFINITY; }
-
-__device__ __forceinline__ uint32_t logit_key(float f) {  // a < b  <=>  key(a) < key(b)
-    const uint32_t b = __float_as_uint(f);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
 // exp((l - m) / T) in 64 bits, within 1e-11 of it (m: the largest logit, not -inf): 2^y as 2^rint(y) times the
 // series of 2^f, |f| <= 1/2, to its tenth power.  (The library's exponential, to the last bit: 28 us for the bins of
 // 64 rows of 151,936 where this takes 20.)
@@ -429,9 +421,6 @@ __device__ __forceinline__ void rank_sort(const unsigned long long* in, unsigned
         sorted[rank] = x;
     }
     __syncthreads();
-}
-__device__ __forceinline__ float key_logit(uint32_t key) {
-    return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 // The first nc of `sorted`, or (nucleus) as many of them as bring the weight `above` them to need(all); in every
 // thread.  (s_w: a word for each entry)
