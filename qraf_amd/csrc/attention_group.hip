@@ -17,6 +17,7 @@
 // unnormalised output) parts, which group_merge_kernel joins in position order.
 // Small calls go without: a workgroup per (row, KV head) takes all its positions.
 // group_any_kernel takes the shapes that the tiles do not.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -82,10 +83,13 @@ __device__ __forceinline__ int group_of(const GroupArgs& a, int r) {
 }
 __device__ __forceinline__ int row_ctx(const GroupArgs& a, int r) { return max(0, min(a.ctx[r], a.max_ctx)); }
 __device__ __forceinline__ int prefix_len(const GroupArgs& a, int g) { return max(0, min(a.prefix[g], a.max_ctx)); }
-// trees: row r's mask behind a cache of `base` positions, below max_ctx; the end of what it attends to
-__device__ __forceinline__ unsigned long long row_mask(const GroupArgs& a, int r, int base) {
+// trees: a mask behind a cache of `base` positions, below max_ctx; row r's; the end of what it attends to
+__device__ __forceinline__ unsigned long long below_ctx(const GroupArgs& a, unsigned long long mask, int base) {
     const int room = a.max_ctx - base;
-    return room >= 64 ? a.masks[r] : a.masks[r] & ((1ull << room) - 1);
+    return room >= 64 ? mask : mask & ((1ull << room) - 1);
+}
+__device__ __forceinline__ unsigned long long row_mask(const GroupArgs& a, int r, int base) {
+    return below_ctx(a, a.masks[r], base);
 }
 __device__ __forceinline__ int mask_end(unsigned long long mask, int base) { return mask ? base + 64 - __clzll(mask) : base; }
 
@@ -482,10 +486,14 @@ __device__ __forceinline__ int wave_sum(int n, F f) {
     for (int i = threadIdx.x & 63; i < n; i += 64) x += f(i);
     return over_wave(x, [](int u, int v) { return u + v; });
 }
+template <bool TREE>
 __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     const int tid = threadIdx.x;
+    static_assert(2 * GTH >= 1024, "rows by thread");
+    unsigned long long masks[2];  // (trees) of rows tid and tid + GTH
+    if (TREE) masks[0] = a.masks[min(tid, a.n - 1)], masks[1] = a.masks[min(tid + GTH, a.n - 1)];
     for (int i = tid; i < max(a.n, a.groups + 1); i += GTH) {  // (all requested at once)
-        const int c = row_ctx(a, min(i, a.n - 1)), s = group_start(a, min(i, a.groups)),
+        const int c = TREE ? 0 : row_ctx(a, min(i, a.n - 1)), s = group_start(a, min(i, a.groups)),
                   t = group_start(a, min(i + 1, a.groups)), e = prefix_len(a, min(i, a.groups - 1));
         if (i < a.n) p.ctx[i] = c;
         if (i <= a.groups) p.gs[i] = s;
@@ -502,7 +510,12 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     const int jobs = p.np + a.tails;
     for (int r = tid; r < a.n; r += GTH) {
         if (r < p.gs[0] || r >= p.gs[a.groups]) continue;
-        const int g = last_at(p.gs, a.groups, r), ctx = p.ctx[r], pre = p.pre[g], all = (p.gs[g + 1] - p.gs[g]) * a.G;
+        const int g = last_at(p.gs, a.groups, r), all = (p.gs[g + 1] - p.gs[g]) * a.G;
+        int ctx = p.ctx[r], pre = p.pre[g];
+        if (TREE) {
+            ctx = p.ctx[r] = mask_end(below_ctx(a, masks[r >= GTH], pre), pre);
+            pre = ctx;
+        }
         const int c0 = (r - p.gs[g]) * a.G, b1 = (c0 + a.G - 1) / BLK;
         for (int b = c0 / BLK; b <= b1 && p.jb[g] + b < p.np; b++)
             atomicMax(&p.tiles[p.jb[g] + b], tiles_of(min(ctx, pre), min(BLK, all - BLK * b)));
@@ -541,8 +554,9 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
             const int g = in ? last_at(p.gs, a.groups, r) : 0;
             const int pos = p.jb[g] * BLK + (r - p.gs[g]) * a.G, b = in ? pos / BLK : 0, t = p.np + (r >> a.tail_log2);
             a.plan[2 * r] = make_int4(in ? pos : -1, p.upto[min(b, jobs)], p.upto[min(b + 1, jobs)], p.upto[min(b + 2, jobs)]);
-            a.plan[2 * r + 1] = make_int4((min(p.ctx[r], p.pre[g]) > 0 ? 1 : 0) | (p.ctx[r] > p.pre[g] ? 2 : 0), p.upto[t],
-                                          p.upto[t + 1], 0);
+            if (TREE) a.plan[2 * r + 1] = make_int4(p.ctx[r] > 0 ? 1 : 0, 0, 0, 0);
+            else a.plan[2 * r + 1] = make_int4((min(p.ctx[r], p.pre[g]) > 0 ? 1 : 0) | (p.ctx[r] > p.pre[g] ? 2 : 0), p.upto[t],
+                                               p.upto[t + 1], 0);
         }
     }
 }
@@ -572,7 +586,9 @@ struct GroupTile<HD, (int)DT_F32> {
 // LDS floats for the tiles: the waves' outputs, [GW][32][hd]; before them q, and two f32 tiles that waves share
 constexpr int tile_floats(int hd) { return GW * 32 * hd; }
 
-template <int HD, int KV, bool DIRECT>
+// TREE: rows attend to their sequence's cache and to the positions behind it that their masks name, all of them shared
+// (the prefix ends where their attention does): tiles that reach behind the cache go by bits.
+template <int HD, int KV, bool DIRECT, bool TREE>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
@@ -584,6 +600,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     int(*const s_vx)[32] = (int(*)[32])s_l;
     constexpr int OWN = -(1 << 20);  // (scores over it are infinite)
     __shared__ int s_ku[2][4], s_vu[2][4];
+    __shared__ unsigned long long s_mask[TREE ? BLK : 1];
     __shared__ long long s_to[BLK];  // where a column's output goes: an element of out, or ~ one of part_o
     constexpr long long NOWHERE = 1ll << 62;
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
@@ -624,7 +641,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             s[k] = group_start(a, min(lane + 64 * k, a.groups));
             e[k] = prefix_len(a, min(lane + 64 * k, a.groups - 1));
         }
-        d_ctx = row_ctx(a, w);
+        if (!TREE) d_ctx = row_ctx(a, w);
         if (w < group_start(a, 0) || w >= group_start(a, a.groups)) return;  // outside every group
         int g = -1;
 #pragma unroll
@@ -635,9 +652,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 d_first = __builtin_amdgcn_readlane(s[k], g & 63);
                 d_pre = __builtin_amdgcn_readlane(e[k], g & 63);
             }
-        d_tiles = (min(d_ctx, d_pre) + 31) >> 5;
+        if (TREE) {
+            d_ctx = mask_end(row_mask(a, w, d_pre), d_pre);
+            d_first = g;  // (whose row of the page table is read)
+        }
+        d_tiles = (TREE ? d_ctx + 31 : min(d_ctx, d_pre) + 31) >> 5;
     } else {
-        group_plan(a, plan, gridDim.x);
+        group_plan<TREE>(a, plan, gridDim.x);
         jobs = plan.np + a.tails;
         pieces = plan.upto[jobs] & 0xFFFF;
     }
@@ -668,11 +689,11 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             first = bfirst = w * G;
             cols = bcols = G;
             // tiles: the prefix's, then the tail's
-            jend = d_tiles + (d_ctx > d_pre ? (d_ctx - tail_base(d_pre) + 31) >> 5 : 0);
-            tail = wave >= d_tiles;
+            jend = d_tiles + (!TREE && d_ctx > d_pre ? (d_ctx - tail_base(d_pre) + 31) >> 5 : 0);
+            tail = !TREE && wave >= d_tiles;
             trow = tail ? w : d_first;
             g = 0;
-        } else if (tail) {             // a row's columns are 1, 2 or 4 waves'
+        } else if (!TREE && tail) {    // a row's columns are 1, 2 or 4 waves'
             wq = 4;
             const int side = 4 >> a.tail_log2, c0 = 32 * (wave & (side - 1));
             const int row = ((j - plan.np) << a.tail_log2) + ((wave & 3) >> (2 - a.tail_log2));
@@ -695,14 +716,15 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         wq = __builtin_amdgcn_readfirstlane(wq);
         cols = __builtin_amdgcn_readfirstlane(max(cols, 0));
         const int wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
-        const int pre = __builtin_amdgcn_readfirstlane(DIRECT ? d_pre : plan.pre[g]), base = tail ? tail_base(pre) : 0;
+        const int cache = __builtin_amdgcn_readfirstlane(DIRECT ? d_pre : plan.pre[g]);  // (trees: ahead of the masks)
+        const int pre = TREE ? INT_MAX : cache, base = tail ? tail_base(pre) : 0;
         int lo = tail ? pre : 0;
         // the page table through scalar loads: an id does not wait for vector loads ahead of it
         typedef const __attribute__((address_space(4))) int32_t ConstInt;
         auto table_of = [&](int row) {
             return (ConstInt*)(uintptr_t)(a.page_table + (size_t)__builtin_amdgcn_readfirstlane(row) * a.max_pages);
         };
-        ConstInt* ptab = table_of(trow);
+        ConstInt* ptab = table_of(TREE && !DIRECT ? g : trow);
 
         // ---- the lane's column (past the last: that again, not written), row and limit
         const int ab = min(first + min(col, max(cols - 1, 0)), a.n * G - 1);
@@ -712,7 +734,15 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         int lim = cols == 0 ? 0 : tail ? ctx : min(ctx, pre);
         // behind the last position that some of the wave's columns attends to
         int kend = __builtin_amdgcn_readfirstlane(DIRECT ? lim : over_wave(lim, imax2)), klast = max(kend - 1, 0);
-        int least = __builtin_amdgcn_readfirstlane(DIRECT ? lim : over_wave(lim, imin2));
+        int least = TREE ? cache : __builtin_amdgcn_readfirstlane(DIRECT ? lim : over_wave(lim, imin2));
+        // (trees) the positions of the tile at t that the lane's column attends to, as bits; those of its half from bit 0
+        auto attended = [&](int t) {
+            const unsigned long long mask = s_mask[qt * 32 + col];
+            const int d = t - cache, in = min(max(d, 0), 63), ahead = min(max(-d, 0), 32);  // (ahead: positions of the cache)
+            const uint32_t b = d >= 64 ? 0u : (uint32_t)((mask >> in) << ahead | ((1ull << ahead) - 1));
+            return b >> (8 * half);
+        };
+        auto bit_of = [](uint32_t b, int x) { return (b >> (16 * (x >> 3) + (x & 7)) & 1) != 0; };  // of register x
 
         // ---- loads of the tile at position t
         GroupTile<HD, KV> tl;
@@ -836,10 +866,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 if (d0 == 0) s_qs[c] = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e);
             }
         };
+        const unsigned long long mask_of =
+            TREE ? row_mask(a, DIRECT ? w : (int)(((float)(bfirst + min(tid % BLK, bcols - 1)) + 0.5f) * inv_g), cache) : 0;
         if (DIRECT || wq == 1) stage_q(std::integral_constant<int, 1>());
         else if (wq == 2) stage_q(std::integral_constant<int, 2>());
         else stage_q(std::integral_constant<int, 4>());
         if (!TURNS) load_v(more ? t : 0, F32 || !shared);  // (behind q: their registers)
+        if (TREE) s_mask[tid % BLK] = mask_of;
         lds_sync();
         const float qs = s_qs[qt * 32 + col];  // scores in powers of two
 
@@ -1094,10 +1127,12 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         v_own = seldom(min(ve[0], ve[1]) == OWN);
                     }
                     // ---- softmax
+                    uint32_t seen = 0;
                     if (edge) {
+                        if (TREE) seen = attended(t);
 #pragma unroll
                         for (int x = 0; x < 16; x++)
-                            s[x] = t + 16 * (x >> 3) + 8 * half + (x & 7) < lim ? s[x] : -INFINITY;
+                            s[x] = (TREE ? bit_of(seen, x) : t + 16 * (x >> 3) + 8 * half + (x & 7) < lim) ? s[x] : -INFINITY;
                     }
                     float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
@@ -1161,7 +1196,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                         f16x8 att[2];
 #pragma unroll
                         for (int x = 0; x < 16; x++)
-                            att[x >> 3][x & 7] = t + 16 * (x >> 3) + 8 * half + (x & 7) < lim ? (_Float16)1.f : (_Float16)0.f;
+                            att[x >> 3][x & 7] = (TREE ? bit_of(seen, x) : t + 16 * (x >> 3) + 8 * half + (x & 7) < lim)
+                                                     ? (_Float16)1.f : (_Float16)0.f;
 #pragma unroll
                         for (int d = 0; d < DT; d++) {
                             f32x16 c;
@@ -1302,11 +1338,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 
             // ---- softmax: register x is position t + 16 (x / 8) + 8 half + x % 8
             float mt = -INFINITY;
+            uint32_t seen = 0;
             if (edge) {
+                if (TREE) seen = attended(t);
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
                     const int pos = t + 16 * (x >> 3) + 8 * half + (x & 7);
-                    s[x] = pos >= lo && pos < lim ? s[x] : -INFINITY;
+                    s[x] = (TREE ? bit_of(seen, x) : pos >= lo && pos < lim) ? s[x] : -INFINITY;
                     if constexpr (I8) vsc[x] = pos < kend ? vsc[x] : 0.f;
                 }
             }
@@ -1436,7 +1474,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 #pragma unroll
                         for (int x = 0; x < 16; x++) {
                             const int pos = t + 16 * (x >> 3) + 8 * half + (x & 7);
-                            att[x >> 3][x & 7] = pos >= lo && pos < lim ? (_Float16)1.f : (_Float16)0.f;
+                            att[x >> 3][x & 7] = (TREE ? bit_of(seen, x) : pos >= lo && pos < lim) ? (_Float16)1.f : (_Float16)0.f;
                         }
 #pragma unroll
                         for (int d = 0; d < DT; d++) {
@@ -1683,12 +1721,12 @@ struct GroupSizes {
     long long slots;
     size_t plan_bytes, ml_bytes, o_bytes;
 };
-static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd) {
+static GroupSizes group_sizes(int n, int groups, int H, int Hkv, int hd, bool tree = false) {
     const int G = H / Hkv;
     GroupSizes z;
     z.job_cap = (int)((long long)n * G / BLK) + groups;
     z.tail_log2 = G <= 32 ? 2 : G <= 64 ? 1 : 0;
-    z.tails = (n + (1 << z.tail_log2) - 1) >> z.tail_log2;
+    z.tails = tree ? 0 : (n + (1 << z.tail_log2) - 1) >> z.tail_log2;
     z.slots = 2ll * n * G + (long long)BLK * group_grid(Hkv);
     z.plan_bytes = ((size_t)n * 32 + 255) / 256 * 256;
     z.ml_bytes = ((size_t)Hkv * z.slots * sizeof(float2) + 255) / 256 * 256;
@@ -1700,10 +1738,11 @@ static size_t group_lds(int hd, int n, int groups, const GroupSizes& z) {
 }
 // shapes of the tiles (their LDS bounds what few very wide layouts would need; offsets inside a page, and of q, are
 // held in 32 bits)
-bool group_attention_tiles(int n, int groups, int H, int Hkv, int hd, int page_size) {
+bool group_attention_tiles(int n, int groups, int H, int Hkv, int hd, int page_size, bool tree) {
     const int G = H / Hkv;
     return (hd == 64 || hd == 128) && G <= BLK && page_size >= 16 && (page_size & (page_size - 1)) == 0 && (long long)page_size * hd <= 1 << 29 &&
-           (long long)n * H * hd <= 1 << 30 && group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd)) + 5120 <= 160 * 1024;
+           (long long)n * H * hd <= 1 << 30 &&
+           group_lds(hd, n, groups, group_sizes(n, groups, H, Hkv, hd, tree)) + (tree ? 6144 : 5120) <= 160 * 1024;
 }
 
 // Small calls: one launch without a plan, a workgroup per (row, KV head), which saves the plan (3 us) and the launch
@@ -1717,14 +1756,16 @@ static bool group_direct(int n, int H, int Hkv, uint32_t kv_dtype, int max_ctx) 
 }
 
 int group_attention_init() {
-#define QH_GROUP_LDS(HDv, KVv)                                                         \
-    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, false>, \
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024)); \
-    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, true>, \
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024));
+#define QH_GROUP_LDS1(HDv, KVv, DIRECTv, TREEv)                                                            \
+    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, DIRECTv, TREEv>,       \
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, (TREEv ? 154 : 155) * 1024));
+#define QH_GROUP_LDS(HDv, KVv)                                                                             \
+    QH_GROUP_LDS1(HDv, KVv, false, false) QH_GROUP_LDS1(HDv, KVv, true, false)                            \
+    QH_GROUP_LDS1(HDv, KVv, false, true) QH_GROUP_LDS1(HDv, KVv, true, true)
     QH_GROUP_LDS(64, DT_F32) QH_GROUP_LDS(64, DT_F16) QH_GROUP_LDS(64, DT_I8)
     QH_GROUP_LDS(128, DT_F32) QH_GROUP_LDS(128, DT_F16) QH_GROUP_LDS(128, DT_I8)
 #undef QH_GROUP_LDS
+#undef QH_GROUP_LDS1
     return QRAF_HIP_OK;
 }
 
@@ -1734,6 +1775,39 @@ size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd
     if (H % Hkv || !group_attention_tiles(n, groups, H, Hkv, hd, 16)) return 16;
     const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
     return z.plan_bytes + z.ml_bytes + z.o_bytes;
+}
+
+// the tiles, and the join of their parts
+template <bool TREE>
+static int group_tiles(GroupArgs& a, uint32_t kv_dtype, int hd, void* ws, bool direct, hipStream_t st) {
+    const GroupSizes z = group_sizes(a.n, a.groups, a.H, a.Hkv, hd, TREE);
+    a.job_cap = z.job_cap;
+    a.tail_log2 = z.tail_log2;
+    a.tails = z.tails;
+    a.slots = z.slots;
+    while ((1 << a.ps_log2) < a.page_size) a.ps_log2++;
+    a.plan = (int4*)ws;
+    a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
+    a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
+    const int gx = group_grid(a.Hkv);
+    const size_t lds = group_lds(hd, a.n, a.groups, z);
+#define QH_GROUP_TILE(HDv, KVv)                                                                                            \
+    if (hd == HDv && kv_dtype == KVv) {                                                                                    \
+        if (direct)                                                                                                        \
+            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true, TREE>), dim3(a.n, a.Hkv), dim3(GTH),               \
+                               tile_floats(HDv) * 4, st, a);                                                               \
+        else hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false, TREE>), dim3(gx, a.Hkv), dim3(GTH), lds, st, a);  \
+    }
+    QH_GROUP_TILE(64, DT_F32) QH_GROUP_TILE(64, DT_F16) QH_GROUP_TILE(64, DT_I8)
+    QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)
+#undef QH_GROUP_TILE
+    QH_CHECK_HIP(hipGetLastError());
+    if (direct) return QRAF_HIP_OK;
+    const dim3 grid(a.n, (a.H + 3) / 4);
+    if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((group_merge_kernel<64>), grid, dim3(256), 0, st, a);
+    QH_CHECK_HIP(hipGetLastError());
+    return QRAF_HIP_OK;
 }
 
 // the plain form, of every shape
@@ -1797,40 +1871,16 @@ int launch_group_attention(const float* q, const void* kc, const void* vc, uint3
     a.max_ctx = max_ctx;
     a.scale = scale;
     if (group_attention_tiles(n, groups, H, Hkv, hd, page_size)) {
-        const GroupSizes z = group_sizes(n, groups, H, Hkv, hd);
-        a.job_cap = z.job_cap;
-        a.tail_log2 = z.tail_log2;
-        a.tails = z.tails;
-        a.slots = z.slots;
-        while ((1 << a.ps_log2) < page_size) a.ps_log2++;
-        a.plan = (int4*)ws;
-        a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
-        a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
-        const int gx = group_grid(Hkv);
-        const size_t lds = group_lds(hd, n, groups, z);
-        const bool direct = group_direct(n, H, Hkv, kv_dtype, max_ctx);
-#define QH_GROUP_TILE(HDv, KVv)                                                                                            \
-    if (hd == HDv && kv_dtype == KVv) {                                                                                    \
-        if (direct)                                                                                                        \
-            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true>), dim3(n, Hkv), dim3(GTH), tile_floats(HDv) * 4, st, a); \
-        else hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false>), dim3(gx, Hkv), dim3(GTH), lds, st, a);          \
-    }
-        QH_GROUP_TILE(64, DT_F32) QH_GROUP_TILE(64, DT_F16) QH_GROUP_TILE(64, DT_I8)
-        QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)
-#undef QH_GROUP_TILE
-        QH_CHECK_HIP(hipGetLastError());
-        if (direct) return QRAF_HIP_OK;
-        if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((group_merge_kernel<64>), dim3(n, (H + 3) / 4), dim3(256), 0, st, a);
-        QH_CHECK_HIP(hipGetLastError());
-        return QRAF_HIP_OK;
+        return group_tiles<false>(a, kv_dtype, hd, ws, group_direct(n, H, Hkv, kv_dtype, max_ctx), st);
     }
     return group_any<false>(a, kv_dtype, hd, st);
 }
 
 size_t tree_attention_workspace_bytes(int n, int seqs, int H, int Hkv, int hd, int max_ctx) {
-    (void)n, (void)seqs, (void)H, (void)Hkv, (void)hd, (void)max_ctx;
-    return 16;
+    (void)max_ctx;
+    if (H % Hkv || !group_attention_tiles(n, seqs, H, Hkv, hd, 16, true)) return 16;
+    const GroupSizes z = group_sizes(n, seqs, H, Hkv, hd, true);
+    return z.plan_bytes + z.ml_bytes + z.o_bytes;
 }
 
 int launch_tree_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype, const int32_t* page_table,
@@ -1878,6 +1928,8 @@ int launch_tree_attention(const float* q, const void* kc, const void* vc, uint32
     a.max_pages = max_pages;
     a.max_ctx = max_ctx;
     a.scale = scale;
+    if (group_attention_tiles(n, seqs, H, Hkv, hd, page_size, true))
+        return group_tiles<true>(a, kv_dtype, hd, ws, group_direct(n, H, Hkv, kv_dtype, max_ctx), st);
     return group_any<true>(a, kv_dtype, hd, st);
 }
 

@@ -239,7 +239,7 @@ int launch_attention(const float* q, const void* kc, const void* vc, uint32_t kv
 // raises the dynamic-LDS limit of its workgroups (qraf_hip_init)
 int group_attention_init();
 // whether a shape's shared positions are read once (elsewhere each row and head reads them by itself)
-bool group_attention_tiles(int n, int groups, int H, int Hkv, int hd, int page_size);
+bool group_attention_tiles(int n, int groups, int H, int Hkv, int hd, int page_size, bool tree = false);
 size_t group_attention_workspace_bytes(int n, int groups, int H, int Hkv, int hd, int max_ctx);
 int launch_group_attention(const float* q, const void* kc, const void* vc, uint32_t kv_dtype,
                            const int32_t* page_table, int max_pages, const int32_t* ctx, const int32_t* group_starts,
