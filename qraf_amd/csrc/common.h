@@ -126,17 +126,6 @@ __device__ __forceinline__ void split_bf16(float v, uint16_t* hi, uint16_t* lo) 
 // SiLU-gate of one gate/up pair (ops.cpp:218-222 then :275-279): silu(g) * u
 __device__ __forceinline__ float silu_gate(float g, float u) { return __fmul_rn(g / (1.0f + expf(-g)), u); }
 
-// a logit as it is ordered and weighed: NaN counts as -inf, -0 as +0
-__device__ __forceinline__ float clean_logit(float l) { return l == l ? l + 0.0f : -INFINITY; }
-
-__device__ __forceinline__ uint32_t logit_key(float f) {  // a < b  <=>  key(a) < key(b)
-    const uint32_t b = __float_as_uint(f);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float key_logit(uint32_t key) {
-    return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
-}
-
 // element e of S slices (GEMM split-K partials) of `slice` floats, summed in
 // slice order.  Up to 8 slices: every load issued before the first add (one
 // round trip); beyond, 8 slices per round trip.

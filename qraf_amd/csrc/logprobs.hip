@@ -9,100 +9,477 @@
 //   alternatives      the n tokens ahead of all others, and d_i - ln S of each
 // NaN counts as -inf, -0 as +0.  Of infinite logits each has the same share; a row
 // without a logit above -inf has log probabilities of -inf and entropy 0.
+//
+// The logits are read once, by many workgroups a row; nothing else is large.  A wave
+// holds E logits a lane and writes its maximum, its sums against that, and how many of
+// its tokens are ahead; for alternatives every lane also writes the largest of its own
+// (a sub-range).  A second launch, a workgroup a row (a wave without alternatives), joins
+// the sums in 64 bits and finds the alternatives: the n-th largest of 512 maxima bounds
+// the n-th logit from below, only sub-ranges that reach the bound are read again, and the
+// few logits that do are ordered by counting.  Rows of up to 8,192 logits take one
+// workgroup and one launch.  Rows with more equal logits at the border than the lists
+// hold take a search over the whole row (flat_tops).
 #include <math.h>
 
 #include <algorithm>
 
 #include "common.h"
+#include "logits.h"
+#include "wave.h"
 
 namespace qraf_hip {
 
-constexpr int LTH = 1024;  // threads of a row
 constexpr int TOP_MAX = 64;
+constexpr int STH = 256;        // threads of a split
+constexpr int JTH = 512;        // threads that join a row
+constexpr int SPLITS = 64;      // splits of a row at most: longer rows give them several chunks
+constexpr int SUBS = 512;       // sub-ranges that are read again, at most
+constexpr int LIST = 2816;      // candidates: what the lanes that reach a bound of 64 hold, of 32 logits each
+constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // logit_key of -inf
 
+struct WaveStats {
+    float m, s, e;  // the largest logit, sum exp(l - m), sum exp(l - m) (l - m)
+    int ahead;      // tokens ahead of the row's given one
+};
 struct LogprobArgs {
     const float* logits;
     const uint32_t* tokens;
     float *logprobs, *entropies, *top_logprobs;
     int32_t* ranks;
     uint32_t* top_tokens;
-    int V, top;
+    WaveStats* stats;  // [rows][S * 4]
+    float* sub;        // [rows][S * STH] largest logits of sub-ranges
+    int V, S, top, rows;
 };
 
 // tokens in their order: a is ahead of b  <=>  key(a) > key(b)
-__device__ __forceinline__ unsigned long long token_key(float clean, int i) {
-    return (unsigned long long)logit_key(clean) << 32 | (0xFFFFFFFFu - (uint32_t)i);
+__device__ __forceinline__ unsigned long long token_key(uint32_t key, int i) {
+    return (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)i);
 }
+__device__ __forceinline__ float add2(float x, float y) { return x + y; }
+__device__ __forceinline__ int iadd2(int x, int y) { return x + y; }
+__device__ __forceinline__ float max2(float x, float y) { return fmaxf(x, y); }
+__device__ __forceinline__ uint32_t umax2(uint32_t x, uint32_t y) { return max(x, y); }
+__device__ __forceinline__ uint32_t umin2(uint32_t x, uint32_t y) { return min(x, y); }
 
-template <typename T, typename F>
-__device__ __forceinline__ T block_all(T x, F op, T* s) {
+// 16 bytes of a row, whose alignment is that of a float
+struct __attribute__((packed, aligned(4))) Four {
+    float v[4];
+};
+// Chunk c of a row, E logits a thread: element u is index chunk_index(c, u); past the row -inf.
+template <int E>
+__device__ __forceinline__ int chunk_index(int c, int t, int u) {
+    return c * (STH * E) + 4 * (t + STH * (u >> 2)) + (u & 3);
+}
+template <int E>
+__device__ __forceinline__ void load_chunk(const float* l, int V, int c, float (&v)[E]) {
+    const int t = threadIdx.x;
+    if ((c + 1) * (STH * E) <= V) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x = op(x, __shfl_xor(x, o));
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = s[0];
-    for (int w = 1; w < LTH / 64; w++) x = op(x, s[w]);
-    __syncthreads();
-    return x;
+        for (int j = 0; j < E; j += 4) {
+            const Four x = *(const Four*)(l + chunk_index<E>(c, t, j));
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[j + k] = x.v[k];
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < E; u++) {
+            const int i = chunk_index<E>(c, t, u);
+            const float x = l[min(i, V - 1)];
+            v[u] = i < V ? x : -INFINITY;
+        }
+    }
 }
 
-__global__ __launch_bounds__(LTH) void logprobs_row_kernel(LogprobArgs a) {
-    __shared__ unsigned long long s_k[LTH / 64];
-    __shared__ double s_d[LTH / 64];
-    __shared__ int s_i[LTH / 64];
-    const int row = blockIdx.x, tid = threadIdx.x, V = a.V;
-    const float* l = a.logits + (size_t)row * V;
-    auto most = [](unsigned long long x, unsigned long long y) { return max(x, y); };
-    auto sum = [](double x, double y) { return x + y; };
-    unsigned long long first = 0;
-    for (int i = tid; i < V; i += LTH) first = max(first, token_key(clean_logit(l[i]), i));
-    first = block_all(first, most, s_k);
-    const float m = key_logit((uint32_t)(first >> 32));
-    const uint32_t token = a.tokens ? a.tokens[row] : 0xFFFFFFFFu;
-    const bool known = token < (uint32_t)V;
-    const unsigned long long mine = known ? token_key(clean_logit(l[token]), (int)token) : ~0ull;
-    double S = 0.0, E = 0.0;
-    int ahead = 0;
-    for (int i = tid; i < V; i += LTH) {
-        const float x = clean_logit(l[i]), d = x == m ? 0.f : x - m, w = expf(d);
-        S += w;
-        E += w > 0.f ? (double)w * d : 0.0;
-        ahead += token_key(x, i) > mine;
+// sums of exp(v - m) and of that times (v - m), by halves: a chain of log2(E) additions.  Below m - 200, and of -inf and
+// NaN, nothing is left of either.
+template <int E>
+__device__ __forceinline__ float2 weights(const float* v, float m) {
+    if constexpr (E == 1) {
+        const float d = fmaxf(v[0] - m, -200.f), w = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+        return make_float2(w, w * d);
+    } else {
+        const float2 x = weights<E / 2>(v, m), y = weights<E / 2>(v + E / 2, m);
+        return make_float2(x.x + y.x, x.y + y.y);
     }
-    S = block_all(S, sum, s_d);
-    E = block_all(E, sum, s_d);
-    ahead = block_all(ahead, [](int x, int y) { return x + y; }, s_i);
-    const double log_s = log(S);
-    auto logprob = [&](float x) {
+}
+
+// A wave's statistics of its part of a chunk; mine: the lane's largest.
+template <int E>
+__device__ __forceinline__ WaveStats wave_stats(const float (&v)[E], int c, uint32_t token, float given, float& mine) {
+    mine = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < E; u++) mine = v[u] > mine ? v[u] : mine;  // (a NaN of either kind is none)
+    WaveStats w;
+    w.m = over_wave(mine, max2);
+    float2 s = make_float2(0.f, 0.f);
+    if (fabsf(w.m) < INFINITY) {
+        s = weights<E>(v, w.m);
+    } else if (w.m == INFINITY) {
+#pragma unroll
+        for (int u = 0; u < E; u++) s.x += v[u] == INFINITY ? 1.f : 0.f;
+    }
+    w.s = over_wave(s.x, add2);
+    w.e = over_wave(s.y, add2);
+    // a larger logit is ahead, an equal one where it lies ahead
+    int ahead = 0;
+    const long long first = (long long)c * (STH * E), end = first + STH * E;
+    if (given == -INFINITY || (token >= first && token < end)) {
+        const unsigned long long key = token_key(logit_key(given), (int)token);
+#pragma unroll
+        for (int u = 0; u < E; u++) {
+            const int i = chunk_index<E>(c, threadIdx.x, u);
+            ahead += token_key(logit_key(clean_logit(v[u])), i) > key;
+        }
+    } else if (token < first) {
+#pragma unroll
+        for (int u = 0; u < E; u++) ahead += v[u] > given;
+    } else {
+#pragma unroll
+        for (int u = 0; u < E; u++) ahead += v[u] >= given;
+    }
+    w.ahead = over_wave(ahead, iadd2);
+    return w;
+}
+// Sums of several of them against the largest of their maxima, in 64 bits.
+struct RunStats {
+    float m = -INFINITY;
+    double s = 0.0, e = 0.0;
+    int ahead = 0;
+    // (m: at least w's)
+    __device__ __forceinline__ void add(const WaveStats& w) {
+        const double f = weight64(w.m, m, 1.0);
+        if (f > 0.0 && w.m > -INFINITY) {
+            const double d = w.m == m ? 0.0 : (double)w.m - (double)m;
+            s += f * w.s;
+            e += f * (w.e + d * w.s);
+        }
+        ahead += w.ahead;
+    }
+    __device__ __forceinline__ void follow(float to) {
+        if (to > m) {
+            const double f = weight64(m, to, 1.0);
+            e = f > 0.0 ? f * (e + ((double)m - (double)to) * s) : 0.0;
+            s *= f;
+            m = to;
+        }
+    }
+};
+
+// the row's token: its logit as it is ordered (+inf of one outside the vocabulary: nothing is ahead of it)
+__device__ __forceinline__ float given_logit(const LogprobArgs& a, int row, uint32_t token) {
+    return token < (uint32_t)a.V ? clean_logit(a.logits[(size_t)row * a.V + token]) : INFINITY;
+}
+__device__ __forceinline__ uint32_t given_token(const LogprobArgs& a, int row) {
+    return a.tokens ? a.tokens[row] : 0xFFFFFFFFu;
+}
+
+struct RowSums {
+    float m;
+    double log_s;
+    __device__ __forceinline__ float logprob(float x) const {
         if (m == -INFINITY) return -INFINITY;
         return x == m ? (float)-log_s : (float)((double)x - (double)m - log_s);
-    };
-    if (tid == 0) {
-        if (a.tokens) {
-            if (a.logprobs) a.logprobs[row] = known ? logprob(clean_logit(l[token])) : -INFINITY;
-            if (a.ranks) a.ranks[row] = known ? ahead : -1;
-        }
-        if (a.entropies) a.entropies[row] = m == -INFINITY ? 0.f : (float)(log_s - E / S);
     }
-    for (int k = 0; k < a.top; k++) {
-        if (k > 0) {
-            unsigned long long next = 0;
-            for (int i = tid; i < V; i += LTH) {
-                const unsigned long long key = token_key(clean_logit(l[i]), i);
-                next = key < first ? max(next, key) : next;
-            }
-            first = block_all(next, most, s_k);
+};
+// A row's sums from those of n waves, by a wave; its outputs but the alternatives.
+__device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, const WaveStats* st, int n, uint32_t token,
+                                            float given) {
+    const int lane = threadIdx.x & 63;
+    RowSums r;
+    WaveStats mine{-INFINITY, 0.f, 0.f, 0};
+    if (lane < n) mine = st[lane];
+    float m = mine.m;
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, st[i].m);
+    RunStats run;
+    run.m = r.m = over_wave(m, max2);
+    for (int i = lane; i < n; i += 64) run.add(i == lane ? mine : st[i]);
+    double s = run.s, e = run.e;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        s += __shfl_xor(s, o);
+        e += __shfl_xor(e, o);
+    }
+    const int ahead = over_wave(run.ahead, iadd2);
+    r.log_s = log(s);
+    if (lane == 0) {
+        const bool known = token < (uint32_t)a.V;
+        if (a.logprobs) a.logprobs[row] = known ? r.logprob(given) : -INFINITY;
+        if (a.ranks) a.ranks[row] = known ? ahead : -1;
+        if (a.entropies) a.entropies[row] = r.m == -INFINITY ? 0.f : (float)(r.log_s - e / s);
+    }
+    return r;
+}
+
+// ---- alternatives
+template <int TH>
+struct TopShared {
+    unsigned long long list[LIST];
+    uint32_t key[TH];
+    int subs[SUBS], cnt[8], wave[TH / 64], n, ns;
+};
+
+// Of TH keys a bound that at least `need` of them, and not many more, reach; by each wave for itself.
+template <int TH>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t* keys, int need) {
+    const int lane = threadIdx.x & 63;
+    uint32_t k[TH / 64], lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+    for (int u = 0; u < TH / 64; u++) {
+        k[u] = keys[lane + 64 * u];
+        lo = min(lo, k[u]);
+        hi = max(hi, k[u]);
+    }
+    lo = __builtin_amdgcn_readfirstlane(over_wave(lo, umin2));
+    hi = __builtin_amdgcn_readfirstlane(over_wave(hi, umax2));
+    int reach = TH;
+    while (lo < hi && reach > need + (need >> 2) + 4) {
+        const uint32_t mid = lo + ((hi - lo) >> 1) + 1;
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < TH / 64; u++) c += __popcll(__ballot(k[u] >= mid));
+        if (c >= need) {
+            lo = mid;
+            reach = c;
+        } else {
+            hi = mid - 1;
         }
-        if (tid == 0) {
-            a.top_tokens[(size_t)row * a.top + k] = 0xFFFFFFFFu - (uint32_t)first;
-            a.top_logprobs[(size_t)row * a.top + k] = logprob(key_logit((uint32_t)(first >> 32)));
+    }
+    return lo;
+}
+
+// The alternatives of a row by search: the n-th largest key three bits at a time, then the logits above it and the
+// first of those at it.  Leaves all of them in the list.
+template <int TH>
+__device__ void flat_tops(const LogprobArgs& a, const float* l, TopShared<TH>& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, V = a.V, need = a.top;
+    uint32_t at = 0;
+    for (int shift = 29; shift >= 0; shift = shift == 2 ? 0 : shift - 3) {
+        const int digits = shift ? 8 : 4;
+        if (tid < 8) sh.cnt[tid] = 0;
+        __syncthreads();
+        int c[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int i = tid; i < V; i += TH) {
+            const uint32_t k = logit_key(clean_logit(l[i]));
+#pragma unroll
+            for (int j = 1; j < 8; j++) c[j] += j < digits && k >= at + ((uint32_t)j << shift);
+        }
+#pragma unroll
+        for (int j = 1; j < 8; j++) {
+            const int x = over_wave(c[j], iadd2);
+            if (lane == 0) atomicAdd(&sh.cnt[j], x);
+        }
+        __syncthreads();
+        int best = 0;
+#pragma unroll
+        for (int j = 1; j < 8; j++)
+            if (j < digits && sh.cnt[j] >= need) best = j;
+        at += (uint32_t)best << shift;
+        __syncthreads();
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    for (int i = tid; i < V; i += TH) {  // fewer than `need`
+        const uint32_t k = logit_key(clean_logit(l[i]));
+        if (k > at) sh.list[atomicAdd(&sh.n, 1)] = token_key(k, i);
+    }
+    __syncthreads();
+    for (int base = 0; base < V; base += TH) {
+        const int i = base + tid;
+        const bool is = i < V && logit_key(clean_logit(l[min(i, V - 1)])) == at;
+        const unsigned long long b = __ballot(is);
+        if (lane == 0) sh.wave[tid >> 6] = __popcll(b);
+        __syncthreads();
+        int before = sh.n, all = before;
+#pragma unroll
+        for (int w = 0; w < TH / 64; w++) {
+            before += w < tid >> 6 ? sh.wave[w] : 0;
+            all += sh.wave[w];
+        }
+        before += __popcll(b & ((1ull << lane) - 1));
+        if (is && before < need) sh.list[before] = token_key(at, i);
+        __syncthreads();
+        if (tid == 0) sh.n = min(all, need);
+        __syncthreads();
+        if (all >= need) break;
+    }
+}
+
+// The alternatives from the candidates in the list (`over`: there were more than it holds, or than could be read
+// again), in order; where fewer logits than that are above -inf, the first of the others behind them.
+template <int TH>
+__device__ void write_tops(const LogprobArgs& a, int row, const float* l, TopShared<TH>& sh, bool over, const RowSums& r) {
+    const int tid = threadIdx.x;
+    if (over) flat_tops(a, l, sh);
+    const int n = sh.n;
+    uint32_t* tokens = a.top_tokens + (size_t)row * a.top;
+    float* lps = a.top_logprobs + (size_t)row * a.top;
+    for (int i = tid; i < n; i += TH) {
+        const unsigned long long x = sh.list[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; j++) rank += sh.list[j] > x;
+        if (rank < a.top) {
+            tokens[rank] = 0xFFFFFFFFu - (uint32_t)x;
+            lps[rank] = r.logprob(key_logit((uint32_t)(x >> 32)));
+        }
+    }
+    if (n < a.top && tid < 64) {
+        int at = n;
+        for (int base = 0; at < a.top && base < a.V; base += 64) {
+            const int i = base + tid;
+            const bool none = i < a.V && clean_logit(l[min(i, a.V - 1)]) == -INFINITY;
+            const unsigned long long b = __ballot(none);
+            const int rank = at + __popcll(b & ((1ull << tid) - 1));
+            if (none && rank < a.top) {
+                tokens[rank] = i;
+                lps[rank] = -INFINITY;
+            }
+            at += __popcll(b);
         }
     }
 }
 
+// ---- rows of up to STH * E logits: one workgroup
+template <int E>
+__global__ __launch_bounds__(STH) void logprobs_small_kernel(LogprobArgs a) {
+    __shared__ TopShared<STH> sh;
+    __shared__ WaveStats s_st[STH / 64];
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const float* l = a.logits + (size_t)row * a.V;
+    const uint32_t token = given_token(a, row);
+    float v[E], mine;
+    load_chunk<E>(l, a.V, 0, v);
+    const float given = given_logit(a, row, token);
+    const WaveStats w = wave_stats<E>(v, 0, token, given, mine);
+    if ((tid & 63) == 0) s_st[tid >> 6] = w;
+    sh.key[tid] = logit_key(mine + 0.f);
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    if (a.top == 0) {
+        if (tid < 64) row_sums(a, row, s_st, STH / 64, token, given);
+        return;
+    }
+    const uint32_t bound = max(bound_of<STH>(sh.key, a.top), KEY_NONE + 1);
+#pragma unroll
+    for (int u = 0; u < E; u++) {
+        const uint32_t k = logit_key(clean_logit(v[u]));
+        if (k >= bound) {
+            const int x = atomicAdd(&sh.n, 1);
+            if (x < LIST) sh.list[x] = token_key(k, chunk_index<E>(0, tid, u));
+        }
+    }
+    RowSums r;
+    r = row_sums(a, row, s_st, STH / 64, token, given);  // (each wave for itself)
+    __syncthreads();
+    const bool over = sh.n > LIST;
+    __syncthreads();
+    write_tops(a, row, l, sh, over, r);
+}
+
+// ---- longer rows: their splits, then a row's join
+template <int E>
+__global__ __launch_bounds__(STH) void logprobs_split_kernel(LogprobArgs a) {
+    const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x;
+    const float* l = a.logits + (size_t)row * a.V;
+    const uint32_t token = given_token(a, row);
+    const int chunks = (a.V + STH * E - 1) / (STH * E);
+    float v[E], most;
+    load_chunk<E>(l, a.V, split, v);
+    const float given = given_logit(a, row, token);
+    WaveStats w = wave_stats<E>(v, split, token, given, most);
+    if (chunks > a.S) {  // (for all workgroups)
+        RunStats run;
+        run.m = w.m;
+        run.add(w);
+        for (int c = split + a.S; c < chunks; c += a.S) {
+            float mine;
+            load_chunk<E>(l, a.V, c, v);
+            w = wave_stats<E>(v, c, token, given, mine);
+            run.follow(w.m);
+            run.add(w);
+            most = fmaxf(most, mine);
+        }
+        w = WaveStats{run.m, (float)run.s, (float)run.e, run.ahead};
+    }
+    if ((tid & 63) == 0) a.stats[((size_t)row * a.S + split) * (STH / 64) + (tid >> 6)] = w;
+    if (a.top) a.sub[((size_t)row * a.S + split) * STH + tid] = most;
+}
+
+__global__ __launch_bounds__(STH) void logprobs_sums_kernel(LogprobArgs a) {
+    const int row = blockIdx.x * (STH / 64) + (threadIdx.x >> 6), n = a.S * (STH / 64);
+    if (row >= a.rows) return;
+    const uint32_t token = given_token(a, row);
+    row_sums(a, row, a.stats + (size_t)row * n, n, token, given_logit(a, row, token));
+}
+
+template <int E>
+__global__ __launch_bounds__(JTH) void logprobs_tops_kernel(LogprobArgs a) {
+    constexpr int R = SPLITS * STH / JTH;  // maxima a thread holds
+    __shared__ TopShared<JTH> sh;
+    __shared__ RowSums s_r;
+    const int row = blockIdx.x, tid = threadIdx.x, n_sub = a.S * STH, waves = a.S * (STH / 64), V = a.V;
+    const float* l = a.logits + (size_t)row * V;
+    const float* sub = a.sub + (size_t)row * n_sub;
+    uint32_t mine[R], most = 0;
+#pragma unroll
+    for (int u = 0; u < R; u++) {
+        mine[u] = 0;
+        if (JTH * u < n_sub) {  // (for the whole workgroup)
+            const int i = tid + JTH * u;
+            const uint32_t k = logit_key(sub[min(i, n_sub - 1)] + 0.f);
+            mine[u] = i < n_sub ? k : 0;
+            most = max(most, mine[u]);
+        }
+    }
+    sh.key[tid] = most;
+    if (tid == 0) sh.n = sh.ns = 0;
+    __syncthreads();
+    const uint32_t bound = max(bound_of<JTH>(sh.key, a.top), KEY_NONE + 1);
+#pragma unroll
+    for (int u = 0; u < R; u++)
+        if (JTH * u < n_sub && mine[u] >= bound) {
+            const int x = atomicAdd(&sh.ns, 1);
+            if (x < SUBS) sh.subs[x] = tid + JTH * u;
+        }
+    __syncthreads();
+    const int ns = sh.ns, chunks = (V + STH * E - 1) / (STH * E), per = (chunks + a.S - 1) / a.S * (E / 4);
+    if (ns <= SUBS)
+        for (int w = tid; w < ns * per; w += JTH) {
+            const int x = sh.subs[w / per], rest = w % per;
+            const int i0 = chunk_index<E>(x / STH + rest / (E / 4) * a.S, x % STH, 4 * (rest % (E / 4)));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t key = logit_key(clean_logit(l[min(i0 + k, V - 1)]));
+                if (i0 + k < V && key >= bound) {
+                    const int y = atomicAdd(&sh.n, 1);
+                    if (y < LIST) sh.list[y] = token_key(key, i0 + k);
+                }
+            }
+        }
+    if (tid >= JTH - 64) {  // the last wave has the least to read
+        const uint32_t token = given_token(a, row);
+        const RowSums r = row_sums(a, row, a.stats + (size_t)row * waves, waves, token, given_logit(a, row, token));
+        if (tid == JTH - 1) s_r = r;
+    }
+    __syncthreads();
+    const bool over = ns > SUBS || sh.n > LIST;
+    __syncthreads();
+    write_tops(a, row, l, sh, over, s_r);
+}
+
+// Splits of 32 logits a thread where these are workgroups enough, of 8 in smaller calls.
+static bool wide_splits(int rows, int V) { return (long long)rows * V >= 256ll * STH * 32; }
+static int splits_of(int rows, int V) {
+    const int per = STH * (wide_splits(rows, V) ? 32 : 8);
+    return std::min(SPLITS, (V + per - 1) / per);
+}
+constexpr int SMALL = STH * 32;  // logits of a row that one workgroup takes
+
 size_t token_logprobs_workspace_bytes(int rows, int V, int top) {
-    (void)rows, (void)V, (void)top;
-    return 16;
+    if (V <= SMALL) return 16;
+    const size_t S = splits_of(rows, V);
+    return (size_t)rows * S * (STH / 64) * sizeof(WaveStats) + (top ? (size_t)rows * S * STH * 4 : 0);
 }
 
 int launch_token_logprobs(const float* logits, int rows, int V, const uint32_t* tokens, float* logprobs, int32_t* ranks,
@@ -121,8 +498,24 @@ int launch_token_logprobs(const float* logits, int rows, int V, const uint32_t* 
     const size_t need = token_logprobs_workspace_bytes(rows, V, top);
     QH_REQUIRE(ws_bytes >= need, QRAF_HIP_ERR_INVALID, "token_logprobs: workspace of %zu bytes, %zu needed", ws_bytes,
                need);
-    const LogprobArgs a{logits, tokens, logprobs, entropies, top_logprobs, ranks, top_tokens, V, top};
-    hipLaunchKernelGGL(logprobs_row_kernel, dim3(rows), dim3(LTH), 0, s, a);
+    LogprobArgs a{logits, tokens, logprobs, entropies, top_logprobs, ranks, top_tokens, nullptr, nullptr, V, 1, top, rows};
+    if (V <= SMALL) {
+        if (V <= STH * 8) hipLaunchKernelGGL(logprobs_small_kernel<8>, dim3(rows), dim3(STH), 0, s, a);
+        else hipLaunchKernelGGL(logprobs_small_kernel<32>, dim3(rows), dim3(STH), 0, s, a);
+        QH_CHECK_HIP(hipGetLastError());
+        return QRAF_HIP_OK;
+    }
+    a.S = splits_of(rows, V);
+    a.stats = (WaveStats*)ws;
+    a.sub = (float*)(a.stats + (size_t)rows * a.S * (STH / 64));
+    const bool wide = wide_splits(rows, V);
+    if (wide) hipLaunchKernelGGL(logprobs_split_kernel<32>, dim3(a.S, rows), dim3(STH), 0, s, a);
+    else hipLaunchKernelGGL(logprobs_split_kernel<8>, dim3(a.S, rows), dim3(STH), 0, s, a);
+    QH_CHECK_HIP(hipGetLastError());
+    if (!top)
+        hipLaunchKernelGGL(logprobs_sums_kernel, dim3((rows + STH / 64 - 1) / (STH / 64)), dim3(STH), 0, s, a);
+    else if (wide) hipLaunchKernelGGL(logprobs_tops_kernel<32>, dim3(rows), dim3(JTH), 0, s, a);
+    else hipLaunchKernelGGL(logprobs_tops_kernel<8>, dim3(rows), dim3(JTH), 0, s, a);
     QH_CHECK_HIP(hipGetLastError());
     return QRAF_HIP_OK;
 }

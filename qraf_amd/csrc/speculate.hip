@@ -52,32 +52,13 @@
 #include <algorithm>
 
 #include "common.h"
+#include "logits.h"
 
 namespace qraf_hip {
 
 constexpr int PNT = 1024;  // threads per row
 
-// exp((l - m) / T) in 64 bits, within 1e-11 of it (m: the largest logit, not -inf): 2^y as 2^rint(y) times the
-// series of 2^f, |f| <= 1/2, to its tenth power.  (The library's exponential, to the last bit: 28 us for the bins of
-// 64 rows of 151,936 where this takes 20.)
-__device__ __forceinline__ double weight64(float l, float m, double T) {
-    const double y = fmax(((double)l - (double)m) * (1.4426950408889634074 / T), -1100.0), n = rint(y), f = y - n;
-    double p = 7.0549116208011233e-9;
-    p = __builtin_fma(p, f, 1.0178086009239699e-7);
-    p = __builtin_fma(p, f, 1.3215486790144309e-6);
-    p = __builtin_fma(p, f, 1.5252733804059841e-5);
-    p = __builtin_fma(p, f, 1.5403530393381610e-4);
-    p = __builtin_fma(p, f, 1.3333558146428443e-3);
-    p = __builtin_fma(p, f, 9.6181291076284772e-3);
-    p = __builtin_fma(p, f, 5.5504108664821580e-2);
-    p = __builtin_fma(p, f, 2.4022650695910071e-1);
-    p = __builtin_fma(p, f, 6.9314718055994531e-1);
-    p = __builtin_fma(p, f, 1.0);
-    p = ldexp(p, (int)n);
-    return l == m ? 1.0 : l == -INFINITY || m == INFINITY ? 0.0 : p;
-}
-
-// the same in 32 bits, off by at most 3 units of the last place: the exponent's
+// weight64 in 32 bits, off by at most 3 units of the last place: the exponent's
 // rounding errors (of l - m, of its product with log2(e) / T) as a factor behind it.
 // l and m by halves: their difference may leave fp32's range where T brings it back
 struct Weight32 {

@@ -150,6 +150,20 @@ def test_top_in_one_place(hip, V):
     check(call(hip, x, tokens, 64)[0], x, tokens, 64)
 
 
+@pytest.mark.parametrize("rows,V", [(1, 524289), (2, 600001), (1, 2100000)])
+def test_long_rows(hip, rows, V):
+    """More splits than a row has: several chunks each, the largest in the first, in the last, rising maxima."""
+    rng = np.random.default_rng(V)
+    x, tokens = logits(rng, rows, V), rng.integers(0, V, rows)
+    check(call(hip, x, tokens, 20)[0], x, tokens, 20)
+    x[:, -5:] = 30.0
+    check(call(hip, x, tokens, 20)[0], x, tokens, 20)
+    x += np.linspace(-90, 0, V, dtype=np.float32)
+    check(call(hip, x, tokens, 20)[0], x, tokens, 20)
+    x[:, :V // 2] = -np.inf
+    check(call(hip, x, tokens, 20)[0], x, tokens, 20)
+
+
 @pytest.mark.parametrize("offset", [0, 1, 2, 3])
 @pytest.mark.parametrize("V", [1003, 4096, 50257, 151936])
 def test_alignments(hip, V, offset):
