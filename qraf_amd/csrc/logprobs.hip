@@ -19,6 +19,8 @@
 // few logits that do are ordered by counting.  Rows of up to 8,192 logits take one
 // workgroup and one launch.  Rows with more equal logits at the border than the lists
 // hold take a search over the whole row (flat_tops).
+// Measured: 512 rows of 151,936 (311 MB) 55.7 us, 5.6 TB/s; 160 rows with 20 alternatives (97 MB) 24.5, of which the
+// pass 17 and the join 6.4; 8 rows of 49,152 with 4 7.7.
 #include <math.h>
 
 #include <algorithm>
@@ -33,7 +35,7 @@ constexpr int TOP_MAX = 64;
 constexpr int STH = 256;        // threads of a split
 constexpr int JTH = 512;        // threads that join a row
 constexpr int SPLITS = 64;      // splits of a row at most: longer rows give them several chunks
-constexpr int SUBS = 512;       // sub-ranges that are read again, at most
+constexpr int SUBS = 128;       // sub-ranges that a wave reads again, at most
 constexpr int LIST = 2816;      // candidates: what the lanes that reach a bound of 64 hold, of 32 logits each
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // logit_key of -inf
 
@@ -182,24 +184,21 @@ struct RowSums {
         return x == m ? (float)-log_s : (float)((double)x - (double)m - log_s);
     }
 };
-// A row's sums from those of n waves, by a wave; its outputs but the alternatives.
-__device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, const WaveStats* st, int n, uint32_t token,
-                                            float given) {
+// A row's sums from those of n waves, by a wave; its outputs but the alternatives.  mine: st[lane], requested ahead.
+__device__ __forceinline__ WaveStats lane_stats(const WaveStats* st, int n) {
+    const int lane = threadIdx.x & 63;
+    return lane < n ? st[lane] : WaveStats{-INFINITY, 0.f, 0.f, 0};
+}
+__device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, const WaveStats* st, int n,
+                                            const WaveStats& mine, uint32_t token, float given) {
     const int lane = threadIdx.x & 63;
     RowSums r;
-    WaveStats mine{-INFINITY, 0.f, 0.f, 0};
-    if (lane < n) mine = st[lane];
     float m = mine.m;
     for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, st[i].m);
     RunStats run;
     run.m = r.m = over_wave(m, max2);
     for (int i = lane; i < n; i += 64) run.add(i == lane ? mine : st[i]);
-    double s = run.s, e = run.e;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        s += __shfl_xor(s, o);
-        e += __shfl_xor(e, o);
-    }
+    const double s = wave_sum64(run.s), e = wave_sum64(run.e);
     const int ahead = over_wave(run.ahead, iadd2);
     r.log_s = log(s);
     if (lane == 0) {
@@ -212,11 +211,12 @@ __device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, const
 }
 
 // ---- alternatives
+// (of TH threads)
 template <int TH>
 struct TopShared {
     unsigned long long list[LIST];
     uint32_t key[TH];
-    int subs[SUBS], cnt[8], wave[TH / 64], n, ns;
+    int cnt[8], wave[TH / 64], n;
 };
 
 // Of TH keys a bound that at least `need` of them, and not many more, reach; by each wave for itself.
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(STH) void logprobs_small_kernel(LogprobArgs a) {
     if (tid == 0) sh.n = 0;
     __syncthreads();
     if (a.top == 0) {
-        if (tid < 64) row_sums(a, row, s_st, STH / 64, token, given);
+        if (tid < 64) row_sums(a, row, s_st, STH / 64, lane_stats(s_st, STH / 64), token, given);
         return;
     }
     const uint32_t bound = max(bound_of<STH>(sh.key, a.top), KEY_NONE + 1);
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(STH) void logprobs_small_kernel(LogprobArgs a) {
         }
     }
     RowSums r;
-    r = row_sums(a, row, s_st, STH / 64, token, given);  // (each wave for itself)
+    r = row_sums(a, row, s_st, STH / 64, lane_stats(s_st, STH / 64), token, given);  // (each wave for itself)
     __syncthreads();
     const bool over = sh.n > LIST;
     __syncthreads();
@@ -409,61 +409,86 @@ __global__ __launch_bounds__(STH) void logprobs_split_kernel(LogprobArgs a) {
 __global__ __launch_bounds__(STH) void logprobs_sums_kernel(LogprobArgs a) {
     const int row = blockIdx.x * (STH / 64) + (threadIdx.x >> 6), n = a.S * (STH / 64);
     if (row >= a.rows) return;
+    const WaveStats* st = a.stats + (size_t)row * n;
+    const WaveStats mine = lane_stats(st, n);
     const uint32_t token = given_token(a, row);
-    row_sums(a, row, a.stats + (size_t)row * n, n, token, given_logit(a, row, token));
+    row_sums(a, row, st, n, mine, token, given_logit(a, row, token));
 }
 
-template <int E>
-__global__ __launch_bounds__(JTH) void logprobs_tops_kernel(LogprobArgs a) {
-    constexpr int R = SPLITS * STH / JTH;  // maxima a thread holds
-    __shared__ TopShared<JTH> sh;
+// A wave more than the maxima's for the sums, which nothing waits for but the log probabilities of the alternatives.
+// The others keep their sub-ranges to themselves up to the candidates: two barriers.  R: maxima a thread holds, all
+// requested at once.  Cycles of a row of 151,936, 20 alternatives: maxima 2,800 (a read of what another launch wrote),
+// barrier 500, bound 1,600, list 800, second read 2,400, barriers 1,300, order and output 2,000: 11,500.  (20,000 with one
+// list of sub-ranges by atomics, maxima requested one after another and the sums by one of these waves.)
+template <int E, int R>
+__global__ __launch_bounds__(JTH + 64) void logprobs_tops_kernel(LogprobArgs a) {
+    __shared__ TopShared<JTH + 64> sh;
+    __shared__ int s_subs[JTH / 64][SUBS];
     __shared__ RowSums s_r;
     const int row = blockIdx.x, tid = threadIdx.x, n_sub = a.S * STH, waves = a.S * (STH / 64), V = a.V;
     const float* l = a.logits + (size_t)row * V;
-    const float* sub = a.sub + (size_t)row * n_sub;
-    uint32_t mine[R], most = 0;
+    if (tid >= JTH) {
+        const WaveStats* st = a.stats + (size_t)row * waves;
+        const WaveStats stats = lane_stats(st, waves);
+        const uint32_t token = given_token(a, row);
+        const float given = given_logit(a, row, token);
+        __syncthreads();
+        const RowSums r = row_sums(a, row, st, waves, stats, token, given);
+        if (tid == JTH) s_r = r;
+        __syncthreads();
+    } else {
+        const float* sub = a.sub + (size_t)row * n_sub;
+        float x[R];
 #pragma unroll
-    for (int u = 0; u < R; u++) {
-        mine[u] = 0;
-        if (JTH * u < n_sub) {  // (for the whole workgroup)
-            const int i = tid + JTH * u;
-            const uint32_t k = logit_key(sub[min(i, n_sub - 1)] + 0.f);
-            mine[u] = i < n_sub ? k : 0;
+        for (int u = 0; u < R; u++) x[u] = sub[min(tid + JTH * u, n_sub - 1)];
+        uint32_t mine[R], most = 0;
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+            mine[u] = tid + JTH * u < n_sub ? logit_key(x[u] + 0.f) : 0;
             most = max(most, mine[u]);
         }
-    }
-    sh.key[tid] = most;
-    if (tid == 0) sh.n = sh.ns = 0;
-    __syncthreads();
-    const uint32_t bound = max(bound_of<JTH>(sh.key, a.top), KEY_NONE + 1);
+        sh.key[tid] = most;
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        const uint32_t bound = max(bound_of<JTH>(sh.key, a.top), KEY_NONE + 1);
+        const int lane = tid & 63;
+        int *const subs = s_subs[tid >> 6], ns = 0;
 #pragma unroll
-    for (int u = 0; u < R; u++)
-        if (JTH * u < n_sub && mine[u] >= bound) {
-            const int x = atomicAdd(&sh.ns, 1);
-            if (x < SUBS) sh.subs[x] = tid + JTH * u;
+        for (int u = 0; u < R; u++) {
+            const unsigned long long b = __ballot(mine[u] >= bound);
+            if (!b) continue;  // (nearly always)
+            const int at = ns + __popcll(b & ((1ull << lane) - 1));
+            if (mine[u] >= bound && at < SUBS) subs[at] = tid + JTH * u;
+            ns += __popcll(b);
         }
-    __syncthreads();
-    const int ns = sh.ns, chunks = (V + STH * E - 1) / (STH * E), per = (chunks + a.S - 1) / a.S * (E / 4);
-    if (ns <= SUBS)
-        for (int w = tid; w < ns * per; w += JTH) {
-            const int x = sh.subs[w / per], rest = w % per;
-            const int i0 = chunk_index<E>(x / STH + rest / (E / 4) * a.S, x % STH, 4 * (rest % (E / 4)));
+        __builtin_amdgcn_wave_barrier();  // (of one wave: its writes are in order with its reads)
+        const int chunks = (V + STH * E - 1) / (STH * E), per = (chunks + a.S - 1) / a.S * (E / 4);
+        if (ns > SUBS && lane == 0) atomicAdd(&sh.n, LIST + 1);
+        for (int w0 = 0; w0 < (ns <= SUBS ? ns * per : 0); w0 += 64) {
+            const int w = w0 + lane, in = min(w, ns * per - 1), y = subs[in / per], rest = in % per;
+            const int i0 = chunk_index<E>(y / STH + rest / (E / 4) * a.S, y % STH, 4 * (rest % (E / 4)));
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = l[min(i0 + k, V - 1)];
+            uint32_t key[4];
+            int at[4], all = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const uint32_t key = logit_key(clean_logit(l[min(i0 + k, V - 1)]));
-                if (i0 + k < V && key >= bound) {
-                    const int y = atomicAdd(&sh.n, 1);
-                    if (y < LIST) sh.list[y] = token_key(key, i0 + k);
-                }
+                key[k] = w == in && i0 + k < V ? logit_key(clean_logit(v[k])) : 0;
+                const unsigned long long b = __ballot(key[k] >= bound);
+                at[k] = all + __popcll(b & ((1ull << lane) - 1));
+                all += __popcll(b);
             }
+            int first = 0;
+            if (lane == 0) first = atomicAdd(&sh.n, all);
+            first = __builtin_amdgcn_readfirstlane(first);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (key[k] >= bound && first + at[k] < LIST) sh.list[first + at[k]] = token_key(key[k], i0 + k);
         }
-    if (tid >= JTH - 64) {  // the last wave has the least to read
-        const uint32_t token = given_token(a, row);
-        const RowSums r = row_sums(a, row, a.stats + (size_t)row * waves, waves, token, given_logit(a, row, token));
-        if (tid == JTH - 1) s_r = r;
+        __syncthreads();
     }
-    __syncthreads();
-    const bool over = ns > SUBS || sh.n > LIST;
+    const bool over = sh.n > LIST;
     __syncthreads();
     write_tops(a, row, l, sh, over, s_r);
 }
@@ -514,8 +539,20 @@ int launch_token_logprobs(const float* logits, int rows, int V, const uint32_t* 
     QH_CHECK_HIP(hipGetLastError());
     if (!top)
         hipLaunchKernelGGL(logprobs_sums_kernel, dim3((rows + STH / 64 - 1) / (STH / 64)), dim3(STH), 0, s, a);
-    else if (wide) hipLaunchKernelGGL(logprobs_tops_kernel<32>, dim3(rows), dim3(JTH), 0, s, a);
-    else hipLaunchKernelGGL(logprobs_tops_kernel<8>, dim3(rows), dim3(JTH), 0, s, a);
+    else {
+#define QH_TOPS(Ev, Rv) hipLaunchKernelGGL((logprobs_tops_kernel<Ev, Rv>), dim3(rows), dim3(JTH + 64), 0, s, a)
+        const int per = (a.S * STH + JTH - 1) / JTH;
+        if (wide) {
+            if (per <= 4) QH_TOPS(32, 4);
+            else if (per <= 12) QH_TOPS(32, 12);
+            else QH_TOPS(32, 32);
+        } else {
+            if (per <= 4) QH_TOPS(8, 4);
+            else if (per <= 12) QH_TOPS(8, 12);
+            else QH_TOPS(8, 32);
+        }
+#undef QH_TOPS
+    }
     QH_CHECK_HIP(hipGetLastError());
     return QRAF_HIP_OK;
 }

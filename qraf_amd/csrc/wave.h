@@ -53,4 +53,32 @@ __device__ __forceinline__ T over_wave(T x, F op) {
     return over_halves(over_rows(over_row(x, op), op), op);
 }
 
+// the sum of a 64-bit value over all lanes, the same in every lane
+__device__ __forceinline__ double wave_sum64(double x) {
+    auto halves = [](double v, int& lo, int& hi) {
+        lo = (int)__double_as_longlong(v);
+        hi = (int)(__double_as_longlong(v) >> 32);
+    };
+    auto whole = [](unsigned lo, unsigned hi) { return __longlong_as_double((long long)hi << 32 | lo); };
+    int lo, hi;
+    halves(x, lo, hi);
+    x += whole(gdpp<GDPP_XOR1>(lo), gdpp<GDPP_XOR1>(hi));
+    halves(x, lo, hi);
+    x += whole(gdpp<GDPP_XOR2>(lo), gdpp<GDPP_XOR2>(hi));
+    halves(x, lo, hi);
+    x += whole(gdpp<GDPP_ROR4>(lo), gdpp<GDPP_ROR4>(hi));
+    halves(x, lo, hi);
+    x += whole(gdpp<GDPP_ROR8>(lo), gdpp<GDPP_ROR8>(hi));
+    halves(x, lo, hi);
+    auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    auto h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    x = whole(l[0], h[0]) + whole(l[1], h[1]);
+    halves(x, lo, hi);
+    l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    x = whole(l[0], h[0]) + whole(l[1], h[1]);
+    halves(x, lo, hi);  // (rows rotated by 4 and 8 add in another order)
+    return whole(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi));
+}
+
 }  // namespace qraf_hip
