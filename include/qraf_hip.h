@@ -726,6 +726,38 @@ int qraf_engine_verify(qraf_engine* engine, int32_t row0, int32_t n_seqs, const 
                        int32_t recent_stride, const uint32_t* draft_tokens, const float* draft_probs,
                        const float* accept_uniforms, const float* pick_uniforms, int32_t* accepted,
                        uint32_t* tokens);
+/* One step whose rows are the nodes of trees of drafted tokens, as qraf_engine_step
+ * otherwise.  A sequence's rows lie side by side: the first is its last token that is
+ * certain, at position positions[i] (at most the sequence's length; of the others
+ * positions is not read) with parent -1; every other row i drafts tokens[i] behind
+ * row parents[i], a row of this call of the same sequence ahead of it.  A node
+ * attends to its sequence's positions ahead of the tree, its ancestors and itself,
+ * and is rotated for its depth (qraf_hip_tree_append_dev,
+ * qraf_hip_tree_attention_dev); node j of a tree takes the cache's position
+ * positions[first] + j.  Up to 64 nodes a sequence.  Sequences that
+ * qraf_engine_set_repetition_penalty counts for are refused (QRAF_HIP_ERR_STATE):
+ * drafts would be counted; qraf_engine_accept_tree takes the penalty with the call.
+ * No reference counterpart. */
+int qraf_engine_step_tree(qraf_engine* engine, int32_t n_rows, const int32_t* seq_ids, const uint32_t* tokens,
+                          const int32_t* parents, const int32_t* positions, const uint8_t* want_logits, float* logits,
+                          uint32_t* next_tokens);
+/* The trees of the step before, a qraf_engine_step_tree with the logits of all its
+ * rows: a token sampled behind every node (qraf_engine_sample's parameters, histories
+ * and uniforms, a row each; a node's history holds its ancestors' drafts and its
+ * own), the path along them (qraf_hip_tree_accept_dev), and the path's keys and
+ * values moved to the positions behind the root (qraf_hip_kv_compact_dev).
+ * accepted [sequences of the step] and tokens [rows] as there.  The sequence's next
+ * step begins at its root's position + 1 + accepted.  Once a step: the cache has
+ * moved (QRAF_HIP_ERR_STATE otherwise).  No reference counterpart. */
+int qraf_engine_accept_tree(qraf_engine* engine, const qraf_sampling_params* params, const uint32_t* recent,
+                            const int32_t* recent_count, int32_t recent_stride, const float* uniforms,
+                            int32_t* accepted, uint32_t* tokens);
+/* qraf_hip_token_logprobs_dev on the last step's logit rows row0 .. row0+rows-1, all
+ * arrays on the host: log probabilities and ranks of tokens [rows] (NULL: neither),
+ * entropies, the top alternatives.  A repetition penalty of an earlier call on these
+ * rows has changed them.  No reference counterpart. */
+int qraf_engine_logprobs(qraf_engine* engine, int32_t row0, int32_t rows, const uint32_t* tokens, float* logprobs,
+                         int32_t* ranks, float* entropies, int32_t top, uint32_t* top_tokens, float* top_logprobs);
 /* The last step's logit rows row0 .. row0+rows-1 (the rows it returned
  * logits or argmax for, in order) copied from HBM to out [rows][vocab]: a
  * step can keep its logits on the device and a caller read back only the

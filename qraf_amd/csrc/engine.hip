@@ -479,7 +479,8 @@ struct qraf_engine {
     uint16_t *ah = nullptr, *al = nullptr;  // SwiGLU activation planes [max_batch][F] (fused gate/up epilogue)
     uint32_t* amax = nullptr;
     int32_t* d_in = nullptr;  // tokens | positions | ctx | logit rows | token sources | penalty slots | penalties |
-                              // group prefixes | group starts | page table rows
+                              // group prefixes | group starts | page table rows | trees: cache positions, sequences,
+                              // parents (a node of the tree), masks
     // Pinned staging, one slot per step in flight: a step's inputs are written
     // into slot `slot` while the previous step (the other slot) may still be
     // queued; its tokens come back into h_amax of the same slot.
@@ -496,6 +497,10 @@ struct qraf_engine {
     size_t attn_ws_bytes = 0;
     void* group_ws = nullptr;  // attention by group (group_rows), allocated when that is first turned on
     size_t group_ws_bytes = 0;
+    void* tree_ws = nullptr;   // attention of trees, allocated by the first step of one
+    size_t tree_ws_bytes = 0;
+    // the last step's trees while they can be accepted: nodes (0: none), sequences, rows of its layout in d_in
+    int tree_nodes = 0, tree_seqs = 0, tree_n = 0;
     void* gemm_ws = nullptr;  // split-K partial tiles of the batched projections
     size_t gemm_ws_bytes = 0;
     float* am_val = nullptr;  // argmax chunk winners [max_batch][32]
@@ -516,7 +521,7 @@ struct qraf_engine {
     struct StepGraph {
         int n = 0, n_logit_rows = 0, ctx = 0;
         int head = 0;  // 0: no head, 1: logits (and argmax), 2: argmax only
-        bool grouped = false;
+        bool grouped = false, tree = false;
         uint32_t gen = 0;
         hipGraphExec_t exec = nullptr;
         uint64_t used = 0;
@@ -667,7 +672,7 @@ int qraf_engine_create(const qraf_model_config* cfg, const qraf_engine_options* 
     A(e->am_idx, (size_t)B * ARGMAX_CHUNKS * 4);
     e->am_keys_bytes = qgemm_argmax_keys_bytes((int)V, (int)B);
     A(e->am_keys, e->am_keys_bytes);
-    e->in_words = (size_t)B * (9 + e->max_pages) + 1;
+    e->in_words = (size_t)B * (14 + e->max_pages) + 2;
     A(e->d_in, e->in_words * 4);
     e->attn_ws_bytes = attn_workspace_bytes(B, (int)c.num_heads, (int)kvh, hd, e->capacity);
     A(e->attn_ws, e->attn_ws_bytes);
@@ -1064,13 +1069,27 @@ static double now_us() {
     return std::chrono::duration<double, std::micro>(std::chrono::steady_clock::now().time_since_epoch()).count();
 }
 
+// word of a step's staging at which the masks of its trees lie (8-byte aligned), n rows with padding
+static size_t tree_masks_at(int n, int max_pages) { return ((size_t)n * (12 + max_pages) + 2) / 2 * 2; }
+static int tree_workspace(qraf_engine* e) {
+    if (e->tree_ws) return QRAF_HIP_OK;
+    size_t bytes = 16;
+    for (int n = 1; n <= (int)e->o.max_batch; n++)  // (not monotone: the largest batches take another form)
+        bytes = std::max(bytes, tree_attention_workspace_bytes(n, n, (int)e->c.num_heads, (int)e->c.num_kv_heads, e->hd,
+                                                               e->capacity));
+    QH_TRY(ealloc(e, &e->tree_ws, bytes));
+    e->tree_ws_bytes = bytes;
+    return QRAF_HIP_OK;
+}
+
 // Validates one step and issues it on the engine's stream: its inputs into
 // staging slot e->slot, the staging copy, the captured (or eager) launches,
 // the logits copy (logits != null) and the greedy tokens' copy into the
 // slot's h_amax (tok_out), then the slot's event.  The step joins e->pending.
+// parents: the rows are nodes of trees (qraf_engine_step_tree), checked; a sequence's rows lie side by side.
 static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const uint32_t* tokens,
                       const int32_t* token_src, const int32_t* positions, const uint8_t* want_logits, float* logits,
-                      bool tok_out) {
+                      bool tok_out, const int32_t* parents = nullptr) {
     const double t_enter = now_us();
     QH_REQUIRE(e && seq_ids && tokens && positions, QRAF_HIP_ERR_INVALID, "step: null argument");
     QH_REQUIRE(e->finalized, QRAF_HIP_ERR_STATE, "step: engine not finalized");
@@ -1109,13 +1128,28 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     int32_t* gpre = (int32_t*)(ppen + n_pad);
     int32_t* gstart = gpre + n_pad;
     int32_t* ptab = gstart + n_pad + 1;
+    const bool tree = parents != nullptr;
+    int32_t* slots = ptab + (size_t)n_pad * MP;
+    int32_t* row_seq = slots + n_pad;
+    int32_t* node_parent = row_seq + n_pad;
+    uint64_t* masks = (uint64_t*)(e->h_in[e->slot] + tree_masks_at(n_pad, MP));
+    std::vector<int32_t> places;  // trees: a node's place in the cache
+    if (tree) {
+        QH_TRY(tree_workspace(e));
+        places.resize(n);
+        for (int i = 0, first = 0; i < n; i++) {
+            if (i > 0 && seq_ids[i] != seq_ids[i - 1]) first = i;
+            places[i] = (int32_t)std::min<int64_t>((int64_t)positions[first] + (i - first), INT_MAX);
+        }
+    }
     // the rows' sequences and positions checked, their new pages taken from
     // the pool and their page-table rows written (nothing changes on failure);
     // step_ctx, the longest context of this step, sizes the attention grid
     // (and skips the merge)
     int step_ctx = 1;
-    QH_TRY(e->pages.plan_step(n, seq_ids, positions, ptab, &step_ctx));
+    QH_TRY(e->pages.plan_step(n, seq_ids, tree ? places.data() : positions, ptab, &step_ctx));
     e->last_logit_rows = 0;  // set again once this step's launches are issued
+    e->tree_nodes = 0;
     for (int i = 0; i < n; i++) {
         src[i] = token_src ? token_src[i] : -1;
         tok[i] = src[i] >= 0 ? 0 : (int32_t)tokens[i];
@@ -1140,7 +1174,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     // unused entries empty ones.  By group when that spares enough (group_least), in shapes that it reads shared
     // positions of once.
     bool grouped = false;
-    if (e->group_rows) {
+    if (e->group_rows && !tree) {
         int groups = 0;
         long long spared = 0;  // positions
         for (int i = 0; i < n_pad; i++) {
@@ -1165,6 +1199,30 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
                 }
     }
     e->group_steps += grouped;
+    // Trees: a node is rotated for its depth behind its sequence's cache, lies behind the nodes ahead of it and attends
+    // to its parent's nodes and itself.  The page table gets a row for each sequence (its last row's is the whole); pad
+    // rows are one more, unused entries empty ones.
+    int tree_seqs = 0;
+    if (tree) {
+        for (int i = 0, first = 0; i < n_pad; i++) {
+            if (i == 0 || (i < n ? seq_ids[i] != seq_ids[i - 1] : i == n)) {
+                first = i;
+                gstart[tree_seqs] = i;
+                gpre[tree_seqs++] = i < n ? positions[i] : 0;
+            }
+            const int q = tree_seqs - 1, node = i < n ? i - first : 0, up = i < n && i > first ? parents[i] : -1;
+            row_seq[i] = q;
+            slots[i] = gpre[q] + node;
+            node_parent[i] = up < 0 ? -1 : up - first;
+            masks[i] = (up < 0 ? 0 : masks[up]) | 1ull << node;
+            pos[i] = i < n ? (up < 0 ? positions[first] : pos[up] + 1) : 0;
+            if (i + 1 == n_pad || (i < n ? i + 1 == n || seq_ids[i + 1] != seq_ids[i] : false))
+                memmove(ptab + (size_t)q * MP, ptab + (size_t)i * MP, (size_t)MP * 4);
+        }
+        for (int q = tree_seqs; q < n_pad; q++) gpre[q] = 0;
+        for (int q = tree_seqs; q <= n_pad; q++) gstart[q] = n_pad;
+        if (n_pad > n_real) tree_seqs--;
+    }
     const int n_logit_real = n_logit_rows;
     if (n_pad != n && n_logit_rows > 0) {
         const int nl = std::min((n_logit_rows + e->row_pad - 1) / e->row_pad * e->row_pad, n_pad);
@@ -1173,7 +1231,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     }
     n = n_pad;
     hipStream_t s = e->stream;
-    const size_t words = (size_t)n * (9 + MP) + 1;
+    const size_t words = tree ? tree_masks_at(n, MP) + 2 * (size_t)n : (size_t)n * (9 + MP) + 1;
     const bool head = n_logit_rows > 0 && (logits || tok_out);
     // greedy-only step (no logits wanted, none kept): the head's argmax fused into its GEMM where it runs one
     const bool argmax_only = head && !logits && tok_out && !e->keep_logits && e->pen_live == 0;
@@ -1188,6 +1246,9 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     const int32_t* d_gpre = (const int32_t*)(d_ppen + n);
     const int32_t* d_gstart = d_gpre + n;
     const int32_t* d_ptab = d_gstart + n + 1;
+    const int32_t* d_slots = tree ? d_ptab + (size_t)n * MP : nullptr;
+    const int32_t* d_row_seq = tree ? d_slots + n : nullptr;
+    const uint64_t* d_masks = (const uint64_t*)(e->d_in + tree_masks_at(n, MP));
 
     const int D = (int)c.hidden_size, F = (int)c.intermediate_size, V = (int)c.vocab_size;
     const int H = (int)c.num_heads, Hkv = (int)c.num_kv_heads, hd = e->hd;
@@ -1242,6 +1303,9 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     };
 
     auto attention = [&](const uint8_t* kc, const uint8_t* vc, int ctx_grid, float* out, uint16_t* hi, uint16_t* lo) {
+        if (tree)
+            return launch_tree_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_gpre, d_gstart, d_masks, n, n, H, Hkv, hd, ps,
+                                         scale, ctx_grid, out, e->tree_ws, e->tree_ws_bytes, s, hi, lo);
         if (grouped)
             return launch_group_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_ctx, d_gstart, d_gpre, n, n, H, Hkv, hd,
                                           ps, scale, ctx_grid, out, e->group_ws, e->group_ws_bytes, s, hi, lo);
@@ -1280,7 +1344,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
                 QH_TRY(launch_qgemm(L.wqkv_t, L.dt_attn, 32, e->qkvd, D, e->xh, e->xl, n, e->qkv, nullptr, P,
                                     e->part_ws_bytes, s, true, &S));
                 QH_TRY(launch_rope_append(P, L.has_bias ? L.bqkv : nullptr, n, H, Hkv, hd, d_pos, e->rope, e->q, kc, vc,
-                                          e->o.kv_dtype, d_ptab, MP, ps, s, S, (size_t)n * e->qkvd));
+                                          e->o.kv_dtype, d_ptab, MP, ps, s, S, (size_t)n * e->qkvd, d_slots, d_row_seq));
                 QH_TRY(attention(kc, vc, ctx_grid, nullptr, e->xh, e->xl));
                 QH_TRY(launch_qgemm(L.wo_t, L.dt_attn, 32, D, e->qd, e->xh, e->xl, n, e->qkv, nullptr, P, e->part_ws_bytes,
                                     s, true, &S));
@@ -1326,10 +1390,10 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
             rope.kv_dtype = e->o.kv_dtype;
             bool fused = false;
             QH_TRY(proj(L.wqkv, L.wqkv_t, L.dt_attn, e->qkvd, D, e->h, n, e->qkv, nullptr, &attn_norm,
-                        e->fuse_rope && e->o.kv_dtype != DT_I8 ? &rope : nullptr, &fused));
+                        e->fuse_rope && !tree && e->o.kv_dtype != DT_I8 ? &rope : nullptr, &fused));
             if (!fused)
                 QH_TRY(launch_rope_append(e->qkv, L.has_bias ? L.bqkv : nullptr, n, H, Hkv, hd, d_pos, e->rope, e->q,
-                                          kc, vc, e->o.kv_dtype, d_ptab, MP, ps, s));
+                                          kc, vc, e->o.kv_dtype, d_ptab, MP, ps, s, 1, 0, d_slots, d_row_seq));
             QH_TRY(attention(kc, vc, ctx_grid, e->att, nullptr, nullptr));
             QH_TRY(proj(L.wo, L.wo_t, L.dt_attn, D, e->qd, e->att, n, e->h, e->h));  // + residual (transformer.cpp:593)
             const MvPrep ffn_norm{XP_NORM, L.fn, c.rms_norm_eps, e->xn};  // transformer.cpp:595
@@ -1392,13 +1456,13 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         qraf_engine::StepGraph* g = nullptr;
         for (auto& sg : e->graphs)
             if (sg.n == n && sg.n_logit_rows == n_logit_rows && sg.ctx == ctx_grid && sg.head == head_mode &&
-                sg.grouped == grouped && sg.gen == gen)
+                sg.grouped == grouped && sg.tree == tree && sg.gen == gen)
                 g = &sg;
         bool second = false;
         if (!g) {
             for (auto it = e->seen.begin(); it != e->seen.end(); ++it)
                 if (it->n == n && it->n_logit_rows == n_logit_rows && it->ctx == ctx_grid && it->head == head_mode &&
-                    it->grouped == grouped && it->gen == gen) {
+                    it->grouped == grouped && it->tree == tree && it->gen == gen) {
                     second = true;
                     e->seen.erase(it);
                     break;
@@ -1410,6 +1474,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
                 sg.ctx = ctx_grid;
                 sg.head = head_mode;
                 sg.grouped = grouped;
+                sg.tree = tree;
                 sg.gen = gen;
                 if (e->seen.size() >= 4 * MAX_STEP_GRAPHS) e->seen.erase(e->seen.begin());
                 e->seen.push_back(sg);
@@ -1449,6 +1514,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
             sg.ctx = ctx_grid;
             sg.head = head_mode;
             sg.grouped = grouped;
+            sg.tree = tree;
             sg.gen = gen;
             sg.exec = exec;
             e->graphs.push_back(sg);
@@ -1465,6 +1531,11 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     }
     e->last_logit_rows = head ? n_logit_real : 0;
     e->last_logits_kept = !argmax_only;
+    if (tree && e->last_logit_rows == n_real) {
+        e->tree_nodes = n_real;
+        e->tree_seqs = tree_seqs;
+        e->tree_n = n;
+    }
     if (head && logits)
         QH_CHECK_HIP(hipMemcpyAsync(logits, e->logits, (size_t)n_logit_real * V * 4, hipMemcpyDeviceToHost, s));
     // tokens come back through pinned staging: an async copy into pageable
@@ -1494,6 +1565,37 @@ int qraf_engine_step(qraf_engine* e, int32_t n, const int32_t* seq_ids, const ui
     e->n_pending = 0;
     const double t0 = now_us();
     QH_CHECK_HIP(hipStreamSynchronize(e->stream));  // also completes a logits copy into pageable memory
+    e->stats.wait_us += now_us() - t0;
+    if (next_tokens && p.n_tok) memcpy(next_tokens, e->h_amax[p.slot], (size_t)p.n_tok * 4);
+    return QRAF_HIP_OK;
+}
+
+// One step whose rows are the nodes of trees of drafted tokens.
+int qraf_engine_step_tree(qraf_engine* e, int32_t n, const int32_t* seq_ids, const uint32_t* tokens, const int32_t* parents,
+                          const int32_t* positions, const uint8_t* want_logits, float* logits, uint32_t* next_tokens) {
+    clear_error();
+    QH_REQUIRE(e && seq_ids && tokens && parents && positions, QRAF_HIP_ERR_INVALID, "step_tree: null argument");
+    QH_REQUIRE(e->n_pending == 0, QRAF_HIP_ERR_STATE, "step_tree: %d asynchronous steps not collected", e->n_pending);
+    QH_REQUIRE(n > 0 && n <= (int32_t)e->o.max_batch, QRAF_HIP_ERR_INVALID, "step_tree: %d rows (max_batch %u)", n,
+               e->o.max_batch);
+    for (int i = 0, first = 0; i < n; i++) {
+        if (i > 0 && seq_ids[i] != seq_ids[i - 1]) {
+            first = i;
+            for (int k = 0; k < i; k++)
+                QH_REQUIRE(seq_ids[k] != seq_ids[i], QRAF_HIP_ERR_INVALID,
+                           "step_tree: rows %d and %d of sequence %d do not lie side by side", k, i, seq_ids[i]);
+        }
+        QH_REQUIRE(i - first < 64, QRAF_HIP_ERR_INVALID, "step_tree: sequence %d has more than 64 nodes", seq_ids[i]);
+        QH_REQUIRE(i == first ? parents[i] == -1 : parents[i] >= first && parents[i] < i, QRAF_HIP_ERR_INVALID,
+                   "step_tree: row %d of sequence %d, whose rows begin at %d, has parent %d", i, seq_ids[i], first, parents[i]);
+        QH_REQUIRE(seq_ids[i] < 0 || seq_ids[i] >= (int32_t)e->pen_slot.size() || e->pen_slot[seq_ids[i]] < 0,
+                   QRAF_HIP_ERR_STATE, "step_tree: sequence %d counts its tokens for a repetition penalty", seq_ids[i]);
+    }
+    QH_TRY(step_issue(e, n, seq_ids, tokens, nullptr, positions, want_logits, logits, next_tokens != nullptr, parents));
+    const qraf_engine::Pending p = e->pending[0];
+    e->n_pending = 0;
+    const double t0 = now_us();
+    QH_CHECK_HIP(hipStreamSynchronize(e->stream));
     e->stats.wait_us += now_us() - t0;
     if (next_tokens && p.n_tok) memcpy(next_tokens, e->h_amax[p.slot], (size_t)p.n_tok * 4);
     return QRAF_HIP_OK;
@@ -1590,12 +1692,11 @@ int qraf_engine_get_stats(qraf_engine* e, qraf_engine_stats* out, int32_t reset)
 }
 
 // Sampler::apply_repetition_penalty + Sampler::sample on the last step's
-// logit rows (sampler.cpp:37-128), where they lie in HBM.
-int qraf_engine_sample(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sampling_params* p,
-                       const uint32_t* recent, const int32_t* counts, int32_t stride, const float* uniforms,
-                       uint32_t* tokens) {
-    clear_error();
-    QH_REQUIRE(e && p && tokens && rows > 0 && row0 >= 0, QRAF_HIP_ERR_INVALID, "sample: bad arguments");
+// logit rows (sampler.cpp:37-128), where they lie in HBM: their tokens to *tokens
+// on the device.  extra: bytes of staging behind them, at *rest.
+static int sample_rows(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sampling_params* p, const uint32_t* recent,
+                       const int32_t* counts, int32_t stride, const float* uniforms, uint32_t** tokens, size_t extra,
+                       uint8_t** rest) {
     QH_REQUIRE(row0 + rows <= e->last_logit_rows, QRAF_HIP_ERR_STATE,
                "sample: rows %d..%d, the last step left %d logit rows", row0, row0 + rows - 1, e->last_logit_rows);
     QH_REQUIRE(e->last_logits_kept, QRAF_HIP_ERR_STATE,
@@ -1606,7 +1707,7 @@ int qraf_engine_sample(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sa
     QH_REQUIRE(greedy || uniforms, QRAF_HIP_ERR_INVALID, "sample: temperature %g needs uniforms", p->temperature);
     const size_t rb = ((size_t)rows * 4 + 255) / 256 * 256;
     const size_t rec = pen ? ((size_t)rows * stride * 4 + 255) / 256 * 256 : 0;
-    const size_t need = 3 * rb + rec;  // tokens, uniforms, counts, recent
+    const size_t need = 3 * rb + rec + extra;  // tokens, uniforms, counts, recent
     if (need > e->samp_cap) {
         const size_t cap = std::max(need, (size_t)1 << 20);
         QH_TRY(ealloc(e, (void**)&e->samp, cap));  // held until the engine is destroyed
@@ -1630,7 +1731,51 @@ int qraf_engine_sample(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sa
     QH_TRY(launch_sample(e->logits + (size_t)row0 * e->c.vocab_size, rows, (int)e->c.vocab_size, *p,
                          pen ? d_rec : nullptr, pen ? d_cnt : nullptr, stride, greedy ? nullptr : d_uni, d_tok,
                          e->sort_ws, e->sort_cap, s));
-    QH_CHECK_HIP(hipMemcpyAsync(tokens, d_tok, (size_t)rows * 4, hipMemcpyDeviceToHost, s));
+    *tokens = d_tok;
+    if (rest) *rest = e->samp + 3 * rb + rec;
+    return QRAF_HIP_OK;
+}
+
+int qraf_engine_sample(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sampling_params* p,
+                       const uint32_t* recent, const int32_t* counts, int32_t stride, const float* uniforms,
+                       uint32_t* tokens) {
+    clear_error();
+    QH_REQUIRE(e && p && tokens && rows > 0 && row0 >= 0, QRAF_HIP_ERR_INVALID, "sample: bad arguments");
+    uint32_t* d_tok = nullptr;
+    QH_TRY(sample_rows(e, row0, rows, p, recent, counts, stride, uniforms, &d_tok, 0, nullptr));
+    QH_CHECK_HIP(hipMemcpyAsync(tokens, d_tok, (size_t)rows * 4, hipMemcpyDeviceToHost, e->stream));
+    QH_CHECK_HIP(hipStreamSynchronize(e->stream));
+    return QRAF_HIP_OK;
+}
+
+// The last step's trees: a token sampled behind every node, the paths along them, and their keys and values moved to
+// where the sequences go on.
+int qraf_engine_accept_tree(qraf_engine* e, const qraf_sampling_params* p, const uint32_t* recent, const int32_t* counts,
+                            int32_t stride, const float* uniforms, int32_t* accepted, uint32_t* tokens) {
+    clear_error();
+    QH_REQUIRE(e && p && accepted && tokens, QRAF_HIP_ERR_INVALID, "accept_tree: null argument");
+    QH_REQUIRE(e->n_pending == 0, QRAF_HIP_ERR_STATE, "accept_tree: %d asynchronous steps not collected", e->n_pending);
+    QH_REQUIRE(e->tree_nodes > 0, QRAF_HIP_ERR_STATE,
+               "accept_tree: the last step was no qraf_engine_step_tree with the logits of all its rows, or its trees were "
+               "accepted before");
+    const int n = e->tree_nodes, seqs = e->tree_seqs, at = e->tree_n, MP = e->max_pages;
+    const size_t rb = ((size_t)n * 4 + 255) / 256 * 256;
+    uint32_t* d_pick = nullptr;
+    uint8_t* rest = nullptr;
+    QH_TRY(sample_rows(e, 0, n, p, recent, counts, stride, uniforms, &d_pick, 3 * rb, &rest));
+    e->tree_nodes = 0;  // (the cache moves)
+    int32_t *d_acc = (int32_t*)rest, *d_path = (int32_t*)(rest + rb);
+    uint32_t* d_tok = (uint32_t*)(rest + 2 * rb);
+    const int32_t* d_gpre = e->d_in + 7 * (size_t)at;
+    const int32_t* d_gstart = d_gpre + at;
+    const int32_t* d_ptab = d_gstart + at + 1;
+    const int32_t* d_parent = d_ptab + (size_t)at * MP + 2 * (size_t)at;
+    hipStream_t s = e->stream;
+    QH_TRY(launch_tree_accept(d_pick, (const uint32_t*)e->d_in, d_parent, d_gstart, seqs, n, d_acc, d_path, d_tok, s));
+    QH_TRY(launch_kv_compact(e->kpool, e->vpool, e->o.kv_dtype, (int)e->c.num_layers, e->layer_kv_bytes, d_ptab, MP, d_gpre,
+                             d_gstart, d_path, seqs, n, (int)e->c.num_kv_heads, e->hd, (int)e->o.page_size, s));
+    QH_CHECK_HIP(hipMemcpyAsync(accepted, d_acc, (size_t)seqs * 4, hipMemcpyDeviceToHost, s));
+    QH_CHECK_HIP(hipMemcpyAsync(tokens, d_tok, (size_t)n * 4, hipMemcpyDeviceToHost, s));
     QH_CHECK_HIP(hipStreamSynchronize(s));
     return QRAF_HIP_OK;
 }
@@ -1686,6 +1831,45 @@ int qraf_engine_probs(qraf_engine* e, int32_t row0, int32_t rows, const qraf_sam
     }
     QH_TRY(launch_sample_probs(e->logits + (size_t)row0 * V, rows, V, *p, rec ? d_rec : nullptr, rec ? d_cnt : nullptr,
                                stride, probs, e->spec, ws, s));
+    QH_CHECK_HIP(hipStreamSynchronize(s));
+    return QRAF_HIP_OK;
+}
+
+// What is said about tokens beside them, of the last step's logit rows.
+int qraf_engine_logprobs(qraf_engine* e, int32_t row0, int32_t rows, const uint32_t* tokens, float* logprobs, int32_t* ranks,
+                         float* entropies, int32_t top, uint32_t* top_tokens, float* top_logprobs) {
+    clear_error();
+    QH_REQUIRE(e && rows > 0 && row0 >= 0, QRAF_HIP_ERR_INVALID, "logprobs: bad arguments");
+    QH_REQUIRE(rows <= e->last_logit_rows - row0, QRAF_HIP_ERR_STATE, "logprobs: rows %d..%lld, the last step left %d logit rows",
+               row0, (long long)row0 + rows - 1, e->last_logit_rows);
+    QH_REQUIRE(e->last_logits_kept, QRAF_HIP_ERR_STATE,
+               "logprobs: the last step was greedy-only and kept no logits (qraf_engine_set_keep_logits)");
+    QH_REQUIRE(tokens || (!logprobs && !ranks), QRAF_HIP_ERR_INVALID, "logprobs: log probabilities and ranks need tokens");
+    QH_REQUIRE(top >= 0 && top <= 64 && top <= (int64_t)e->c.vocab_size, QRAF_HIP_ERR_INVALID,
+               "logprobs: %d alternatives (at most 64, and the vocabulary)", top);
+    QH_REQUIRE(top == 0 || (top_tokens && top_logprobs), QRAF_HIP_ERR_INVALID,
+               "logprobs: %d alternatives need their tokens and log probabilities", top);
+    const int V = (int)e->c.vocab_size;
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    const size_t ws = up(token_logprobs_workspace_bytes(rows, V, top)), rb = up((size_t)rows * 4), tb = up((size_t)rows * top * 4);
+    QH_TRY(spec_storage(e, ws + 4 * rb + 2 * tb));
+    uint8_t* b = (uint8_t*)e->spec + ws;
+    uint32_t* d_t = (uint32_t*)b;
+    float *d_lp = (float*)(b + rb), *d_ent = (float*)(b + 3 * rb), *d_tl = (float*)(b + 4 * rb + tb);
+    int32_t* d_rank = (int32_t*)(b + 2 * rb);
+    uint32_t* d_tt = (uint32_t*)(b + 4 * rb);
+    hipStream_t s = e->stream;
+    if (tokens) QH_CHECK_HIP(hipMemcpyAsync(d_t, tokens, (size_t)rows * 4, hipMemcpyHostToDevice, s));
+    QH_TRY(launch_token_logprobs(e->logits + (size_t)row0 * V, rows, V, tokens ? d_t : nullptr, logprobs ? d_lp : nullptr,
+                                 ranks ? d_rank : nullptr, entropies ? d_ent : nullptr, top, top ? d_tt : nullptr,
+                                 top ? d_tl : nullptr, e->spec, ws, s));
+    if (logprobs) QH_CHECK_HIP(hipMemcpyAsync(logprobs, d_lp, (size_t)rows * 4, hipMemcpyDeviceToHost, s));
+    if (ranks) QH_CHECK_HIP(hipMemcpyAsync(ranks, d_rank, (size_t)rows * 4, hipMemcpyDeviceToHost, s));
+    if (entropies) QH_CHECK_HIP(hipMemcpyAsync(entropies, d_ent, (size_t)rows * 4, hipMemcpyDeviceToHost, s));
+    if (top) {
+        QH_CHECK_HIP(hipMemcpyAsync(top_tokens, d_tt, (size_t)rows * top * 4, hipMemcpyDeviceToHost, s));
+        QH_CHECK_HIP(hipMemcpyAsync(top_logprobs, d_tl, (size_t)rows * top * 4, hipMemcpyDeviceToHost, s));
+    }
     QH_CHECK_HIP(hipStreamSynchronize(s));
     return QRAF_HIP_OK;
 }

@@ -310,6 +310,67 @@ class Engine:
             rec[i, :len(r)] = r
         return rec, cnt, rec.shape[1]
 
+    def step_tree(self, seq_ids, tokens, parents, positions, want_logits=None, logits=False, argmax=True):
+        """One step whose rows are the nodes of trees of drafted tokens (qraf_engine_step_tree): a sequence's rows side
+        by side, the first its last certain token at positions[i] with parent -1, every other a draft behind row
+        parents[i].  Returns as step()."""
+        sid = np.ascontiguousarray(seq_ids, dtype=np.int32)
+        tok = np.ascontiguousarray(tokens, dtype=np.uint32)
+        par = np.ascontiguousarray(parents, dtype=np.int32)
+        pos = np.ascontiguousarray(positions, dtype=np.int32)
+        n = sid.size
+        wl = None if want_logits is None else np.ascontiguousarray(want_logits, dtype=np.uint8)
+        for name, a in (("tokens", tok), ("parents", par), ("positions", pos), ("want_logits", wl)):
+            if a is not None and a.size != n:
+                raise ValueError(f"{name}: {a.size} for {n}")
+        k = n if wl is None else int(np.count_nonzero(wl))
+        lg = np.empty((k, self.vocab), np.float32) if logits else None
+        nx = np.empty(k, np.uint32) if argmax else None
+        call("qraf_engine_step_tree", self.h, n, sid.ctypes.data_as(i32p), tok.ctypes.data_as(u32p),
+             par.ctypes.data_as(i32p), pos.ctypes.data_as(i32p),
+             wl.ctypes.data_as(C.POINTER(C.c_uint8)) if wl is not None else None,
+             lg.ctypes.data_as(fp) if lg is not None else None, nx.ctypes.data_as(u32p) if nx is not None else None)
+        self._trees = [int(np.count_nonzero(sid == s)) for s in dict.fromkeys(sid.tolist())]
+        return lg, nx
+
+    def accept_tree(self, params: SamplingParams, recent=None, uniforms=None):
+        """The trees of the step_tree() before, whose rows all left logits: the tokens that each sequence emits, its
+        accepted drafts and the one behind them; their keys and values move behind its root (qraf_engine_accept_tree).
+        recent, uniforms: a list and a draw for each row."""
+        trees = getattr(self, "_trees", [])
+        n = sum(trees)
+        rec, cnt, stride = self._penalty(params, recent, n)
+        uni = None if uniforms is None else np.ascontiguousarray(uniforms, dtype=np.float32)
+        if uni is not None and uni.size != n:
+            raise ValueError(f"uniforms: {uni.size} for {n}")
+        accepted, out = np.empty(max(len(trees), 1), np.int32), np.empty(max(n, 1), np.uint32)
+        call("qraf_engine_accept_tree", self.h, C.byref(params), rec.ctypes.data_as(u32p) if rec is not None else None,
+             cnt.ctypes.data_as(i32p) if cnt is not None else None, stride,
+             uni.ctypes.data_as(fp) if uni is not None else None, accepted.ctypes.data_as(i32p),
+             out.ctypes.data_as(u32p))
+        at = np.concatenate([[0], np.cumsum(trees)]).astype(int)
+        return [[int(t) for t in out[a:a + k + 1]] for a, k in zip(at, accepted)]
+
+    def logprobs(self, tokens=None, top=0, row0=0, rows=None) -> dict:
+        """What is said about a token beside it, of rows row0.. of the last step's logit rows (qraf_engine_logprobs):
+        "logprobs" and "ranks" of `tokens` (one a row), "entropies", and with top > 0 "top_tokens" and "top_logprobs"
+        [rows][top], the most likely first."""
+        tok = None if tokens is None else np.ascontiguousarray(tokens, dtype=np.uint32)
+        n = rows if rows is not None else (tok.size if tok is not None else 1)
+        if tok is not None and tok.size != n:
+            raise ValueError(f"tokens: {tok.size} for {n}")
+        if n < 0 or top < 0:
+            raise ValueError(f"{top} alternatives of {n} rows")
+        res = {"entropies": np.empty(n, np.float32)}
+        if tok is not None:
+            res["logprobs"], res["ranks"] = np.empty(n, np.float32), np.empty(n, np.int32)
+        if top:
+            res["top_tokens"], res["top_logprobs"] = np.empty((n, top), np.uint32), np.empty((n, top), np.float32)
+        p = lambda k, t: res[k].ctypes.data_as(t) if k in res else None  # noqa: E731
+        call("qraf_engine_logprobs", self.h, row0, n, tok.ctypes.data_as(u32p) if tok is not None else None,
+             p("logprobs", fp), p("ranks", i32p), p("entropies", fp), top, p("top_tokens", u32p), p("top_logprobs", fp))
+        return res
+
     def probs(self, params: SamplingParams, out: int, recent=None, row0=0, rows=1) -> None:
         """The distributions that sample() draws from, for rows row0.. of the last step's logit rows, to the device
         memory at `out` [rows][vocab] (qraf_engine_probs)."""
@@ -507,6 +568,79 @@ class InferenceEngine:
             drafter.close()
         return out
 
+    def score(self, tokens, top: int = 0) -> dict:
+        """Log probabilities of a text: entry i of every array is about tokens[i + 1] behind tokens[:i + 1], as
+        Engine.logprobs gives them ("logprobs", "ranks", "entropies", and "top_tokens" and "top_logprobs")."""
+        if len(tokens) < 2:
+            raise ValueError("a text of two tokens at least")
+        e = self.transformer.engine
+        self.transformer.reset()
+        seq, parts, n = -1, [], len(tokens) - 1
+        try:
+            seq = e.seq_create()
+            for a in range(0, n, e.max_batch):
+                b = min(a + e.max_batch, n)
+                e.step([seq] * (b - a), tokens[a:b], range(a, b), logits=False, argmax=True)
+                parts.append(e.logprobs(tokens[a + 1:b + 1], top))
+        finally:
+            if seq >= 0:
+                e.seq_release(seq)
+        return {k: np.concatenate([p[k] for p in parts]) for k in parts[0]}
+
+    def generate_tree(self, prompt_tokens, max_tokens=256, stop_tokens=(), sampling: SamplingConfig | None = None,
+                      depth: int = 4, width: int = 4, draft: Transformer | None = None, ngram: int = 3):
+        """generate_speculative with a tree of drafts to a step: up to `width` drafted tokens at each of `depth` depths
+        behind the last token.  With a draft model each depth holds the continuations of the one above that it finds
+        most likely (Engine.logprobs), its greedy path among them; without one the tree is what followed the last
+        `ngram` tokens (or fewer) at the latest places where these occurred, up to `width` of them.  A step samples a
+        token behind every node and emits the path along them (Engine.accept_tree), so tokens are generate_tokens' when
+        greedy, as far as rows of one step round as steps of one row do, and distributed as its tokens are when
+        sampled.  The engines' max_batch has to hold depth * width + 1 rows, of which there are at most 64."""
+        if len(prompt_tokens) == 0:
+            raise ValueError("empty prompt")
+        e = self.transformer.engine
+        if depth < 0 or width < 1 or depth * width + 1 > min(64, e.max_batch):
+            raise ValueError(f"{depth} x {width} drafts and the last token: at most {min(64, e.max_batch)} rows")
+        if draft is not None and draft.engine.vocab != e.vocab:
+            raise ValueError("the draft model has another vocabulary")
+        if draft is not None and depth * width + 1 > draft.engine.max_batch:
+            raise ValueError(f"the draft model's steps hold {draft.engine.max_batch} rows")
+        if draft is not None and width > 64:
+            raise ValueError(f"{width} alternatives of a node (at most 64)")
+        if sampling is None:
+            sampling = SamplingConfig(temperature=0.0, top_k=0, top_p=1.0, repetition_penalty=1.0, deterministic=True)
+        sampler = Sampler(sampling) if not sampling.greedy else None
+        params = sampling.params()
+        stops = set(stop_tokens) | ({self.eos} if self.eos is not None else set())
+        self.transformer.reset()
+        drafter = _TreeDrafter(draft, depth, width, ngram)
+        history, out, seq = list(prompt_tokens), [], -1
+        try:
+            seq = e.seq_create()
+            for a in range(0, len(history) - 1, e.max_batch):  # the prompt but its last token
+                chunk = history[a:min(a + e.max_batch, len(history) - 1)]
+                e.step([seq] * len(chunk), chunk, range(a, a + len(chunk)), want_logits=[0] * len(chunk), argmax=False)
+            while len(out) < max_tokens:
+                pos = len(history) - 1  # of the last token, not fed yet
+                guess, parents = drafter.propose(history, max(0, min(depth, max_tokens - len(out) - 1)),
+                                                 max(0, e.capacity - pos - 1))
+                rows, paths = [history[-1], *guess], [[]]
+                for t, up in zip(guess, parents):
+                    paths.append(paths[up] + [t])
+                e.step_tree([seq] * len(rows), rows, [-1, *parents], [pos] * len(rows))
+                recent = [history + p for p in paths] if params.repetition_penalty != 1.0 else None
+                got = e.accept_tree(params, recent, None if sampler is None else sampler.uniforms(len(rows)))[0]
+                for t in got:
+                    if t in stops:
+                        return out
+                    out.append(t)
+                    history.append(t)
+        finally:
+            if seq >= 0:
+                e.seq_release(seq)
+            drafter.close()
+        return out
+
     @staticmethod
     def _penalised_greedy_pipelined(e, seq, prompt, max_tokens, stops, penalty):
         e.set_repetition_penalty(seq, penalty)
@@ -584,6 +718,85 @@ class _Drafter:
             guess.append(int(e.sample(once, None, [self.sampler.uniform()], rows=1)[0]))
         self.held = history + guess[:-1]
         return guess, self.q.ptr if self.q is not None and guess else None
+
+
+class _TreeDrafter:
+    """Trees of drafted tokens: a model's most likely continuations, or what followed the last tokens before."""
+
+    def __init__(self, model: Transformer | None, depth, width, ngram):
+        self.model, self.depth, self.width, self.ngram = model, depth, width, ngram
+        self.seq, self.held = -1, []
+        if model is not None:
+            self.seq = model.engine.seq_create()
+
+    def close(self):
+        if self.seq >= 0:
+            self.model.engine.seq_release(self.seq)
+            self.seq = -1
+
+    def propose(self, history, depth, most):
+        """At most `most` tokens in `depth` depths behind `history`, and the parent of each: 0 for the last token of
+        the history, i + 1 for token i."""
+        if depth <= 0 or most <= 0:
+            return [], []
+        return self._from_text(history, depth, most) if self.model is None else self._from_model(history, depth, most)
+
+    def _from_text(self, history, depth, most):
+        guess, parents, child, found = [], [], {}, 0
+        for n in range(min(self.ngram, len(history) - 1), 0, -1):
+            tail = history[-n:]
+            for at in range(len(history) - n - 1, -1, -1):  # the latest occurrence first
+                if history[at:at + n] != tail:
+                    continue
+                up = 0
+                for t in history[at + n:at + n + depth]:
+                    if (up, t) not in child:
+                        if len(guess) == most:
+                            return guess, parents
+                        guess.append(t)
+                        parents.append(up)
+                        child[up, t] = len(guess)
+                    up = child[up, t]
+                found += 1
+                if found == self.width:
+                    return guess, parents
+            if found:
+                break
+        return guess, parents
+
+    def _from_model(self, history, depth, most):
+        e, pos = self.model.engine, len(history) - 1
+        if pos >= e.capacity:
+            return [], []  # the draft model's cache ends here
+        most = min(most, e.capacity - pos - 1)
+        same = 0  # positions of the draft's cache that still hold this history
+        while same < min(len(self.held), pos) and self.held[same] == history[same]:
+            same += 1
+        for a in range(same, pos, e.max_batch):
+            chunk = history[a:min(a + e.max_batch, pos)]
+            e.step([self.seq] * len(chunk), chunk, range(a, a + len(chunk)), want_logits=[0] * len(chunk), argmax=False)
+        # of the nodes, the last token's first; those of the depth above; the end of the greedy path, which is always kept
+        guess, parents, weight, level, greedy = [], [], [0.0], [0], 0
+        top = min(self.width, e.vocab)
+        for _ in range(depth):
+            rows = [history[-1], *guess]
+            want = [int(i in level) for i in range(len(rows))]
+            e.step_tree([self.seq] * len(rows), rows, [-1, *parents], [pos] * len(rows), want)
+            alt = e.logprobs(top=top, rows=len(level))
+            best = sorted(((up != greedy or k > 0, -weight[up] - float(lp), up, int(t)) for up, ts, lps in
+                           zip(level, alt["top_tokens"], alt["top_logprobs"]) for k, (t, lp) in enumerate(zip(ts, lps))
+                           if lp > -np.inf))[:min(self.width, most - len(guess))]
+            level = []
+            for other, less, up, t in sorted(best, key=lambda x: x[2]):
+                guess.append(t)
+                parents.append(up)
+                weight.append(-less)
+                level.append(len(guess))
+                greedy = greedy if other else len(guess)
+            if not level:
+                break
+        self.held = list(history)
+        return guess, parents
 
 
 @dataclass
