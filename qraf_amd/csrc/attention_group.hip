@@ -396,6 +396,15 @@ __device__ __forceinline__ int last_at(const int* v, int n, int x) {
     }
     return lo;
 }
+// the same of two numbers at once
+__device__ __forceinline__ void last_at(const int* v, int n, int x0, int x1, int& at0, int& at1) {
+    at0 = at1 = 0;
+    for (int step = 1 << (31 - __clz(n)); step; step >>= 1) {
+        const int m0 = at0 + step, m1 = at1 + step, v0 = v[min(m0, n - 1)], v1 = v[min(m1, n - 1)];
+        at0 = m0 < n && v0 <= x0 ? m0 : at0;
+        at1 = m1 < n && v1 <= x1 ? m1 : at1;
+    }
+}
 // the same by a whole wave, n <= 4096, of entries' bits in `mask`: two reads instead of one per halving
 __device__ __forceinline__ int wave_last_at(const int* v, int n, int x, int mask = -1) {
     const int lane = threadIdx.x & 63, step = (n + 63) >> 6;
@@ -462,12 +471,17 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     lds_sync();
     p.np = min(p.jb[a.groups], a.job_cap);
     const int jobs = p.np + a.tails;
-    for (int r = tid; r < a.n; r += GTH) {
-        if (r < p.gs[0] || r >= p.gs[a.groups]) continue;
-        const int g = last_at(p.gs, a.groups, r), all = (p.gs[g + 1] - p.gs[g]) * a.G;
+    const int r_first = p.gs[0], r_end = p.gs[a.groups];
+    int group[2];  // of rows tid and tid + GTH
+    last_at(p.gs, a.groups, max(tid, r_first), max(tid + GTH, r_first), group[0], group[1]);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int r = tid + k * GTH, g = group[k];
+        if (r >= a.n || r < r_first || r >= r_end) continue;
+        const int all = (p.gs[g + 1] - p.gs[g]) * a.G;
         int ctx = p.ctx[r], pre = p.pre[g];
         if (TREE) {
-            ctx = p.ctx[r] = mask_end(below_ctx(a, masks[r >= GTH], pre), pre);
+            ctx = p.ctx[r] = mask_end(below_ctx(a, masks[k], pre), pre);
             pre = ctx;
         }
         const int c0 = (r - p.gs[g]) * a.G, b1 = (c0 + a.G - 1) / BLK;
@@ -487,8 +501,17 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
             all = (unsigned)wave_sum(jobs, [&](int j) { return p.tiles[j] & 0xFFFF; });
             all += (uint64_t)wave_sum(jobs, [&](int j) { return p.tiles[j] >> 16; }) << 16;
         }
+        int few[4];  // up to 256 jobs: a lane's, in registers through the search
+#pragma unroll
+        for (int k = 0; k < 4; k++) few[k] = p.tiles[max(min(tid + 64 * k, jobs - 1), 0)];
         const int lo = shortest_piece(all, full, room, [&](int most) {
             const float per = 1.f / (float)most;
+            if (jobs <= 256 && !longs) {
+                int x = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) x += tid + 64 * k < jobs ? pieces_of(few[k], most, per) : 0;
+                return __builtin_amdgcn_readfirstlane(over_wave(x, [](int u, int v) { return u + v; }));
+            }
             if (longs) return wave_sum(jobs, [&](int j) { return pieces_of_long(p.tiles[j], most); });
             return wave_sum(jobs, [&](int j) { return pieces_of(p.tiles[j], most, per); });
         });
@@ -503,9 +526,12 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         // {first column among the prefix jobs' (-1: outside every group), pieces ahead of its block, of the next, of
         // the one behind}, {which parts, pieces ahead of its tail, behind it}; a row's columns are in two blocks at most
-        for (int r = tid; r < a.n; r += GTH) {
-            const bool in = r >= p.gs[0] && r < p.gs[a.groups];
-            const int g = in ? last_at(p.gs, a.groups, r) : 0;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int r = tid + k * GTH;
+            if (r >= a.n) continue;
+            const bool in = r >= r_first && r < r_end;
+            const int g = in ? group[k] : 0;
             const int pos = p.jb[g] * BLK + (r - p.gs[g]) * a.G, b = in ? pos / BLK : 0, t = p.np + (r >> a.tail_log2);
             a.plan[2 * r] = make_int4(in ? pos : -1, p.upto[min(b, jobs)], p.upto[min(b + 1, jobs)], p.upto[min(b + 2, jobs)]);
             if (TREE) a.plan[2 * r + 1] = make_int4(p.ctx[r] > 0 ? 1 : 0, 0, 0, 0);
@@ -547,7 +573,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
     extern __shared__ __align__(16) float s_dyn[];
-    __shared__ float s_m[GW][32], s_l[GW][32], s_by[BLK], s_qs[BLK];
+    __shared__ float s_m[GW][32], s_l[GW][32], s_qs[BLK];
     // f32 tiles that four waves share: the exponents of K's and V's powers of two, of 8 positions each, or (OWN) of each,
     // where the waves' maxima and sums lie behind the tiles
     int(*const s_kx)[32] = (int(*)[32])s_m;
@@ -555,7 +581,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int OWN = -(1 << 20);  // (scores over it are infinite)
     __shared__ int s_ku[2][4], s_vu[2][4];
     __shared__ unsigned long long s_mask[TREE ? BLK : 1];
-    __shared__ long long s_to[BLK];  // where a column's output goes: an element of out, or ~ one of part_o
+    __shared__ long long s_to[BLK];  // where a column's output goes: an element of out, or ~ a slot of part_o
     constexpr long long NOWHERE = 1ll << 62;
     // [GW][32][HD] the waves' outputs, behind a segment's tiles; 16-byte piece c of a column's row lies at
     // c ^ (column % 16), which spreads a wave's writes over the banks
@@ -1255,6 +1281,9 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     fs = 1.f;
                 }
             } else {
+                // (int8: the wave at its products goes ahead of the one beside it, which widens and weighs meanwhile: 24 trees of
+                // 26 nodes at 8,000 positions 100.8 -> 97.2 us; the others gained nothing)
+                if (I8) __builtin_amdgcn_s_setprio(2);
 #pragma unroll
                 for (int kk = 0; kk < KS; kk++) {
                     f16x8 kf;
@@ -1270,6 +1299,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh, s, 0, 0, 0);
                 }
             }
+            if (I8) __builtin_amdgcn_s_setprio(0);
             float vsc[16];
             if constexpr (I8) {
 #pragma unroll
@@ -1484,6 +1514,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[b], o[d], 0, 0, 0);
                 }
             };
+            if (I8) __builtin_amdgcn_s_setprio(2);
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 float by[8];  // (f32: a half's 8 positions; 8 at a time: registers)
@@ -1493,6 +1524,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 for (int d = 0; d < DT; d++) product(d, b, [&](int k) { return by[k]; });
                 if (F32) __builtin_amdgcn_sched_barrier(0);
             }
+            if (I8) __builtin_amdgcn_s_setprio(0);
             if (TURNS) load_k(tn, go);
             else load_v(tn, go);
             more = go;
@@ -1513,6 +1545,16 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         if (half == 0) {
             s_m[wave][col] = m;
             s_l[wave][col] = l;
+        }
+        // where a column's joined output goes (pieces ahead, less one for each of their jobs: a job's columns are at most
+        // 128, so slots stay apart)
+        if (kw == 0 && half == 0) {
+            const bool any_pre = min(ctx, pre) > 0, any_tail = ctx > pre;
+            const bool alone = DIRECT || (whole && (tail ? !any_pre : any_pre && !any_tail));
+            const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab +
+                                (size_t)BLK * ((here & 0xFFFF) - (here >> 16) + i_of);
+            const bool mine = col < cols, part = mine && !alone && (tail || any_pre);
+            s_to[qt * 32 + col] = mine && alone ? (long long)orow : part ? ~(long long)slot : NOWHERE;
         }
         const float unit = F16 ? 1.f : ldexpf(1.f, -vexp - (F32 ? (int)P_UNIT : 0));
         if (col < cols) {
@@ -1537,33 +1579,6 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             }
         }
         lds_sync();
-        // per column: the waves' factors, and where the joined output goes
-        if (kw == 0 && half == 0) {
-            float mv[GW], lv[GW], M = -INFINITY, L = 0.f;
-#pragma unroll
-            for (int k = 0; k < GW; k++) {
-                const int v = min(qt + wq * k, GW - 1);
-                mv[k] = k < wk ? s_m[v][col] : -INFINITY;
-                lv[k] = k < wk ? s_l[v][col] : 0.f;
-                M = fmaxf(M, mv[k]);
-            }
-            const float mu = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int k = 0; k < GW; k++) {
-                const float f = __builtin_amdgcn_exp2f(mv[k] - mu);
-                L = __builtin_fmaf(lv[k], f, L);
-                if (k < wk) s_m[qt + wq * k][col] = f;
-            }
-            const bool any_pre = min(ctx, pre) > 0, any_tail = ctx > pre;
-            const bool alone = DIRECT || (whole && (tail ? !any_pre : any_pre && !any_tail));
-            // (pieces ahead, less one for each of their jobs: a job's columns are at most 128, so slots stay apart)
-            const size_t slot = (size_t)kvh * a.slots + (tail ? (size_t)a.n * G : 0) + ab +
-                                (size_t)BLK * ((here & 0xFFFF) - (here >> 16) + i_of);
-            const bool mine = col < cols, part = mine && !alone && (tail || any_pre);
-            s_to[qt * 32 + col] = mine && alone ? (long long)orow : part ? ~(long long)(slot * HD) : NOWHERE;
-            s_by[qt * 32 + col] = DIRECT && ctx == 0 ? 0.f : alone ? 1.f / L : 1.f;
-            if (part) a.part_ml[slot] = make_float2(M, L);
-        }
         lanes_again();
         lds_sync();
         auto join = [&](auto wk_c) {
@@ -1574,24 +1589,31 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 const long long to = s_to[c];
                 if (to == NOWHERE) continue;
                 float4 x[WK];
-                float f[WK];
+                float f[WK], M = -INFINITY, L = 0.f;
 #pragma unroll
                 for (int k = 0; k < WK; k++) {
                     x[k] = *(const float4*)(s_o + ((cq + WQ * k) * 32 + ci) * HD + (d ^ 4 * (ci & 15)));
                     f[k] = s_m[cq + WQ * k][ci];
+                    M = fmaxf(M, f[k]);
                 }
+                const float mu = M == -INFINITY ? 0.f : M;
                 float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int k = 0; k < WK; k++) {  // (a wave without positions holds zeros)
+                    f[k] = __builtin_amdgcn_exp2f(f[k] - mu);
+                    L = __builtin_fmaf(s_l[cq + WQ * k][ci], f[k], L);
                     O.x = __builtin_fmaf(x[k].x, f[k], O.x);
                     O.y = __builtin_fmaf(x[k].y, f[k], O.y);
                     O.z = __builtin_fmaf(x[k].z, f[k], O.z);
                     O.w = __builtin_fmaf(x[k].w, f[k], O.w);
                 }
-                const float by = s_by[c];
-                O = make_float4(O.x * by, O.y * by, O.z * by, O.w * by);
-                if (to < 0) *(float4*)(a.part_o + ~to + d) = O;
-                else group_store4(a, to + d, O);
+                if (to < 0) {
+                    *(float4*)(a.part_o + (size_t)~to * HD + d) = O;
+                    if (d == 0) a.part_ml[~to] = make_float2(M, L);
+                } else {
+                    const float by = DIRECT && d_ctx == 0 ? 0.f : 1.f / L;
+                    group_store4(a, to + d, make_float4(O.x * by, O.y * by, O.z * by, O.w * by));
+                }
             }
         };
         if (wk == 2) join(std::integral_constant<int, 2>());
@@ -1605,7 +1627,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
 // whose one part was the output itself is left; one without any is zero.
 template <int HD>
 __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
-    constexpr int DPL = HD / 64;
+    constexpr int DPL = HD / 64, FLIGHT = 8;  // dimensions a lane; parts in flight
     const int r = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (h >= a.H) return;
     const int lane = threadIdx.x & 63, kvh = h / a.G, hh = h - kvh * a.G;
@@ -1636,11 +1658,11 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
     float m = -INFINITY, l = 0.f, O[DPL];  // running, as in the tiles
 #pragma unroll
     for (int k = 0; k < DPL; k++) O[k] = 0.f;
-    for (int i0 = 0; i0 < all; i0 += 8) {  // 8 parts in flight
-        float v[8][DPL];
-        float2 ml[8];
+    for (int i0 = 0; i0 < all; i0 += FLIGHT) {
+        float v[FLIGHT][DPL];
+        float2 ml[FLIGHT];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < FLIGHT; u++) {
             const size_t at = slot(min(i0 + u, all - 1));
             ml[u] = a.part_ml[at];
 #pragma unroll
@@ -1648,13 +1670,13 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
         }
         float mn = m;
 #pragma unroll
-        for (int u = 0; u < 8; u++) mn = i0 + u < all ? fmaxf(mn, ml[u].x) : mn;
+        for (int u = 0; u < FLIGHT; u++) mn = i0 + u < all ? fmaxf(mn, ml[u].x) : mn;
         const float mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
         l *= alpha;
 #pragma unroll
         for (int k = 0; k < DPL; k++) O[k] *= alpha;
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < FLIGHT; u++) {
             const float f = i0 + u < all ? __builtin_amdgcn_exp2f(ml[u].x - mu) : 0.f;
             l = __builtin_fmaf(ml[u].y, f, l);
 #pragma unroll
