@@ -68,25 +68,25 @@ __device__ __forceinline__ uint32_t umin2(uint32_t x, uint32_t y) { return min(x
 struct __attribute__((packed, aligned(4))) Four {
     float v[4];
 };
-// Chunk c of a row, E logits a thread: element u is index chunk_index(c, u); past the row -inf.
-template <int E>
+// Chunk c of a row, E logits of TH threads each: element u is index chunk_index(c, u); past the row -inf.
+template <int E, int TH = STH>
 __device__ __forceinline__ int chunk_index(int c, int t, int u) {
-    return c * (STH * E) + 4 * (t + STH * (u >> 2)) + (u & 3);
+    return c * (TH * E) + 4 * (t + TH * (u >> 2)) + (u & 3);
 }
-template <int E>
+template <int E, int TH = STH>
 __device__ __forceinline__ void load_chunk(const float* l, int V, int c, float (&v)[E]) {
     const int t = threadIdx.x;
-    if ((c + 1) * (STH * E) <= V) {
+    if ((c + 1) * (TH * E) <= V) {
 #pragma unroll
         for (int j = 0; j < E; j += 4) {
-            const Four x = *(const Four*)(l + chunk_index<E>(c, t, j));
+            const Four x = *(const Four*)(l + chunk_index<E, TH>(c, t, j));
 #pragma unroll
             for (int k = 0; k < 4; k++) v[j + k] = x.v[k];
         }
     } else {
 #pragma unroll
         for (int u = 0; u < E; u++) {
-            const int i = chunk_index<E>(c, t, u);
+            const int i = chunk_index<E, TH>(c, t, u);
             const float x = l[min(i, V - 1)];
             v[u] = i < V ? x : -INFINITY;
         }
@@ -107,7 +107,7 @@ __device__ __forceinline__ float2 weights(const float* v, float m) {
 }
 
 // A wave's statistics of its part of a chunk; mine: the lane's largest.
-template <int E>
+template <int E, int TH = STH>
 __device__ __forceinline__ WaveStats wave_stats(const float (&v)[E], int c, uint32_t token, float given, float& mine) {
     mine = -INFINITY;
 #pragma unroll
@@ -125,12 +125,12 @@ __device__ __forceinline__ WaveStats wave_stats(const float (&v)[E], int c, uint
     w.e = over_wave(s.y, add2);
     // a larger logit is ahead, an equal one where it lies ahead
     int ahead = 0;
-    const long long first = (long long)c * (STH * E), end = first + STH * E;
+    const long long first = (long long)c * (TH * E), end = first + TH * E;
     if (given == -INFINITY || (token >= first && token < end)) {
         const unsigned long long key = token_key(logit_key(given), (int)token);
 #pragma unroll
         for (int u = 0; u < E; u++) {
-            const int i = chunk_index<E>(c, threadIdx.x, u);
+            const int i = chunk_index<E, TH>(c, threadIdx.x, u);
             ahead += token_key(logit_key(clean_logit(v[u])), i) > key;
         }
     } else if (token < first) {
@@ -340,41 +340,60 @@ __device__ void write_tops(const LogprobArgs& a, int row, const float* l, TopSha
     }
 }
 
-// ---- rows of up to STH * E logits: one workgroup
-template <int E>
-__global__ __launch_bounds__(STH) void logprobs_small_kernel(LogprobArgs a) {
-    __shared__ TopShared<STH> sh;
-    __shared__ WaveStats s_st[STH / 64];
-    const int row = blockIdx.x, tid = threadIdx.x;
+// ---- rows of up to TH * E logits: one workgroup, and with alternatives a wave more for the sums
+template <int E, int TH>
+__global__ __launch_bounds__(TH + 64) void logprobs_small_kernel(LogprobArgs a) {
+    __shared__ TopShared<TH + 64> sh;
+    __shared__ WaveStats s_st[TH / 64];
+    __shared__ RowSums s_r;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const float* l = a.logits + (size_t)row * a.V;
     const uint32_t token = given_token(a, row);
-    float v[E], mine;
-    load_chunk<E>(l, a.V, 0, v);
-    const float given = given_logit(a, row, token);
-    const WaveStats w = wave_stats<E>(v, 0, token, given, mine);
-    if ((tid & 63) == 0) s_st[tid >> 6] = w;
-    sh.key[tid] = logit_key(mine + 0.f);
-    if (tid == 0) sh.n = 0;
-    __syncthreads();
-    if (a.top == 0) {
-        if (tid < 64) row_sums(a, row, s_st, STH / 64, lane_stats(s_st, STH / 64), token, given);
-        return;
-    }
-    const uint32_t bound = max(bound_of<STH>(sh.key, a.top), KEY_NONE + 1);
-#pragma unroll
-    for (int u = 0; u < E; u++) {
-        const uint32_t k = logit_key(clean_logit(v[u]));
-        if (k >= bound) {
-            const int x = atomicAdd(&sh.n, 1);
-            if (x < LIST) sh.list[x] = token_key(k, chunk_index<E>(0, tid, u));
+    if (tid >= TH) {
+        const float given = given_logit(a, row, token);
+        __syncthreads();
+        const RowSums r = row_sums(a, row, s_st, TH / 64, lane_stats(s_st, TH / 64), token, given);
+        if (tid == TH) s_r = r;
+        __syncthreads();
+    } else {
+        float v[E], mine;
+        load_chunk<E, TH>(l, a.V, 0, v);
+        const float given = given_logit(a, row, token);
+        const WaveStats w = wave_stats<E, TH>(v, 0, token, given, mine);
+        if (lane == 0) s_st[tid >> 6] = w;
+        sh.key[tid] = logit_key(mine + 0.f);
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        if (a.top == 0) {  // (without the wave more)
+            if (tid < 64) row_sums(a, row, s_st, TH / 64, lane_stats(s_st, TH / 64), token, given);
+            return;
         }
+        const uint32_t bound = max(bound_of<TH>(sh.key, a.top), KEY_NONE + 1);
+        if (__any(sh.key[tid] >= bound)) {
+            uint32_t key[E];
+            int all = 0;
+#pragma unroll
+            for (int u = 0; u < E; u++) {
+                key[u] = logit_key(clean_logit(v[u]));
+                all += __popcll(__ballot(key[u] >= bound));
+            }
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.n, all);
+            at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+            for (int u = 0; u < E; u++) {
+                const unsigned long long b = __ballot(key[u] >= bound);
+                if (!b) continue;
+                const int x = at + __popcll(b & ((1ull << lane) - 1));
+                if (key[u] >= bound && x < LIST) sh.list[x] = token_key(key[u], chunk_index<E, TH>(0, tid, u));
+                at += __popcll(b);
+            }
+        }
+        __syncthreads();
     }
-    RowSums r;
-    r = row_sums(a, row, s_st, STH / 64, lane_stats(s_st, STH / 64), token, given);  // (each wave for itself)
-    __syncthreads();
     const bool over = sh.n > LIST;
     __syncthreads();
-    write_tops(a, row, l, sh, over, r);
+    write_tops(a, row, l, sh, over, s_r);
 }
 
 // ---- longer rows: their splits, then a row's join
@@ -525,8 +544,9 @@ int launch_token_logprobs(const float* logits, int rows, int V, const uint32_t* 
                need);
     LogprobArgs a{logits, tokens, logprobs, entropies, top_logprobs, ranks, top_tokens, nullptr, nullptr, V, 1, top, rows};
     if (V <= SMALL) {
-        if (V <= STH * 8) hipLaunchKernelGGL(logprobs_small_kernel<8>, dim3(rows), dim3(STH), 0, s, a);
-        else hipLaunchKernelGGL(logprobs_small_kernel<32>, dim3(rows), dim3(STH), 0, s, a);
+        const int more = top ? 64 : 0;
+        if (V <= STH * 8) hipLaunchKernelGGL((logprobs_small_kernel<8, STH>), dim3(rows), dim3(STH + more), 0, s, a);
+        else hipLaunchKernelGGL((logprobs_small_kernel<16, 512>), dim3(rows), dim3(512 + more), 0, s, a);
         QH_CHECK_HIP(hipGetLastError());
         return QRAF_HIP_OK;
     }
