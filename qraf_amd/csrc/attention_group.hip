@@ -413,18 +413,21 @@ __device__ __forceinline__ int wave_last_at(const int* v, int n, int x, int mask
     i = b + lane;
     return b + __popcll(__ballot(lane < step && i < n && (v[min(i, n - 1)] & mask) <= x)) - 1;
 }
+// x summed over the lanes up to each: rows of 16, then rows 1 and 3, then 2 and 3
+__device__ __forceinline__ int over_lanes_ahead(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+}
 // v[0..n) to its exclusive prefix sums, v[n] the sum, by one wave
 __device__ __forceinline__ void wave_prefix_sum(int* v, int n) {
     const int lane = threadIdx.x & 63, per = (n + 63) >> 6, i0 = min(n, lane * per), i1 = min(n, i0 + per);
     int sum = 0;
     for (int i = i0; i < i1; i++) sum += v[i];
-    int inc = sum;  // over the lanes: rows of 16, then rows 1 and 3, then 2 and 3
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xF, 0xF, false);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xF, 0xF, false);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xF, 0xF, false);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xF, 0xF, false);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xA, 0xF, false);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xC, 0xF, false);
+    const int inc = over_lanes_ahead(sum);
     int run = inc - sum;
     for (int i = i0; i < i1; i++) {
         const int x = v[i];
@@ -541,6 +544,56 @@ __device__ void group_plan(const GroupArgs& a, GroupPlan& p, int shares) {
     }
 }
 
+// ---- the plan of trees of up to 64 sequences: a lane to a sequence, by each wave for itself, in registers.  A sequence's
+// blocks but the last are alike; its positions are taken to end where a mask's highest bit may lie (tiles that no row
+// attends to are skipped), so the masks are not waited for.  No barrier, a read, 3,300 cycles to the piece where the plan
+// in LDS takes 9,000 to 12,000 (1 to 48 sequences).
+struct LanePlan {
+    int first, end, base;  // rows, cache
+    int blocks, tiles, last;    // blocks of columns; tiles of each, of the last
+    int pieces, last_pieces;    // of those
+    int upto;                   // pieces ahead of the sequence's, and from bit 16 on its blocks ahead
+    int all;                    // pieces of all sequences
+};
+__device__ __forceinline__ LanePlan lane_plan(const GroupArgs& a, int shares) {
+    const int s = threadIdx.x & 63;
+    LanePlan p;
+    // (ascending, whatever is given: no two sequences share a row, and past the last there are none)
+    int first = group_start(a, min(s, a.groups));
+    first = max(first, __builtin_amdgcn_update_dpp(0, first, 0x111, 0xF, 0xF, false));
+    first = max(first, __builtin_amdgcn_update_dpp(0, first, 0x112, 0xF, 0xF, false));
+    first = max(first, __builtin_amdgcn_update_dpp(0, first, 0x114, 0xF, 0xF, false));
+    first = max(first, __builtin_amdgcn_update_dpp(0, first, 0x118, 0xF, 0xF, false));
+    first = max(first, __builtin_amdgcn_update_dpp(0, first, 0x142, 0xA, 0xF, false));
+    p.first = max(first, __builtin_amdgcn_update_dpp(0, first, 0x143, 0xC, 0xF, false));
+    p.end = __shfl_down(p.first, 1);
+    if (s == 63) p.end = max(p.first, group_start(a, a.groups));
+    p.base = prefix_len(a, min(s, a.groups - 1));
+    const int cols = (p.end - p.first) * a.G, to = min(p.base + 64, a.max_ctx);
+    p.blocks = (cols + BLK - 1) / BLK;
+    p.tiles = p.blocks > 1 ? tiles_of(to, BLK) : 0;
+    p.last = p.blocks > 0 ? tiles_of(to, cols - BLK * (p.blocks - 1)) : 0;
+    auto sum = [](int x) { return __builtin_amdgcn_readfirstlane(over_wave(x, [](int u, int v) { return u + v; })); };
+    const bool longs = __any(max(p.tiles, p.last) >= LONG_JOB);
+    // (at most 1,088 blocks, of fewer than LONG_JOB tiles or of 2^24)
+    const uint64_t mine = (uint64_t)max(p.blocks - 1, 0) * p.tiles + p.last;
+    const uint64_t all = longs ? (unsigned)sum((int)(mine & 0xFFFF)) + ((uint64_t)(unsigned)sum((int)(mine >> 16)) << 16)
+                               : (unsigned)sum((int)mine);
+    const int full = sum(p.blocks), room = piece_room(full, shares);
+    auto cut = [&](int most, int& pieces, int& last) {
+        const float per = 1.f / (float)most;
+        pieces = longs ? pieces_of_long(p.tiles, most) : pieces_of(p.tiles, most, per);
+        last = longs ? pieces_of_long(p.last, most) : pieces_of(p.last, most, per);
+        return max(p.blocks - 1, 0) * pieces + last;
+    };
+    int x, y;
+    const int most = shortest_piece(all, full, room, [&](int m) { return sum(cut(m, x, y)); });
+    const int own = cut(most, p.pieces, p.last_pieces) | p.blocks << 16, inc = over_lanes_ahead(own);
+    p.upto = inc - own;
+    p.all = __builtin_amdgcn_readlane(inc, 63) & 0xFFFF;
+    return p;
+}
+
 // ---- a wave's K and V of one tile
 template <int HD, int KV>
 struct GroupTile;
@@ -568,7 +621,8 @@ constexpr int tile_floats(int hd) { return GW * 32 * hd; }
 
 // TREE: rows attend to their sequence's cache and to the positions behind it that their masks name, all of them shared
 // (the prefix ends where their attention does): tiles that reach behind the cache go by bits.
-template <int HD, int KV, bool DIRECT, bool TREE>
+// LANES: the plan is lane_plan's.
+template <int HD, int KV, bool DIRECT, bool TREE, bool LANES>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
     constexpr bool F32 = KV == (int)DT_F32, F16 = KV == (int)DT_F16, I8 = KV == (int)DT_I8;
@@ -591,6 +645,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int QB = 33, QT = 2 * KS * QB, QHI = 4 * QT;
     uint4 *s_qlo = (uint4*)s_dyn, *s_qhi = s_qlo + QHI;
     GroupPlan plan;
+    unsigned long long* const masks = (unsigned long long*)(s_dyn + tile_floats(HD));  // LANES: all rows'
+    LanePlan lp;
     plan.tiles = (int*)(s_dyn + tile_floats(HD));
     plan.upto = plan.tiles + a.job_cap + a.tails;
     plan.jb = plan.upto + a.job_cap + a.tails + 1;
@@ -637,22 +693,46 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             d_first = g;  // (whose row of the page table is read)
         }
         d_tiles = (TREE ? d_ctx + 31 : min(d_ctx, d_pre) + 31) >> 5;
+    } else if constexpr (LANES) {
+        const unsigned long long m0 = a.masks[min(tid, a.n - 1)], m1 = a.masks[min(tid + GTH, a.n - 1)];
+        lp = lane_plan(a, gridDim.x);
+        if (tid < a.n) masks[tid] = m0;
+        if (tid + GTH < a.n) masks[tid + GTH] = m1;
+        pieces = lp.all;
+        lds_sync();
     } else {
         group_plan<TREE>(a, plan, gridDim.x);
         jobs = plan.np + a.tails;
         pieces = plan.upto[jobs] & 0xFFFF;
     }
+    // (trees) behind the last position that row r of a sequence with `cache` positions attends to
+    auto row_end = [&](int r, int cache) { return LANES ? mask_end(below_ctx(a, masks[r], cache), cache) : plan.ctx[r]; };
 
     for (int piece = w; piece < pieces; piece += gridDim.x) {
         lanes_again();
         int j = 0, here = 0, i_of = 0, ja = 0, jend = 0;
         bool whole = true;  // tiles [ja, jend) of the job
+        int l_seq = 0, l_first = 0, l_end = 0, l_block = 0;  // LANES: the piece's sequence, its rows, the block
         if constexpr (!DIRECT) {
-            j = __builtin_amdgcn_readfirstlane(wave_last_at(plan.upto, jobs, piece, 0xFFFF));
-            here = __builtin_amdgcn_readfirstlane(plan.upto[j]);
-            const int next = __builtin_amdgcn_readfirstlane(plan.upto[j + 1]);
-            const int tiles = __builtin_amdgcn_readfirstlane(plan.tiles[j]);
-            const int n_of = (next & 0xFFFF) - (here & 0xFFFF);
+            int tiles, n_of;
+            if constexpr (LANES) {
+                const int at = lp.upto & 0xFFFF, of = max(lp.blocks - 1, 0) * lp.pieces + lp.last_pieces;
+                l_seq = __ffsll((unsigned long long)__ballot(piece >= at && piece < at + of)) - 1;
+                auto its = [&](int x) { return __builtin_amdgcn_readlane(x, l_seq); };
+                const int upto = its(lp.upto), k = its(lp.pieces), last = its(lp.blocks) - 1, local = piece - (upto & 0xFFFF);
+                l_block = last > 0 ? min((int)(((float)local + 0.5f) / (float)k), last) : 0;
+                here = upto + l_block * (k | 1 << 16);
+                n_of = l_block < last ? k : its(lp.last_pieces);
+                tiles = l_block < last ? its(lp.tiles) : its(lp.last);
+                l_first = its(lp.first);
+                l_end = its(lp.end);
+            } else {
+                j = __builtin_amdgcn_readfirstlane(wave_last_at(plan.upto, jobs, piece, 0xFFFF));
+                here = __builtin_amdgcn_readfirstlane(plan.upto[j]);
+                const int next = __builtin_amdgcn_readfirstlane(plan.upto[j + 1]);
+                tiles = __builtin_amdgcn_readfirstlane(plan.tiles[j]);
+                n_of = (next & 0xFFFF) - (here & 0xFFFF);
+            }
             i_of = piece - (here & 0xFFFF);
             const int each = (int)((unsigned)tiles / (unsigned)n_of), odd = tiles - each * n_of;  // `odd` pieces of one more
             ja = i_of * each + min(i_of, odd);
@@ -661,7 +741,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         }
 
         // ---- the wave's place: qt of wq waves side by side along the job's columns, kw of wk along the positions
-        bool tail = !DIRECT && j >= plan.np;
+        bool tail = !DIRECT && !LANES && j >= plan.np;
         int g, trow, first, cols, wq;  // group; the row whose table is read; first column (among all rows'), columns
         int bfirst = 0, bcols = 0;     // those of the workgroup (of a prefix)
         if constexpr (DIRECT) {
@@ -683,10 +763,10 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             first = trow * G + c0;
             cols = in && plan.ctx[trow] > plan.pre[g] ? min(32, G - c0) : 0;
         } else {
-            g = wave_last_at(plan.jb, a.groups, j);
-            const int b = j - plan.jb[g];
-            trow = plan.gs[g];
-            cols = bcols = min(BLK, (plan.gs[g + 1] - trow) * G - BLK * b);
+            g = LANES ? l_seq : wave_last_at(plan.jb, a.groups, j);
+            const int b = LANES ? l_block : j - plan.jb[g];
+            trow = LANES ? l_first : plan.gs[g];
+            cols = bcols = min(BLK, ((LANES ? l_end : plan.gs[g + 1]) - trow) * G - BLK * b);
             wq = waves_over(cols);
             const int c0 = 32 * (wave & (wq - 1));
             bfirst = trow * G + BLK * b;
@@ -696,7 +776,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         wq = __builtin_amdgcn_readfirstlane(wq);
         cols = __builtin_amdgcn_readfirstlane(max(cols, 0));
         const int wk = GW / wq, qt = wave & (wq - 1), kw = wave / wq;
-        const int cache = __builtin_amdgcn_readfirstlane(DIRECT ? d_pre : plan.pre[g]);  // (trees: ahead of the masks)
+        const int cache = __builtin_amdgcn_readfirstlane(DIRECT ? d_pre : LANES ? __builtin_amdgcn_readlane(lp.base, l_seq) : plan.pre[g]);  // (trees: ahead of the masks)
         const int pre = TREE ? INT_MAX : cache, base = tail ? tail_base(pre) : 0;
         int lo = tail ? pre : 0;
         // the page table through scalar loads: an id does not wait for vector loads ahead of it
@@ -710,7 +790,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         const int ab = min(first + min(col, max(cols - 1, 0)), a.n * G - 1);
         const int r = DIRECT ? w : (int)(((float)ab + 0.5f) * inv_g);  // (ab < 2^17: exact)
         const size_t orow = ((size_t)r * a.H + kvh * G + (ab - r * G)) * HD;
-        const int ctx = DIRECT ? d_ctx : plan.ctx[r];
+        const int ctx = DIRECT ? d_ctx : row_end(r, cache);
         int lim = cols == 0 ? 0 : tail ? ctx : min(ctx, pre);
         // behind the last position that some of the wave's columns attends to
         int kend = __builtin_amdgcn_readfirstlane(DIRECT ? lim : over_wave(lim, imax2)), klast = max(kend - 1, 0);
@@ -847,7 +927,8 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             }
         };
         const unsigned long long mask_of =
-            TREE ? row_mask(a, DIRECT ? w : (int)(((float)(bfirst + min(tid % BLK, bcols - 1)) + 0.5f) * inv_g), cache) : 0;
+            LANES ? below_ctx(a, masks[(int)(((float)(bfirst + min(tid % BLK, bcols - 1)) + 0.5f) * inv_g)], cache)
+            : TREE ? row_mask(a, DIRECT ? w : (int)(((float)(bfirst + min(tid % BLK, bcols - 1)) + 0.5f) * inv_g), cache) : 0;
         if (DIRECT || wq == 1) stage_q(std::integral_constant<int, 1>());
         else if (wq == 2) stage_q(std::integral_constant<int, 2>());
         else stage_q(std::integral_constant<int, 4>());
@@ -913,7 +994,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 int kl = 0;
 #pragma unroll
                 for (int c = 0; c < BLK; c += 64)
-                    kl = max(kl, plan.ctx[(int)(((float)(bfirst + min(lane + c, bcols - 1)) + 0.5f) * inv_g)]);
+                    kl = max(kl, row_end((int)(((float)(bfirst + min(lane + c, bcols - 1)) + 0.5f) * inv_g), cache));
                 kl = max(min(__builtin_amdgcn_readfirstlane(over_wave(kl, imax2)), pre), 1) - 1;
                 typedef float vpart __attribute__((ext_vector_type(NP)));
                 std::conditional_t<F32, float[NP][8], int> kx;
@@ -1621,6 +1702,26 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         else join(std::integral_constant<int, 8>());
         lds_sync();  // s_o, s_m, s_l are written again
     }
+    // where each row's parts lie, for the join: as group_plan writes it, by the workgroup that has least to do
+    if (LANES && blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {
+        int* seq = (int*)s_dyn;  // [7][64]
+        if (tid < 64) {
+            const int of[7] = {lp.first, lp.end, lp.base, lp.blocks, lp.pieces, lp.last_pieces, lp.upto};
+#pragma unroll
+            for (int k = 0; k < 7; k++) seq[64 * k + tid] = of[k];
+        }
+        lds_sync();
+        for (int r = tid; r < a.n; r += GTH) {
+            const int* q = seq + last_at(seq, a.groups, r);
+            const bool in = r >= q[0] && r < q[64];
+            const int pos = (r - q[0]) * G, b = pos / BLK, block = q[256] | 1 << 16;
+            auto upto = [&](int k) {
+                return q[384] + (k < q[192] ? k * block : (q[192] - 1) * block + (q[320] | 1 << 16));
+            };
+            a.plan[2 * r] = make_int4(in ? pos : -1, upto(b), upto(b + 1), upto(b + 2));
+            a.plan[2 * r + 1] = make_int4(in && row_end(r, q[128]) > 0 ? 1 : 0, 0, 0, 0);
+        }
+    }
 }
 
 // The parts of a column, joined in order: one wave per (row, query head).  A row
@@ -1732,12 +1833,13 @@ static bool group_direct(int n, int H, int Hkv, uint32_t kv_dtype, int max_ctx) 
 }
 
 int group_attention_init() {
-#define QH_GROUP_LDS1(HDv, KVv, DIRECTv, TREEv)                                                            \
-    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, DIRECTv, TREEv>,       \
+#define QH_GROUP_LDS1(HDv, KVv, DIRECTv, TREEv, LANESv)                                                   \
+    QH_CHECK_HIP(hipFuncSetAttribute((const void*)group_tile_kernel<HDv, (int)KVv, DIRECTv, TREEv, LANESv>, \
                                      hipFuncAttributeMaxDynamicSharedMemorySize, (TREEv ? 154 : 155) * 1024));
 #define QH_GROUP_LDS(HDv, KVv)                                                                             \
-    QH_GROUP_LDS1(HDv, KVv, false, false) QH_GROUP_LDS1(HDv, KVv, true, false)                            \
-    QH_GROUP_LDS1(HDv, KVv, false, true) QH_GROUP_LDS1(HDv, KVv, true, true)
+    QH_GROUP_LDS1(HDv, KVv, false, false, false) QH_GROUP_LDS1(HDv, KVv, true, false, false)              \
+    QH_GROUP_LDS1(HDv, KVv, false, true, false) QH_GROUP_LDS1(HDv, KVv, true, true, false)                \
+    QH_GROUP_LDS1(HDv, KVv, false, true, true)
     QH_GROUP_LDS(64, DT_F32) QH_GROUP_LDS(64, DT_F16) QH_GROUP_LDS(64, DT_I8)
     QH_GROUP_LDS(128, DT_F32) QH_GROUP_LDS(128, DT_F16) QH_GROUP_LDS(128, DT_I8)
 #undef QH_GROUP_LDS
@@ -1766,13 +1868,17 @@ static int group_tiles(GroupArgs& a, uint32_t kv_dtype, int hd, void* ws, bool d
     a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
     a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
     const int gx = group_grid(a.Hkv);
-    const size_t lds = group_lds(hd, a.n, a.groups, z);
+    const bool lanes = TREE && a.groups <= 64;
+    const size_t lds = lanes ? (size_t)tile_floats(hd) * 4 + (size_t)a.n * 8 : group_lds(hd, a.n, a.groups, z);
 #define QH_GROUP_TILE(HDv, KVv)                                                                                            \
     if (hd == HDv && kv_dtype == KVv) {                                                                                    \
         if (direct)                                                                                                        \
-            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true, TREE>), dim3(a.n, a.Hkv), dim3(GTH),               \
+            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, true, TREE, false>), dim3(a.n, a.Hkv), dim3(GTH),        \
                                tile_floats(HDv) * 4, st, a);                                                               \
-        else hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false, TREE>), dim3(gx, a.Hkv), dim3(GTH), lds, st, a);  \
+        else if (lanes)                                                                                                    \
+            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false, TREE, TREE>), dim3(gx, a.Hkv), dim3(GTH), lds, st, a); \
+        else                                                                                                               \
+            hipLaunchKernelGGL((group_tile_kernel<HDv, (int)KVv, false, TREE, false>), dim3(gx, a.Hkv), dim3(GTH), lds, st, a); \
     }
     QH_GROUP_TILE(64, DT_F32) QH_GROUP_TILE(64, DT_F16) QH_GROUP_TILE(64, DT_I8)
     QH_GROUP_TILE(128, DT_F32) QH_GROUP_TILE(128, DT_F16) QH_GROUP_TILE(128, DT_I8)

@@ -521,7 +521,8 @@ struct qraf_engine {
     struct StepGraph {
         int n = 0, n_logit_rows = 0, ctx = 0;
         int head = 0;  // 0: no head, 1: logits (and argmax), 2: argmax only
-        bool grouped = false, tree = false;
+        bool grouped = false;
+        int trees = 0;  // sequences of a step of trees, as attention is given them
         uint32_t gen = 0;
         hipGraphExec_t exec = nullptr;
         uint64_t used = 0;
@@ -1074,8 +1075,8 @@ static size_t tree_masks_at(int n, int max_pages) { return ((size_t)n * (12 + ma
 static int tree_workspace(qraf_engine* e) {
     if (e->tree_ws) return QRAF_HIP_OK;
     size_t bytes = 16;
-    for (int n = 1; n <= (int)e->o.max_batch; n++)  // (not monotone: the largest batches take another form)
-        bytes = std::max(bytes, tree_attention_workspace_bytes(n, n, (int)e->c.num_heads, (int)e->c.num_kv_heads, e->hd,
+    for (int n = 1; n <= (int)e->o.max_batch; n++)  // (fewer sequences never need less)
+        bytes = std::max(bytes, tree_attention_workspace_bytes(n, 1, (int)e->c.num_heads, (int)e->c.num_kv_heads, e->hd,
                                                                e->capacity));
     QH_TRY(ealloc(e, &e->tree_ws, bytes));
     e->tree_ws_bytes = bytes;
@@ -1202,7 +1203,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     // Trees: a node is rotated for its depth behind its sequence's cache, lies behind the nodes ahead of it and attends
     // to its parent's nodes and itself.  The page table gets a row for each sequence (its last row's is the whole); pad
     // rows are one more, unused entries empty ones.
-    int tree_seqs = 0;
+    int tree_seqs = 0, trees = 0;
     if (tree) {
         for (int i = 0, first = 0; i < n_pad; i++) {
             if (i == 0 || (i < n ? seq_ids[i] != seq_ids[i - 1] : i == n)) {
@@ -1221,6 +1222,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         }
         for (int q = tree_seqs; q < n_pad; q++) gpre[q] = 0;
         for (int q = tree_seqs; q <= n_pad; q++) gstart[q] = n_pad;
+        trees = std::min((tree_seqs + 15) / 16 * 16, n_pad);  // (steps of nearby numbers share a graph)
         if (n_pad > n_real) tree_seqs--;
     }
     const int n_logit_real = n_logit_rows;
@@ -1304,7 +1306,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
 
     auto attention = [&](const uint8_t* kc, const uint8_t* vc, int ctx_grid, float* out, uint16_t* hi, uint16_t* lo) {
         if (tree)
-            return launch_tree_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_gpre, d_gstart, d_masks, n, n, H, Hkv, hd, ps,
+            return launch_tree_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_gpre, d_gstart, d_masks, n, trees, H, Hkv, hd, ps,
                                          scale, ctx_grid, out, e->tree_ws, e->tree_ws_bytes, s, hi, lo);
         if (grouped)
             return launch_group_attention(e->q, kc, vc, e->o.kv_dtype, d_ptab, MP, d_ctx, d_gstart, d_gpre, n, n, H, Hkv, hd,
@@ -1456,13 +1458,13 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
         qraf_engine::StepGraph* g = nullptr;
         for (auto& sg : e->graphs)
             if (sg.n == n && sg.n_logit_rows == n_logit_rows && sg.ctx == ctx_grid && sg.head == head_mode &&
-                sg.grouped == grouped && sg.tree == tree && sg.gen == gen)
+                sg.grouped == grouped && sg.trees == trees && sg.gen == gen)
                 g = &sg;
         bool second = false;
         if (!g) {
             for (auto it = e->seen.begin(); it != e->seen.end(); ++it)
                 if (it->n == n && it->n_logit_rows == n_logit_rows && it->ctx == ctx_grid && it->head == head_mode &&
-                    it->grouped == grouped && it->tree == tree && it->gen == gen) {
+                    it->grouped == grouped && it->trees == trees && it->gen == gen) {
                     second = true;
                     e->seen.erase(it);
                     break;
@@ -1474,7 +1476,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
                 sg.ctx = ctx_grid;
                 sg.head = head_mode;
                 sg.grouped = grouped;
-                sg.tree = tree;
+                sg.trees = trees;
                 sg.gen = gen;
                 if (e->seen.size() >= 4 * MAX_STEP_GRAPHS) e->seen.erase(e->seen.begin());
                 e->seen.push_back(sg);
@@ -1514,7 +1516,7 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
             sg.ctx = ctx_grid;
             sg.head = head_mode;
             sg.grouped = grouped;
-            sg.tree = tree;
+            sg.trees = trees;
             sg.gen = gen;
             sg.exec = exec;
             e->graphs.push_back(sg);

@@ -205,6 +205,25 @@ def test_many_ragged(hip, kv):
 
 
 @KINDS
+@pytest.mark.parametrize("seqs", [63, 64, 65, 130])
+@pytest.mark.parametrize("H,hd", [(6, 64), (32, 128)])
+def test_many_sequences(hip, kv, seqs, H, hd):
+    """Up to 64 sequences are planned by lane, more in LDS; bounds that choose the planned form; sequences without rows."""
+    rng = np.random.default_rng(seqs)
+    trees = [(int(rng.integers(0, 150)), tree(rng, int(rng.integers(0, 8)))) for _ in range(seqs)]
+    trees[7] = (1200, tree(rng, 33))
+    run(hip, Trees(rng, trees, 2, hd, 16, kv, max_ctx=3000, ahead=1, behind=2), H, rng)
+
+
+@KINDS
+def test_rows_of_two_blocks(hip, kv):
+    """Rows whose query heads lie in two blocks of columns: 40 heads a KV head, and 128."""
+    rng = np.random.default_rng(11)
+    for H, n in ((40, 13), (128, 3), (100, 5)):
+        run(hip, Trees(rng, [(700, tree(rng, n)), (33, tree(rng, 2))], 1, 64, 16, kv, max_ctx=2000), H, rng)
+
+
+@KINDS
 @pytest.mark.parametrize("max_ctx", [None, 9000])
 def test_long(hip, kv, max_ctx):
     """Contexts that are split along their positions; bounds far above them."""
