@@ -879,10 +879,56 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         const bool shared = !DIRECT && !I8 && !tail && wq == 4;
         bool more = i < jend && (DIRECT || t < kend);
         ids(more ? t : 0);
-        // No load of K and V depends on a branch, here and below: where paths with more and with fewer loads behind
-        // one meet, a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
+        // No load of K and V depends on a branch, here and below (but whether waves share tiles): where paths with more and
+        // with fewer loads behind one meet, a wait for it is a wait for all.  A wave without tiles reads its pool's first page.
         pg0 = more ? pg0 : 0;
         pg1 = more ? pg1 : 0;
+
+        // Tiles that four waves share (below): a wave's 8 positions of a tile; fp16's first is requested ahead of q's end.
+        constexpr bool SHARES = !DIRECT && !I8;
+        constexpr int NP = HD / 64, PCS = HD / 8, RP = 64 / PCS;  // K: passes, pieces of a row, rows of a pass
+        typedef float vpart __attribute__((ext_vector_type(NP)));
+        std::conditional_t<SHARES && F32, float[NP][8], int> kx;
+        std::conditional_t<SHARES && F32, vpart[8], int> vx;
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        std::conditional_t<SHARES && F16, u32x4[NP], int> kr, vr;  // 8 dims of K, 8 positions of V
+        int kl = 0, id = 0;  // the last position that some column of the block attends to; the next request's page
+        bool some = true;    // (there is one; else no page is named, and the first is read)
+        auto id_of = [&](int at) { return some ? ptab[min(at + 8 * qt, kl) >> psl] : 0; };
+        auto request = [&](int at, int page) {
+            if constexpr (SHARES) {
+                const char *kp = block(a.kc, page), *vp = block(a.vc, page);
+                lanes_again();
+#pragma unroll
+                for (int u = 0; u < NP; u++) {
+                    const uint32_t off = (uint32_t)((min(at + 8 * qt + u * RP + lane / PCS, kl) & psm) * HD + 8 * (lane % PCS));
+                    if constexpr (F32) {
+                        const float4 x = *(const float4*)(kp + 4u * off), y = *(const float4*)(kp + (4u * off + 16u));
+                        kx[u][0] = x.x, kx[u][1] = x.y, kx[u][2] = x.z, kx[u][3] = x.w;
+                        kx[u][4] = y.x, kx[u][5] = y.y, kx[u][6] = y.z, kx[u][7] = y.w;
+                    } else {
+                        kr[u] = *(const u32x4*)(kp + 2u * off);
+                        vr[u] = *(const u32x4*)(vp + 2u * (uint32_t)((64 * u + lane) * a.page_size + ((at + 8 * qt) & psm)));
+                    }
+                }
+                if constexpr (F32) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        vx[k] = *(const vpart*)(vp + (uint32_t)(((min(at + 8 * qt + k, kl) & psm) * HD + NP * lane) * 4));
+                }
+            }
+        };
+        int id0 = 0;
+        if (SHARES && shared) {
+#pragma unroll
+            for (int c = 0; c < BLK; c += 64)
+                kl = max(kl, row_end((int)(((float)(bfirst + min(lane + c, bcols - 1)) + 0.5f) * inv_g), cache));
+            kl = min(__builtin_amdgcn_readfirstlane(over_wave(kl, imax2)), pre);
+            some = kl > 0;
+            kl = max(kl, 1) - 1;
+            id0 = id_of(t);
+            id = id_of(t + dt);
+        }
 
         // ---- q as fp16 hi + lo, scaled per column: 32 (HD 128) or 16 neighbouring lanes to a column, 16 bytes each,
         // all waves (a lane to a column, as the products take it, is a line of memory per lane and load: 2 us more)
@@ -905,9 +951,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
                 }
                 x[u] = *(const float4*)(a.q + (uint32_t)((row * a.H + kvh * G + h) * HD + d0));
             }
-            // (behind q, which is waited for alone; of tiles that are shared nothing is used: fp16 then reads one address,
-            // 28.0 -> 27.5 us of 128 rows behind 2,048 + 512 positions; f32 gained nothing)
-            load_k(more ? t : 0, F32 || !shared);
+            // (behind q, which is waited for alone)
+            if constexpr (SHARES && decltype(tiles_c)::value == 4) {
+                if (!shared) load_k(more ? t : 0);
+                else if (F16) request(t, id0);  // (f32: registers)
+            } else {
+                load_k(more ? t : 0);
+            }
             const int kk = I8 ? 2 * (d0 >> 5) + ((d0 >> 3) & 1) : d0 >> 4, hf = I8 ? (d0 >> 4) & 1 : (d0 >> 3) & 1;
 #pragma unroll
             for (int u = 0; u < NQ; u++) {
@@ -932,7 +982,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         if (DIRECT || wq == 1) stage_q(std::integral_constant<int, 1>());
         else if (wq == 2) stage_q(std::integral_constant<int, 2>());
         else stage_q(std::integral_constant<int, 4>());
-        if (!TURNS) load_v(more ? t : 0, F32 || !shared);  // (behind q: their registers)
+        if (!TURNS && !(SHARES && shared)) load_v(more ? t : 0);  // (behind q: their registers)
         if (TREE) s_mask[tid % BLK] = mask_of;
         lds_sync();
         const float qs = s_qs[qt * 32 + col];  // scores in powers of two
@@ -975,7 +1025,7 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             vexp += down;
         };
 
-        if constexpr (!DIRECT && !I8) {
+        if constexpr (SHARES) {
             // Tiles of more than 64 columns: the four waves side by side load a quarter of a tile each, 8 positions, and
             // write it as operands for all of them, f32 split (alone each would load and split it all, and a lane to a
             // position reads a line of memory per lane).  The tiles lie where q's hi halves were, which stay in
@@ -983,49 +1033,13 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
             // 32,768 positions, 16/2 heads of 128: f32 in 0.63 and fp16 in 0.89 of the time of waves alone; int8 gained
             // nothing and goes on alone.
             if (shared) {
-                constexpr int NP = HD / 64, PCS = HD / 8, RP = 64 / PCS;  // K: passes, pieces of a row, rows of a pass
                 constexpr int HL = F32 ? 2 : 1, KP = HL * QT, VP = 2 * 64 * DT, TP = KP + HL * VP;  // 16-byte pieces: hi, lo
                 static_assert((QHI + 2 * TP) * 16 <= 4 * tile_floats(HD), "q's lo halves and a tile of each kw");
                 uint4* tile = s_qhi + kw * TP;
                 f16x8 qh[KS];
 #pragma unroll
                 for (int kk = 0; kk < KS; kk++) qh[kk] = __builtin_bit_cast(f16x8, s_qhi[qt * QT + half * QB + col + 2 * QB * kk]);
-                // behind the last position that some column of the block attends to
-                int kl = 0;
-#pragma unroll
-                for (int c = 0; c < BLK; c += 64)
-                    kl = max(kl, row_end((int)(((float)(bfirst + min(lane + c, bcols - 1)) + 0.5f) * inv_g), cache));
-                kl = max(min(__builtin_amdgcn_readfirstlane(over_wave(kl, imax2)), pre), 1) - 1;
-                typedef float vpart __attribute__((ext_vector_type(NP)));
-                std::conditional_t<F32, float[NP][8], int> kx;
-                std::conditional_t<F32, vpart[8], int> vx;
-                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-                std::conditional_t<F16, u32x4[NP], int> kr, vr;  // 8 dims of K, 8 positions of V
-                auto id_of = [&](int at) { return ptab[min(at + 8 * qt, kl) >> psl]; };
-                auto request = [&](int at, int id) {
-                    const char *kp = block(a.kc, id), *vp = block(a.vc, id);
-                    lanes_again();
-#pragma unroll
-                    for (int u = 0; u < NP; u++) {
-                        const uint32_t off = (uint32_t)((min(at + 8 * qt + u * RP + lane / PCS, kl) & psm) * HD + 8 * (lane % PCS));
-                        if constexpr (F32) {
-                            const float4 x = *(const float4*)(kp + 4u * off), y = *(const float4*)(kp + (4u * off + 16u));
-                            kx[u][0] = x.x, kx[u][1] = x.y, kx[u][2] = x.z, kx[u][3] = x.w;
-                            kx[u][4] = y.x, kx[u][5] = y.y, kx[u][6] = y.z, kx[u][7] = y.w;
-                        } else {
-                            kr[u] = *(const u32x4*)(kp + 2u * off);
-                            vr[u] = *(const u32x4*)(vp + 2u * (uint32_t)((64 * u + lane) * a.page_size + ((at + 8 * qt) & psm)));
-                        }
-                    }
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            vx[k] = *(const vpart*)(vp + (uint32_t)(((min(at + 8 * qt + k, kl) & psm) * HD + NP * lane) * 4));
-                    }
-                };
-                t = __builtin_amdgcn_readfirstlane(t);
-                request(t, id_of(t));
-                int id = id_of(t + dt);
+                if (F32) request(t, id0);
                 for (; i < jend; i++, t += dt) {
                     lds_sync();  // what lay there is read
                     // ---- this wave's quarter
@@ -1664,36 +1678,48 @@ __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
         lds_sync();
         auto join = [&](auto wk_c) {
             constexpr int WK = decltype(wk_c)::value, WQ = GW / WK;
-#pragma unroll 4
-            for (int e = tid; e < WQ * 32 * (HD / 4); e += GTH) {
-                const int c = e / (HD / 4), d = e % (HD / 4) * 4, cq = c >> 5, ci = c & 31;
-                const long long to = s_to[c];
-                if (to == NOWHERE) continue;
-                float4 x[WK];
-                float f[WK], M = -INFINITY, L = 0.f;
+            // U pieces of 16 bytes at a time, all read ahead of the first branch (one by one a piece was 600 cycles)
+            constexpr int U = 8 / WK < WQ * 32 * (HD / 4) / GTH ? 8 / WK : WQ * 32 * (HD / 4) / GTH;
+            for (int e0 = tid; e0 < WQ * 32 * (HD / 4); e0 += U * GTH) {
+                long long to[U];
+                float4 x[U][WK];
+                float f[U][WK], lw[U][WK];
 #pragma unroll
-                for (int k = 0; k < WK; k++) {
-                    x[k] = *(const float4*)(s_o + ((cq + WQ * k) * 32 + ci) * HD + (d ^ 4 * (ci & 15)));
-                    f[k] = s_m[cq + WQ * k][ci];
-                    M = fmaxf(M, f[k]);
-                }
-                const float mu = M == -INFINITY ? 0.f : M;
-                float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int u = 0; u < U; u++) {
+                    const int e = e0 + u * GTH, c = e / (HD / 4), d = e % (HD / 4) * 4, cq = c >> 5, ci = c & 31;
+                    to[u] = s_to[c];
 #pragma unroll
-                for (int k = 0; k < WK; k++) {  // (a wave without positions holds zeros)
-                    f[k] = __builtin_amdgcn_exp2f(f[k] - mu);
-                    L = __builtin_fmaf(s_l[cq + WQ * k][ci], f[k], L);
-                    O.x = __builtin_fmaf(x[k].x, f[k], O.x);
-                    O.y = __builtin_fmaf(x[k].y, f[k], O.y);
-                    O.z = __builtin_fmaf(x[k].z, f[k], O.z);
-                    O.w = __builtin_fmaf(x[k].w, f[k], O.w);
+                    for (int k = 0; k < WK; k++) {
+                        x[u][k] = *(const float4*)(s_o + ((cq + WQ * k) * 32 + ci) * HD + (d ^ 4 * (ci & 15)));
+                        f[u][k] = s_m[cq + WQ * k][ci];
+                        lw[u][k] = s_l[cq + WQ * k][ci];
+                    }
                 }
-                if (to < 0) {
-                    *(float4*)(a.part_o + (size_t)~to * HD + d) = O;
-                    if (d == 0) a.part_ml[~to] = make_float2(M, L);
-                } else {
-                    const float by = DIRECT && d_ctx == 0 ? 0.f : 1.f / L;
-                    group_store4(a, to + d, make_float4(O.x * by, O.y * by, O.z * by, O.w * by));
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int d = (e0 + u * GTH) % (HD / 4) * 4;
+                    float M = -INFINITY, L = 0.f;
+#pragma unroll
+                    for (int k = 0; k < WK; k++) M = fmaxf(M, f[u][k]);
+                    const float mu = M == -INFINITY ? 0.f : M;
+                    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int k = 0; k < WK; k++) {  // (a wave without positions holds zeros)
+                        const float by = __builtin_amdgcn_exp2f(f[u][k] - mu);
+                        L = __builtin_fmaf(lw[u][k], by, L);
+                        O.x = __builtin_fmaf(x[u][k].x, by, O.x);
+                        O.y = __builtin_fmaf(x[u][k].y, by, O.y);
+                        O.z = __builtin_fmaf(x[u][k].z, by, O.z);
+                        O.w = __builtin_fmaf(x[u][k].w, by, O.w);
+                    }
+                    if (to[u] == NOWHERE) continue;
+                    if (to[u] < 0) {
+                        *(float4*)(a.part_o + (size_t)~to[u] * HD + d) = O;
+                        if (d == 0) a.part_ml[~to[u]] = make_float2(M, L);
+                    } else {
+                        const float by = DIRECT && d_ctx == 0 ? 0.f : 1.f / L;
+                        group_store4(a, to[u] + d, make_float4(O.x * by, O.y * by, O.z * by, O.w * by));
+                    }
                 }
             }
         };
