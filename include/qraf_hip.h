@@ -270,7 +270,8 @@ int qraf_hip_group_attention_dev(const float* q, const void* k_cache, const void
  * ahead of them.  A row attends to all of its sequence's cache and, of the
  * positions behind it, to those that its mask names.  The batch of
  * qraf_hip_paged_attention_dev (its caches, page types, scale and out), but:
- *   page_table [n_seqs][max_pages_per_seq], a row for each sequence
+ *   page_table [n_seqs][max_pages_per_seq], a row for each sequence, which maps
+ *            every position up to the last that some row of it attends to
  *   row_starts [n_seqs + 1] ascending (a sequence may have no rows)
  *   base_lens [n_seqs] positions that every row of the sequence attends to
  *   masks [n_rows]: bit b set: the row attends to position base_lens[s] + b

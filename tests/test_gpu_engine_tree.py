@@ -388,3 +388,15 @@ def test_a_pool_without_pages_for_a_tree(hip):
     assert x.value.code == ERR_NOMEM and e.seq_length(a) == 3 and e.free_pages() == 1
     e.step_tree([a] * 20, [1] * 20, [-1] + [0] * 19, [3] * 20)
     e.close()
+
+
+def test_an_engine_of_one_row(hip):
+    """A tree of its root alone: generate_tokens' steps."""
+    from qraf_amd.engine import InferenceEngine
+    tf, kw = transformer("q8_llama", max_batch=1)
+    prompt = tokens(np.random.default_rng(2), kw, 5)
+    want, sure = reference_stream(tf, prompt, 10)
+    got = InferenceEngine(tf, eos_token=None).generate_tree(prompt, 10, depth=0, width=1)
+    assert len(got) == 10 and got[:sure] == want[:sure]
+    assert len(InferenceEngine(tf, eos_token=None).score(prompt)["logprobs"]) == 4
+    tf.engine.close()

@@ -96,6 +96,32 @@ def test_sizes(hip, rows, V, top):
     check(call(hip, x, tokens, top)[0], x, tokens, top)
 
 
+@pytest.mark.parametrize("V", [2047, 2048, 2049, 8191, 8192, 8193, 16385, 131072, 524288])
+@pytest.mark.parametrize("top", [0, 3, 64])
+def test_where_the_form_changes(hip, V, top):
+    """The last row of a form and the first of the next, one row and several."""
+    rng = np.random.default_rng(V)
+    for rows in (1, 9):
+        if rows * V > 1 << 21:
+            continue
+        x, tokens = logits(rng, rows, V), rng.integers(0, V, rows)
+        check(call(hip, x, tokens, top)[0], x, tokens, top)
+
+
+@pytest.mark.parametrize("V", [5000, 8192, 300000])
+def test_flat_rows(hip, V):
+    """More equal logits at the border than the lists hold, the ties behind a few larger ones, at the end, everywhere."""
+    rng = np.random.default_rng(V)
+    x = np.full((4, V), 1.5, np.float32)
+    x[0, rng.choice(V, 7, replace=False)] = 2 + rng.random(7)
+    x[1, :V // 2] = -3.0
+    x[2] = np.round(rng.standard_normal(V))
+    x[3, V - 3:] = 9.0
+    tokens = np.array([5, V - 1, 0, V - 2])
+    for top in (1, 20, 64):
+        check(call(hip, x, tokens, top)[0], x, tokens, top)
+
+
 @pytest.mark.parametrize("V", [1000, 49152, 151936])
 @pytest.mark.parametrize("rows", [63, 300])
 def test_many_rows(hip, rows, V):

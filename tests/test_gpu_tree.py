@@ -261,3 +261,102 @@ def test_append_is_rope_append_at_another_place(hip, kv, H, Hkv, hd, bias):
             want[cell[0, table[of[i], slots[i] // ps], :, slots[i] % ps]] = r[fcell[0, own[i, pos[i] // ps], :,
                                                                                    pos[i] % ps]]
         assert np.array_equal(g, want)
+
+
+# ------------------------------------------------------------------ a step of all of them
+
+@KINDS
+def test_a_captured_step_of_trees(hip, kv):
+    """Append, attention, sampling, acceptance, compaction and log probabilities in one graph, replayed on new inputs
+    with the same calls made eagerly between: equal bit for bit, the cache among them."""
+    from qraf_amd._lib import SamplingParams, lib
+    from qraf_amd.backend import DeviceBuffer, Graph, Stream
+    rng = np.random.default_rng(21)
+    H, Hkv, hd, ps, V, sizes, bases = 8, 2, 64, 16, 700, (9, 5), (45, 100)
+    up, n, wide = DeviceBuffer.from_array, sum(sizes), 8
+    starts = np.cumsum([0, *sizes]).astype(np.int32)
+    of = np.repeat([0, 1], sizes).astype(np.int32)
+    table = rng.permutation(2 * wide).astype(np.int32).reshape(2, wide)
+    rope = np.zeros((128, hd), np.float32)
+    hip._lib.call("qraf_hip_rope_table_host", 128, hd, 1e4, rope.ctypes.data_as(hip._lib.fp))
+    if kv == I8:  # bytes with scales
+        block = np.concatenate([rng.integers(0, 256, (2 * wide * Hkv, ps * hd)).astype(np.uint8),
+                                np.full((2 * wide * Hkv, ps), 0.02, np.float32).view(np.uint8)], 1)
+        cache = block.reshape(-1)
+    else:
+        cache = rng.standard_normal(2 * wide * Hkv * ps * hd).astype(np.float16 if kv == F16 else np.float32).view(np.uint8)
+    d = {k: up(v) for k, v in dict(starts=starts, of=of, table=table, rope=rope, base=np.array(bases, np.int32),
+                                   k=cache, v=cache).items()}
+    for k, size in dict(qkv=n * (H + 2 * Hkv) * hd * 4, pos=n * 4, slots=n * 4, masks=n * 8, parents=n * 4, draft=n * 4,
+                        logits=n * V * 4, q=n * H * hd * 4, out=n * H * hd * 4, picks=n * 4, acc=8, path=n * 4,
+                        tokens=n * 4, lp=n * 4, rank=n * 4, ent=n * 4, tt=n * 16, tl=n * 16).items():
+        d[k] = up(np.zeros(size, np.uint8))
+    params = SamplingParams(0.0, 0, 1.0, 1.0)
+    aw, lw = lib.qraf_hip_tree_attention_workspace_bytes(n, 2, H, Hkv, hd, 128), \
+        lib.qraf_hip_token_logprobs_workspace_bytes(n, V, 4)
+    d["aw"], d["lw"] = up(np.zeros(aw, np.uint8)), up(np.zeros(lw, np.uint8))
+    p = {k: b.ptr for k, b in d.items()}
+
+    def step(st):
+        import ctypes
+        call = hip._lib.call
+        call("qraf_hip_tree_append_dev", p["qkv"], None, n, H, Hkv, hd, p["pos"], p["slots"], p["of"], p["rope"], p["q"],
+             p["k"], p["v"], kv, p["table"], wide, ps, st)
+        call("qraf_hip_tree_attention_dev", p["q"], p["k"], p["v"], kv, p["table"], wide, p["base"], p["starts"],
+             p["masks"], n, 2, H, Hkv, hd, ps, 0.125, 128, p["out"], p["aw"], aw, st)
+        call("qraf_hip_sample_dev", p["logits"], n, V, ctypes.byref(params), None, None, 0, None, p["picks"], st)
+        call("qraf_hip_tree_accept_dev", p["picks"], p["draft"], p["parents"], p["starts"], 2, n, p["acc"], p["path"],
+             p["tokens"], st)
+        call("qraf_hip_kv_compact_dev", p["k"], p["v"], kv, 1, cache.size, p["table"], wide, p["base"], p["starts"],
+             p["path"], 2, n, Hkv, hd, ps, st)
+        call("qraf_hip_token_logprobs_dev", p["logits"], n, V, p["picks"], p["lp"], p["rank"], p["ent"], 4, p["tt"],
+             p["tl"], p["lw"], lw, st)
+
+    def inputs():
+        trees = [random_tree(rng, k, 0.9, V) for k in sizes]
+        masks, depth = [], []
+        for parents, _, _ in trees:
+            m, at = [], []
+            for i, u in enumerate(parents):
+                m.append((m[u] if i else 0) | 1 << i)
+                at.append(at[u] + 1 if i else 0)
+            masks += m
+            depth += at
+        x = rng.standard_normal((n, V)).astype(np.float32)
+        for i, t in enumerate(sum((list(t[2]) for t in trees), [])):
+            x[i, t] = 20.0
+        d["logits"].upload(x)
+        d["qkv"].upload(rng.standard_normal((n, (H + 2 * Hkv) * hd)).astype(np.float32))
+        d["masks"].upload(np.array(masks, np.uint64))
+        d["pos"].upload((np.array(bases)[of] + depth).astype(np.int32))
+        d["slots"].upload((np.array(bases)[of] + np.arange(n) - starts[of]).astype(np.int32))
+        d["parents"].upload(np.array(sum((t[0] for t in trees), []), np.int32))
+        d["draft"].upload(np.array(sum((list(t[1]) for t in trees), []), np.uint32))
+        return trees
+
+    names = ("k", "v", "out", "acc", "path", "tokens", "lp", "rank", "ent", "tt", "tl")
+    st = Stream()
+    inputs()
+    step(st.h)
+    st.synchronize()
+    g = Graph(st)
+    with g:
+        step(st.h)
+    for _ in range(4):
+        trees = inputs()
+        results = []
+        for way in (lambda: g.launch(), lambda: step(None)):
+            d["k"].upload(cache)
+            d["v"].upload(cache)
+            way()
+            st.synchronize()
+            hip._lib.call("qraf_hip_device_synchronize")
+            results.append({k: d[k].download(np.uint8, d[k].nbytes) for k in names})
+        for k in names:
+            assert np.array_equal(results[0][k], results[1][k]), k
+        acc, path, toks = expect(trees)
+        assert list(results[0]["acc"].view(np.int32)) == acc and list(results[0]["path"].view(np.int32)) == path
+        assert list(results[0]["tokens"].view(np.uint32)) == toks
+        assert list(results[0]["rank"].view(np.int32)) == [0] * n
+    g.destroy()
+    st.destroy()
