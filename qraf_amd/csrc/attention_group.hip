@@ -17,6 +17,11 @@
 // unnormalised output) parts, which group_merge_kernel joins in position order.
 // Small calls go without: a workgroup per (row, KV head) takes all its positions.
 // group_any_kernel takes the shapes that the tiles do not.
+//
+// Trees of drafted tokens (qraf_hip_tree_attention_dev) are groups all of whose positions
+// are shared: a sequence's rows attend to its cache and, behind it, to the positions that
+// their 64-bit masks name.  The same jobs, pieces and tiles; tiles that reach behind the
+// cache take a bit for each position instead of a length.
 #include <limits.h>
 #include <math.h>
 
@@ -622,6 +627,10 @@ constexpr int tile_floats(int hd) { return GW * 32 * hd; }
 // TREE: rows attend to their sequence's cache and to the positions behind it that their masks name, all of them shared
 // (the prefix ends where their attention does): tiles that reach behind the cache go by bits.
 // LANES: the plan is lane_plan's.
+// Trees, measured (16/2 heads of 128, us a call): 64 nodes at 8,000 positions, fp16, 25.9, of which the join's launch 4.7
+// and in the tiles' 40,000 cycles the plan 4,500, the piece and q 10,000, four tiles 18,000 and the outputs 8,000; 48
+// trees of up to 16 at 128..4,096, fp16, 56.6: 114 MB at a plain read's rate in 30 behind as much that is fixed; 24 of up
+// to 26 at 3,000..8,000, int8, 95: widening and softmax (VALU) beside the products; 8 of 64 at 777..2,000, f32, 45.9.
 template <int HD, int KV, bool DIRECT, bool TREE, bool LANES>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
@@ -1815,6 +1824,67 @@ __global__ __launch_bounds__(256) void group_merge_kernel(GroupArgs a) {
     for (int k = 0; k < DPL; k++) group_store(a, out + lane + 64 * k, O[k] / l);
 }
 
+// The same of trees, whose columns have parts of one kind: HD / 4 lanes hold a part, so 2 or 4 parts lie side by side in
+// a wave's registers, 4 or 8 times; their maxima, sums and outputs meet at the end.  (64 nodes at 8,000 positions, 32
+// parts a column: 4.7 us, of which two reads one after another and the launch; eight parts of two dimensions a lane at
+// a time 6.1.)
+template <int HD>
+__global__ __launch_bounds__(256) void tree_merge_kernel(GroupArgs a) {
+    constexpr int W = HD / 4, NP = 64 / W;
+    const int r = blockIdx.x, h = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (h >= a.H) return;
+    const int lane = threadIdx.x & 63, kvh = h / a.G, hh = h - kvh * a.G, d = 4 * (lane % W), side = lane / W;
+    const int4 at = a.plan[2 * r];
+    const bool some = a.plan[2 * r + 1].x != 0;
+    if (at.x < 0) return;  // of no sequence
+    const bool second = (at.x + hh) / BLK != at.x / BLK;
+    const int x = second ? at.z : at.y, y = second ? at.w : at.z;
+    const int all = some ? (y & 0xFFFF) - (x & 0xFFFF) : 0;
+    const size_t out = ((size_t)r * a.H + h) * HD + d;
+    if (all == 0 && side == 0) group_store4(a, out, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (all <= 1) return;
+    const size_t column = (size_t)kvh * a.slots + (size_t)r * a.G + hh + (size_t)BLK * ((x & 0xFFFF) - (x >> 16));
+    float m = -INFINITY, l = 0.f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto take = [&](int i0, auto many) {
+        constexpr int U = decltype(many)::value;
+        float4 v[U];
+        float2 ml[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const size_t slot = column + (size_t)BLK * min(i0 + u * NP + side, all - 1);
+            ml[u] = a.part_ml[slot];
+            v[u] = *(const float4*)(a.part_o + slot * HD + d);
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; u++) mn = i0 + u * NP + side < all ? fmaxf(mn, ml[u].x) : mn;
+        const float mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
+        l *= alpha;
+        O = make_float4(O.x * alpha, O.y * alpha, O.z * alpha, O.w * alpha);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const bool in = i0 + u * NP + side < all;
+            const float f = in ? __builtin_amdgcn_exp2f(ml[u].x - mu) : 0.f;
+            l = in ? __builtin_fmaf(ml[u].y, f, l) : l;
+            O.x = in ? __builtin_fmaf(v[u].x, f, O.x) : O.x;
+            O.y = in ? __builtin_fmaf(v[u].y, f, O.y) : O.y;
+            O.z = in ? __builtin_fmaf(v[u].z, f, O.z) : O.z;
+            O.w = in ? __builtin_fmaf(v[u].w, f, O.w) : O.w;
+        }
+        m = mn;
+    };
+    if (all <= 4 * NP) take(0, std::integral_constant<int, 4>());
+    else
+        for (int i0 = 0; i0 < all; i0 += 8 * NP) take(i0, std::integral_constant<int, 8>());
+    auto sides = [](float v, auto op) { return NP == 4 ? over_halves(over_rows(v, op), op) : over_halves(v, op); };
+    const float M = sides(m, fmax2), by = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+    auto sum = [&](float v) { return sides(v * by, [](float p, float q) { return p + q; }); };
+    l = sum(l);
+    O = make_float4(sum(O.x), sum(O.y), sum(O.z), sum(O.w));
+    if (side == 0) group_store4(a, out, make_float4(O.x / l, O.y / l, O.z / l, O.w / l));
+}
+
 // workgroups per KV head: as many as are resident at once, one per CU, whose
 // registers its 8 waves fill
 static int group_grid(int Hkv) { return std::max(1, 256 / Hkv); }
@@ -1912,8 +1982,8 @@ static int group_tiles(GroupArgs& a, uint32_t kv_dtype, int hd, void* ws, bool d
     QH_CHECK_HIP(hipGetLastError());
     if (direct) return QRAF_HIP_OK;
     const dim3 grid(a.n, (a.H + 3) / 4);
-    if (hd == 128) hipLaunchKernelGGL((group_merge_kernel<128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((group_merge_kernel<64>), grid, dim3(256), 0, st, a);
+    if (hd == 128) hipLaunchKernelGGL((TREE ? tree_merge_kernel<128> : group_merge_kernel<128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((TREE ? tree_merge_kernel<64> : group_merge_kernel<64>), grid, dim3(256), 0, st, a);
     QH_CHECK_HIP(hipGetLastError());
     return QRAF_HIP_OK;
 }
