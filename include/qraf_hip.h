@@ -610,9 +610,9 @@ int qraf_hip_tree_accept_dev(const uint32_t* picks, const uint32_t* draft_tokens
  * -inf and entropy 0.  The logits are as the model left them (temperature 1, no
  * penalty).  Exponentials in 32 bits, sums of whole rows and logarithms in 64:
  * log probabilities and entropies are within 2^-19 of (1 + their size).  The
- * workspace (qraf_hip_token_logprobs_workspace_bytes, 16-byte aligned) needs no
- * initialisation; calls that share one must not overlap.  The same from call to
- * call.  No counterpart in the reference. */
+ * workspace (qraf_hip_token_logprobs_workspace_bytes, 16-byte aligned; no more for
+ * fewer rows or alternatives) needs no initialisation; calls that share one must not
+ * overlap.  The same from call to call.  No counterpart in the reference. */
 uint64_t qraf_hip_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top);
 int qraf_hip_token_logprobs_dev(const float* logits, int32_t rows, int32_t vocab, const uint32_t* tokens,
                                 float* logprobs, int32_t* ranks, float* entropies, int32_t top, uint32_t* top_tokens,

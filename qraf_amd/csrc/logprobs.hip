@@ -19,8 +19,8 @@
 // few logits that do are ordered by counting.  Rows of up to 8,192 logits take one
 // workgroup and one launch.  Rows with more equal logits at the border than the lists
 // hold take a search over the whole row (flat_tops).
-// Measured: 512 rows of 151,936 (311 MB) 55.7 us, 5.6 TB/s; 160 rows with 20 alternatives (97 MB) 24.5, of which the
-// pass 17 and the join 6.4; 8 rows of 49,152 with 4 7.7.
+// Measured: 512 rows of 151,936 (311 MB) 55.6 us, 5.6 TB/s; 160 rows with 20 alternatives (97 MB) 24.1, of which the
+// pass 17 and the join 6.3; 8 rows of 49,152 with 4 7.6.
 #include <math.h>
 
 #include <algorithm>
@@ -82,6 +82,19 @@ __device__ __forceinline__ void load_chunk(const float* l, int V, int c, float (
             const Four x = *(const Four*)(l + chunk_index<E, TH>(c, t, j));
 #pragma unroll
             for (int k = 0; k < 4; k++) v[j + k] = x.v[k];
+        }
+    } else if (V >= 4) {
+        // (A row's last chunk one logit at a time took four times its loads: 512 rows of 128,256 logits 57 us, so 50.)
+        const int end = V & ~3, rest = V & 3;
+        float last[3];
+#pragma unroll
+        for (int k = 0; k < 3; k++) last[k] = l[min(end + k, V - 1)];
+#pragma unroll
+        for (int j = 0; j < E; j += 4) {
+            const int i = chunk_index<E, TH>(c, t, j);
+            const Four x = *(const Four*)(l + min(i, V - 4));
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[j + k] = i < end ? x.v[k] : k < rest && i == end ? last[k % 3] : -INFINITY;
         }
     } else {
 #pragma unroll
@@ -512,18 +525,29 @@ __global__ __launch_bounds__(JTH + 64) void logprobs_tops_kernel(LogprobArgs a) 
     write_tops(a, row, l, sh, over, s_r);
 }
 
-// Splits of 32 logits a thread where these are workgroups enough, of 8 in smaller calls.
-static bool wide_splits(int rows, int V) { return (long long)rows * V >= 256ll * STH * 32; }
+// Splits of 32 logits a thread, or of 8, which reach more CUs with fewer rows and leave less of a short row's last split
+// empty, but take a row past 131,072 in turns.  Of 8 against of 32, us, 20 alternatives: 8 rows of 32,000 / 49,152 /
+// 80,000 / 128,256 / 151,936 logits 8.1 / 8.2 / 9.6 / 10.2 / 11.5 against 9.5 / 8.7 / 9.6 / 9.7 / 9.7; 128 rows 11.6 /
+// 12.9 / 16.5 / 20.9 / 28.9 against 12.4 / 13.2 / 15.9 / 19.4 / 20.9; 512 rows 20.3 / 28.5 / 44.4 / 64.8 / 83.8 against
+// 20.8 / 25.5 / 38.3 / 58.3 / 64.3.  100,003 logits: of 32 from the first row on (9.3 against 10.0).
+constexpr int WIDE = 3 << 15, NARROW = 40000, WIDE_ALL = 1 << 23;  // logits of a row, of a row, of a call
+static bool wide_splits(int rows, int V) {
+    return V >= WIDE || (V >= NARROW && (long long)rows * V >= WIDE_ALL);
+}
 static int splits_of(int rows, int V) {
     const int per = STH * (wide_splits(rows, V) ? 32 : 8);
     return std::min(SPLITS, (V + per - 1) / per);
 }
-constexpr int SMALL = STH * 32;  // logits of a row that one workgroup takes
+// Logits of a row that one workgroup takes.  8 rows of 8,000, 20 alternatives: 7.8 us where splits take 8.3; 512 rows 10.7
+// and 15.0.  (Up to 2,048 by 256 threads: 1,000 logits 4.9 where 512 take 5.2.)
+constexpr int SMALL = STH * 32;
 
 size_t token_logprobs_workspace_bytes(int rows, int V, int top) {
     if (V <= SMALL) return 16;
-    const size_t S = splits_of(rows, V);
-    return (size_t)rows * S * (STH / 64) * sizeof(WaveStats) + (top ? (size_t)rows * S * STH * 4 : 0);
+    auto bytes = [&](size_t n) { return n * splits_of((int)n, V) * ((STH / 64) * sizeof(WaveStats) + (top ? STH * 4 : 0)); };
+    // never less than of fewer rows, whose splits may be more
+    const int narrow = V >= NARROW && V < WIDE ? std::min(rows, (WIDE_ALL - 1) / V) : rows;
+    return std::max(bytes(rows), bytes(narrow));
 }
 
 int launch_token_logprobs(const float* logits, int rows, int V, const uint32_t* tokens, float* logprobs, int32_t* ranks,

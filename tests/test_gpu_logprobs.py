@@ -231,3 +231,33 @@ def test_graph_replays(hip, rows, V, top):
         assert all(np.array_equal(a, b) for a, b in zip(read(), got))
     g.destroy()
     st.destroy()
+
+
+@pytest.mark.parametrize("V", [4, 5, 6, 7, 1022, 2050, 4099, 8191, 8194, 16387, 40001, 49155, 98301, 98305, 98306, 98307])
+def test_ends_of_rows(hip, V):
+    """Rows that end inside 16 bytes: the largest logits, NaN and -inf next to the end, behind which the next row begins."""
+    rng = np.random.default_rng(V)
+    x = logits(rng, 5, V)
+    x[0, -3:] = 40.0, 41.0, 40.0
+    x[1, -4:] = np.nan, 39.0, np.nan, -np.inf
+    x[2, -1] = -np.inf
+    x[3, :4] = 60.0
+    x[4, -2:] = np.inf
+    tokens = np.array([V - 1, V - 3, V - 1, V - 2, V - 1])
+    for top in (0, 4):
+        check(call(hip, x, tokens, top, offset=1)[0], x, tokens, top)
+
+
+@pytest.mark.parametrize("rows,V", [(170, 49152), (171, 49152), (209, 40001), (210, 40001), (85, 98303), (86, 98303)])
+def test_splits_of_either_size(hip, rows, V):
+    """The last call whose splits are short and the first whose are long, in the workspace of the larger."""
+    assert hip.lib.qraf_hip_token_logprobs_workspace_bytes(rows, V, 5) <= \
+        hip.lib.qraf_hip_token_logprobs_workspace_bytes(rows + 1, V, 5)
+    rng = np.random.default_rng(rows)
+    x = np.tile(logits(rng, 5, V), (rows // 5 + 1, 1))[:rows]
+    tokens = rng.integers(0, V, rows)
+    got = call(hip, x, tokens, 5)[0]
+    check([g[-9:] for g in got], x[-9:], tokens[-9:], 5)
+    check([g[:3] for g in got], x[:3], tokens[:3], 5)
+    for g in got[2:]:
+        assert np.array_equal(g[:5], g[5:10])

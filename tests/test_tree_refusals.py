@@ -105,3 +105,13 @@ def test_workspace_queries_of_bad_shapes_are_zero():
     assert lib.qraf_hip_tree_attention_workspace_bytes(4, 1, 8, -2, 64, 128) == 0
     assert lib.qraf_hip_token_logprobs_workspace_bytes(0, 100, 5) == 0
     assert lib.qraf_hip_token_logprobs_workspace_bytes(3, 100, -1) == 0
+
+
+@pytest.mark.parametrize("vocab", [8192, 8193, 39999, 40000, 98303, 98304, 151936])
+def test_logprobs_workspace_grows_with_rows_and_alternatives(vocab):
+    size = lib.qraf_hip_token_logprobs_workspace_bytes
+    rows = [1, 2, 84, 85, 86, 87, 208, 209, 210, 211, 1024, 65535]
+    for top in (0, 1, 64):
+        sizes = [size(r, vocab, top) for r in rows]
+        assert sizes == sorted(sizes) and sizes[0] > 0
+        assert top == 0 or all(size(r, vocab, 0) <= s for r, s in zip(rows, sizes))
