@@ -483,7 +483,7 @@ struct qraf_engine {
                               // parents (a node of the tree), masks
     // Pinned staging, one slot per step in flight: a step's inputs are written
     // into slot `slot` while the previous step (the other slot) may still be
-    // queued; its tokens come back into h_amax of the same slot.
+    // queued; its tokens come back into h_amax of the same slot (accepted trees: their lengths and tokens).
     int32_t* h_in[2] = {nullptr, nullptr};
     uint32_t* h_amax[2] = {nullptr, nullptr};
     hipEvent_t done_ev[2] = {nullptr, nullptr};  // recorded after a step's last copy
@@ -700,7 +700,7 @@ int qraf_engine_create(const qraf_model_config* cfg, const qraf_engine_options* 
         return fail(set_error(QRAF_HIP_ERR_HIP, "engine: workspace set-up failed"));
     for (int k = 0; k < 2; k++)
         if (hipHostMalloc((void**)&e->h_in[k], e->in_words * 4, hipHostMallocDefault) != hipSuccess ||
-            hipHostMalloc((void**)&e->h_amax[k], (size_t)B * 4, hipHostMallocDefault) != hipSuccess ||
+            hipHostMalloc((void**)&e->h_amax[k], (size_t)B * 8, hipHostMallocDefault) != hipSuccess ||
             hipEventCreateWithFlags(&e->done_ev[k], hipEventDisableTiming) != hipSuccess)
             return fail(set_error(QRAF_HIP_ERR_HIP, "engine: staging set-up failed"));
     // RoPE table from the host libm (RopeCache::init, ops.cpp:179-193)
@@ -1580,13 +1580,14 @@ int qraf_engine_step_tree(qraf_engine* e, int32_t n, const int32_t* seq_ids, con
     QH_REQUIRE(e->n_pending == 0, QRAF_HIP_ERR_STATE, "step_tree: %d asynchronous steps not collected", e->n_pending);
     QH_REQUIRE(n > 0 && n <= (int32_t)e->o.max_batch, QRAF_HIP_ERR_INVALID, "step_tree: %d rows (max_batch %u)", n,
                e->o.max_batch);
+    std::vector<int32_t> ids;  // a sequence's, once
+    for (int i = 0; i < n; i++)
+        if (i == 0 || seq_ids[i] != seq_ids[i - 1]) ids.push_back(seq_ids[i]);
+    std::sort(ids.begin(), ids.end());
+    const auto twice = std::adjacent_find(ids.begin(), ids.end());
+    QH_REQUIRE(twice == ids.end(), QRAF_HIP_ERR_INVALID, "step_tree: the rows of sequence %d do not lie side by side", *twice);
     for (int i = 0, first = 0; i < n; i++) {
-        if (i > 0 && seq_ids[i] != seq_ids[i - 1]) {
-            first = i;
-            for (int k = 0; k < i; k++)
-                QH_REQUIRE(seq_ids[k] != seq_ids[i], QRAF_HIP_ERR_INVALID,
-                           "step_tree: rows %d and %d of sequence %d do not lie side by side", k, i, seq_ids[i]);
-        }
+        if (i > 0 && seq_ids[i] != seq_ids[i - 1]) first = i;
         QH_REQUIRE(i - first < 64, QRAF_HIP_ERR_INVALID, "step_tree: sequence %d has more than 64 nodes", seq_ids[i]);
         QH_REQUIRE(i == first ? parents[i] == -1 : parents[i] >= first && parents[i] < i, QRAF_HIP_ERR_INVALID,
                    "step_tree: row %d of sequence %d, whose rows begin at %d, has parent %d", i, seq_ids[i], first, parents[i]);
@@ -1766,8 +1767,8 @@ int qraf_engine_accept_tree(qraf_engine* e, const qraf_sampling_params* p, const
     uint8_t* rest = nullptr;
     QH_TRY(sample_rows(e, 0, n, p, recent, counts, stride, uniforms, &d_pick, 3 * rb, &rest));
     e->tree_nodes = 0;  // (the cache moves)
-    int32_t *d_acc = (int32_t*)rest, *d_path = (int32_t*)(rest + rb);
-    uint32_t* d_tok = (uint32_t*)(rest + 2 * rb);
+    int32_t *d_path = (int32_t*)rest, *d_acc = (int32_t*)(rest + rb);
+    uint32_t* d_tok = (uint32_t*)(d_acc + seqs);  // (one copy with the lengths, into pinned memory)
     const int32_t* d_gpre = e->d_in + 7 * (size_t)at;
     const int32_t* d_gstart = d_gpre + at;
     const int32_t* d_ptab = d_gstart + at + 1;
@@ -1776,9 +1777,10 @@ int qraf_engine_accept_tree(qraf_engine* e, const qraf_sampling_params* p, const
     QH_TRY(launch_tree_accept(d_pick, (const uint32_t*)e->d_in, d_parent, d_gstart, seqs, n, d_acc, d_path, d_tok, s));
     QH_TRY(launch_kv_compact(e->kpool, e->vpool, e->o.kv_dtype, (int)e->c.num_layers, e->layer_kv_bytes, d_ptab, MP, d_gpre,
                              d_gstart, d_path, seqs, n, (int)e->c.num_kv_heads, e->hd, (int)e->o.page_size, s));
-    QH_CHECK_HIP(hipMemcpyAsync(accepted, d_acc, (size_t)seqs * 4, hipMemcpyDeviceToHost, s));
-    QH_CHECK_HIP(hipMemcpyAsync(tokens, d_tok, (size_t)n * 4, hipMemcpyDeviceToHost, s));
+    QH_CHECK_HIP(hipMemcpyAsync(e->h_amax[0], d_acc, (size_t)(seqs + n) * 4, hipMemcpyDeviceToHost, s));
     QH_CHECK_HIP(hipStreamSynchronize(s));
+    memcpy(accepted, e->h_amax[0], (size_t)seqs * 4);
+    memcpy(tokens, e->h_amax[0] + seqs, (size_t)n * 4);
     return QRAF_HIP_OK;
 }
 

@@ -330,7 +330,7 @@ class Engine:
              par.ctypes.data_as(i32p), pos.ctypes.data_as(i32p),
              wl.ctypes.data_as(C.POINTER(C.c_uint8)) if wl is not None else None,
              lg.ctypes.data_as(fp) if lg is not None else None, nx.ctypes.data_as(u32p) if nx is not None else None)
-        self._trees = [int(np.count_nonzero(sid == s)) for s in dict.fromkeys(sid.tolist())]
+        self._trees = np.diff(np.concatenate([[0], np.flatnonzero(np.diff(sid)) + 1, [n]]))  # rows of each sequence
         return lg, nx
 
     def accept_tree(self, params: SamplingParams, recent=None, uniforms=None):
@@ -338,7 +338,7 @@ class Engine:
         accepted drafts and the one behind them; their keys and values move behind its root (qraf_engine_accept_tree).
         recent, uniforms: a list and a draw for each row."""
         trees = getattr(self, "_trees", [])
-        n = sum(trees)
+        n = int(np.sum(trees))
         rec, cnt, stride = self._penalty(params, recent, n)
         uni = None if uniforms is None else np.ascontiguousarray(uniforms, dtype=np.float32)
         if uni is not None and uni.size != n:
