@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void group_any_kernel(GroupArgs a) {
 // Measured (16/2 heads of 128, us): 48 sequences of 5 rows at 128..4,096 fp16 positions
 // 41, of which the tiles 34 (117 MB read in the 28 beside 6 of plan and prologue: the
 // rate of a plain read); 128 rows behind 2,048 shared and 512 own ones 27, half of it
-// plan, prologue and join; 4 chunks of 128 rows at 400..2,000 f32 positions 46 (matrix
+// plan, prologue and join; 4 chunks of 128 rows at 400..2,000 f32 positions 41 (matrix
 // cores 18% busy, VALU 44%, 23% of the waves' time waiting for an instruction's turn);
 // 256 rows of 32,768: fp16 154 (446 TFLOP/s of products with q and p in 22 bits: 893
 // of the matrix cores'), int8 198, f32 266.  Powers of two by position and column cost
