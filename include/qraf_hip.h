@@ -286,7 +286,8 @@ int qraf_hip_group_attention_dev(const float* q, const void* k_cache, const void
  * (qraf_hip_tree_attention_workspace_bytes) needs no initialisation; calls that
  * share one must not overlap.  The same from call to call; what is held of each
  * operand is as for qraf_hip_group_attention_dev, whose shapes and blocks these
- * are: a sequence's positions are read once by each 128 query vectors.  Values of
+ * are: a sequence's positions are read once by each 128 query vectors (few rows on
+ * f32 pages: once by each row, and all of it in fp32).  Values of
  * positions that a row does not attend to do not reach it, an infinity or NaN
  * among them.  No counterpart in the reference, which has no drafts. */
 uint64_t qraf_hip_tree_attention_workspace_bytes(int32_t n_rows, int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
@@ -735,7 +736,8 @@ int qraf_engine_verify(qraf_engine* engine, int32_t row0, int32_t n_seqs, const 
  * attends to its sequence's positions ahead of the tree, its ancestors and itself,
  * and is rotated for its depth (qraf_hip_tree_append_dev,
  * qraf_hip_tree_attention_dev); node j of a tree takes the cache's position
- * positions[first] + j.  Up to 64 nodes a sequence.  Sequences that
+ * positions[first] + j.  Up to 64 nodes a sequence; a step of roots alone is
+ * qraf_engine_step's, bit for bit.  Sequences that
  * qraf_engine_set_repetition_penalty counts for are refused (QRAF_HIP_ERR_STATE):
  * drafts would be counted; qraf_engine_accept_tree takes the penalty with the call.
  * No reference counterpart. */

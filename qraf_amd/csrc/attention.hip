@@ -51,7 +51,8 @@
 // f32 / fp16 pages on request) is plain fp32 VALU code on the chunk grid:
 // scores with thread = position, output with thread = (head, dimension).
 // attn_few_kernel takes f32 pages where one workgroup per query head (or KV
-// head) does not fill the chip: fp32 VALU code, latency-bound.
+// head) does not fill the chip: fp32 VALU code, latency-bound; also for rows of
+// trees of drafted tokens.
 #include <math.h>
 
 #include <algorithm>
@@ -98,6 +99,11 @@ struct AttnArgs {
     float scale;
     int gx;                    // split kernel: workgroups per KV head
     int ps_log2;               // matrix-core kernels: page_size = 1 << ps_log2
+    // Trees (attn_few_kernel): page_table is [groups][max_pages], ctx unused.  Sequence g has rows starts[g] ..
+    // starts[g + 1] - 1 and base[g] positions of cache; a row attends to these and to base + b where bit b of its mask is.
+    const int32_t *starts, *base;
+    const unsigned long long* masks;
+    int groups;  // at most 64
 };
 
 // final output element: f32, or split into the two planes a GEMM consumes
@@ -334,6 +340,11 @@ __global__ __launch_bounds__(ACH) void attn_decode_kernel(AttnArgs a) {
 // zeros costs about what clamping its position did; zeroing what it loaded
 // took 3.42 us instead of 3.24 (9/3 heads of 64, 161 positions, warm) and
 // 4.23 instead of 3.88 inside a step, where the code is not in the caches.
+//
+// TREE: rows of trees of drafted tokens.  The sequences' first rows and cache lengths
+// are requested with the row's mask, a lane to a sequence; the page ids wait for them
+// where there is more than one.  Positions that a row does not attend to are as those
+// past the context.
 // ---------------------------------------------------------------------------
 // lane exchanges without LDS: DPP controls inside rows of 16 lanes (quad_perm
 // for xor 1 and 2, row_ror, row_newbcast), lane-row swaps across them
@@ -364,7 +375,7 @@ typedef float f4_raw __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(1))) f4_raw GlobalF4;
 // a maximum to subtract: scores that are all -inf stay -inf, and count as 0
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
-template <int HD, int G, int TPW>
+template <int HD, int G, int TPW, bool TREE>
 __global__ __launch_bounds__(1024, 4) void attn_few_kernel(AttnArgs a) {
     constexpr int NW = 16, KQ = HD / 16, VQ = HD / 64;  // float4s of a lane's K quarter, of its V dimensions
     __shared__ __align__(16) float s_o[NW][G][HD];
@@ -377,11 +388,28 @@ __global__ __launch_bounds__(1024, 4) void attn_few_kernel(AttnArgs a) {
 
     // requested together: the context length, the page id of the lane's
     // position per tile (table index clamped into the table), q
-    const int ctx_raw = a.ctx[s];
+    int ctx_raw = 0, seq = s, base = 0;
+    unsigned long long mask = 0;
+    bool inside = true;  // some sequence's row
+    if constexpr (TREE) {
+        auto start = [&](int g) { return max(0, min(a.starts[g], a.n)); };
+        mask = a.masks[s];
+        const int first = start(min(lane, a.groups - 1)), end = start(a.groups), cache = a.base[min(lane, a.groups - 1)];
+        const int upto = __popcll(__ballot(lane < a.groups && first <= s));
+        inside = upto > 0 && s < end;
+        seq = a.groups == 1 ? 0 : max(upto - 1, 0);
+        base = max(0, min(__builtin_amdgcn_readlane(cache, max(upto - 1, 0)), a.max_ctx));
+        const int room = a.max_ctx - base;
+        if (room < 64) mask &= (1ull << room) - 1;
+        ctx_raw = mask ? base + 64 - __clzll(mask) : base;
+    } else {
+        ctx_raw = a.ctx[s];
+    }
+    auto attends = [&](int p) { return p < base || (p - base < 64 && mask >> (p - base) & 1); };
     int pg[TPW];
 #pragma unroll
     for (int t = 0; t < TPW; t++)
-        pg[t] = a.page_table[(size_t)s * a.max_pages + min(16 * (wave + NW * t) + i, a.max_ctx - 1) / a.page_size];
+        pg[t] = a.page_table[(size_t)seq * a.max_pages + min(16 * (wave + NW * t) + i, a.max_ctx - 1) / a.page_size];
     const float* qp = a.q + ((size_t)s * a.H + head) * HD + 4 * j;
     float4 q[G][KQ];
 #pragma unroll
@@ -389,7 +417,11 @@ __global__ __launch_bounds__(1024, 4) void attn_few_kernel(AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < KQ; k++) q[h][k] = *(const float4*)(qp + h * HD + 16 * k);
     const int ctx = min(ctx_raw, a.max_ctx);
-    if (ctx <= 0) return;
+    if (TREE && !inside) return;
+    if (ctx <= 0) {
+        if (TREE && tid < G * HD) attn_store(a, ((size_t)s * a.H + head) * HD + tid, 0.f);
+        return;
+    }
 
     const float* kc = (const float*)a.kc;
     const float* vc = (const float*)a.vc;
@@ -407,7 +439,7 @@ __global__ __launch_bounds__(1024, 4) void attn_few_kernel(AttnArgs a) {
             for (int k = 0; k < KQ; k++) kr[t][k] = *(const float4*)(kp + 16 * k);
             auto vrow = [&](int x, int id, float4 (&v)[VQ]) {
                 const uint64_t at = (uint64_t)(vc + row(p0 + x, id));
-                const uint64_t vp = (p0 + x < ctx ? at : (uint64_t)g_zero_row) + 16 * c;
+                const uint64_t vp = ((TREE ? attends(p0 + x) : p0 + x < ctx) ? at : (uint64_t)g_zero_row) + 16 * c;
 #pragma unroll
                 for (int y = 0; y < VQ; y++) v[y] = __builtin_bit_cast(float4, *((const GlobalF4*)vp + 16 * y));
             };
@@ -444,7 +476,7 @@ __global__ __launch_bounds__(1024, 4) void attn_few_kernel(AttnArgs a) {
                 x += dpp<DPP_XOR1>(x);
                 x += dpp<DPP_XOR2>(x);
                 x *= a.scale;  // attention.cpp:134: dot * scale
-                sc[t][h] = p0 + i < ctx ? x : -INFINITY;
+                sc[t][h] = (TREE ? attends(p0 + i) : p0 + i < ctx) ? x : -INFINITY;
                 m[h] = fmaxf(m[h], sc[t][h]);
             }
         }
@@ -1682,6 +1714,58 @@ static int few_heads(int n, int H, int Hkv, int hd, int max_ctx) {
     return hd == 64 && max_ctx <= 512 && n * Hkv <= 256 && (G < 4 || (G == 4 && max_ctx <= 256)) ? G : 0;
 }
 
+// attn_few_kernel for `few` query heads a workgroup (few_heads)
+template <bool TREE>
+static void launch_few(const AttnArgs& a, int few, int hd, int max_ctx, hipStream_t st) {
+    const dim3 grid(a.n, a.H / few);
+    const int tpw = (max_ctx + 255) / 256;  // 16-position tiles per wave
+    if (hd == 128 && tpw == 1) hipLaunchKernelGGL((attn_few_kernel<128, 1, 1, TREE>), grid, dim3(1024), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((attn_few_kernel<128, 1, 2, TREE>), grid, dim3(1024), 0, st, a);
+    else if (tpw > 2) hipLaunchKernelGGL((attn_few_kernel<64, 1, 4, TREE>), grid, dim3(1024), 0, st, a);
+#define QH_ATTN_FEW(Gv)                                                                                      \
+    else if (few == Gv) {                                                                                    \
+        if (tpw == 1) hipLaunchKernelGGL((attn_few_kernel<64, Gv, 1, TREE>), grid, dim3(1024), 0, st, a);    \
+        else hipLaunchKernelGGL((attn_few_kernel<64, Gv, 2, TREE>), grid, dim3(1024), 0, st, a);             \
+    }
+    QH_ATTN_FEW(1) QH_ATTN_FEW(2) QH_ATTN_FEW(3) QH_ATTN_FEW(4)
+#undef QH_ATTN_FEW
+}
+// Trees on f32 pages: whether a call of these sizes goes to attn_few_kernel (0: to group_tile_kernel, in one launch or
+// planned), and that.  The rule of steps without trees holds for them.  Here against there, us: trees of 8 / 28 nodes at
+// 300 positions, 9/3 heads of 64, 5.6 / 5.8 against 10.7 / 11.2, of 8 at 1,000 8.8 against 14.2; 4 trees of 8 / 20 at 300 7.7 /
+// 8.1 against 11.8 / 14.7; 16/2 heads of 128, of 8 / 16 at 300 10.4 / 11.4 against 14.5 / 15.1, of 8 at 500 11.8 against 19.5.
+int tree_few_heads(int n, int seqs, int H, int Hkv, int hd, int page_size, int max_ctx) {
+    const bool shape = (hd == 64 || hd == 128) && H / Hkv <= 16 && page_size % 4 == 0 && (page_size & (page_size - 1)) == 0;
+    return shape && seqs <= 64 ? few_heads(n, H, Hkv, hd, max_ctx) : 0;
+}
+int launch_tree_few(const float* q, const void* kc, const void* vc, const int32_t* page_table, int max_pages,
+                    const int32_t* base, const int32_t* row_starts, const uint64_t* masks, int n, int seqs, int H, int Hkv,
+                    int hd, int page_size, float scale, int max_ctx, int few, float* out, hipStream_t st, uint16_t* out_hi,
+                    uint16_t* out_lo) {
+    AttnArgs a{};
+    a.q = q;
+    a.kc = kc;
+    a.vc = vc;
+    a.page_table = page_table;
+    a.out = out;
+    a.out_hi = out_hi;
+    a.out_lo = out_lo;
+    a.n = n;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.page_size = page_size;
+    a.max_pages = max_pages;
+    a.max_ctx = max_ctx;
+    a.scale = scale;
+    a.starts = row_starts;
+    a.base = base;
+    a.masks = (const unsigned long long*)masks;
+    a.groups = seqs;
+    launch_few<true>(a, few, hd, max_ctx, st);
+    QH_CHECK_HIP(hipGetLastError());
+    return QRAF_HIP_OK;
+}
+
 // query heads per KV head that attn_decode_kernel is built for at head_dim 64
 static bool valu_group(int G) { return G <= 4 || G == 6 || G == 8 || G == 12 || G == 16; }
 
@@ -1743,7 +1827,7 @@ int launch_attention(const float* q, const void* kc, const void* vc, uint32_t kv
                "attention: workspace too small");
     const int items = n * ((max_ctx + ACH - 1) / ACH);
     const size_t slots = attn_slots(n, Hkv, hd, max_ctx);
-    AttnArgs a;
+    AttnArgs a{};
     a.q = q;
     a.kc = kc;
     a.vc = vc;
@@ -1779,18 +1863,7 @@ int launch_attention(const float* q, const void* kc, const void* vc, uint32_t kv
     const int few = kv_dtype == DT_F32 && mfma_shape && g_attn_form == 0 && !refused
                         ? few_heads(n, H, Hkv, hd, max_ctx) : 0;
     if (few) {
-        const dim3 grid(n, H / few);
-        const int tpw = (max_ctx + 255) / 256;  // 16-position tiles per wave
-        if (hd == 128 && tpw == 1) hipLaunchKernelGGL((attn_few_kernel<128, 1, 1>), grid, dim3(1024), 0, st, a);
-        else if (hd == 128) hipLaunchKernelGGL((attn_few_kernel<128, 1, 2>), grid, dim3(1024), 0, st, a);
-        else if (tpw > 2) hipLaunchKernelGGL((attn_few_kernel<64, 1, 4>), grid, dim3(1024), 0, st, a);
-#define QH_ATTN_FEW(Gv)                                                                                      \
-    else if (few == Gv) {                                                                                    \
-        if (tpw == 1) hipLaunchKernelGGL((attn_few_kernel<64, Gv, 1>), grid, dim3(1024), 0, st, a);    \
-        else hipLaunchKernelGGL((attn_few_kernel<64, Gv, 2>), grid, dim3(1024), 0, st, a);                   \
-    }
-        QH_ATTN_FEW(1) QH_ATTN_FEW(2) QH_ATTN_FEW(3) QH_ATTN_FEW(4)
-#undef QH_ATTN_FEW
+        launch_few<false>(a, few, hd, max_ctx, st);
         QH_CHECK_HIP(hipGetLastError());
         return QRAF_HIP_OK;
     }

@@ -21,7 +21,8 @@
 // Trees of drafted tokens (qraf_hip_tree_attention_dev) are groups all of whose positions
 // are shared: a sequence's rows attend to its cache and, behind it, to the positions that
 // their 64-bit masks name.  The same jobs, pieces and tiles; tiles that reach behind the
-// cache take a bit for each position instead of a length.
+// cache take a bit for each position instead of a length.  Few rows on f32 pages go to
+// attn_few_kernel (attention.hip).
 #include <limits.h>
 #include <math.h>
 
@@ -2086,6 +2087,9 @@ int launch_tree_attention(const float* q, const void* kc, const void* vc, uint32
     const size_t need = tree_attention_workspace_bytes(n, seqs, H, Hkv, hd, max_ctx);
     QH_REQUIRE(ws_bytes >= need, QRAF_HIP_ERR_INVALID, "tree attention: workspace of %zu bytes, %zu needed", ws_bytes,
                need);
+    if (const int few = kv_dtype == DT_F32 ? tree_few_heads(n, seqs, H, Hkv, hd, page_size, max_ctx) : 0)
+        return launch_tree_few(q, kc, vc, page_table, max_pages, base, row_starts, masks, n, seqs, H, Hkv, hd, page_size, scale,
+                               max_ctx, few, out, st, out_hi, out_lo);
     GroupArgs a{};
     a.q = q;
     a.kc = kc;

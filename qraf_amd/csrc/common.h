@@ -243,6 +243,12 @@ int launch_tree_attention(const float* q, const void* kc, const void* vc, uint32
                           int seqs, int H, int Hkv, int hd, int page_size, float scale, int max_ctx, float* out,
                           void* ws, size_t ws_bytes, hipStream_t st, uint16_t* out_hi = nullptr,
                           uint16_t* out_lo = nullptr);
+// the same for few rows on f32 pages, a workgroup per row and `few` heads (attention.hip); 0: another form's
+int tree_few_heads(int n, int seqs, int H, int Hkv, int hd, int page_size, int max_ctx);
+int launch_tree_few(const float* q, const void* kc, const void* vc, const int32_t* page_table, int max_pages,
+                    const int32_t* base, const int32_t* row_starts, const uint64_t* masks, int n, int seqs, int H, int Hkv,
+                    int hd, int page_size, float scale, int max_ctx, int few, float* out, hipStream_t st, uint16_t* out_hi,
+                    uint16_t* out_lo);
 // the accepted path of each tree, and its keys and values moved together (tree.hip)
 int launch_tree_accept(const uint32_t* picks, const uint32_t* drafts, const int32_t* parents, const int32_t* starts,
                        int seqs, int rows, int32_t* accepted, int32_t* path, uint32_t* tokens, hipStream_t st);

@@ -499,7 +499,8 @@ struct qraf_engine {
     size_t group_ws_bytes = 0;
     void* tree_ws = nullptr;   // attention of trees, allocated by the first step of one
     size_t tree_ws_bytes = 0;
-    // the last step's trees while they can be accepted: nodes (0: none), sequences, rows of its layout in d_in
+    // the last step's trees while they can be accepted: nodes (0: none), sequences, rows of its layout in d_in (0: roots
+    // alone, a step as any other)
     int tree_nodes = 0, tree_seqs = 0, tree_n = 0;
     void* gemm_ws = nullptr;  // split-K partial tiles of the batched projections
     size_t gemm_ws_bytes = 0;
@@ -1594,7 +1595,13 @@ int qraf_engine_step_tree(qraf_engine* e, int32_t n, const int32_t* seq_ids, con
         QH_REQUIRE(seq_ids[i] < 0 || seq_ids[i] >= (int32_t)e->pen_slot.size() || e->pen_slot[seq_ids[i]] < 0,
                    QRAF_HIP_ERR_STATE, "step_tree: sequence %d counts its tokens for a repetition penalty", seq_ids[i]);
     }
-    QH_TRY(step_issue(e, n, seq_ids, tokens, nullptr, positions, want_logits, logits, next_tokens != nullptr, parents));
+    const bool drafts = (int32_t)ids.size() < n;
+    QH_TRY(step_issue(e, n, seq_ids, tokens, nullptr, positions, want_logits, logits, next_tokens != nullptr,
+                      drafts ? parents : nullptr));
+    if (!drafts && e->last_logit_rows == n) {
+        e->tree_nodes = e->tree_seqs = n;
+        e->tree_n = 0;
+    }
     const qraf_engine::Pending p = e->pending[0];
     e->n_pending = 0;
     const double t0 = now_us();
@@ -1767,6 +1774,13 @@ int qraf_engine_accept_tree(qraf_engine* e, const qraf_sampling_params* p, const
     uint8_t* rest = nullptr;
     QH_TRY(sample_rows(e, 0, n, p, recent, counts, stride, uniforms, &d_pick, 3 * rb, &rest));
     e->tree_nodes = 0;  // (the cache moves)
+    if (at == 0) {
+        QH_CHECK_HIP(hipMemcpyAsync(e->h_amax[0], d_pick, (size_t)n * 4, hipMemcpyDeviceToHost, e->stream));
+        QH_CHECK_HIP(hipStreamSynchronize(e->stream));
+        memset(accepted, 0, (size_t)seqs * 4);
+        memcpy(tokens, e->h_amax[0], (size_t)n * 4);
+        return QRAF_HIP_OK;
+    }
     int32_t *d_path = (int32_t*)rest, *d_acc = (int32_t*)(rest + rb);
     uint32_t* d_tok = (uint32_t*)(d_acc + seqs);  // (one copy with the lengths, into pinned memory)
     const int32_t* d_gpre = e->d_in + 7 * (size_t)at;

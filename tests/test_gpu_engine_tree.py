@@ -400,3 +400,28 @@ def test_an_engine_of_one_row(hip):
     assert len(got) == 10 and got[:sure] == want[:sure]
     assert len(InferenceEngine(tf, eos_token=None).score(prompt)["logprobs"]) == 4
     tf.engine.close()
+
+
+@KINDS
+@pytest.mark.parametrize("rows", [1, 3])
+def test_roots_alone_are_steps_as_any_other(hip, kv, rows):
+    """The same logits bit for bit as qraf_engine_step's, eager, captured and replayed; their tokens, once."""
+    from qraf_amd._lib import ERR_STATE, HipError, SamplingParams
+    tf, kw = make("q4_gqa8_hd128", kv)
+    e, rng = tf.engine, np.random.default_rng(4)
+    params = SamplingParams(0.8, 10, 0.9, 1.0)
+    seqs = [[e.seq_create() for _ in range(rows)] for _ in range(2)]
+    for k in range(5):
+        toks, uni = tokens(rng, kw, rows), rng.random(rows).astype(np.float32)
+        want = e.step(seqs[0], toks, [k] * rows, logits=True)
+        sampled = e.sample(params, uniforms=uni, rows=rows)
+        with pytest.raises(HipError) as x:
+            e.accept_tree(SamplingParams(0.0, 0, 1.0, 1.0))  # no trees
+        assert x.value.code == ERR_STATE
+        got = e.step_tree(seqs[1], toks, [-1] * rows, [k] * rows, logits=True)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        assert e.accept_tree(params, uniforms=uni) == [[int(t)] for t in sampled]
+        with pytest.raises(HipError) as x:
+            e.accept_tree(params, uniforms=uni)
+        assert x.value.code == ERR_STATE
+    e.close()
