@@ -425,3 +425,29 @@ def test_roots_alone_are_steps_as_any_other(hip, kv, rows):
             e.accept_tree(params, uniforms=uni)
         assert x.value.code == ERR_STATE
     e.close()
+
+
+@pytest.mark.parametrize("kv", [po.F32, po.F16], ids=["f32", "f16"])
+def test_a_sequence_released_ahead_of_its_acceptance(hip, kv):
+    """The other's path goes on as if it were alone, and so does the sequence that takes the released pages."""
+    from qraf_amd._lib import SamplingParams
+    tf, kw = make("q4_gqa8_hd128", kv)
+    e, rng, greedy = tf.engine, np.random.default_rng(6), SamplingParams(0.0, 0, 1.0, 1.0)
+    prompt = tokens(rng, kw, 21)
+    alone = e.seq_create()
+    feed(e, alone, prompt[:-1])
+    first = int(e.step([alone], [prompt[-1]], [20], argmax=True)[1][0])
+    want = e.step([alone], [first], [21], logits=True)[0]
+    a, b = e.seq_create(), e.seq_create()
+    for s in (a, b):
+        feed(e, s, prompt[:-1])
+    rows = [prompt[-1], (first + 1) % kw["vocab"], first]
+    e.step_tree([a] * 3 + [b] * 3, rows * 2, [-1, 0, 0, -1, 3, 3], [20] * 6)
+    e.seq_release(a)
+    got = e.accept_tree(greedy)
+    assert [len(g) for g in got] == [2, 2] and got[1][0] == first
+    c = e.seq_create()
+    feed(e, c, prompt)
+    check_logits(e.step([b], [first], [21], logits=True)[0], want)
+    check_logits(e.step([c], [first], [21], logits=True)[0], want)
+    e.close()
