@@ -332,7 +332,8 @@ int qraf_hip_tree_append_dev(const float* qkv, const float* bias, int32_t n_rows
  * In every layer: k_cache and v_cache are n_layers caches of the layouts above,
  * layer_bytes apart (a multiple of 4).  page_table as for
  * qraf_hip_tree_attention_dev; entries of a path past max_pages_per_seq pages end
- * it.  Positions behind the path keep their contents.  n_rows is the number of
+ * it, and so does a base there (a negative one is 0).  Positions behind the path
+ * keep their contents.  n_rows is the number of
  * entries of path, n_seqs up to 65535, head_dim 16, 32, 64 or 128.  No counterpart
  * in the reference. */
 int qraf_hip_kv_compact_dev(void* k_cache, void* v_cache, uint32_t kv_dtype, int32_t n_layers, uint64_t layer_bytes,

@@ -115,7 +115,9 @@ template <int KV, typename Piece>
 __global__ __launch_bounds__(512) void kv_compact_kernel(CompactArgs a) {
     constexpr int ITEM = KV == (int)DT_F32 ? 4 : KV == (int)DT_F16 ? 2 : 1;
     const int s = blockIdx.y, lane = threadIdx.x & 63, ps = a.page_size, hd = a.hd, most = a.max_pages - 1;
-    const int base = max(0, a.base[s]), r0 = max(0, min(a.starts[s], a.rows)), n = max(0, min(a.starts[s + 1], a.rows) - r0);
+    // (a base at or past the table's end, which no path begins ahead of, as that end: at most 2^30, so sums below hold)
+    const int base = max(0, min(a.base[s], a.max_pages * ps));
+    const int r0 = max(0, min(a.starts[s], a.rows)), n = max(0, min(a.starts[s + 1], a.rows) - r0);
     const int32_t* table = a.table + (size_t)s * a.max_pages;
     const int first = base / ps, page_of = table[min(first + lane, most)];  // the tree's pages, a lane to a page
     const size_t block = (size_t)ps * (KV == (int)DT_I8 ? hd + 4 : hd * ITEM);  // bytes of a (page, KV head)

@@ -213,6 +213,30 @@ def test_compact_past_the_table(hip, kv):
     run_compact(hip, kv, [(20, 30, [0, 5, 11, 13, 25])], wide=2)
 
 
+@KINDS
+@pytest.mark.parametrize("base", [5, 6, 100, 2 ** 30, 2 ** 31 - 64, 2 ** 31 - 63, 2 ** 31 - 1, -1, -2 ** 31])
+def test_compact_bases_past_the_table(hip, kv, base):
+    """Pages of one position: a base at the table's end or past it, up to int32's largest, moves nothing and names no
+    page outside the table; a negative one is 0."""
+    from qraf_amd.backend import DeviceBuffer
+    rng, wide, nodes, up = np.random.default_rng(15), 5, 70, DeviceBuffer.from_array
+    pool = Pool(rng, kv, 2, 3 * wide, 2, 1, 64)
+    # the second sequence's table row; those beside it name other pages
+    table = rng.permutation(3 * wide).astype(np.int32).reshape(3, wide)
+    path = np.tile(np.concatenate([[1, 2, 4], np.arange(5, 5 + nodes - 3)]), 3).astype(np.int32)
+    path[:nodes] = path[2 * nodes:] = -1
+    d = [up(x) for x in (pool.k, pool.v, table, np.array([0, base, 0], np.int32),
+                         (np.arange(4) * nodes).astype(np.int32), path)]
+    hip._lib.call("qraf_hip_kv_compact_dev", d[0].ptr, d[1].ptr, kv, 2, pool.layer_bytes, d[2].ptr, wide, d[3].ptr,
+                  d[4].ptr, d[5].ptr, 3, path.size, 2, 64, 1, None)
+    hip._lib.call("qraf_hip_device_synchronize")
+    for v, b, was in ((False, d[0], pool.k), (True, d[1], pool.v)):
+        cell, want = pool.cells(v), was.copy()
+        for to, at in ((0, 1), (1, 2), (2, 4)) if base < 0 else ():
+            want[cell[:, table[1, to], :, 0]] = was[cell[:, table[1, at], :, 0]]
+        assert np.array_equal(b.download(np.uint8, want.size), want)
+
+
 def test_compact_many_layers_and_sequences(hip):
     rng = np.random.default_rng(13)
     seqs = [(int(rng.integers(0, 60)), 12, [0] + sorted(rng.choice(np.arange(1, 12), 4, replace=False)))
