@@ -35,6 +35,7 @@
 
 #include "common.h"
 #include "kv_pages.h"
+#include "tree_rows.h"
 
 namespace qraf_hip {
 
@@ -1139,17 +1140,15 @@ static int step_issue(qraf_engine* e, int32_t n, const int32_t* seq_ids, const u
     if (tree) {
         QH_TRY(tree_workspace(e));
         places.resize(n);
-        for (int i = 0, first = 0; i < n; i++) {
-            if (i > 0 && seq_ids[i] != seq_ids[i - 1]) first = i;
-            places[i] = (int32_t)std::min<int64_t>((int64_t)positions[first] + (i - first), INT_MAX);
-        }
+        tree_places(n, seq_ids, positions, places.data());
+        positions = places.data();  // (the caller's are those of first rows alone)
     }
     // the rows' sequences and positions checked, their new pages taken from
     // the pool and their page-table rows written (nothing changes on failure);
     // step_ctx, the longest context of this step, sizes the attention grid
     // (and skips the merge)
     int step_ctx = 1;
-    QH_TRY(e->pages.plan_step(n, seq_ids, tree ? places.data() : positions, ptab, &step_ctx));
+    QH_TRY(e->pages.plan_step(n, seq_ids, positions, ptab, &step_ctx));
     e->last_logit_rows = 0;  // set again once this step's launches are issued
     e->tree_nodes = 0;
     for (int i = 0; i < n; i++) {

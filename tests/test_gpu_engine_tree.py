@@ -363,6 +363,32 @@ def test_refusals(hip):
     e.close()
 
 
+@KINDS
+def test_positions_of_drafts_are_not_read(hip, kv):
+    """Whatever stands there, int32's ends among it: the same logits bit for bit, eager, captured and replayed, the same
+    paths, and the same steps behind them."""
+    from qraf_amd._lib import SamplingParams
+    tf, kw = make("q8_hd64_gqa3", kv, max_batch=32)
+    e, rng, greedy = tf.engine, np.random.default_rng(7), SamplingParams(0.0, 0, 1.0, 1.0)
+    prompts, ends = [tokens(rng, kw, 19), tokens(rng, kw, 7)], [2 ** 31 - 1, -2 ** 31, -1, 10 ** 6]
+    seqs = [[e.seq_create() for _ in prompts] for _ in range(2)]
+    for p, s, r in zip(prompts, *seqs):
+        feed(e, s, p)
+        feed(e, r, p)
+    bases = [len(p) for p in prompts]
+    for turn in range(4):
+        trees = [(tokens(rng, kw, n), random_tree(rng, n)) for n in (9, 4)]
+        sid, tok, par, pos = flat(trees, seqs[0], bases)
+        want = e.step_tree(sid, tok, par, pos, logits=True)[0]
+        said = e.accept_tree(greedy)
+        sid = flat(trees, seqs[1], bases)[0]
+        pos = [p if up < 0 else ends[(i + turn) % 4] for i, (p, up) in enumerate(zip(pos, par))]
+        assert np.array_equal(e.step_tree(sid, tok, par, pos, logits=True)[0], want)
+        assert e.accept_tree(greedy) == said
+        bases = [b + len(t) for b, t in zip(bases, said)]
+    e.close()
+
+
 def test_more_than_64_nodes_are_refused(hip):
     from qraf_amd._lib import ERR_INVALID, HipError
     tf, kw = transformer("q8_llama", max_batch=128)
