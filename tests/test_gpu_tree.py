@@ -237,6 +237,39 @@ def test_compact_bases_past_the_table(hip, kv, base):
         assert np.array_equal(b.download(np.uint8, want.size), want)
 
 
+@KINDS
+@pytest.mark.parametrize("pad,shift", [(4, 0), (8, 0), (12, 0), (0, 4), (0, 8), (0, 12), (12, 4)])
+@pytest.mark.parametrize("Hkv,hd,ps", [(3, 64, 16), (2, 128, 16), (5, 16, 6), (2, 32, 48)])
+def test_compact_of_caches_that_four_bytes_align(hip, kv, Hkv, hd, ps, pad, shift):
+    """Layers and pools whose alignment is 4 or 8 bytes: keys move in pieces of 4.  Paths of more than eight entries, of
+    neighbours among them; the bytes ahead of a pool and behind a layer stay."""
+    from qraf_amd.backend import DeviceBuffer
+    rng, up, layers = np.random.default_rng(16), DeviceBuffer.from_array, 3
+    seqs = [(37, 30, [0, 3, 4, 5, 6, 7, 9, 12, 13, 19, 28, 29]), (14, 12, [0, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11]),
+            (0, 20, [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18])]
+    per = [-(-(b + n) // ps) for b, n, _ in seqs]
+    pool = Pool(rng, kv, layers, sum(per), Hkv, ps, hd, pad)
+    table, ids = np.zeros((3, max(per)), np.int32), np.split(rng.permutation(sum(per)), np.cumsum(per)[:-1])
+    path = np.concatenate([p + [-1] * (n - len(p)) for _, n, p in seqs]).astype(np.int32)
+    for t, i in zip(table, ids):
+        t[:len(i)] = i
+    base, starts = np.array([b for b, _, _ in seqs], np.int32), np.cumsum([0] + [n for _, n, _ in seqs]).astype(np.int32)
+    ahead = rng.integers(0, 256, shift).astype(np.uint8)
+    k, v, t, bs, st, pt = (up(x) for x in (np.concatenate([ahead, pool.k]), np.concatenate([ahead, pool.v]), table, base,
+                                           starts, path))
+    hip._lib.call("qraf_hip_kv_compact_dev", k.ptr + shift, v.ptr + shift, kv, layers, pool.layer_bytes, t.ptr,
+                  table.shape[1], bs.ptr, st.ptr, pt.ptr, 3, path.size, Hkv, hd, ps, None)
+    hip._lib.call("qraf_hip_device_synchronize")
+    for b, was, by_dim in ((k, pool.k, False), (v, pool.v, True)):
+        cell, want = pool.cells(by_dim), was.copy()
+        for row, (at, _, nodes) in zip(table, seqs):
+            for j, node in enumerate(nodes):
+                src, dst = at + node, at + j
+                want[cell[:, row[dst // ps], :, dst % ps]] = was[cell[:, row[src // ps], :, src % ps]]
+        got = b.download(np.uint8, shift + want.size)
+        assert np.array_equal(got[:shift], ahead) and np.array_equal(got[shift:], want)
+
+
 def test_compact_many_layers_and_sequences(hip):
     rng = np.random.default_rng(13)
     seqs = [(int(rng.integers(0, 60)), 12, [0] + sorted(rng.choice(np.arange(1, 12), 4, replace=False)))
