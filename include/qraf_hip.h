@@ -286,10 +286,11 @@ int qraf_hip_group_attention_dev(const float* q, const void* k_cache, const void
  * (qraf_hip_tree_attention_workspace_bytes) needs no initialisation; calls that
  * share one must not overlap.  The same from call to call; what is held of each
  * operand is as for qraf_hip_group_attention_dev, whose shapes and blocks these
- * are: a sequence's positions are read once by each 128 query vectors (few rows on
- * f32 pages: once by each row, and all of it in fp32).  Values of
- * positions that a row does not attend to do not reach it, an infinity or NaN
- * among them.  No counterpart in the reference, which has no drafts. */
+ * are: a sequence's positions are read once by each block of 128 query vectors, in
+ * small calls and in shapes that the blocks do not take by each row.  (Few rows on
+ * f32 pages: by each row and query head, or by each row and KV head where a workgroup
+ * takes all query heads of one, and all of it in fp32.)  Values of positions that a
+ * row does not attend to do not reach it, an infinity or NaN among them.  No counterpart in the reference, which has no drafts. */
 uint64_t qraf_hip_tree_attention_workspace_bytes(int32_t n_rows, int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
                                                  int32_t head_dim, int32_t max_ctx);
 int qraf_hip_tree_attention_dev(const float* q, const void* k_cache, const void* v_cache, uint32_t kv_dtype,
