@@ -628,10 +628,10 @@ constexpr int tile_floats(int hd) { return GW * 32 * hd; }
 // TREE: rows attend to their sequence's cache and to the positions behind it that their masks name, all of them shared
 // (the prefix ends where their attention does): tiles that reach behind the cache go by bits.
 // LANES: the plan is lane_plan's.
-// Trees, measured (16/2 heads of 128, us a call): 64 nodes at 8,000 positions, fp16, 25.9, of which the join's launch 4.7
+// Trees, measured (16/2 heads of 128, us a call): 64 nodes at 8,000 positions, fp16, 25.4, of which the join's launch 4.7
 // and in the tiles' 40,000 cycles the plan 4,500, the piece and q 10,000, four tiles 18,000 and the outputs 8,000; 48
-// trees of up to 16 at 128..4,096, fp16, 56.6: 114 MB at a plain read's rate in 30 behind as much that is fixed; 24 of up
-// to 26 at 3,000..8,000, int8, 95: widening and softmax (VALU) beside the products; 8 of 64 at 777..2,000, f32, 45.9.
+// trees of up to 16 at 128..4,096, fp16, 52 to 64: 114 MB at a plain read's rate in 30 behind 20 that are fixed; 24 of up
+// to 26 at 3,000..8,000, int8, 89 to 95: widening and softmax (VALU) beside the products; 8 of 64 at 777..2,000, f32, 44 to 48.
 template <int HD, int KV, bool DIRECT, bool TREE, bool LANES>
 __global__ __launch_bounds__(GTH, 2) void group_tile_kernel(GroupArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;  // products per score tile, 32-dim output tiles
@@ -1965,6 +1965,8 @@ static int group_tiles(GroupArgs& a, uint32_t kv_dtype, int hd, void* ws, bool d
     a.part_ml = (float2*)((uint8_t*)ws + z.plan_bytes);
     a.part_o = (float*)((uint8_t*)ws + z.plan_bytes + z.ml_bytes);
     const int gx = group_grid(a.Hkv);
+    // (A lane to a sequence; more take the plan in LDS.  64 / 65 trees of 8, 16/2 heads of 128, us: at 128..4,096 positions f32
+    // 95 / 95, fp16 45.9 / 46.8, int8 44.5 / 45.5, at 300 29.4 / 31.4, 21.0 / 21.3, 21.8 / 21.2.)
     const bool lanes = TREE && a.groups <= 64;
     const size_t lds = lanes ? (size_t)tile_floats(hd) * 4 + (size_t)a.n * 8 : group_lds(hd, a.n, a.groups, z);
 #define QH_GROUP_TILE(HDv, KVv)                                                                                            \

@@ -85,9 +85,9 @@ int launch_tree_accept(const uint32_t* picks, const uint32_t* drafts, const int3
 // scales).  Every wave finds the moves for itself - the path and the pages that the tree
 // spans are requested at once, from lengths alone - and has eight moves in flight: three
 // reads one after another, then the writes, without a barrier.  Elements that become
-// neighbours (values by dimension) are written together.  One sequence: latency, 4.1 us.
-// 64 sequences of 6 nodes in 36 layers, fp16, 23.6 MB of keys and values: 19.6 us, in
-// which values by dimension bring every line of the pages that the tree spans, 76 MB read
+// neighbours (values by dimension) are written together.  One sequence: latency, 4.1 to 4.9 us.
+// 64 sequences of 6 nodes in 36 layers, fp16, 23.6 MB of keys and values: 19.6 to 19.8 us, in
+// which values by dimension bring every line of the pages that the tree spans, 77 MB read
 // and written at 3.9 TB/s.  (Keys alone 7.1; one node after another and keys ahead of
 // values 22.0; elements written one by one 20.3.)
 // ---------------------------------------------------------------------------

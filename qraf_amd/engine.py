@@ -580,6 +580,7 @@ class InferenceEngine:
             seq = e.seq_create()
             for a in range(0, n, e.max_batch):
                 b = min(a + e.max_batch, n)
+                # (argmax: of a step that returns neither logits nor tokens no logits are computed)
                 e.step([seq] * (b - a), tokens[a:b], range(a, b), logits=False, argmax=True)
                 parts.append(e.logprobs(tokens[a + 1:b + 1], top))
         finally:
